@@ -571,6 +571,12 @@ struct TimedLaunch {
 
 }  // namespace
 
+// The same message for the entry points of ccv1d_ops.h, in files of their own.
+namespace ccv1d {
+int report_error(int code, const char* message) { return fail(code, "%s", message); }
+void clear_error() { g_last_error.clear(); }
+}  // namespace ccv1d
+
 extern "C" {
 
 int ccv1d_abi_version(void) { return CCV1D_ABI_VERSION; }

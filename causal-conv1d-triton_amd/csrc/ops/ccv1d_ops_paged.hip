@@ -1,0 +1,202 @@
+// The plan of a batch over paged caches, and the write of keys and values into them.
+#include "ops_common.h"
+
+namespace ccv1d {
+namespace ops {
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------
+// Plan. Everything follows from two running sums over the requests: of the new tokens (where a
+// request's tokens lie) and of the pages that each needs (which free pages are its own). A launch
+// of its own for the sums would cost more than they do, so every workgroup makes them again, 1024
+// requests at a time, and then serves its share: every kPlanTokens-th range of token places that
+// falls into those requests, and the table rows of every gridDim.x-th of them. Nothing that one
+// workgroup writes is read by another: the table entries written are past the cached pages, and
+// those read are before them.
+// ---------------------------------------------------------------------------------------------
+
+constexpr int kPlanThreads = 256;
+constexpr int kPlanItems = 4;
+constexpr int kPlanChunk = kPlanThreads * kPlanItems;
+constexpr int kPlanTokens = 1024;  // token places of a workgroup
+
+__device__ __forceinline__ int64_t wave_scan(int64_t v, int lane) {
+#pragma unroll
+  for (int o = 1; o < kWave; o *= 2) {
+    const int64_t w = __shfl_up(v, o);
+    if (lane >= o) v += w;
+  }
+  return v;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(ccv1d_paged_plan_args p) {
+  __shared__ int64_t s_wave[2][kPlanThreads / kWave];
+  __shared__ int64_t s_start[kPlanChunk];  // first token place of a request
+  __shared__ int64_t s_nth[kPlanChunk];    // pages needed by the requests before it
+  __shared__ int32_t s_cached[kPlanChunk];
+  __shared__ int32_t s_have[kPlanChunk], s_need[kPlanChunk];  // need: -1 when not admitted
+  __shared__ int64_t s_used[kPlanThreads / kWave];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t R = p.requests, ps = p.page_size, M = p.max_pages;
+  const int64_t free = min((int64_t)max(*p.num_free, 0), p.num_free_pages);
+  const int64_t t0 = (int64_t)blockIdx.x * kPlanTokens;
+  const int64_t t1 = min(t0 + kPlanTokens, p.max_tokens);
+  const bool lead = blockIdx.x == 0;
+  int64_t tokens = 0, pages = 0, used = 0;  // over the requests before this chunk; used: my share
+
+  for (int64_t r0 = 0; r0 < R; r0 += kPlanChunk) {
+    int64_t c[kPlanItems], n[kPlanItems], have[kPlanItems], need[kPlanItems];
+    bool fits[kPlanItems];
+    int64_t st = 0, sp = 0;
+#pragma unroll
+    for (int i = 0; i < kPlanItems; ++i) {
+      const int64_t r = r0 + tid * kPlanItems + i;
+      c[i] = r < R ? max(p.cached_lens[r], 0) : 0;
+      n[i] = r < R ? max(p.new_lens[r], 0) : 0;
+      have[i] = (c[i] + ps - 1) / ps;
+      const int64_t want = (c[i] + n[i] + ps - 1) / ps;
+      fits[i] = want <= M;
+      need[i] = fits[i] ? want - have[i] : 0;
+      st += n[i];
+      sp += need[i];
+    }
+    const int64_t it = wave_scan(st, lane), ip = wave_scan(sp, lane);
+    __syncthreads();  // the last chunk's tables have been read
+    if (lane == kWave - 1) {
+      s_wave[0][wave] = it;
+      s_wave[1][wave] = ip;
+    }
+    __syncthreads();
+    int64_t et = tokens + it - st, ep = pages + ip - sp;  // before this lane's first request
+    for (int w = 0; w < kPlanThreads / kWave; ++w) {
+      if (w < wave) {
+        et += s_wave[0][w];
+        ep += s_wave[1][w];
+      }
+      tokens += s_wave[0][w];
+      pages += s_wave[1][w];
+    }
+    const int64_t chunk_start = tokens;  // end of this chunk's tokens
+#pragma unroll
+    for (int i = 0; i < kPlanItems; ++i) {
+      const int j = tid * kPlanItems + i;
+      const int64_t r = r0 + j;
+      const bool ok = fits[i] && (need[i] == 0 || ep + need[i] <= free);
+      s_start[j] = et;
+      s_nth[j] = ep;
+      s_cached[j] = (int32_t)c[i];
+      s_have[j] = (int32_t)have[i];
+      s_need[j] = ok ? (int32_t)need[i] : -1;
+      if (ok && need[i] > 0) used = ep + need[i];
+      if (lead && r < R) {
+        p.seq_lens[r] = (int32_t)(ok ? c[i] + n[i] : c[i]);
+        p.query_start[r] = (int32_t)et;
+      }
+      et += n[i];
+      ep += need[i];
+    }
+    __syncthreads();
+
+    // New pages of every gridDim.x-th request, a wave each.
+    const int live = (int)min((int64_t)kPlanChunk, R - r0);
+    for (int64_t j = blockIdx.x + (int64_t)wave * gridDim.x; j < live;
+         j += (int64_t)gridDim.x * (kPlanThreads / kWave)) {
+      int32_t* row = p.block_tables + (r0 + j) * p.block_table_stride;
+      for (int i = lane; i < s_need[j]; i += kWave)
+        row[s_have[j] + i] = p.free_pages[free - 1 - (s_nth[j] + i)];
+    }
+
+    // My token places inside this chunk's tokens: the last request that starts at or before each.
+    const int64_t lo = max(t0, s_start[0]), hi = min(t1, chunk_start);
+    for (int64_t t = lo + tid; t < hi; t += kPlanThreads) {
+      int a = 0, b = live;  // s_start[a] <= t < s_start[b]
+      while (b - a > 1) {
+        const int m = (a + b) / 2;
+        if (s_start[m] <= t) a = m;
+        else b = m;
+      }
+      int32_t pos = -1, id = -1;
+      int64_t slot = -1;
+      if (s_need[a] >= 0) {
+        id = (int32_t)(r0 + a);
+        pos = s_cached[a] + (int32_t)(t - s_start[a]);
+        const uint32_t pg = (uint32_t)pos / (uint32_t)ps, off = (uint32_t)pos % (uint32_t)ps;
+        const int32_t page = (int32_t)pg < s_have[a]
+                                 ? p.block_tables[(r0 + a) * p.block_table_stride + pg]
+                                 : p.free_pages[free - 1 - (s_nth[a] + pg - s_have[a])];
+        if (page >= 0) slot = (int64_t)page * ps + off;
+      }
+      p.positions[t] = pos;
+      p.request_ids[t] = id;
+      p.slot_mapping[t] = slot;
+    }
+  }
+
+  for (int64_t t = max(t0, tokens) + tid; t < t1; t += kPlanThreads) {
+    p.positions[t] = -1;
+    p.request_ids[t] = -1;
+    p.slot_mapping[t] = -1;
+  }
+  if (lead) {
+#pragma unroll
+    for (int o = kWave / 2; o; o /= 2) used = max(used, (int64_t)__shfl_xor(used, o));
+    if (lane == 0) s_used[wave] = used;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < kPlanThreads / kWave; ++w) used = max(used, s_used[w]);
+      p.query_start[R] = (int32_t)tokens;
+      *p.num_free_out = (int32_t)(free - used);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Write: a wave moves the heads of one token, 16 bytes a lane where rows allow it.
+// ---------------------------------------------------------------------------------------------
+
+template <typename V>
+__global__ __launch_bounds__(256) void paged_write_kernel(ccv1d_paged_write_args p, int per_head) {
+  const int64_t token = blockIdx.x;
+  const int64_t slot = p.slot_mapping[token];
+  if (slot < 0 || slot >= p.num_pages * p.page_size) return;
+  const int64_t page = slot / p.page_size, off = slot % p.page_size;
+  const int n = (int)p.kv_heads * per_head;
+  for (int i = threadIdx.x; i < 2 * n; i += 256) {
+    const bool val = i >= n;
+    const int j = val ? i - n : i;
+    const int64_t h = j / per_head, w = j % per_head;
+    const char* src = static_cast<const char*>(val ? p.v : p.k);
+    char* dst = static_cast<char*>(val ? p.v_cache : p.k_cache);
+    const int64_t from = val ? token * p.v_stride_t + h * p.v_stride_h
+                             : token * p.k_stride_t + h * p.k_stride_h;
+    const int64_t to = val ? page * p.v_cache_stride_p + off * p.v_cache_stride_t + h * p.v_cache_stride_h
+                           : page * p.k_cache_stride_p + off * p.k_cache_stride_t + h * p.k_cache_stride_h;
+    const int es = p.dtype == CCV1D_F32 ? 4 : 2;
+    *reinterpret_cast<V*>(dst + to * es + w * sizeof(V)) =
+        *reinterpret_cast<const V*>(src + from * es + w * sizeof(V));
+  }
+}
+
+}  // namespace
+
+hipError_t paged_plan(const ccv1d_paged_plan_args& a, hipStream_t s) {
+  const int64_t blocks = (a.max_tokens + kPlanTokens - 1) / kPlanTokens;
+  paged_plan_kernel<<<(unsigned)(blocks > 0 ? blocks : 1), kPlanThreads, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+hipError_t paged_write(const ccv1d_paged_write_args& a, hipStream_t s) {
+  const int es = a.dtype == CCV1D_F32 ? 4 : 2;
+  const int64_t bytes = a.head_dim * es;
+  typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
+  if (bytes % 16 == 0)
+    paged_write_kernel<u4><<<(unsigned)a.tokens, 256, 0, s>>>(a, (int)(bytes / 16));
+  else
+    paged_write_kernel<uint16_t><<<(unsigned)a.tokens, 256, 0, s>>>(a, (int)(bytes / 2));
+  return hipGetLastError();
+}
+
+}  // namespace ops
+}  // namespace ccv1d

@@ -1,0 +1,36 @@
+// Shared by the operators around the convolution: element access, launch helpers and the launchers
+// that the C ABI (ccv1d_ops_api.hip) calls after it has checked the arguments.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "ccv1d_ops.h"
+
+namespace ccv1d {
+
+// Defined in ccv1d_api.hip: the thread-local message behind ccv1d_last_error().
+int report_error(int code, const char* message);
+void clear_error();
+
+namespace ops {
+
+constexpr int kWave = 64;
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v) {
+  return static_cast<float>(v);
+}
+
+// Launchers (arguments checked, device current).
+hipError_t rec_fwd(const ccv1d_rec_args& a, hipStream_t s);
+hipError_t rec_bwd(const ccv1d_rec_args& a, hipStream_t s);
+size_t rec_workspace(int64_t B, int64_t T, int64_t D, bool backward);
+hipError_t rec_update(const ccv1d_rec_update_args& a, hipStream_t s);
+hipError_t paged_plan(const ccv1d_paged_plan_args& a, hipStream_t s);
+hipError_t paged_write(const ccv1d_paged_write_args& a, hipStream_t s);
+hipError_t paged_attn(const ccv1d_paged_attn_args& a, hipStream_t s);
+size_t paged_attn_workspace(const ccv1d_paged_attn_args& a);
+
+}  // namespace ops
+}  // namespace ccv1d
