@@ -1,138 +1,55 @@
-// The gated linear recurrence: one lane walks one channel of one sequence.
-#include "ops_rec_math.h"
+// Launch of the gated linear recurrence: workspace, the kernels around the main ones, and the form for
+// single tokens.
+#include "ops_rec_launch.h"
 
 namespace ccv1d {
 namespace ops {
 
 namespace {
 
-// One row's forward: the factor of the state before it and its own contribution.
-template <bool DECAY>
-__device__ __forceinline__ void coefficients(float k, float gate, float& r, float& log2a, float& a,
-                                             float& beta) {
-  if constexpr (DECAY) {
-    r = sigmoid(gate);
-    log2a = k * r;
-    a = __builtin_amdgcn_exp2f(log2a);
-    beta = __builtin_amdgcn_sqrtf(one_minus_square(log2a, a));
-  } else {
-    plain_gate(gate, a, beta);
-    r = a;
-    log2a = 0.0f;
-  }
+__global__ __launch_bounds__(256) void rec_clear_kernel(uint64_t* words, int64_t n) {
+  const int64_t stride = (int64_t)gridDim.x * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) words[i] = 0;
 }
 
-struct Row {
-  bool pad, first;  // padding; the state starts anew
-};
-
-__device__ __forceinline__ Row row_of(const int32_t* seq, int64_t t) {
-  Row w{false, false};
-  if (seq) {
-    const int32_t id = seq[t];
-    w.pad = id < 0;
-    w.first = t > 0 && seq[t - 1] != id;
-  }
-  return w;
+// No rows: the final states are the initial ones, and their gradients likewise; no decay gradient.
+__global__ __launch_bounds__(256) void rec_empty_kernel(const float* from, float* to, int64_t n,
+                                                        float* zero, int64_t nz) {
+  const int64_t stride = (int64_t)gridDim.x * 256;
+  const int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (to)
+    for (int64_t i = i0; i < n; i += stride) to[i] = from ? from[i] : 0.0f;
+  if (zero)
+    for (int64_t i = i0; i < nz; i += stride) zero[i] = 0.0f;
 }
 
-template <typename T, bool DECAY>
-__global__ __launch_bounds__(64) void rec_fwd_kernel(ccv1d_rec_args p) {
-  const int64_t nc = (p.dim + 63) / 64;
-  const int64_t b = blockIdx.x / nc, d = (blockIdx.x % nc) * 64 + threadIdx.x;
-  if (d >= p.dim) return;
-  const T* x = static_cast<const T*>(p.x) + b * p.x_stride_b + d;
-  const T* g = static_cast<const T*>(p.gate) + b * p.gate_stride_b + d;
-  const T* ig = p.input_gate ? static_cast<const T*>(p.input_gate) + b * p.input_gate_stride_b + d
-                             : nullptr;
-  const int32_t* seq = p.seq_idx ? p.seq_idx + b * p.seqlen : nullptr;
-  T* out = static_cast<T*>(p.out) + b * p.seqlen * p.dim + d;
-  const int64_t ns = (p.seqlen + CCV1D_REC_SAVED_ROWS - 1) / CCV1D_REC_SAVED_ROWS;
-  float* saved = p.saved ? p.saved + b * ns * p.dim + d : nullptr;
-  const float k = DECAY ? decay_rate(p.decay[d], p.decay_scale) : 0.0f;
-  float h = p.initial_states ? p.initial_states[b * p.dim + d] : 0.0f;
-  for (int64_t t = 0; t < p.seqlen; ++t) {
-    if (saved && t % CCV1D_REC_SAVED_ROWS == 0) saved[t / CCV1D_REC_SAVED_ROWS * p.dim] = h;
-    float r, l, a, beta;
-    coefficients<DECAY>(k, to_f32(g[t * p.gate_stride_t]), r, l, a, beta);
-    float u = beta * to_f32(x[t * p.x_stride_t]);
-    if (ig) u *= sigmoid(to_f32(ig[t * p.input_gate_stride_t]));
-    const Row w = row_of(seq, t);
-    h = w.pad ? 0.0f : w.first ? u : fmaf(a, h, u);
-    out[t * p.dim] = static_cast<T>(h);
-  }
-  if (p.final_states) p.final_states[b * p.dim + d] = h;
-}
-
-template <typename T, bool DECAY>
-__global__ __launch_bounds__(64) void rec_bwd_kernel(ccv1d_rec_args p) {
-  const int64_t nc = (p.dim + 63) / 64;
-  const int64_t b = blockIdx.x / nc, d = (blockIdx.x % nc) * 64 + threadIdx.x;
-  if (d >= p.dim) return;
-  const T* x = static_cast<const T*>(p.x) + b * p.x_stride_b + d;
-  const T* g = static_cast<const T*>(p.gate) + b * p.gate_stride_b + d;
-  const T* ig = p.input_gate ? static_cast<const T*>(p.input_gate) + b * p.input_gate_stride_b + d
-                             : nullptr;
-  const T* dy = static_cast<const T*>(p.dout) + b * p.dout_stride_b + d;
-  const int32_t* seq = p.seq_idx ? p.seq_idx + b * p.seqlen : nullptr;
-  const int64_t base = b * p.seqlen * p.dim + d;
-  T* dx = static_cast<T*>(p.dx) + base;
-  T* dg = static_cast<T*>(p.dgate) + base;
-  T* dig = ig ? static_cast<T*>(p.dinput_gate) + base : nullptr;
-  float* before = static_cast<float*>(p.workspace) + base;  // the state in front of each row
-  const float k = DECAY ? decay_rate(p.decay[d], p.decay_scale) : 0.0f;
-  float h = p.initial_states ? p.initial_states[b * p.dim + d] : 0.0f;
-  for (int64_t t = 0; t < p.seqlen; ++t) {
-    float r, l, a, beta;
-    coefficients<DECAY>(k, to_f32(g[t * p.gate_stride_t]), r, l, a, beta);
-    float u = beta * to_f32(x[t * p.x_stride_t]);
-    if (ig) u *= sigmoid(to_f32(ig[t * p.input_gate_stride_t]));
-    const Row w = row_of(seq, t);
-    const float hp = w.pad || w.first ? 0.0f : h;
-    before[t * p.dim] = hp;
-    h = w.pad ? 0.0f : fmaf(a, hp, u);
-  }
-  float c = p.dfinal_states ? p.dfinal_states[b * p.dim + d] : 0.0f;  // what reaches row t's state
-  float dk = 0.0f;
-  for (int64_t t = p.seqlen - 1; t >= 0; --t) {
-    const Row w = row_of(seq, t);
-    if (w.pad) {
-      c = 0.0f;
-      dx[t * p.dim] = static_cast<T>(0.0f);
-      dg[t * p.dim] = static_cast<T>(0.0f);
-      if (dig) dig[t * p.dim] = static_cast<T>(0.0f);
-      continue;
-    }
-    float r, l, a, beta;
-    coefficients<DECAY>(k, to_f32(g[t * p.gate_stride_t]), r, l, a, beta);
-    const float xv = to_f32(x[t * p.x_stride_t]), hp = before[t * p.dim];
-    const float i = ig ? sigmoid(to_f32(ig[t * p.input_gate_stride_t])) : 1.0f;
-    const float dh = to_f32(dy[t * p.dout_stride_t]) + c;
-    dx[t * p.dim] = static_cast<T>(dh * beta * i);
-    if (dig) dig[t * p.dim] = static_cast<T>(dh * beta * xv * i * (1.0f - i));
-    if constexpr (DECAY) {
-      const float la = l * kLn2, over = beta > 0.0f ? la / beta : 0.0f;
-      const float q = dh * (la * a * hp - i * xv * a * a * over);
-      dg[t * p.dim] = static_cast<T>(q * (1.0f - r));
-      dk += q;
-    } else {
-      dg[t * p.dim] = static_cast<T>(dh * (hp - i * xv) * a * beta);
-    }
-    c = w.first ? 0.0f : a * dh;
-  }
-  if (p.dinitial_states) p.dinitial_states[b * p.dim + d] = c;
-  if constexpr (DECAY) {
-    static_cast<float*>(p.workspace)[p.batch * p.seqlen * p.dim + b * p.dim + d] = dk;
-  }
-}
-
-__global__ __launch_bounds__(64) void rec_reduce_kernel(const float* part, int64_t rows, int64_t dim,
-                                                        const float* decay, float* ddecay) {
-  const int64_t d = blockIdx.x * 64 + threadIdx.x;
-  if (d >= dim) return;
+// ddecay from the chunks' sums: 32 channels a workgroup, thread y adds rows y, y + 32, ..., 8 requested
+// at a time, and the 32 sums are added in order.
+__global__ __launch_bounds__(1024) void rec_reduce_kernel(const float* part, int64_t rows, int64_t dim,
+                                                          const float* decay, float* ddecay) {
+  __shared__ float sums[32][33];
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int64_t d = (int64_t)blockIdx.x * 32 + x;
   float s = 0.0f;
-  for (int64_t i = 0; i < rows; ++i) s += part[i * dim + d];
-  ddecay[d] = s * decay_ratio(decay[d]);
+  if (d < dim) {
+    int64_t i = y;
+    for (; i + 7 * 32 < rows; i += 8 * 32) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = part[(i + 32 * j) * dim + d];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += v[j];
+    }
+    for (; i < rows; i += 32) s += part[i * dim + d];
+  }
+  sums[y][x] = s;
+  __syncthreads();
+  if (y == 0 && d < dim) {
+    s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) s += sums[j][x];
+    ddecay[d] = s * decay_ratio(decay[d]);
+  }
 }
 
 template <typename T, bool DECAY>
@@ -143,37 +60,17 @@ __global__ __launch_bounds__(64) void rec_update_kernel(ccv1d_rec_update_args p)
   const int64_t slot = p.state_indices ? p.state_indices[row] : row;
   float h = 0.0f;
   if (slot >= 0 && slot < p.slots) {
-    float r, l, a, beta;
+    float a, beta;
     const float k = DECAY ? decay_rate(p.decay[d], p.decay_scale) : 0.0f;
-    coefficients<DECAY>(k, to_f32(static_cast<const T*>(p.gate)[row * p.gate_stride + d]), r, l, a, beta);
+    forget<T, DECAY>(k, to_f32(static_cast<const T*>(p.gate)[row * p.gate_stride + d]), a, beta);
     float u = beta * to_f32(static_cast<const T*>(p.x)[row * p.x_stride + d]);
     if (p.input_gate)
-      u *= sigmoid(to_f32(static_cast<const T*>(p.input_gate)[row * p.input_gate_stride + d]));
+      u *= sigmoid<T>(to_f32(static_cast<const T*>(p.input_gate)[row * p.input_gate_stride + d]));
     float* st = p.state + slot * p.state_stride + d;
     h = fmaf(a, *st, u);
     *st = h;
   }
   static_cast<T*>(p.out)[row * p.dim + d] = static_cast<T>(h);
-}
-
-template <typename T>
-hipError_t fwd_t(const ccv1d_rec_args& a, hipStream_t s) {
-  const dim3 grid((unsigned)(a.batch * ((a.dim + 63) / 64)));
-  if (a.decay) rec_fwd_kernel<T, true><<<grid, 64, 0, s>>>(a);
-  else rec_fwd_kernel<T, false><<<grid, 64, 0, s>>>(a);
-  return hipGetLastError();
-}
-
-template <typename T>
-hipError_t bwd_t(const ccv1d_rec_args& a, hipStream_t s) {
-  const dim3 grid((unsigned)(a.batch * ((a.dim + 63) / 64)));
-  if (a.decay) rec_bwd_kernel<T, true><<<grid, 64, 0, s>>>(a);
-  else rec_bwd_kernel<T, false><<<grid, 64, 0, s>>>(a);
-  if (a.decay)
-    rec_reduce_kernel<<<(unsigned)((a.dim + 63) / 64), 64, 0, s>>>(
-        static_cast<const float*>(a.workspace) + a.batch * a.seqlen * a.dim, a.batch, a.dim, a.decay,
-        a.ddecay);
-  return hipGetLastError();
 }
 
 template <typename T>
@@ -184,27 +81,68 @@ hipError_t update_t(const ccv1d_rec_update_args& a, hipStream_t s) {
   return hipGetLastError();
 }
 
+unsigned fill_blocks(int64_t n) {
+  const int64_t b = (n + 1023) / 1024;
+  return (unsigned)(b < 1 ? 1 : b > 2048 ? 2048 : b);
+}
+
+struct Plan {
+  int64_t chunks, groups, words, part;  // words: of 8 bytes, cleared; part: floats after them
+};
+
+Plan plan_of(int64_t B, int64_t T, int64_t D, bool backward) {
+  Plan p;
+  const int64_t rows = kRecWaves * (backward ? kRecBwdRows : kRecFwdRows);
+  p.chunks = (T + rows - 1) / rows;
+  p.groups = (p.chunks + kRecGroup - 1) / kRecGroup;
+  p.words = p.chunks > 1 ? B * D * (p.chunks + p.groups) + 1 : 0;  // and the ticket
+  p.part = backward ? B * D * p.chunks : 0;
+  return p;
+}
+
+hipError_t run(const ccv1d_rec_args& a, bool backward, hipStream_t s) {
+  if (a.seqlen == 0 || a.batch == 0) {
+    const int64_t n = a.batch * a.dim;
+    const float* from = backward ? a.dfinal_states : a.initial_states;
+    float* to = backward ? a.dinitial_states : a.final_states;
+    float* zero = backward ? a.ddecay : nullptr;
+    if (to || zero) rec_empty_kernel<<<fill_blocks(n), 256, 0, s>>>(from, to, n, zero, a.dim);
+    return hipGetLastError();
+  }
+  const Plan pl = plan_of(a.batch, a.seqlen, a.dim, backward);
+  RecParams p{};
+  p.a = a;
+  p.chunks = (int32_t)pl.chunks;
+  p.groups = (int32_t)pl.groups;
+  if (pl.words) {
+    p.pairs = static_cast<uint64_t*>(a.workspace);
+    p.states = p.pairs + a.batch * a.dim * pl.chunks;
+    p.ticket = reinterpret_cast<uint32_t*>(p.pairs + pl.words - 1);
+    rec_clear_kernel<<<fill_blocks(pl.words), 256, 0, s>>>(p.pairs, pl.words);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
+  p.part = reinterpret_cast<float*>(static_cast<uint64_t*>(a.workspace) + pl.words);
+  hipError_t e;
+  switch (a.dtype) {
+    case CCV1D_BF16: e = rec_launch_bf16(p, backward, s); break;
+    case CCV1D_F16: e = rec_launch_f16(p, backward, s); break;
+    default: e = rec_launch_f32(p, backward, s); break;
+  }
+  if (e != hipSuccess || !backward || !a.decay) return e;
+  rec_reduce_kernel<<<(unsigned)((a.dim + 31) / 32), 1024, 0, s>>>(p.part, a.batch * pl.chunks, a.dim,
+                                                                   a.decay, a.ddecay);
+  return hipGetLastError();
+}
+
 }  // namespace
 
 size_t rec_workspace(int64_t B, int64_t T, int64_t D, bool backward) {
-  return backward ? (size_t)(B * T * D + B * D) * 4 : 0;
+  const Plan p = plan_of(B, T, D, backward);
+  return (size_t)p.words * 8 + (size_t)p.part * 4;
 }
 
-hipError_t rec_fwd(const ccv1d_rec_args& a, hipStream_t s) {
-  switch (a.dtype) {
-    case CCV1D_BF16: return fwd_t<__bf16>(a, s);
-    case CCV1D_F16: return fwd_t<_Float16>(a, s);
-    default: return fwd_t<float>(a, s);
-  }
-}
-
-hipError_t rec_bwd(const ccv1d_rec_args& a, hipStream_t s) {
-  switch (a.dtype) {
-    case CCV1D_BF16: return bwd_t<__bf16>(a, s);
-    case CCV1D_F16: return bwd_t<_Float16>(a, s);
-    default: return bwd_t<float>(a, s);
-  }
-}
+hipError_t rec_fwd(const ccv1d_rec_args& a, hipStream_t s) { return run(a, false, s); }
+hipError_t rec_bwd(const ccv1d_rec_args& a, hipStream_t s) { return run(a, true, s); }
 
 hipError_t rec_update(const ccv1d_rec_update_args& a, hipStream_t s) {
   switch (a.dtype) {

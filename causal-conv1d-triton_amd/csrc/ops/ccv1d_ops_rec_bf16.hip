@@ -1,0 +1,12 @@
+#include "ops_rec_launch.h"
+
+namespace ccv1d {
+namespace ops {
+
+// Two channels a lane, 256 bytes a row and wave; a single channel has no pair.
+hipError_t rec_launch_bf16(const RecParams& p, bool backward, hipStream_t s) {
+  return p.a.dim == 1 ? rec_launch<__bf16, 1>(p, backward, s) : rec_launch<__bf16, 2>(p, backward, s);
+}
+
+}  // namespace ops
+}  // namespace ccv1d

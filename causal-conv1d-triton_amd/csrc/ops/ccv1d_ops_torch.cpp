@@ -164,6 +164,7 @@ void rec_inputs(PyObject* const* o, Rec& r) {
         "seq_idx must hold integers");
   check(!r.decay.defined() || r.decay.is_floating_point(), "decay must be floating point");
   check(!r.init.defined() || r.init.is_floating_point(), "initial_states must be floating point");
+  check(a.decay_scale >= 0.0f, "decay_scale must not be negative");
   check(r.x.is_cuda(), "x must be on a GPU");
   const int64_t dev = r.x.get_device();
   check(r.gate.get_device() == dev, "gate must be on the device of x");
@@ -268,6 +269,7 @@ PyObject* rec_update(PyObject* const* o) {
   at::Tensor idx = optional(o[5], "state_indices must be a tensor or None");
   ccv1d_rec_update_args a{};
   a.decay_scale = (float)number(o[6]);
+  check(a.decay_scale >= 0.0f, "decay_scale must not be negative");
   check(x.dim() == 2, "x must be (rows, dim)");
   a.rows = x.size(0), a.dim = x.size(1);
   check(gate.sizes() == x.sizes(), "gate must have the shape of x");

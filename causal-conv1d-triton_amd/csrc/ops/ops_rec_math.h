@@ -13,10 +13,35 @@ namespace ccv1d {
 namespace ops {
 
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2eLow = 1.92596299112661746887e-8f;  // log2 e - kLog2e
 constexpr float kLn2 = 0.69314718055994530942f;
 
+// exp(-z) = 2^t, t = -z log2 e. The rounding of t, |t| 2^-24, is a relative error of the result that
+// grows with |z|. For fp32 inputs its residue is added back (4 operations, and twice the bytes per
+// element to hide them); for 16-bit ones it lies far below the rounding of what is stored. t is held
+// at 126, so that 1 / (1 + 2^t) stays a normal number; a NaN passes.
+template <typename T>
+__device__ __forceinline__ float exp_minus(float z) {
+  float t = -kLog2e * z;
+  if constexpr (sizeof(T) == 4) {
+    const float rest = fmaf(z, -kLog2eLow, fmaf(z, -kLog2e, -t));
+    const float e = __builtin_amdgcn_exp2f(t > 126.0f ? 126.0f : t);
+    return t > 126.0f ? e : fmaf(e, kLn2 * rest, e);
+  }
+  return __builtin_amdgcn_exp2f(t > 126.0f ? 126.0f : t);
+}
+
+// s = sigmoid(z), and 1 - s without cancellation.
+template <typename T>
+__device__ __forceinline__ void sigmoid_pair(float z, float& s, float& rest) {
+  const float e = exp_minus<T>(z);
+  s = __builtin_amdgcn_rcpf(1.0f + e);
+  rest = e * s;
+}
+
+template <typename T>
 __device__ __forceinline__ float sigmoid(float z) {
-  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
+  return __builtin_amdgcn_rcpf(1.0f + exp_minus<T>(z));
 }
 
 // k of a channel: log2 a = k * r.
@@ -46,13 +71,16 @@ __device__ __forceinline__ float one_minus_square(float log2a, float a) {
   return y > -0.35f ? -y * p : fmaf(-a, a, 1.0f);
 }
 
-// Without decay: a = sigmoid(g), beta = 1 - a without cancellation. Past 2^126 the exponential is
-// held there (a stays a normal number and beta is 1); a NaN passes.
-__device__ __forceinline__ void plain_gate(float g, float& a, float& beta) {
-  const float z = -kLog2e * g;
-  const float e = __builtin_amdgcn_exp2f(z > 126.0f ? 126.0f : z);
-  a = __builtin_amdgcn_rcpf(1.0f + e);
-  beta = e * a;
+// The factor of the state before a row and that of the row's own i * x.
+template <typename T, bool DECAY>
+__device__ __forceinline__ void forget(float k, float gate, float& a, float& beta) {
+  if constexpr (DECAY) {
+    const float l = k * sigmoid<T>(gate);
+    a = __builtin_amdgcn_exp2f(l);
+    beta = __builtin_amdgcn_sqrtf(one_minus_square(l, a));
+  } else {
+    sigmoid_pair<T>(gate, a, beta);
+  }
 }
 
 }  // namespace ops

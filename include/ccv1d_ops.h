@@ -47,7 +47,7 @@ struct ccv1d_rec_args {
   int64_t input_gate_stride_b, input_gate_stride_t;
   int dtype;
   const float* decay; /* (dim,) or NULL */
-  float decay_scale;
+  float decay_scale; /* not negative */
   const int32_t* seq_idx;      /* (batch, seqlen) contiguous, or NULL */
   const float* initial_states; /* (batch, dim) or NULL */
   int64_t batch, seqlen, dim;
@@ -89,7 +89,7 @@ struct ccv1d_rec_update_args {
   int64_t input_gate_stride;
   int dtype;
   const float* decay; /* (dim,) or NULL */
-  float decay_scale;
+  float decay_scale; /* not negative */
   float* state; /* (slots, dim), unit channel stride */
   int64_t state_stride;
   const int32_t* state_indices; /* (rows,) or NULL: row r uses slot r */
