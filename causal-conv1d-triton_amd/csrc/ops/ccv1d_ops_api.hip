@@ -91,8 +91,8 @@ int check_attn(const ccv1d_paged_attn_args* a) {
                 CCV1D_PAGED_MAX_HEAD_DIM);
   if (a->kv_heads == 0 ? a->q_heads != 0 : a->q_heads % a->kv_heads != 0)
     return invalid("q_heads must be a multiple of kv_heads");
-  if (!product_within(a->max_pages, a->page_size, kMaxGrid))
-    return fail(CCV1D_ERR_UNSUPPORTED, "max_pages * page_size must be below 2^31");
+  if (a->page_size > (int64_t(1) << 30) || !product_within(a->max_pages, a->page_size, int64_t(1) << 30))
+    return fail(CCV1D_ERR_UNSUPPORTED, "max_pages * page_size must be at most 2^30");
   if (!product_within(a->rows, a->q_heads, kMaxGrid / 256))
     return fail(CCV1D_ERR_UNSUPPORTED, "rows * q_heads too large for one launch");
   return CCV1D_OK;

@@ -1,74 +1,107 @@
-// Attention of one token per row over a paged cache: a wave per (row, query head), its lanes along
-// the head's elements, one position after the other with the running maximum and sum of a softmax.
-#include "ops_common.h"
+// Launch of the paged attention: how rows are split, and the join of their spans.
+#include "ops_attn.h"
 
 namespace ccv1d {
 namespace ops {
 
 namespace {
 
+// Joins the spans of a row and query head: 4 waves take the spans in turn, 64 lanes the elements, and
+// the waves' sums meet in LDS. Rows of one span have been written by the main kernel.
 template <typename T>
-__global__ __launch_bounds__(64) void paged_attn_kernel(ccv1d_paged_attn_args p) {
-  const int64_t row = blockIdx.x / p.q_heads, head = blockIdx.x % p.q_heads;
-  const int64_t kvh = head / (p.q_heads / p.kv_heads);
-  const int lane = threadIdx.x, Dh = (int)p.head_dim;
-  float q[4], o[4] = {0, 0, 0, 0};
+__global__ __launch_bounds__(256) void paged_join_kernel(AttnParams p) {
+  const ccv1d_paged_attn_args& a = p.a;
+  const int64_t at = blockIdx.x, row = at / a.q_heads;
+  int64_t request;
+  const Span sp = span_of(p, row, request);
+  const int spans = (sp.end - sp.base + p.span - 1) / p.span;
+  if (spans <= 1) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, Dh = (int)a.head_dim;
+  const float* ml = p.part_ml + at * p.splits * 2;
+  const float* part = p.part + at * p.splits * Dh;
+  float top = kLowest;
+  for (int i = lane; i < spans; i += 64) top = fmaxf(top, ml[2 * i]);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int d = lane + 64 * j;
-    q[j] = d < Dh ? to_f32(static_cast<const T*>(p.q)[row * p.q_stride_r + head * p.q_stride_h + d]) : 0;
+  for (int o = 32; o; o /= 2) top = fmaxf(top, __shfl_xor(top, o));
+  float total = 0.0f, sum[4] = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int i = wave; i < spans; i += 4) {
+    const float f = __builtin_amdgcn_exp2f(ml[2 * i] - top);
+    total = fmaf(ml[2 * i + 1], f, total);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (lane + 64 * j < Dh) sum[j] = fmaf(part[(int64_t)i * Dh + lane + 64 * j], f, sum[j]);
   }
-  const int64_t req = p.request_ids ? p.request_ids[row] : row;
-  int64_t len = req >= 0 && req < p.requests ? p.seq_lens[row] : 0;
-  len = min(len, p.max_pages * p.page_size);
-  const int64_t first = p.window && len > p.window ? len - p.window : 0;
-  float m = -3.4028235e38f, l = 0.0f;  // finite, so that no difference of infinities arises
-  for (int64_t t = first; t < len; ++t) {
-    const int64_t page = p.block_tables[req * p.block_table_stride + t / p.page_size];
-    if (page < 0 || page >= p.num_pages) continue;
-    const int64_t off = t % p.page_size;
-    const T* k = static_cast<const T*>(p.k_cache) + page * p.k_cache_stride_p + off * p.k_cache_stride_t +
-                 kvh * p.k_cache_stride_h;
-    const T* v = static_cast<const T*>(p.v_cache) + page * p.v_cache_stride_p + off * p.v_cache_stride_t +
-                 kvh * p.v_cache_stride_h;
-    float s = 0.0f;
+  __shared__ float s_sum[4][256], s_total[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int d = lane + 64 * j;
-      if (d < Dh) s = fmaf(q[j], to_f32(k[d]), s);
-    }
-#pragma unroll
-    for (int w = 32; w; w /= 2) s += __shfl_xor(s, w);
-    s *= p.scale;
-    const float mn = fmaxf(m, s);
-    const float f = expf(m - mn), e = expf(s - mn);
-    m = mn;
-    l = l * f + e;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int d = lane + 64 * j;
-      if (d < Dh) o[j] = o[j] * f + e * to_f32(v[d]);
-    }
+  for (int j = 0; j < 4; ++j) s_sum[wave][lane + 64 * j] = sum[j];
+  if (lane == 0) s_total[wave] = total;
+  __syncthreads();
+  total = s_total[0] + s_total[1] + s_total[2] + s_total[3];
+  const int d = threadIdx.x;
+  if (d < Dh) {
+    const float s = s_sum[0][d] + s_sum[1][d] + s_sum[2][d] + s_sum[3][d];
+    static_cast<T*>(a.out)[at * Dh + d] = static_cast<T>(total == 0.0f ? 0.0f : s / total);
   }
-  T* out = static_cast<T*>(p.out) + (row * p.q_heads + head) * Dh;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int d = lane + 64 * j;
-    if (d < Dh) out[d] = static_cast<T>(l > 0.0f ? o[j] / l : l == 0.0f ? 0.0f : l);
-  }
-  if (p.lse && lane == 0) p.lse[row * p.q_heads + head] = m + logf(l);
+  if (a.lse && d == 0) a.lse[at] = (top + __log2f(total)) * 0.69314718055994530942f;
+}
+
+AttnParams plan(const ccv1d_paged_attn_args& a) {
+  AttnParams p{};
+  p.a = a;
+  uint32_t s = 0;
+  while ((int64_t(1) << s) < a.page_size) ++s;
+  p.by_page.shift = 31 + s;
+  p.by_page.magic = (uint32_t)(((uint64_t(1) << p.by_page.shift) + (uint64_t)a.page_size - 1) /
+                               (uint64_t)a.page_size);
+  const int64_t group = a.q_heads / a.kv_heads;
+  p.tiles = (int32_t)((group + kAttnHeads - 1) / kAttnHeads);
+  int64_t limit = a.max_pages * a.page_size;
+  if (a.max_seq_len && a.max_seq_len < limit) limit = a.max_seq_len;
+  p.limit = (int32_t)limit;
+  // Spans: as many as fill the card with 1024 workgroups, of at least two steps a wave (256
+  // positions), and of at most 2048 positions, so that one long row beside short ones is spread too;
+  // at most 256 of them.
+  int64_t most = a.window && a.window + 31 < limit ? a.window + 31 : limit;
+  if (most < 1) most = 1;
+  const int64_t wgs = a.rows * a.kv_heads * p.tiles;
+  int64_t splits = (1024 + wgs - 1) / wgs;
+  int64_t span = (most + splits - 1) / splits;
+  if (span > 2048) span = 2048;
+  if (span < 256) span = 256;
+  if (span < (most + 255) / 256) span = (most + 255) / 256;
+  span = (span + 127) / 128 * 128;
+  p.span = (int32_t)span;
+  p.splits = (int32_t)((most + span - 1) / span);
+  return p;
 }
 
 }  // namespace
 
-size_t paged_attn_workspace(const ccv1d_paged_attn_args&) { return 0; }
+size_t paged_attn_workspace(const ccv1d_paged_attn_args& a) {
+  const AttnParams p = plan(a);
+  if (p.splits <= 1) return 0;
+  return (size_t)(a.rows * a.q_heads * p.splits * (a.head_dim + 2)) * 4;
+}
 
 hipError_t paged_attn(const ccv1d_paged_attn_args& a, hipStream_t s) {
+  AttnParams p = plan(a);
+  p.part = static_cast<float*>(a.workspace);
+  p.part_ml = p.part + a.rows * a.q_heads * p.splits * a.head_dim;
+  const int step = a.dtype == CCV1D_F32 ? 16 : 32;
+  const int mode = a.page_size % step == 0 ? kPageStep : a.page_size % 4 == 0 ? kPageFour : kPageAny;
+  hipError_t e;
+  switch (a.dtype) {
+    case CCV1D_BF16: e = paged_attn_bf16(p, mode, s); break;
+    case CCV1D_F16: e = paged_attn_f16(p, mode, s); break;
+    default: e = paged_attn_f32(p, mode, s); break;
+  }
+  if (e != hipSuccess || p.splits <= 1) return e;
   const unsigned grid = (unsigned)(a.rows * a.q_heads);
   switch (a.dtype) {
-    case CCV1D_BF16: paged_attn_kernel<__bf16><<<grid, 64, 0, s>>>(a); break;
-    case CCV1D_F16: paged_attn_kernel<_Float16><<<grid, 64, 0, s>>>(a); break;
-    default: paged_attn_kernel<float><<<grid, 64, 0, s>>>(a); break;
+    case CCV1D_BF16: paged_join_kernel<__bf16><<<grid, 256, 0, s>>>(p); break;
+    case CCV1D_F16: paged_join_kernel<_Float16><<<grid, 256, 0, s>>>(p); break;
+    default: paged_join_kernel<float><<<grid, 256, 0, s>>>(p); break;
   }
   return hipGetLastError();
 }

@@ -124,8 +124,8 @@ def assert_close(got, want, what=""):
 
 def plan(cached, new, tables, free, num_free, page_size, max_tokens):
     """One request after the other, in Python integers."""
+    M = tables.shape[1]
     tables = [list(map(int, row)) for row in tables.tolist()]
-    M = len(tables[0]) if tables else 0
     free = free.tolist()
     nf = min(max(int(num_free), 0), len(free))
     seq_lens, start = [], [0]
@@ -144,7 +144,7 @@ def plan(cached, new, tables, free, num_free, page_size, max_tokens):
         upto += need
         seq_lens.append(c + n if ok else c)
         start.append(start[-1] + n)
-        for t in range(n):
+        for t in range(min(n, max(0, max_tokens - len(pos)))):
             p = c + t
             page = tables[r][p // page_size] if ok else -1
             pos.append(p if ok else -1)

@@ -79,7 +79,7 @@ def test_plan_edges():
     check_plan([20], [4], [[-1, -1]], [3, 4], 2, 16, 4)  # a cached page that is not there
     check_plan([0], [4], [[-1]], [], 0, 16, 4)
     check_plan([0, 0], [9, 9], [[-1], [-1]], [3, 4], 2, 16, 11)  # fewer places than tokens
-    check_plan([2 ** 31 - 1, 0], [2 ** 31 - 1, 1], [[-1], [-1]], [3, 4], 2, 16, 8)
+    check_plan([2 ** 31 - 1, 0], [2 ** 31 - 2, 1], [[-1], [-1]], [3, 4], 2, 16, 8)  # the sums' limit
 
 
 def test_plan_leaves_cached_pages_and_strided_tables():
