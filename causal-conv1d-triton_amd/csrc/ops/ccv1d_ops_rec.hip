@@ -62,7 +62,7 @@ __global__ __launch_bounds__(64) void rec_update_kernel(ccv1d_rec_update_args p)
   if (slot >= 0 && slot < p.slots) {
     float a, beta;
     const float k = DECAY ? decay_rate(p.decay[d], p.decay_scale) : 0.0f;
-    forget<T, DECAY>(k, to_f32(static_cast<const T*>(p.gate)[row * p.gate_stride + d]), a, beta);
+    forget<T, DECAY, false>(k, sinh_tail(k), to_f32(static_cast<const T*>(p.gate)[row * p.gate_stride + d]), a, beta);
     float u = beta * to_f32(static_cast<const T*>(p.x)[row * p.x_stride + d]);
     if (p.input_gate)
       u *= sigmoid<T>(to_f32(static_cast<const T*>(p.input_gate)[row * p.input_gate_stride + d]));
@@ -87,12 +87,12 @@ unsigned fill_blocks(int64_t n) {
 }
 
 struct Plan {
-  int64_t chunks, groups, words, part;  // words: of 8 bytes, cleared; part: floats after them
+  int64_t chunks, groups, words, part;  // words of 8 bytes, cleared; floats after them
 };
 
 Plan plan_of(int64_t B, int64_t T, int64_t D, bool backward) {
   Plan p;
-  const int64_t rows = kRecWaves * (backward ? kRecBwdRows : kRecFwdRows);
+  const int64_t rows = backward ? kBwdWaves * kBwdRows : kFwdWaves * kFwdRows;
   p.chunks = (T + rows - 1) / rows;
   p.groups = (p.chunks + kRecGroup - 1) / kRecGroup;
   p.words = p.chunks > 1 ? B * D * (p.chunks + p.groups) + 1 : 0;  // and the ticket
@@ -114,14 +114,14 @@ hipError_t run(const ccv1d_rec_args& a, bool backward, hipStream_t s) {
   p.a = a;
   p.chunks = (int32_t)pl.chunks;
   p.groups = (int32_t)pl.groups;
+  p.pairs = static_cast<uint64_t*>(a.workspace);
+  p.part = reinterpret_cast<float*>(p.pairs + pl.words);
   if (pl.words) {
-    p.pairs = static_cast<uint64_t*>(a.workspace);
     p.states = p.pairs + a.batch * a.dim * pl.chunks;
     p.ticket = reinterpret_cast<uint32_t*>(p.pairs + pl.words - 1);
     rec_clear_kernel<<<fill_blocks(pl.words), 256, 0, s>>>(p.pairs, pl.words);
-    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    if (hipError_t err = hipGetLastError(); err != hipSuccess) return err;
   }
-  p.part = reinterpret_cast<float*>(static_cast<uint64_t*>(a.workspace) + pl.words);
   hipError_t e;
   switch (a.dtype) {
     case CCV1D_BF16: e = rec_launch_bf16(p, backward, s); break;

@@ -1,6 +1,6 @@
 // The gated linear recurrence in one pass over its inputs, forward and backward.
 //
-// h[t] = f[t] h[t-1] + u[t] is cut along time into chunks of kRecWaves waves of R rows, a workgroup
+// h[t] = f[t] h[t-1] + u[t] is cut along time into chunks of NW waves of R rows, a workgroup
 // each; a lane holds the factors of its R rows and CPL channels in registers. A stretch of rows acts
 // on the state before it as h -> A h + H, and such pairs combine: every wave forms the pair of its
 // rows, the workgroup that of its chunk, and once the state in front of a wave is known it walks its
@@ -30,13 +30,14 @@
 // without out's rounding.
 #pragma once
 
+#include <type_traits>
+
 #include "../ccv1d_device.h"
 #include "ops_rec_math.h"
 
 namespace ccv1d {
 namespace ops {
 
-constexpr int kRecWaves = 8;
 constexpr int kRecGroup = 16;
 constexpr uint32_t kReady = 0x80000000u;
 constexpr float kTiny = 1.17549435e-38f;
@@ -78,23 +79,86 @@ __device__ __forceinline__ float product(float A0, float A) {
 // The rows of one wave that are not plain: bit j of each mask is row t0 + j.
 struct Rows {
   uint32_t first, pad;  // a sequence's first row; padding
-  int valid;            // rows inside the sequence, from 0 to R
 };
 
 template <int R>
 __device__ __forceinline__ Rows rows_of(const int32_t* seq, int64_t t0, int64_t T, int lane) {
-  Rows w{0, 0, (int)max((int64_t)0, min((int64_t)R, T - t0))};
-  if (seq && w.valid > 0) {  // lane l looks at row t0 - 1 + l
+  Rows w{0, 0};
+  if (t0 < T) {  // lane l looks at row t0 - 1 + l
     const int64_t t = t0 - 1 + lane;
     const int32_t id = seq[min(max(t, (int64_t)0), T - 1)];
     const int32_t prev = __shfl_up(id, 1);
     const uint64_t pad = __ballot(id < 0);
     const uint64_t first = __ballot(t > 0 && id != prev);
-    const uint32_t live = (1u << w.valid) - 1;
+    const uint32_t live = T - t0 < R ? (1u << (int)(T - t0)) - 1 : (1u << R) - 1;
     w.pad = (uint32_t)(pad >> 1) & live;
     w.first = (uint32_t)(first >> 1) & live;
   }
   return w;
+}
+
+// The rows of one tensor under a wave, from row t0 on: a uniform address (kept in scalar registers, which
+// the compiler would otherwise fold into a vector address per row) and a lane's byte offset from it.
+template <typename T, int CPL>
+struct RowWalk {
+  using V = VecIO<T, CPL>;
+  typedef char __attribute__((address_space(1))) byte;
+  typedef typename V::mem __attribute__((address_space(1))) cell;
+  byte* row;
+  int64_t step;
+  __device__ __forceinline__ RowWalk(const void* base, int64_t stride_b, int64_t stride_t, int64_t b,
+                                     int64_t t, int64_t c0)
+      : row((byte*)base + (b * stride_b + t * stride_t + c0) * (int64_t)sizeof(T)),
+        step(stride_t * (int64_t)sizeof(T)) {}
+  // Every row is read and written once: kept out of the caches' way (forward and backward at B=4
+  // T=8192 D=1024 bf16: 219 us with cached loads and stores, 213 with cached loads, 207 with neither).
+  __device__ __forceinline__ typename V::raw load(uint32_t lane_bytes) const {
+    return __builtin_nontemporal_load((const cell*)(row + lane_bytes));
+  }
+  __device__ __forceinline__ void store(uint32_t lane_bytes, const float (&v)[CPL]) {
+    __builtin_nontemporal_store(V::pack(v), (cell*)(row + lane_bytes));
+  }
+  __device__ __forceinline__ void move(int64_t bytes) {
+    row += bytes;
+    asm volatile("" : "+s"(row));
+  }
+};
+
+template <int CPL>
+__device__ __forceinline__ void settle(float (&v)[CPL]) {
+#pragma unroll
+  for (int i = 0; i < CPL; ++i) asm volatile("" : "+v"(v[i]));
+}
+
+// Loads R rows; those past the last one, `valid` - 1, repeat it.
+template <typename T, int CPL, int R>
+__device__ __forceinline__ void load_rows(RowWalk<T, CPL> w, int valid, uint32_t lane_bytes,
+                                          typename VecIO<T, CPL>::raw (&to)[R]) {
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    to[j] = w.load(lane_bytes);
+    w.move(j + 1 < valid ? w.step : 0);
+  }
+}
+
+// Makes the compiler forget what it knows of a loaded row: values made from it before are made again
+// rather than kept, and nothing is made from it before this point. Statements of this kind keep their
+// order, so a pair of them around a row's arithmetic keeps rows apart: interleaved by the scheduler, they
+// needed more registers than four waves have.
+template <typename RAW>
+__device__ __forceinline__ void forget_row(RAW& v) {
+  if constexpr (sizeof(RAW) == 2) {
+    uint32_t t = v;
+    asm volatile("" : "+v"(t));
+    v = (RAW)t;
+  } else {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(RAW) / 4; ++i) {
+      uint32_t t = v[i];
+      asm volatile("" : "+v"(t));
+      v[i] = t;
+    }
+  }
 }
 
 // Deals a chunk to this workgroup: (batch row and wave column, chunk from the walk's start).
@@ -112,134 +176,207 @@ __device__ __forceinline__ void deal(const RecParams& p, int& bc, int& chunk, ui
 }
 
 // The pairs of the waves of a workgroup, and of the chunks before it, in LDS.
-template <int CPL>
+template <int NW, int CPL>
 struct Pairs {
-  float A[kRecWaves][CPL][kWave], H[kRecWaves][CPL][kWave];
+  float A[NW][CPL][kWave], H[NW][CPL][kWave];
 };
 
-// Combines the chunks between the group before and this chunk: wave w the two from 2 w on, into `got`;
-// the state in front of the group goes to `base`. `chunk` counts from the walk's start.
-template <int CPL>
-__device__ __forceinline__ void look_back(const RecParams& p, int64_t b, int64_t c, int chunk, int dir,
-                                          const float (&start)[CPL], Pairs<CPL>& got,
-                                          float (&base)[CPL][kWave], int wave, int lane) {
+// Words of (batch, n, dim) rows: a uniform row and the lane's place in it.
+__device__ __forceinline__ uint64_t* word_row(uint64_t* words, int64_t row, int64_t D, int64_t c0) {
+  return words + row * D + c0;
+}
+
+// Combines the chunks between the group before and this chunk, kLook of them a wave in order, into
+// `got`; the state in front of the group goes to `base`. `chunk` counts from the walk's start.
+template <int NW>
+constexpr int kLook = (kRecGroup - 2) / NW + 1;
+
+template <int NW, int CPL>
+__device__ __forceinline__ void look_back(const RecParams& p, int64_t b, int64_t c0, uint32_t lane_c,
+                                          int chunk, int dir, const float* start,
+                                          Pairs<NW, CPL>& got, float (&base)[CPL][kWave], int wave,
+                                          int lane) {
+  constexpr int N = kLook<NW>;
   const int64_t D = p.a.dim;
-  const int g = chunk / kRecGroup, j0 = g * kRecGroup;
-  auto word = [&](int j) {  // chunks are stored in order of time
-    const int64_t at = dir > 0 ? j : p.chunks - 1 - j;
-    return p.pairs + (b * p.chunks + at) * D + c;
+  const int g = chunk / kRecGroup, j0 = g * kRecGroup + N * wave;
+  // chunks are stored in order of time
+  auto pair = [&](int j) {
+    return word_row(p.pairs, b * p.chunks + (dir > 0 ? j : p.chunks - 1 - j), D, c0) + lane_c;
   };
-  const int j = j0 + 2 * wave;
-  uint64_t v[2][CPL], s[CPL];
-  const uint64_t* gs = p.states + (b * p.groups + (g - 1)) * D + c;
+  const uint64_t* gs = word_row(p.states, b * p.groups + (g - 1), D, c0) + lane_c;
+  uint64_t v[N][CPL], s[CPL];
 #pragma unroll
-  for (int i = 0; i < CPL; ++i) {  // requested together
-    if (j < chunk) v[0][i] = peek(word(j) + i);
-    if (j + 1 < chunk) v[1][i] = peek(word(j + 1) + i);
-    if (wave == 0 && g > 0) s[i] = peek(gs + i);
+  for (int n = 0; n < N; ++n)  // requested together
+    if (j0 + n < chunk) {
+#pragma unroll
+      for (int i = 0; i < CPL; ++i) v[n][i] = peek(pair(j0 + n) + i);
+    }
+  if (wave == 0 && g > 0) {
+#pragma unroll
+    for (int i = 0; i < CPL; ++i) s[i] = peek(gs + i);
   }
+  if (j0 < chunk) {
+    float A[CPL], H[CPL];
 #pragma unroll
-  for (int i = 0; i < CPL; ++i) {
-    float A = 1.0f, H = 0.0f;
-    if (j < chunk) {
-      const uint64_t w = await(word(j) + i, v[0][i]);
-      A = __uint_as_float((uint32_t)w & ~kReady);
-      H = __uint_as_float((uint32_t)(w >> 32));
+    for (int n = 0; n < N; ++n)
+      if (j0 + n < chunk) {
+#pragma unroll
+        for (int i = 0; i < CPL; ++i) {
+          const uint64_t w = await(pair(j0 + n) + i, v[n][i]);
+          const float A1 = __uint_as_float((uint32_t)w & ~kReady);
+          const float H1 = __uint_as_float((uint32_t)(w >> 32));
+          H[i] = n == 0 ? H1 : after(H[i], A1, H1);
+          A[i] = n == 0 ? A1 : product(A[i], A1);
+        }
+      }
+#pragma unroll
+    for (int i = 0; i < CPL; ++i) {
+      got.A[wave][i][lane] = A[i];
+      got.H[wave][i][lane] = H[i];
     }
-    if (j + 1 < chunk) {
-      const uint64_t w = await(word(j + 1) + i, v[1][i]);
-      const float A1 = __uint_as_float((uint32_t)w & ~kReady);
-      H = after(H, A1, __uint_as_float((uint32_t)(w >> 32)));
-      A = product(A, A1);
-    }
-    got.A[wave][i][lane] = A;
-    got.H[wave][i][lane] = H;
-    if (wave == 0)
-      base[i][lane] = g > 0 ? __uint_as_float((uint32_t)(await(gs + i, s[i]) >> 32)) : start[i];
+  }
+  if (wave == 0) {
+#pragma unroll
+    for (int i = 0; i < CPL; ++i)
+      base[i][lane] = g > 0 ? __uint_as_float((uint32_t)(await(gs + i, s[i]) >> 32))
+                            : start ? (start + b * D + c0)[lane_c + i] : 0.0f;
   }
 }
 
+// The state in front of the chunk from what look_back left, and the chunk's pair from its waves'.
+template <int NW, int CPL>
+__device__ __forceinline__ float look_back_state(const Pairs<NW, CPL>& got,
+                                                 const float (&base)[CPL][kWave], int chunk, int i,
+                                                 int lane) {
+  float h = base[i][lane];
+  const int n = chunk % kRecGroup;
+  for (int w = 0; w * kLook<NW> < n; ++w) h = after(h, got.A[w][i][lane], got.H[w][i][lane]);
+  return h;
+}
+
+// What the kernels share at their start: which rows and channels a wave has.
+template <int CPL, int NW, int R>
+struct Place {
+  int lane, wave, valid;  // valid: rows inside the sequence
+  int64_t b, t0, t1, c0;  // batch row, first row (and a row inside), the wave column's first channel
+  uint32_t lane_c;        // the lane's first channel, from c0 on
+  // The last lanes of a row share its last CPL channels and compute the same values twice.
+  __device__ __forceinline__ Place(const RecParams& p, int bc, int chunk)
+      : lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {
+    const int64_t D = p.a.dim, T = p.a.seqlen;
+    b = bc / p.cols;
+    t0 = ((int64_t)chunk * NW + wave) * R;
+    t1 = min(t0, T - 1);
+    valid = (int)max((int64_t)0, min((int64_t)R, T - t0));
+    c0 = min((int64_t)(bc % p.cols) * (kWave * CPL), D - CPL);
+    lane_c = (uint32_t)min((int64_t)lane * CPL, D - CPL - c0);
+  }
+};
+
 // ------------------------------------------------------------------------------------- forward
 
-template <typename T, int CPL, bool DECAY, bool IG, int R>
-__global__ __launch_bounds__(kRecWaves* kWave, 4) void rec_fwd_kernel(RecParams p) {
+template <typename T, int CPL, bool DECAY, bool IG, bool SEQ, int NW, int R>
+__global__ __launch_bounds__(NW* kWave, 4) void rec_fwd_kernel(RecParams p) {
   using V = VecIO<T, CPL>;
-  __shared__ Pairs<CPL> mine, got;
+  static_assert(NW * R % CCV1D_REC_SAVED_ROWS == 0 && CCV1D_REC_SAVED_ROWS % R == 0, "saved states");
+  __shared__ Pairs<NW, CPL> mine, got;
   __shared__ float base[CPL][kWave];
   __shared__ uint32_t s_ticket;
   const ccv1d_rec_args& a = p.a;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int bc, chunk;
   deal(p, bc, chunk, &s_ticket);
-  const int64_t b = bc / p.cols, T_ = a.seqlen, D = a.dim;
-  const int64_t t0 = ((int64_t)chunk * kRecWaves + wave) * R;
-  // The last lanes of a row share its last CPL channels and compute the same values twice.
-  const int64_t c = min((int64_t)((bc % p.cols) * kWave + lane) * CPL, D - CPL);
-  const int32_t* seq = a.seq_idx ? a.seq_idx + b * T_ : nullptr;
-  const Rows rows = rows_of<R>(seq, t0, T_, lane);
+  const Place<CPL, NW, R> at(p, bc, chunk);
+  const int lane = at.lane, wave = at.wave, valid = at.valid;
+  const int64_t b = at.b, T_ = a.seqlen, D = a.dim, t0 = at.t0, c0 = at.c0;
+  const uint32_t lane_c = at.lane_c;
+  const uint32_t lane_bytes = at.lane_c * (uint32_t)sizeof(T);
 
-  const T* xp = static_cast<const T*>(a.x) + b * a.x_stride_b;
-  const T* gp = static_cast<const T*>(a.gate) + b * a.gate_stride_b;
-  const T* ip = IG ? static_cast<const T*>(a.input_gate) + b * a.input_gate_stride_b : nullptr;
+  Rows rows{0, 0};
+  if constexpr (SEQ) rows = rows_of<R>(a.seq_idx + b * T_, t0, T_, lane);
+  const uint32_t cut = rows.first | rows.pad;
+
   typename V::raw xr[R], gr[R], ir[R];
-#pragma unroll
-  for (int j = 0; j < R; ++j) {
-    const int64_t t = min(t0 + j, T_ - 1);
-    gr[j] = V::ld(gp + t * a.gate_stride_t + c);
-    xr[j] = V::ld(xp + t * a.x_stride_t + c);
-    if constexpr (IG) ir[j] = V::ld(ip + t * a.input_gate_stride_t + c);
-  }
-  float k[CPL], start[CPL];
+  load_rows<T, CPL, R>({a.gate, a.gate_stride_b, a.gate_stride_t, b, at.t1, at.c0}, valid, lane_bytes, gr);
+  load_rows<T, CPL, R>({a.x, a.x_stride_b, a.x_stride_t, b, at.t1, at.c0}, valid, lane_bytes, xr);
+  if constexpr (IG)
+    load_rows<T, CPL, R>({a.input_gate, a.input_gate_stride_b, a.input_gate_stride_t, b, at.t1, at.c0},
+                         valid, lane_bytes, ir);
+  float k[CPL];
+  bool slow = true;
 #pragma unroll
   for (int i = 0; i < CPL; ++i) {
-    k[i] = DECAY ? decay_rate(a.decay[c + i], a.decay_scale) : 0.0f;
-    start[i] = a.initial_states ? a.initial_states[b * D + c + i] : 0.0f;
+    k[i] = DECAY ? decay_rate((a.decay + c0)[lane_c + i], a.decay_scale) : 0.0f;
+    slow = slow && slow_channel(k[i]);
   }
 
   float f[R][CPL], u[R][CPL], A[CPL], H[CPL];
+  auto coefficients = [&](auto is_slow) {
+    constexpr int kTogether = decltype(is_slow)::value ? 2 : 1;  // rows
+    float tail[CPL];
 #pragma unroll
-  for (int i = 0; i < CPL; ++i) A[i] = 1.0f, H[i] = 0.0f;
+    for (int i = 0; i < CPL; ++i) tail[i] = sinh_tail(k[i]);
 #pragma unroll
-  for (int j = 0; j < R; ++j) {
-    float x[CPL], g[CPL], ig[CPL];
-    V::unpack(xr[j], x);
-    V::unpack(gr[j], g);
-    if constexpr (IG) V::unpack(ir[j], ig);
+    for (int j = 0; j < R; ++j) {
+      if (j % kTogether == 0) {
 #pragma unroll
-    for (int i = 0; i < CPL; ++i) {
-      float beta;
-      forget<T, DECAY>(k[i], g[i], f[j][i], beta);
-      u[j][i] = beta * x[i];
-      if constexpr (IG) u[j][i] *= sigmoid<T>(ig[i]);
+        for (int n = j; n < j + kTogether; ++n) {
+          forget_row(xr[n]);
+          forget_row(gr[n]);
+          if constexpr (IG) forget_row(ir[n]);
+        }
+      }
+      float x[CPL], g[CPL], ig[CPL];
+      V::unpack(xr[j], x);
+      V::unpack(gr[j], g);
+      if constexpr (IG) V::unpack(ir[j], ig);
+#pragma unroll
+      for (int i = 0; i < CPL; ++i) {
+        float beta;
+        forget<T, DECAY, decltype(is_slow)::value>(k[i], tail[i], g[i], f[j][i], beta);
+        u[j][i] = beta * x[i];
+        if constexpr (IG) u[j][i] *= sigmoid<T>(ig[i]);
+      }
+      if ((j + 1) % kTogether == 0) {
+#pragma unroll
+        for (int n = j + 1 - kTogether; n <= j; ++n) {
+          settle(f[n]);
+          settle(u[n]);
+        }
+      }
     }
+  };
+  if (DECAY && !__all(slow)) coefficients(std::false_type{});
+  else coefficients(std::true_type{});
+  if (valid < R) {  // past the end nothing happens
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+#pragma unroll
+      for (int i = 0; i < CPL; ++i)
+        if (j >= valid) f[j][i] = 1.0f, u[j][i] = 0.0f;
   }
-  const uint32_t cut = rows.first | rows.pad;
-  const bool plain = cut == 0 && rows.valid == R;
-  if (plain) {
+  // One row's step from the state before it; MASKED: where a row of the wave cuts the state.
+  auto step = [&](auto masked, int j, int i, float h) {
+    const float next = fmaf(f[j][i], h, u[j][i]);
+    if constexpr (decltype(masked)::value) return cut >> j & 1 ? u[j][i] : next;
+    return next;
+  };
+  auto pair = [&](auto masked) {
+#pragma unroll
+    for (int i = 0; i < CPL; ++i) A[i] = 1.0f, H[i] = 0.0f;
 #pragma unroll
     for (int j = 0; j < R; ++j)
 #pragma unroll
       for (int i = 0; i < CPL; ++i) {
-        H[i] = fmaf(f[j][i], H[i], u[j][i]);
+        if (decltype(masked)::value && (rows.pad >> j & 1)) u[j][i] = 0.0f;
+        H[i] = step(masked, j, i, H[i]);
         A[i] *= f[j][i];
       }
-#pragma unroll
-    for (int i = 0; i < CPL; ++i) A[i] = fmaxf(A[i], kTiny);
-  } else {
-#pragma unroll
-    for (int j = 0; j < R; ++j)
-#pragma unroll
-      for (int i = 0; i < CPL; ++i) {
-        if (j >= rows.valid) f[j][i] = 1.0f, u[j][i] = 0.0f;  // past the end: nothing happens
-        if (rows.pad >> j & 1) u[j][i] = 0.0f;
-        H[i] = cut >> j & 1 ? u[j][i] : fmaf(f[j][i], H[i], u[j][i]);
-        A[i] *= f[j][i];
-      }
-#pragma unroll
-    for (int i = 0; i < CPL; ++i) A[i] = cut ? 0.0f : fmaxf(A[i], kTiny);
-  }
+  };
+  if (SEQ && cut) pair(std::true_type{});
+  else pair(std::false_type{});
 #pragma unroll
   for (int i = 0; i < CPL; ++i) {
+    A[i] = SEQ && cut ? 0.0f : fmaxf(A[i], kTiny);
     mine.A[wave][i][lane] = A[i];
     mine.H[wave][i][lane] = H[i];
   }
@@ -247,67 +384,59 @@ __global__ __launch_bounds__(kRecWaves* kWave, 4) void rec_fwd_kernel(RecParams 
 
   float h[CPL];
   if (p.chunks > 1) {
-    if (wave == 0 && chunk + 1 < p.chunks) {
+    if (wave == NW - 1 && chunk + 1 < p.chunks) {
 #pragma unroll
       for (int i = 0; i < CPL; ++i) {
-        float A0 = 1.0f, H0 = 0.0f;
+        float A0 = mine.A[0][i][lane], H0 = mine.H[0][i][lane];
 #pragma unroll
-        for (int w = 0; w < kRecWaves; ++w) {
+        for (int w = 1; w < NW; ++w) {
           H0 = after(H0, mine.A[w][i][lane], mine.H[w][i][lane]);
           A0 = product(A0, mine.A[w][i][lane]);
         }
-        publish(p.pairs + (b * p.chunks + chunk) * D + c + i, A0, H0);
+        publish(word_row(p.pairs, b * p.chunks + chunk, D, at.c0) + at.lane_c + i, A0, H0);
       }
     }
-    look_back<CPL>(p, b, c, chunk, 1, start, got, base, wave, lane);
+    look_back<NW, CPL>(p, b, at.c0, at.lane_c, chunk, 1, a.initial_states, got, base, wave, lane);
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < CPL; ++i) {
-      h[i] = base[i][lane];
-      for (int w = 0; w < kRecWaves && chunk / kRecGroup * kRecGroup + 2 * w < chunk; ++w)
-        h[i] = after(h[i], got.A[w][i][lane], got.H[w][i][lane]);
-    }
+    for (int i = 0; i < CPL; ++i) h[i] = look_back_state<NW, CPL>(got, base, chunk, i, lane);
   } else {
 #pragma unroll
-    for (int i = 0; i < CPL; ++i) h[i] = start[i];
+    for (int i = 0; i < CPL; ++i) h[i] = a.initial_states ? (a.initial_states + b * D + c0)[lane_c + i] : 0.0f;
   }
+  for (int w = 0; w < wave; ++w)
 #pragma unroll
-  for (int i = 0; i < CPL; ++i)
-    for (int w = 0; w < wave; ++w) h[i] = after(h[i], mine.A[w][i][lane], mine.H[w][i][lane]);
-  if (wave == kRecWaves - 1 && chunk % kRecGroup == kRecGroup - 1 && chunk + 1 < p.chunks) {
+    for (int i = 0; i < CPL; ++i) h[i] = after(h[i], mine.A[w][i][lane], mine.H[w][i][lane]);
+  if (wave == NW - 1 && chunk % kRecGroup == kRecGroup - 1 && chunk + 1 < p.chunks) {
 #pragma unroll
     for (int i = 0; i < CPL; ++i)
-      publish(p.states + (b * p.groups + chunk / kRecGroup) * D + c + i, 0.0f, after(h[i], A[i], H[i]));
+      publish(word_row(p.states, b * p.groups + chunk / kRecGroup, D, at.c0) + at.lane_c + i, 0.0f,
+              after(h[i], mine.A[wave][i][lane], mine.H[wave][i][lane]));
   }
-  if (rows.valid == 0) return;
+  if (valid == 0) return;
   if (a.saved && t0 % CCV1D_REC_SAVED_ROWS == 0) {
     const int64_t ns = (T_ + CCV1D_REC_SAVED_ROWS - 1) / CCV1D_REC_SAVED_ROWS;
 #pragma unroll
     for (int i = 0; i < CPL; ++i)
-      a.saved[(b * ns + t0 / CCV1D_REC_SAVED_ROWS) * D + c + i] = h[i];
+      (a.saved + (b * ns + t0 / CCV1D_REC_SAVED_ROWS) * D + c0)[lane_c + i] = h[i];
   }
-  T* out = static_cast<T*>(a.out) + (b * T_ + t0) * D + c;
-  if (plain) {
+  RowWalk<T, CPL> out(a.out, T_ * D, D, b, t0, at.c0);
+  auto walk = [&](auto masked) {
 #pragma unroll
     for (int j = 0; j < R; ++j) {
+      if (j < valid) {
 #pragma unroll
-      for (int i = 0; i < CPL; ++i) h[i] = fmaf(f[j][i], h[i], u[j][i]);
-      V::st(out + j * D, V::pack(h));
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-      if (j < rows.valid) {
-#pragma unroll
-        for (int i = 0; i < CPL; ++i)
-          h[i] = cut >> j & 1 ? u[j][i] : fmaf(f[j][i], h[i], u[j][i]);
-        V::st(out + j * D, V::pack(h));
+        for (int i = 0; i < CPL; ++i) h[i] = step(masked, j, i, h[i]);
+        out.store(lane_bytes, h);
+        out.move(out.step);
       }
     }
-  }
-  if (a.final_states && t0 + rows.valid == T_) {
+  };
+  if (SEQ && cut) walk(std::true_type{});
+  else walk(std::false_type{});
+  if (a.final_states && t0 + valid == T_) {
 #pragma unroll
-    for (int i = 0; i < CPL; ++i) a.final_states[b * D + c + i] = h[i];
+    for (int i = 0; i < CPL; ++i) (a.final_states + b * D + c0)[lane_c + i] = h[i];
   }
 }
 
@@ -318,125 +447,147 @@ __global__ __launch_bounds__(kRecWaves* kWave, 4) void rec_fwd_kernel(RecParams 
 // m = h[t-1] - w (h[t-1] taken as zero where the state is cut):
 //   dx = dh beta i, dinput_gate = dx x (1 - i)
 //   with decay:     w = i x a / beta,  q = dh (ln a) a m,  dgate = q (1 - r),  ddecay from the sum of q
-//                   (a / beta comes from d beta / d(ln a) = -a^2 / beta; 0 where a is exactly 1)
+//                   (a / beta comes from d beta / d(ln a) = -a^2 / beta; where a is exactly 1, ln a = 0
+//                   makes q zero, and 1 / beta is held finite)
 //   without decay:  w = i x,           dgate = dh a beta m
 
-template <typename T, int CPL, bool DECAY, bool IG, int R>
-__global__ __launch_bounds__(kRecWaves* kWave, 2) void rec_bwd_kernel(RecParams p) {
+template <typename T, int CPL, bool DECAY, bool IG, bool SEQ, int NW, int R>
+__global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
   using V = VecIO<T, CPL>;
-  static_assert(kRecWaves * R == CCV1D_REC_SAVED_ROWS, "one saved state per chunk");
-  __shared__ Pairs<CPL> mine, got;
-  __shared__ float s_h[kRecWaves][CPL][kWave];
+  static_assert(NW * R == CCV1D_REC_SAVED_ROWS, "one saved state per chunk");
+  __shared__ Pairs<NW, CPL> mine, got;
+  __shared__ float s_h[NW][CPL][kWave];
   __shared__ float base[CPL][kWave];
   __shared__ uint32_t s_ticket;
   const ccv1d_rec_args& a = p.a;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int bc, from_end;
   deal(p, bc, from_end, &s_ticket);
   const int chunk = p.chunks - 1 - from_end;
-  const int64_t b = bc / p.cols, T_ = a.seqlen, D = a.dim;
-  const int64_t t0 = ((int64_t)chunk * kRecWaves + wave) * R;
-  const int64_t c = min((int64_t)((bc % p.cols) * kWave + lane) * CPL, D - CPL);
-  const int32_t* seq = a.seq_idx ? a.seq_idx + b * T_ : nullptr;
-  const Rows rows = rows_of<R>(seq, t0, T_, lane);
+  const Place<CPL, NW, R> at(p, bc, chunk);
+  const int lane = at.lane, wave = at.wave, valid = at.valid;
+  const int64_t b = at.b, T_ = a.seqlen, D = a.dim, t0 = at.t0, c0 = at.c0;
+  const uint32_t lane_c = at.lane_c;
+  const uint32_t lane_bytes = at.lane_c * (uint32_t)sizeof(T);
 
-  const T* xp = static_cast<const T*>(a.x) + b * a.x_stride_b;
-  const T* gp = static_cast<const T*>(a.gate) + b * a.gate_stride_b;
-  const T* ip = IG ? static_cast<const T*>(a.input_gate) + b * a.input_gate_stride_b : nullptr;
-  const T* yp = static_cast<const T*>(a.dout) + b * a.dout_stride_b;
-  typename V::raw xr[R], gr[R], ir[R], yr[R];
-#pragma unroll
-  for (int j = 0; j < R; ++j) {
-    const int64_t t = min(t0 + j, T_ - 1);
-    gr[j] = V::ld(gp + t * a.gate_stride_t + c);
-    xr[j] = V::ld(xp + t * a.x_stride_t + c);
-    if constexpr (IG) ir[j] = V::ld(ip + t * a.input_gate_stride_t + c);
-    yr[j] = V::ld(yp + t * a.dout_stride_t + c);
-  }
-  float k[CPL], start[CPL], h[CPL];
-#pragma unroll
-  for (int i = 0; i < CPL; ++i) {
-    k[i] = DECAY ? decay_rate(a.decay[c + i], a.decay_scale) : 0.0f;
-    start[i] = a.dfinal_states ? a.dfinal_states[b * D + c + i] : 0.0f;
-    h[i] = a.saved[(b * p.chunks + chunk) * D + c + i];
-  }
-
+  Rows rows{0, 0};
+  if constexpr (SEQ) rows = rows_of<R>(a.seq_idx + b * T_, t0, T_, lane);
   const uint32_t cut = rows.first | rows.pad;
-  const bool plain = cut == 0 && rows.valid == R;
-  float f[R][CPL], bi[R][CPL];          // a; beta i
-  float w[R][CPL];                      // then m
-  float la[R][CPL], rest[R][CPL];       // decay: a ln a, 1 - r; else a beta
-  float xi[R][CPL];                     // x (1 - i)
-  float A[CPL], H[CPL], G[CPL];
-#pragma unroll
-  for (int i = 0; i < CPL; ++i) A[i] = 1.0f, H[i] = 0.0f, G[i] = 0.0f;
-#pragma unroll
-  for (int j = 0; j < R; ++j) {
-    float x[CPL], g[CPL], ig[CPL];
-    V::unpack(xr[j], x);
-    V::unpack(gr[j], g);
-    if constexpr (IG) V::unpack(ir[j], ig);
-#pragma unroll
-    for (int i = 0; i < CPL; ++i) {
-      float in = 1.0f, not_in = 0.0f;
-      if constexpr (IG) sigmoid_pair<T>(ig[i], in, not_in);
-      if constexpr (DECAY) {
-        float r;
-        sigmoid_pair<T>(g[i], r, rest[j][i]);
-        const float l = k[i] * r;
-        const float av = __builtin_amdgcn_exp2f(l);
-        const float s = one_minus_square(l, av);
-        const float inv = s > 0.0f ? __builtin_amdgcn_rsqf(s) : s == 0.0f ? 0.0f : s;
-        f[j][i] = av;
-        bi[j][i] = s * inv * in;
-        la[j][i] = kLn2 * l * av;
-        w[j][i] = in * x[i] * av * inv;
-      } else {
-        float beta;
-        sigmoid_pair<T>(g[i], f[j][i], beta);
-        bi[j][i] = beta * in;
-        la[j][i] = f[j][i] * beta;
-        w[j][i] = in * x[i];
-      }
-      if constexpr (IG) xi[j][i] = x[i] * not_in;
-    }
-  }
-  // Forward over the rows: the pair (A, H).
-#pragma unroll
-  for (int j = 0; j < R; ++j) {
-    float x[CPL];
-    V::unpack(xr[j], x);
-#pragma unroll
-    for (int i = 0; i < CPL; ++i) {
-      float u = bi[j][i] * x[i];
-      if (!plain) {
-        if (j >= rows.valid) f[j][i] = 1.0f, u = 0.0f;
-        if (rows.pad >> j & 1) u = 0.0f;
-        H[i] = cut >> j & 1 ? u : fmaf(f[j][i], H[i], u);
-      } else {
-        H[i] = fmaf(f[j][i], H[i], u);
-      }
-      A[i] *= f[j][i];
-    }
-  }
-  // Backward over them: the pair (A, G).
-#pragma unroll
-  for (int j = R - 1; j >= 0; --j) {
-    float y[CPL];
-    V::unpack(yr[j], y);
-#pragma unroll
-    for (int i = 0; i < CPL; ++i) {
-      if (!plain) {
-        if (j >= rows.valid) y[i] = 0.0f;
-        G[i] = cut >> j & 1 ? 0.0f : f[j][i] * (y[i] + G[i]);
-      } else {
-        G[i] = f[j][i] * (y[i] + G[i]);
-      }
-    }
-  }
+
+  typename V::raw xr[R], gr[R], ir[R], yr[R];
+  load_rows<T, CPL, R>({a.gate, a.gate_stride_b, a.gate_stride_t, b, at.t1, at.c0}, valid, lane_bytes, gr);
+  load_rows<T, CPL, R>({a.x, a.x_stride_b, a.x_stride_t, b, at.t1, at.c0}, valid, lane_bytes, xr);
+  if constexpr (IG)
+    load_rows<T, CPL, R>({a.input_gate, a.input_gate_stride_b, a.input_gate_stride_t, b, at.t1, at.c0},
+                         valid, lane_bytes, ir);
+  load_rows<T, CPL, R>({a.dout, a.dout_stride_b, a.dout_stride_t, b, at.t1, at.c0}, valid, lane_bytes, yr);
+  float k[CPL], h[CPL];
+  bool slow = true;
 #pragma unroll
   for (int i = 0; i < CPL; ++i) {
-    A[i] = cut ? 0.0f : fmaxf(A[i], kTiny);
+    k[i] = DECAY ? decay_rate((a.decay + c0)[lane_c + i], a.decay_scale) : 0.0f;
+    slow = slow && slow_channel(k[i]);
+    h[i] = (a.saved + (b * p.chunks + chunk) * D + c0)[lane_c + i];
+  }
+
+  // Kept per element: a, beta i and w (then m). The gates' other factors are made again from the inputs
+  // in the last walk: keeping them too would leave half of the waves.
+  float f[R][CPL], bi[R][CPL], w[R][CPL];
+  auto coefficients = [&](auto is_slow) {
+    constexpr int kTogether = decltype(is_slow)::value ? 2 : 1;  // rows
+    float tail[CPL];
+#pragma unroll
+    for (int i = 0; i < CPL; ++i) tail[i] = sinh_tail(k[i]);
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      if (j % kTogether == 0) {
+#pragma unroll
+        for (int n = j; n < j + kTogether; ++n) {
+          forget_row(xr[n]);
+          forget_row(gr[n]);
+          if constexpr (IG) forget_row(ir[n]);
+        }
+      }
+      float x[CPL], g[CPL], ig[CPL];
+      V::unpack(xr[j], x);
+      V::unpack(gr[j], g);
+      if constexpr (IG) V::unpack(ir[j], ig);
+#pragma unroll
+      for (int i = 0; i < CPL; ++i) {
+        const float in = IG ? sigmoid<T>(ig[i]) : 1.0f;
+        if constexpr (DECAY) {
+          const float l = k[i] * sigmoid<T>(g[i]);
+          f[j][i] = __builtin_amdgcn_exp2f(l);
+          const float s = one_minus_square<decltype(is_slow)::value>(tail[i], l, f[j][i]);
+          const float inv = __builtin_amdgcn_rsqf(fmaxf(s, kTiny));
+          bi[j][i] = s * inv * in;
+          w[j][i] = in * x[i] * (f[j][i] * inv);
+        } else {
+          float beta;
+          sigmoid_pair<T>(g[i], f[j][i], beta);
+          bi[j][i] = beta * in;
+          w[j][i] = in * x[i];
+        }
+      }
+      if ((j + 1) % kTogether == 0) {
+#pragma unroll
+        for (int n = j + 1 - kTogether; n <= j; ++n) {
+          settle(f[n]);
+          settle(bi[n]);
+          settle(w[n]);
+        }
+      }
+    }
+  };
+  if (DECAY && !__all(slow)) coefficients(std::false_type{});
+  else coefficients(std::true_type{});
+  if (valid < R) {  // past the end nothing happens
+    const float zero[CPL] = {};
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+      if (j >= valid) {
+        xr[j] = yr[j] = V::pack(zero);
+#pragma unroll
+        for (int i = 0; i < CPL; ++i) f[j][i] = 1.0f, bi[j][i] = 0.0f;
+      }
+  }
+
+  // Forward over the rows: the pair (A, H); backward over them: (A, G).
+  float A[CPL], H[CPL], G[CPL];
+  auto forward = [&](auto masked, int j, int i, float x, float h) {
+    const float u = bi[j][i] * x;
+    if constexpr (decltype(masked)::value)
+      return rows.pad >> j & 1 ? 0.0f : cut >> j & 1 ? u : fmaf(f[j][i], h, u);
+    return fmaf(f[j][i], h, u);
+  };
+  auto pairs = [&](auto masked) {
+#pragma unroll
+    for (int i = 0; i < CPL; ++i) A[i] = 1.0f, H[i] = 0.0f, G[i] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      float x[CPL];
+      V::unpack(xr[j], x);
+#pragma unroll
+      for (int i = 0; i < CPL; ++i) {
+        H[i] = forward(masked, j, i, x[i], H[i]);
+        A[i] *= f[j][i];
+      }
+    }
+#pragma unroll
+    for (int j = R - 1; j >= 0; --j) {
+      float y[CPL];
+      V::unpack(yr[j], y);
+#pragma unroll
+      for (int i = 0; i < CPL; ++i) {
+        G[i] = f[j][i] * (y[i] + G[i]);
+        if (decltype(masked)::value && (cut >> j & 1)) G[i] = 0.0f;
+      }
+    }
+  };
+  if (SEQ && cut) pairs(std::true_type{});
+  else pairs(std::false_type{});
+#pragma unroll
+  for (int i = 0; i < CPL; ++i) {
+    A[i] = SEQ && cut ? 0.0f : fmaxf(A[i], kTiny);
     mine.A[wave][i][lane] = A[i];
     mine.H[wave][i][lane] = G[i];
     s_h[wave][i][lane] = H[i];
@@ -445,93 +596,107 @@ __global__ __launch_bounds__(kRecWaves* kWave, 2) void rec_bwd_kernel(RecParams 
 
   float cc[CPL];
   if (p.chunks > 1) {
-    if (wave == 0 && chunk > 0) {
+    if (wave == NW - 1 && chunk > 0) {
 #pragma unroll
       for (int i = 0; i < CPL; ++i) {
-        float A0 = 1.0f, G0 = 0.0f;
+        float A0 = mine.A[NW - 1][i][lane], G0 = mine.H[NW - 1][i][lane];
 #pragma unroll
-        for (int v = kRecWaves - 1; v >= 0; --v) {
+        for (int v = NW - 2; v >= 0; --v) {
           G0 = after(G0, mine.A[v][i][lane], mine.H[v][i][lane]);
           A0 = product(A0, mine.A[v][i][lane]);
         }
-        publish(p.pairs + (b * p.chunks + chunk) * D + c + i, A0, G0);
+        publish(word_row(p.pairs, b * p.chunks + chunk, D, at.c0) + at.lane_c + i, A0, G0);
       }
     }
-    look_back<CPL>(p, b, c, from_end, -1, start, got, base, wave, lane);
+    look_back<NW, CPL>(p, b, at.c0, at.lane_c, from_end, -1, a.dfinal_states, got, base, wave, lane);
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < CPL; ++i) {
-      cc[i] = base[i][lane];
-      for (int v = 0; v < kRecWaves && from_end / kRecGroup * kRecGroup + 2 * v < from_end; ++v)
-        cc[i] = after(cc[i], got.A[v][i][lane], got.H[v][i][lane]);
-    }
+    for (int i = 0; i < CPL; ++i) cc[i] = look_back_state<NW, CPL>(got, base, from_end, i, lane);
   } else {
 #pragma unroll
-    for (int i = 0; i < CPL; ++i) cc[i] = start[i];
+    for (int i = 0; i < CPL; ++i) cc[i] = a.dfinal_states ? (a.dfinal_states + b * D + c0)[lane_c + i] : 0.0f;
   }
+  for (int v = NW - 1; v > wave; --v)
 #pragma unroll
-  for (int i = 0; i < CPL; ++i) {
-    for (int v = kRecWaves - 1; v > wave; --v)
-      cc[i] = after(cc[i], mine.A[v][i][lane], mine.H[v][i][lane]);
-    for (int v = 0; v < wave; ++v) h[i] = after(h[i], mine.A[v][i][lane], s_h[v][i][lane]);
-  }
+    for (int i = 0; i < CPL; ++i) cc[i] = after(cc[i], mine.A[v][i][lane], mine.H[v][i][lane]);
+  for (int v = 0; v < wave; ++v)
+#pragma unroll
+    for (int i = 0; i < CPL; ++i) h[i] = after(h[i], mine.A[v][i][lane], s_h[v][i][lane]);
   if (wave == 0 && from_end % kRecGroup == kRecGroup - 1 && chunk > 0) {
 #pragma unroll
     for (int i = 0; i < CPL; ++i)
-      publish(p.states + (b * p.groups + from_end / kRecGroup) * D + c + i, 0.0f,
-              after(cc[i], A[i], G[i]));
+      publish(word_row(p.states, b * p.groups + from_end / kRecGroup, D, at.c0) + at.lane_c + i, 0.0f,
+              after(cc[i], mine.A[wave][i][lane], mine.H[wave][i][lane]));
   }
 
-  // The states again, row by row: w becomes m.
-#pragma unroll
-  for (int j = 0; j < R; ++j) {
-    float x[CPL];
-    V::unpack(xr[j], x);
-#pragma unroll
-    for (int i = 0; i < CPL; ++i) {
-      const float u = bi[j][i] * x[i];
-      if (!plain) {
-        const bool stop = cut >> j & 1;
-        w[j][i] = (stop ? 0.0f : h[i]) - w[j][i];
-        h[i] = rows.pad >> j & 1 ? 0.0f : stop ? u : fmaf(f[j][i], h[i], u);
-      } else {
-        w[j][i] = h[i] - w[j][i];
-        h[i] = fmaf(f[j][i], h[i], u);
-      }
-    }
-  }
   float sum[CPL];
 #pragma unroll
   for (int i = 0; i < CPL; ++i) sum[i] = 0.0f;
-  const int64_t at = (b * T_ + t0) * D + c;
-  T* dx = static_cast<T*>(a.dx) + at;
-  T* dg = static_cast<T*>(a.dgate) + at;
-  T* di = IG ? static_cast<T*>(a.dinput_gate) + at : nullptr;
+  const int64_t last = t0 + valid - 1;  // stored from the last row back
+  RowWalk<T, CPL> dx(a.dx, T_ * D, D, b, last, at.c0), dg(a.dgate, T_ * D, D, b, last, at.c0);
+  RowWalk<T, CPL> di(a.dinput_gate, T_ * D, D, b, last, at.c0);
+  // The states again, row by row (w becomes m), then the gradients from the last row back.
+  auto walk = [&](auto masked) {
+    constexpr bool kMasked = decltype(masked)::value;
 #pragma unroll
-  for (int j = R - 1; j >= 0; --j) {
-    if (!plain && j >= rows.valid) continue;
-    float y[CPL], ox[CPL], og[CPL], oi[CPL];
-    V::unpack(yr[j], y);
-    const bool pad = !plain && (rows.pad >> j & 1), stop = !plain && (cut >> j & 1);
+    for (int j = 0; j < R; ++j) {
+      forget_row(xr[j]);
+      float x[CPL];
+      V::unpack(xr[j], x);
 #pragma unroll
-    for (int i = 0; i < CPL; ++i) {
-      const float dh = y[i] + cc[i];
-      ox[i] = dh * bi[j][i];
-      if constexpr (IG) oi[i] = ox[i] * xi[j][i];
-      const float q = dh * la[j][i] * w[j][i];
-      og[i] = DECAY ? q * rest[j][i] : q;
-      if (DECAY && !pad) sum[i] += q;
-      cc[i] = stop ? 0.0f : f[j][i] * dh;
-      if (pad) ox[i] = og[i] = 0.0f;
-      if (IG && pad) oi[i] = 0.0f;
+      for (int i = 0; i < CPL; ++i) {
+        w[j][i] = (kMasked && (cut >> j & 1) ? 0.0f : h[i]) - w[j][i];
+        h[i] = forward(masked, j, i, x[i], h[i]);
+      }
     }
-    V::st(dx + j * D, V::pack(ox));
-    V::st(dg + j * D, V::pack(og));
-    if constexpr (IG) V::st(di + j * D, V::pack(oi));
-  }
+#pragma unroll
+    for (int j = R - 1; j >= 0; --j) {
+      if (j >= valid) continue;
+      forget_row(xr[j]);
+      forget_row(gr[j]);
+      forget_row(yr[j]);
+      if constexpr (IG) forget_row(ir[j]);
+      const bool pad = kMasked && (rows.pad >> j & 1);
+      float y[CPL], x[CPL], g[CPL], ig[CPL], ox[CPL], og[CPL], oi[CPL];
+      V::unpack(yr[j], y);
+      V::unpack(xr[j], x);
+      V::unpack(gr[j], g);
+      if constexpr (IG) V::unpack(ir[j], ig);
+#pragma unroll
+      for (int i = 0; i < CPL; ++i) {
+        const float dh = y[i] + cc[i];
+        cc[i] = kMasked && (cut >> j & 1) ? 0.0f : f[j][i] * dh;
+        ox[i] = dh * bi[j][i];
+        if constexpr (IG) {
+          float in, not_in;
+          sigmoid_pair<T>(ig[i], in, not_in);
+          oi[i] = ox[i] * (x[i] * not_in);
+        }
+        float r, not_r;
+        sigmoid_pair<T>(g[i], r, not_r);
+        float q = dh * f[j][i] * w[j][i];
+        if constexpr (DECAY) {
+          q *= kLn2 * k[i] * r;
+          sum[i] += pad ? 0.0f : q;
+        }
+        og[i] = q * not_r;
+        if (pad) ox[i] = og[i] = oi[i] = 0.0f;
+      }
+      dx.store(lane_bytes, ox);
+      dg.store(lane_bytes, og);
+      dx.move(-dx.step);
+      dg.move(-dg.step);
+      if constexpr (IG) {
+        di.store(lane_bytes, oi);
+        di.move(-di.step);
+      }
+    }
+  };
+  if (SEQ && cut) walk(std::true_type{});
+  else walk(std::false_type{});
   if (a.dinitial_states && chunk == 0 && wave == 0) {
 #pragma unroll
-    for (int i = 0; i < CPL; ++i) a.dinitial_states[b * D + c + i] = cc[i];
+    for (int i = 0; i < CPL; ++i) (a.dinitial_states + b * D + c0)[lane_c + i] = cc[i];
   }
   if constexpr (DECAY) {  // the chunk's sum, its waves in order
     __syncthreads();
@@ -543,8 +708,8 @@ __global__ __launch_bounds__(kRecWaves* kWave, 2) void rec_bwd_kernel(RecParams 
       for (int i = 0; i < CPL; ++i) {
         float s = 0.0f;
 #pragma unroll
-        for (int v = 0; v < kRecWaves; ++v) s += s_h[v][i][lane];
-        p.part[(b * p.chunks + chunk) * D + c + i] = s;
+        for (int v = 0; v < NW; ++v) s += s_h[v][i][lane];
+        (p.part + (b * p.chunks + chunk) * D + c0)[lane_c + i] = s;
       }
     }
   }

@@ -39,14 +39,24 @@ __device__ __forceinline__ void sigmoid_pair(float z, float& s, float& rest) {
   rest = e * s;
 }
 
+// sigmoid(z) alone, where 2^t may pass the largest number and the result reach zero.
 template <typename T>
 __device__ __forceinline__ float sigmoid(float z) {
-  return __builtin_amdgcn_rcpf(1.0f + exp_minus<T>(z));
+  if constexpr (sizeof(T) == 4) return __builtin_amdgcn_rcpf(1.0f + exp_minus<T>(z));
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
 }
 
-// k of a channel: log2 a = k * r.
+// k of a channel: log2 a = k * r. softplus = log(1 + e), e = exp(decay): for e below 0.1, where a decay
+// that lets a channel remember lies, its series (the next term is 2e-8 of it), else the library's.
 __device__ __forceinline__ float decay_rate(float decay, float scale) {
-  const float sp = decay > 20.0f ? decay : log1pf(expf(decay));
+  const float e = exp_minus<float>(-decay);
+  float sp = fmaf(e, 1.0f / 7.0f, -1.0f / 6.0f);
+  sp = fmaf(e, sp, 1.0f / 5.0f);
+  sp = fmaf(e, sp, -1.0f / 4.0f);
+  sp = fmaf(e, sp, 1.0f / 3.0f);
+  sp = fmaf(e, sp, -1.0f / 2.0f);
+  sp = fmaf(e * e, sp, e);
+  if (!(decay < -2.3f)) sp = decay > 20.0f ? decay : log1pf(expf(decay));
   return -scale * sp * kLog2e;
 }
 
@@ -58,26 +68,46 @@ __device__ __forceinline__ float decay_ratio(float decay) {
   return 1.0f / ((1.0f + expf(-decay)) * sp);
 }
 
-// 1 - a^2 from log2 a: below 0.35 of -2 ln a the difference cancels, and the series of
-// -expm1(y), y = 2 ln a, is used instead (its next term is 2e-8 of the result there).
-__device__ __forceinline__ float one_minus_square(float log2a, float a) {
-  const float y = log2a * (2.0f * kLn2);
-  float p = fmaf(y, 1.0f / 5040.0f, 1.0f / 720.0f);
-  p = fmaf(y, p, 1.0f / 120.0f);
-  p = fmaf(y, p, 1.0f / 24.0f);
-  p = fmaf(y, p, 1.0f / 6.0f);
-  p = fmaf(y, p, 0.5f);
-  p = fmaf(y, p, 1.0f);
-  return y > -0.35f ? -y * p : fmaf(-a, a, 1.0f);
+// 1 - a^2 = 2 a sinh(-ln a) from log2 a, without the difference's cancellation: sinh's series, to the
+// 11th power, up to |ln a| = 1 (the next term is 3e-8 of it), beyond which 1 - a^2 itself is exact
+// enough. A slow channel, |ln a| <= 1/4 even at an open gate (which its decay alone decides), does
+// with the 5th power (5e-8). Where all channels of a wave are slow the rest is left out (SLOW); where
+// not, a slow channel's higher powers count zero times, so that its values do not depend on its
+// neighbours.
+__device__ __forceinline__ bool slow_channel(float k) { return k >= -0.25f * kLog2e; }
+
+constexpr float sinh_coefficient(double factorial, int power) {
+  double v = -2.0 / factorial;
+  for (int i = 0; i < power; ++i) v *= 0.69314718055994530942;
+  return (float)v;
+}
+
+// 0 for a slow channel, which leaves the higher powers out; else 1.
+__device__ __forceinline__ float sinh_tail(float k) { return slow_channel(k) ? 0.0f : 1.0f; }
+
+template <bool SLOW>
+__device__ __forceinline__ float one_minus_square(float tail, float log2a, float a) {
+  const float l2 = log2a * log2a;
+  float p = sinh_coefficient(120.0, 5);
+  if constexpr (!SLOW) {
+    float t = fmaf(l2, sinh_coefficient(39916800.0, 11), sinh_coefficient(362880.0, 9));
+    t = fmaf(l2, t, sinh_coefficient(5040.0, 7));
+    p = fmaf(l2 * tail, t, p);
+  }
+  p = fmaf(l2, p, sinh_coefficient(6.0, 3));
+  p = fmaf(l2, p, sinh_coefficient(1.0, 1));
+  p = log2a * a * p;
+  if constexpr (SLOW) return p;
+  return log2a < -kLog2e ? fmaf(-a, a, 1.0f) : p;
 }
 
 // The factor of the state before a row and that of the row's own i * x.
-template <typename T, bool DECAY>
-__device__ __forceinline__ void forget(float k, float gate, float& a, float& beta) {
+template <typename T, bool DECAY, bool SLOW>
+__device__ __forceinline__ void forget(float k, float tail, float gate, float& a, float& beta) {
   if constexpr (DECAY) {
     const float l = k * sigmoid<T>(gate);
     a = __builtin_amdgcn_exp2f(l);
-    beta = __builtin_amdgcn_sqrtf(one_minus_square(l, a));
+    beta = __builtin_amdgcn_sqrtf(one_minus_square<SLOW>(tail, l, a));
   } else {
     sigmoid_pair<T>(gate, a, beta);
   }
