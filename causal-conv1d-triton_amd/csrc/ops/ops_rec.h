@@ -49,6 +49,12 @@ struct RecParams {
   uint64_t* states;              // (batch, groups, dim): word of the state after a group
   uint32_t* ticket;
   float* part;  // backward: (batch, chunks, dim) sums behind ddecay
+  // Rows whose starts and ends lie on the 128-byte lines are read and written once and kept out of the
+  // caches' way (forward and backward at B=4 T=8192 D=1024 bf16: 219 us with cached accesses, 213 with
+  // streamed stores, 207 with loads too). Other rows share lines with their neighbours, which another
+  // wave reads at another time. (STREAM in the kernels: chosen at run time inside them, the stores'
+  // branches cost B=4 T=16384 D=4096 without decay 836 -> 903 us.)
+  bool stream;
 };
 
 __device__ __forceinline__ void publish(uint64_t* at, float A, float H) {
@@ -110,13 +116,15 @@ struct RowWalk {
                                      int64_t t, int64_t c0)
       : row((byte*)base + (b * stride_b + t * stride_t + c0) * (int64_t)sizeof(T)),
         step(stride_t * (int64_t)sizeof(T)) {}
-  // Every row is read and written once: kept out of the caches' way (forward and backward at B=4
-  // T=8192 D=1024 bf16: 219 us with cached loads and stores, 213 with cached loads, 207 with neither).
+  template <bool STREAM>
   __device__ __forceinline__ typename V::raw load(uint32_t lane_bytes) const {
-    return __builtin_nontemporal_load((const cell*)(row + lane_bytes));
+    if constexpr (STREAM) return __builtin_nontemporal_load((const cell*)(row + lane_bytes));
+    return *(const cell*)(row + lane_bytes);
   }
+  template <bool STREAM>
   __device__ __forceinline__ void store(uint32_t lane_bytes, const float (&v)[CPL]) {
-    __builtin_nontemporal_store(V::pack(v), (cell*)(row + lane_bytes));
+    if constexpr (STREAM) __builtin_nontemporal_store(V::pack(v), (cell*)(row + lane_bytes));
+    else *(cell*)(row + lane_bytes) = V::pack(v);
   }
   __device__ __forceinline__ void move(int64_t bytes) {
     row += bytes;
@@ -131,12 +139,12 @@ __device__ __forceinline__ void settle(float (&v)[CPL]) {
 }
 
 // Loads R rows; those past the last one, `valid` - 1, repeat it.
-template <typename T, int CPL, int R>
+template <bool STREAM, typename T, int CPL, int R>
 __device__ __forceinline__ void load_rows(RowWalk<T, CPL> w, int valid, uint32_t lane_bytes,
                                           typename VecIO<T, CPL>::raw (&to)[R]) {
 #pragma unroll
   for (int j = 0; j < R; ++j) {
-    to[j] = w.load(lane_bytes);
+    to[j] = w.template load<STREAM>(lane_bytes);
     w.move(j + 1 < valid ? w.step : 0);
   }
 }
@@ -275,7 +283,7 @@ struct Place {
 
 // ------------------------------------------------------------------------------------- forward
 
-template <typename T, int CPL, bool DECAY, bool IG, bool SEQ, int NW, int R>
+template <typename T, int CPL, bool DECAY, bool IG, bool SEQ, bool STREAM, int NW, int R>
 __global__ __launch_bounds__(NW* kWave, 4) void rec_fwd_kernel(RecParams p) {
   using V = VecIO<T, CPL>;
   static_assert(NW * R % CCV1D_REC_SAVED_ROWS == 0 && CCV1D_REC_SAVED_ROWS % R == 0, "saved states");
@@ -296,11 +304,12 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_fwd_kernel(RecParams p) {
   const uint32_t cut = rows.first | rows.pad;
 
   typename V::raw xr[R], gr[R], ir[R];
-  load_rows<T, CPL, R>({a.gate, a.gate_stride_b, a.gate_stride_t, b, at.t1, at.c0}, valid, lane_bytes, gr);
-  load_rows<T, CPL, R>({a.x, a.x_stride_b, a.x_stride_t, b, at.t1, at.c0}, valid, lane_bytes, xr);
+  load_rows<STREAM, T, CPL, R>({a.gate, a.gate_stride_b, a.gate_stride_t, b, at.t1, c0}, valid,
+                                lane_bytes, gr);
+  load_rows<STREAM, T, CPL, R>({a.x, a.x_stride_b, a.x_stride_t, b, at.t1, c0}, valid, lane_bytes, xr);
   if constexpr (IG)
-    load_rows<T, CPL, R>({a.input_gate, a.input_gate_stride_b, a.input_gate_stride_t, b, at.t1, at.c0},
-                         valid, lane_bytes, ir);
+    load_rows<STREAM, T, CPL, R>(
+        {a.input_gate, a.input_gate_stride_b, a.input_gate_stride_t, b, at.t1, c0}, valid, lane_bytes, ir);
   float k[CPL];
   bool slow = true;
 #pragma unroll
@@ -427,7 +436,7 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_fwd_kernel(RecParams p) {
       if (j < valid) {
 #pragma unroll
         for (int i = 0; i < CPL; ++i) h[i] = step(masked, j, i, h[i]);
-        out.store(lane_bytes, h);
+        out.template store<STREAM>(lane_bytes, h);
         out.move(out.step);
       }
     }
@@ -451,7 +460,7 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_fwd_kernel(RecParams p) {
 //                   makes q zero, and 1 / beta is held finite)
 //   without decay:  w = i x,           dgate = dh a beta m
 
-template <typename T, int CPL, bool DECAY, bool IG, bool SEQ, int NW, int R>
+template <typename T, int CPL, bool DECAY, bool IG, bool SEQ, bool STREAM, int NW, int R>
 __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
   using V = VecIO<T, CPL>;
   static_assert(NW * R == CCV1D_REC_SAVED_ROWS, "one saved state per chunk");
@@ -474,12 +483,14 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
   const uint32_t cut = rows.first | rows.pad;
 
   typename V::raw xr[R], gr[R], ir[R], yr[R];
-  load_rows<T, CPL, R>({a.gate, a.gate_stride_b, a.gate_stride_t, b, at.t1, at.c0}, valid, lane_bytes, gr);
-  load_rows<T, CPL, R>({a.x, a.x_stride_b, a.x_stride_t, b, at.t1, at.c0}, valid, lane_bytes, xr);
+  load_rows<STREAM, T, CPL, R>({a.gate, a.gate_stride_b, a.gate_stride_t, b, at.t1, c0}, valid,
+                                lane_bytes, gr);
+  load_rows<STREAM, T, CPL, R>({a.x, a.x_stride_b, a.x_stride_t, b, at.t1, c0}, valid, lane_bytes, xr);
   if constexpr (IG)
-    load_rows<T, CPL, R>({a.input_gate, a.input_gate_stride_b, a.input_gate_stride_t, b, at.t1, at.c0},
-                         valid, lane_bytes, ir);
-  load_rows<T, CPL, R>({a.dout, a.dout_stride_b, a.dout_stride_t, b, at.t1, at.c0}, valid, lane_bytes, yr);
+    load_rows<STREAM, T, CPL, R>(
+        {a.input_gate, a.input_gate_stride_b, a.input_gate_stride_t, b, at.t1, c0}, valid, lane_bytes, ir);
+  load_rows<STREAM, T, CPL, R>({a.dout, a.dout_stride_b, a.dout_stride_t, b, at.t1, c0}, valid,
+                                lane_bytes, yr);
   float k[CPL], h[CPL];
   bool slow = true;
 #pragma unroll
@@ -489,9 +500,11 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
     h[i] = (a.saved + (b * p.chunks + chunk) * D + c0)[lane_c + i];
   }
 
-  // Kept per element: a, beta i and w (then m). The gates' other factors are made again from the inputs
-  // in the last walk: keeping them too would leave half of the waves.
+  // Kept per element: a, beta i and w (then m). With two channels a lane the gates' other factors are
+  // made again from the inputs in the last walk: keeping them too would leave half of the waves.
+  constexpr bool kKeep = CPL == 1;
   float f[R][CPL], bi[R][CPL], w[R][CPL];
+  float kr[R][CPL], kn[R][CPL], kx[R][CPL];  // kKeep: r, 1 - r, x (1 - i)
   auto coefficients = [&](auto is_slow) {
     constexpr int kTogether = decltype(is_slow)::value ? 2 : 1;  // rows
     float tail[CPL];
@@ -513,9 +526,21 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
       if constexpr (IG) V::unpack(ir[j], ig);
 #pragma unroll
       for (int i = 0; i < CPL; ++i) {
-        const float in = IG ? sigmoid<T>(ig[i]) : 1.0f;
+        float in = 1.0f, not_in, r;
+        if constexpr (IG && kKeep) {
+          sigmoid_pair<T>(ig[i], in, not_in);
+          kx[j][i] = x[i] * not_in;
+        } else if constexpr (IG) {
+          in = sigmoid<T>(ig[i]);
+        }
         if constexpr (DECAY) {
-          const float l = k[i] * sigmoid<T>(g[i]);
+          if constexpr (kKeep) {
+            sigmoid_pair<T>(g[i], r, kn[j][i]);
+            kr[j][i] = r;
+          } else {
+            r = sigmoid<T>(g[i]);
+          }
+          const float l = k[i] * r;
           f[j][i] = __builtin_amdgcn_exp2f(l);
           const float s = one_minus_square<decltype(is_slow)::value>(tail[i], l, f[j][i]);
           const float inv = __builtin_amdgcn_rsqf(fmaxf(s, kTiny));
@@ -524,6 +549,7 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
         } else {
           float beta;
           sigmoid_pair<T>(g[i], f[j][i], beta);
+          if constexpr (kKeep) kn[j][i] = beta;
           bi[j][i] = beta * in;
           w[j][i] = in * x[i];
         }
@@ -640,7 +666,7 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
     constexpr bool kMasked = decltype(masked)::value;
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      forget_row(xr[j]);
+      if constexpr (!kKeep) forget_row(xr[j]);
       float x[CPL];
       V::unpack(xr[j], x);
 #pragma unroll
@@ -652,10 +678,12 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
 #pragma unroll
     for (int j = R - 1; j >= 0; --j) {
       if (j >= valid) continue;
-      forget_row(xr[j]);
-      forget_row(gr[j]);
-      forget_row(yr[j]);
-      if constexpr (IG) forget_row(ir[j]);
+      if constexpr (!kKeep) {
+        forget_row(xr[j]);
+        forget_row(gr[j]);
+        forget_row(yr[j]);
+        if constexpr (IG) forget_row(ir[j]);
+      }
       const bool pad = kMasked && (rows.pad >> j & 1);
       float y[CPL], x[CPL], g[CPL], ig[CPL], ox[CPL], og[CPL], oi[CPL];
       V::unpack(yr[j], y);
@@ -667,13 +695,16 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
         const float dh = y[i] + cc[i];
         cc[i] = kMasked && (cut >> j & 1) ? 0.0f : f[j][i] * dh;
         ox[i] = dh * bi[j][i];
-        if constexpr (IG) {
+        if constexpr (IG && kKeep) {
+          oi[i] = ox[i] * kx[j][i];
+        } else if constexpr (IG) {
           float in, not_in;
           sigmoid_pair<T>(ig[i], in, not_in);
           oi[i] = ox[i] * (x[i] * not_in);
         }
         float r, not_r;
-        sigmoid_pair<T>(g[i], r, not_r);
+        if constexpr (kKeep) r = kr[j][i], not_r = kn[j][i];
+        else sigmoid_pair<T>(g[i], r, not_r);
         float q = dh * f[j][i] * w[j][i];
         if constexpr (DECAY) {
           q *= kLn2 * k[i] * r;
@@ -682,12 +713,12 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
         og[i] = q * not_r;
         if (pad) ox[i] = og[i] = oi[i] = 0.0f;
       }
-      dx.store(lane_bytes, ox);
-      dg.store(lane_bytes, og);
+      dx.template store<STREAM>(lane_bytes, ox);
+      dg.template store<STREAM>(lane_bytes, og);
       dx.move(-dx.step);
       dg.move(-dg.step);
       if constexpr (IG) {
-        di.store(lane_bytes, oi);
+        di.template store<STREAM>(lane_bytes, oi);
         di.move(-di.step);
       }
     }

@@ -16,24 +16,40 @@ hipError_t rec_launch(RecParams p, bool backward, hipStream_t s) {
   p.cols = (int32_t)((a.dim + kWave * CPL - 1) / (kWave * CPL));
   const dim3 grid((unsigned)(a.batch * p.cols * p.chunks));
   const dim3 block((backward ? kBwdWaves : kFwdWaves) * kWave);
-  auto with = [&](auto decay, auto input_gate, auto seq) {
+  const auto lines = [](const void* at, int64_t stride_b, int64_t stride_t) {
+    return !at || (reinterpret_cast<uintptr_t>(at) % 128 == 0 && stride_b * (int64_t)sizeof(T) % 128 == 0 &&
+                   stride_t * (int64_t)sizeof(T) % 128 == 0);
+  };
+  const int64_t sb = a.seqlen * a.dim;
+  p.stream = a.dim * (int64_t)sizeof(T) % 128 == 0 && lines(a.x, a.x_stride_b, a.x_stride_t) &&
+             lines(a.gate, a.gate_stride_b, a.gate_stride_t) &&
+             lines(a.input_gate, a.input_gate_stride_b, a.input_gate_stride_t) &&
+             (backward ? lines(a.dout, a.dout_stride_b, a.dout_stride_t) && lines(a.dx, sb, a.dim) &&
+                             lines(a.dgate, sb, a.dim) && lines(a.dinput_gate, sb, a.dim)
+                       : lines(a.out, sb, a.dim));
+  auto run = [&](auto decay, auto input_gate, auto seq, auto stream) {
     constexpr bool kDecay = decltype(decay)::value, kGate = decltype(input_gate)::value;
-    constexpr bool kSeq = decltype(seq)::value;
+    constexpr bool kSeq = decltype(seq)::value, kStream = decltype(stream)::value;
     if (backward)
-      rec_bwd_kernel<T, CPL, kDecay, kGate, kSeq, kBwdWaves, kBwdRows><<<grid, block, 0, s>>>(p);
+      rec_bwd_kernel<T, CPL, kDecay, kGate, kSeq, kStream, kBwdWaves, kBwdRows><<<grid, block, 0, s>>>(p);
     else
-      rec_fwd_kernel<T, CPL, kDecay, kGate, kSeq, kFwdWaves, kFwdRows><<<grid, block, 0, s>>>(p);
+      rec_fwd_kernel<T, CPL, kDecay, kGate, kSeq, kStream, kFwdWaves, kFwdRows><<<grid, block, 0, s>>>(p);
   };
-  auto with_gate = [&](auto decay, auto seq) {
-    if (a.input_gate) with(decay, std::true_type{}, seq);
-    else with(decay, std::false_type{}, seq);
+  // A flag at a time becomes a type.
+  auto choose = [](bool flag, auto&& then) {
+    if (flag) then(std::true_type{});
+    else then(std::false_type{});
   };
-  auto with_seq = [&](auto decay) {
-    if (a.seq_idx) with_gate(decay, std::true_type{});
-    else with_gate(decay, std::false_type{});
-  };
-  if (a.decay) with_seq(std::true_type{});
-  else with_seq(std::false_type{});
+  choose(a.decay != nullptr, [&](auto decay) {
+    choose(a.input_gate != nullptr, [&](auto gate) {
+      choose(a.seq_idx != nullptr, [&](auto seq) {
+        if constexpr (CPL * sizeof(T) >= 4)
+          choose(p.stream, [&](auto stream) { run(decay, gate, seq, stream); });
+        else  // a single channel
+          run(decay, gate, seq, std::false_type{});
+      });
+    });
+  });
   return hipGetLastError();
 }
 
