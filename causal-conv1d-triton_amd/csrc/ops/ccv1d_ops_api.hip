@@ -144,9 +144,9 @@ int ccv1d_paged_plan(const struct ccv1d_paged_plan_args* args) {
     return invalid("negative size");
   if (a.page_size < 1) return invalid("page_size must be at least 1");
   if (a.requests >= kMaxGrid || a.max_tokens > kMaxGrid || a.num_free_pages > kMaxGrid ||
-      !product_within(a.max_pages, a.page_size, kMaxGrid))
+      a.page_size > (int64_t(1) << 30) || !product_within(a.max_pages, a.page_size, kMaxGrid))
     return fail(CCV1D_ERR_UNSUPPORTED,
-                "requests, max_tokens and max_pages * page_size must be below 2^31");
+                "requests, max_tokens, page_size and max_pages * page_size too large");
   if (!a.num_free || !a.num_free_out || !a.query_start) return invalid("num_free or query_start is null");
   if (a.requests &&
       (!a.cached_lens || !a.new_lens || !a.seq_lens || (a.max_pages && !a.block_tables)))

@@ -6,69 +6,87 @@ namespace ops {
 
 namespace {
 
-// Joins the spans of a row and query head: 4 waves take the spans in turn, 64 lanes the elements, and
-// the waves' sums meet in LDS. Rows of one span have been written by the main kernel.
+// Joins the spans of a row and query head: the workgroup's waves (kJoinWaves at most, one a span where
+// there are fewer) take the spans in turn, 64 lanes the elements, and the waves' sums meet in LDS.
+// Rows of one span have been written by the main kernel. Bound by its two dependent reads (the length,
+// then maxima and sums together): two rows of 128 spans and 32 heads of 128 take 6 us (4 waves that read
+// the maxima first 17).
+constexpr int kJoinWaves = 16;
+
 template <typename T>
-__global__ __launch_bounds__(256) void paged_join_kernel(AttnParams p) {
+__global__ __launch_bounds__(kJoinWaves * 64) void paged_join_kernel(AttnParams p) {
+  __shared__ float s_sum[kJoinWaves][256], s_total[kJoinWaves];
   const ccv1d_paged_attn_args& a = p.a;
   const int64_t at = blockIdx.x, row = at / a.q_heads;
   int64_t request;
   const Span sp = span_of(p, row, request);
   const int spans = (sp.end - sp.base + p.span - 1) / p.span;
   if (spans <= 1) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, Dh = (int)a.head_dim;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int Dh = (int)a.head_dim;
   const float* ml = p.part_ml + at * p.splits * 2;
   const float* part = p.part + at * p.splits * Dh;
-  float top = kLowest;
-  for (int i = lane; i < spans; i += 64) top = fmaxf(top, ml[2 * i]);
+  float top = kLowest, total = 0.0f, sum[4] = {0, 0, 0, 0};
+  constexpr int kBatch = 8;  // spans of a wave that are requested together, the first before the maxima
+  for (int i0 = wave; i0 < spans; i0 += kBatch * waves) {
+    float v[kBatch][4];
 #pragma unroll
-  for (int o = 32; o; o /= 2) top = fmaxf(top, __shfl_xor(top, o));
-  float total = 0.0f, sum[4] = {0, 0, 0, 0};
-#pragma unroll 4
-  for (int i = wave; i < spans; i += 4) {
-    const float f = __builtin_amdgcn_exp2f(ml[2 * i] - top);
-    total = fmaf(ml[2 * i + 1], f, total);
+    for (int n = 0; n < kBatch; ++n) {
+      const float* from = part + (int64_t)min(i0 + n * waves, spans - 1) * Dh;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (lane + 64 * j < Dh) sum[j] = fmaf(part[(int64_t)i * Dh + lane + 64 * j], f, sum[j]);
+      for (int j = 0; j < 4; ++j) v[n][j] = lane + 64 * j < Dh ? from[lane + 64 * j] : 0.0f;
+    }
+    if (i0 == wave) {
+      for (int i = lane; i < spans; i += 64) top = fmaxf(top, ml[2 * i]);
+#pragma unroll
+      for (int o = 32; o; o /= 2) top = fmaxf(top, __shfl_xor(top, o));
+    }
+#pragma unroll
+    for (int n = 0; n < kBatch; ++n) {
+      const int i = i0 + n * waves;
+      if (i < spans) {
+        const float f = __builtin_amdgcn_exp2f(ml[2 * i] - top);
+        total = fmaf(ml[2 * i + 1], f, total);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] = fmaf(v[n][j], f, sum[j]);
+      }
+    }
   }
-  __shared__ float s_sum[4][256], s_total[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) s_sum[wave][lane + 64 * j] = sum[j];
   if (lane == 0) s_total[wave] = total;
   __syncthreads();
-  total = s_total[0] + s_total[1] + s_total[2] + s_total[3];
-  const int d = threadIdx.x;
-  if (d < Dh) {
-    const float s = s_sum[0][d] + s_sum[1][d] + s_sum[2][d] + s_sum[3][d];
+  total = 0.0f;
+  for (int w = 0; w < waves; ++w) total += s_total[w];
+  for (int d = threadIdx.x; d < Dh; d += blockDim.x) {
+    float s = 0.0f;
+    for (int w = 0; w < waves; ++w) s += s_sum[w][d];
     static_cast<T*>(a.out)[at * Dh + d] = static_cast<T>(total == 0.0f ? 0.0f : s / total);
   }
-  if (a.lse && d == 0) a.lse[at] = (top + __log2f(total)) * 0.69314718055994530942f;
+  if (a.lse && threadIdx.x == 0) a.lse[at] = (top + __log2f(total)) * 0.69314718055994530942f;
 }
 
 AttnParams plan(const ccv1d_paged_attn_args& a) {
   AttnParams p{};
   p.a = a;
-  uint32_t s = 0;
-  while ((int64_t(1) << s) < a.page_size) ++s;
-  p.by_page.shift = 31 + s;
-  p.by_page.magic = (uint32_t)(((uint64_t(1) << p.by_page.shift) + (uint64_t)a.page_size - 1) /
-                               (uint64_t)a.page_size);
+  p.by_page = divisor(a.page_size);
   const int64_t group = a.q_heads / a.kv_heads;
   p.tiles = (int32_t)((group + kAttnHeads - 1) / kAttnHeads);
   int64_t limit = a.max_pages * a.page_size;
   if (a.max_seq_len && a.max_seq_len < limit) limit = a.max_seq_len;
   p.limit = (int32_t)limit;
-  // Spans: as many as fill the card with 1024 workgroups, of at least two steps a wave (256
-  // positions), and of at most 2048 positions, so that one long row beside short ones is spread too;
-  // at most 256 of them.
+  // Spans: as many as make 2048 workgroups, of at least a step of every wave (128 positions) and at most
+  // 1024 positions, so that a long row beside short ones is spread too; at most 256 of them. (64
+  // requests of 512 to 8192 positions, 8 key heads of 128: spans of 2048 293 us, 1024 254, 512 253; two
+  // rows of 131072: 194, 202, 211; 256 rows of 1000 to 3000, heads of 64: 358, 278, 314. 16 rows of a
+  // 1024 window: spans of 256 20.1 us, 128 17.3.)
   int64_t most = a.window && a.window + 31 < limit ? a.window + 31 : limit;
   if (most < 1) most = 1;
   const int64_t wgs = a.rows * a.kv_heads * p.tiles;
-  int64_t splits = (1024 + wgs - 1) / wgs;
+  int64_t splits = (2048 + wgs - 1) / wgs;
   int64_t span = (most + splits - 1) / splits;
-  if (span > 2048) span = 2048;
-  if (span < 256) span = 256;
+  if (span > 1024) span = 1024;
+  if (span < 128) span = 128;
   if (span < (most + 255) / 256) span = (most + 255) / 256;
   span = (span + 127) / 128 * 128;
   p.span = (int32_t)span;
@@ -98,10 +116,11 @@ hipError_t paged_attn(const ccv1d_paged_attn_args& a, hipStream_t s) {
   }
   if (e != hipSuccess || p.splits <= 1) return e;
   const unsigned grid = (unsigned)(a.rows * a.q_heads);
+  const unsigned block = 64 * (p.splits < kJoinWaves ? p.splits : kJoinWaves);
   switch (a.dtype) {
-    case CCV1D_BF16: paged_join_kernel<__bf16><<<grid, 256, 0, s>>>(p); break;
-    case CCV1D_F16: paged_join_kernel<_Float16><<<grid, 256, 0, s>>>(p); break;
-    default: paged_join_kernel<float><<<grid, 256, 0, s>>>(p); break;
+    case CCV1D_BF16: paged_join_kernel<__bf16><<<grid, block, 0, s>>>(p); break;
+    case CCV1D_F16: paged_join_kernel<_Float16><<<grid, block, 0, s>>>(p); break;
+    default: paged_join_kernel<float><<<grid, block, 0, s>>>(p); break;
   }
   return hipGetLastError();
 }

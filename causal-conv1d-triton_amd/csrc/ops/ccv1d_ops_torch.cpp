@@ -80,12 +80,23 @@ at::Tensor unit_last(const at::Tensor& t) {
   return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
 }
 
-at::Tensor as_f32(const at::Tensor& t) {
-  return t.defined() ? t.to(at::kFloat).contiguous() : t;
+// Contiguous and of a type; as it is where it is both (a call into torch costs 0.2 us also then).
+at::Tensor as_type(const at::Tensor& t, at::ScalarType type) {
+  if (!t.defined() || (t.scalar_type() == type && t.is_contiguous())) return t;
+  return t.to(type).contiguous();
 }
 
-at::Tensor as_i32(const at::Tensor& t) {
-  return t.defined() ? t.to(at::kInt).contiguous() : t;
+at::Tensor as_f32(const at::Tensor& t) { return as_type(t, at::kFloat); }
+at::Tensor as_i32(const at::Tensor& t) { return as_type(t, at::kInt); }
+
+// A contiguous tensor in the storage of `base`, from byte `at` on (a multiple of its element's size):
+// several small outputs share one allocation.
+at::Tensor inside(const at::Tensor& base, int64_t at, at::ScalarType type, int64_t n) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(
+      c10::Storage(base.storage()), base.key_set(), c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_storage_offset(at / (int64_t)c10::elementSize(type));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(at::IntArrayRef(&n, 1));
+  return t;
 }
 
 template <typename P = void>
@@ -350,10 +361,17 @@ PyObject* paged_plan(PyObject* const* o) {
         "block_tables must be int32 on the device of cached_lens");
   check(tables.size(1) <= 1 || tables.stride(1) == 1, "rows of block_tables must be contiguous");
   check(R <= 1 || tables.stride(0) >= tables.size(1), "rows of block_tables must not overlap");
-  const auto i32 = cached.options();
-  at::Tensor lens = at::empty({R}, i32), start = at::empty({R + 1}, i32);
-  at::Tensor pos = at::empty({a.max_tokens}, i32), ids = at::empty({a.max_tokens}, i32);
-  at::Tensor slots = at::empty({a.max_tokens}, i32.dtype(at::kLong)), left = at::empty({1}, i32);
+  const int64_t N = a.max_tokens;
+  // slot_mapping first: its elements are 8 bytes
+  const at::Tensor all = at::empty({16 * N + 4 * (R + R + 1 + 1)}, cached.options().dtype(at::kByte));
+  int64_t at = 0;
+  auto next = [&](at::ScalarType type, int64_t n) {
+    at::Tensor t = inside(all, at, type, n);
+    at += n * (int64_t)c10::elementSize(type);
+    return t;
+  };
+  at::Tensor slots = next(at::kLong, N), pos = next(at::kInt, N), ids = next(at::kInt, N);
+  at::Tensor lens = next(at::kInt, R), start = next(at::kInt, R + 1), left = next(at::kInt, 1);
   a.cached_lens = ptr<int32_t>(cached), a.new_lens = ptr<int32_t>(fresh);
   a.block_tables = ptr<int32_t>(tables), a.block_table_stride = tables.stride(0);
   a.free_pages = ptr<int32_t>(free), a.num_free = ptr<int32_t>(num);
@@ -401,7 +419,7 @@ PyObject* paged_cache_write(PyObject* const* o) {
   no_grad_through({&k, &v, &kc, &vc},
                   "paged_cache_write has no backward: call it under torch.no_grad()");
   k = unit_last(k), v = unit_last(v);
-  const at::Tensor s = slots.to(at::kLong).contiguous();
+  const at::Tensor s = as_type(slots, at::kLong);
   a.k = ptr(k), a.k_stride_t = k.stride(0), a.k_stride_h = k.stride(1);
   a.v = ptr(v), a.v_stride_t = v.stride(0), a.v_stride_h = v.stride(1);
   a.k_cache = ptr(kc), a.v_cache = ptr(vc);

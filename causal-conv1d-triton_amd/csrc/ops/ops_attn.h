@@ -42,11 +42,6 @@ constexpr int kAttnWaves = 4;
 constexpr int kAttnHeads = 16;  // query heads of a workgroup
 constexpr float kLowest = -3.402823466e38f;
 
-// x / d for 0 <= x < 2^31.
-struct Divisor {
-  uint32_t magic, shift;
-};
-
 struct AttnParams {
   ccv1d_paged_attn_args a;
   Divisor by_page;
@@ -71,10 +66,6 @@ __device__ __forceinline__ Span span_of(const AttnParams& p, int64_t row, int64_
   if (p.a.window && s.end > p.a.window) s.first = s.end - (int32_t)p.a.window;
   s.base = s.first & ~31;
   return s;
-}
-
-__device__ __forceinline__ uint32_t divide(uint32_t x, Divisor d) {
-  return (uint32_t)(((uint64_t)x * d.magic) >> d.shift);
 }
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -158,7 +149,7 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
 enum PageMode : int { kPageStep = 0, kPageFour = 1, kPageAny = 2 };
 
 template <typename T, int DH, int MODE>
-__global__ __launch_bounds__(kAttnWaves* kWave, sizeof(T) * DH > 512 ? 1 : 2) void paged_attn_kernel(
+__global__ __launch_bounds__(kAttnWaves* kWave, sizeof(T) * DH > 768 ? 1 : 2) void paged_attn_kernel(
     AttnParams p) {
   using St = Step<T>;
   using Pc = Pieces<T, DH>;
@@ -171,11 +162,18 @@ __global__ __launch_bounds__(kAttnWaves* kWave, sizeof(T) * DH > 512 ? 1 : 2) vo
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int Dh = (int)a.head_dim, group = (int)(a.q_heads / a.kv_heads);
-  int64_t id = blockIdx.x;
+  // Workgroups go to the 8 XCDs in turn: ids are dealt anew so that the key heads of one span, whose rows
+  // lie side by side in memory, share an XCD's L2 at the same time (256 rows of 1000 to 3000 positions,
+  // heads of 64: 278 -> 246 us). The spans move on by one XCD from 8 to 8, or with 8 spans a row one XCD
+  // would get all the last ones, which short rows do not have.
+  uint32_t id = blockIdx.x;
+  const uint32_t together = (uint32_t)(a.kv_heads * p.tiles), block = 8 * together;
+  const uint32_t in = id % block, start = id - in;
+  if (start + block <= gridDim.x) id = start + (in + start / block) % 8 * together + in / 8;
   const int tile = (int)(id % p.tiles);
   id /= p.tiles;
-  const int64_t kvh = id % a.kv_heads;
-  id /= a.kv_heads;
+  const int64_t kvh = id % (uint32_t)a.kv_heads;
+  id /= (uint32_t)a.kv_heads;
   const int split = (int)(id % p.splits);
   const int64_t row = id / p.splits;
 
@@ -280,17 +278,23 @@ __global__ __launch_bounds__(kAttnWaves* kWave, sizeof(T) * DH > 512 ? 1 : 2) vo
       for (int t = 0; t < kTiles; ++t) load_words<4>(kp[t] + (d < Dh ? d : 0), kw[t][c]);
     }
     uint32_t vw[kMine][kVW];
+    auto load_values = [&]() {
 #pragma unroll
-    for (int e = 0; e < kMine; ++e)
+      for (int e = 0; e < kMine; ++e)
 #pragma unroll
-      for (int k = 0; k < Pc::kCount; ++k) {
-        constexpr int kPer = St::kPer;
-        const int d = 16 * Pc::before(k) + n * Pc::width(k);
-        const T* v = vp[e] + (d < Dh ? d : 0);
-        if (Pc::width(k) / kPer == 4) load_words<4>(v, &vw[e][Pc::before(k) / kPer]);
-        else if (Pc::width(k) / kPer == 2) load_words<2>(v, &vw[e][Pc::before(k) / kPer]);
-        else load_words<1>(v, &vw[e][Pc::before(k) / kPer]);
-      }
+        for (int k = 0; k < Pc::kCount; ++k) {
+          constexpr int kPer = St::kPer;
+          const int d = 16 * Pc::before(k) + n * Pc::width(k);
+          const T* v = vp[e] + (d < Dh ? d : 0);
+          if (Pc::width(k) / kPer == 4) load_words<4>(v, &vw[e][Pc::before(k) / kPer]);
+          else if (Pc::width(k) / kPer == 2) load_words<2>(v, &vw[e][Pc::before(k) / kPer]);
+          else load_words<1>(v, &vw[e][Pc::before(k) / kPer]);
+        }
+    };
+    // Requested with the keys, except where the registers of both would leave one wave per SIMD (heads
+    // of 256, 64 rows of 512 to 4096 positions: 119 us so, 92 with the values requested after the scores).
+    constexpr bool kLate = DH == 256 || (sizeof(T) == 4 && DH > 128);
+    if constexpr (!kLate) load_values();
 
     // Scores.
     float x[kMine];
@@ -308,6 +312,10 @@ __global__ __launch_bounds__(kAttnWaves* kWave, sizeof(T) * DH > 512 ? 1 : 2) vo
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[4 * t + i] = s[i] * to2;
+    }
+    if constexpr (kLate) {
+      __builtin_amdgcn_sched_barrier(0);
+      load_values();
     }
     if (!whole) {
 #pragma unroll

@@ -22,6 +22,23 @@ __device__ __forceinline__ float to_f32(T v) {
   return static_cast<float>(v);
 }
 
+// x / d for 0 <= x < 2^31 and 1 <= d < 2^31 as a product: with magic = 2^(31 + s) / d rounded up, 2^s the
+// power of two from d on, the excess is below d <= 2^s and stays below 2^(31 + s) times any x.
+struct Divisor {
+  uint32_t magic, shift;
+};
+
+inline Divisor divisor(int64_t d) {
+  uint32_t s = 0;
+  while ((int64_t(1) << s) < d) ++s;
+  const uint64_t one = uint64_t(1) << (31 + s);
+  return {(uint32_t)((one + (uint64_t)d - 1) / (uint64_t)d), 31 + s};
+}
+
+__device__ __forceinline__ uint32_t divide(uint32_t x, Divisor d) {
+  return (uint32_t)(((uint64_t)x * d.magic) >> d.shift);
+}
+
 // Launchers (arguments checked, device current).
 hipError_t rec_fwd(const ccv1d_rec_args& a, hipStream_t s);
 hipError_t rec_bwd(const ccv1d_rec_args& a, hipStream_t s);
