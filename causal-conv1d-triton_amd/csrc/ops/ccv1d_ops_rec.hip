@@ -52,32 +52,71 @@ __global__ __launch_bounds__(1024) void rec_reduce_kernel(const float* part, int
   }
 }
 
-template <typename T, bool DECAY>
+// One token of a request: CPL channels a lane, the last lane of a row those that are left. Bound by
+// latency for a small batch (16 rows of 2048 channels: 3 us), by memory for a large one.
+template <typename T, bool DECAY, int CPL>
 __global__ __launch_bounds__(64) void rec_update_kernel(ccv1d_rec_update_args p) {
-  const int64_t nc = (p.dim + 63) / 64;
-  const int64_t row = blockIdx.x / nc, d = (blockIdx.x % nc) * 64 + threadIdx.x;
+  using V = VecIO<T, CPL>;
+  using S = VecIO<float, CPL>;
+  const uint32_t cols = (uint32_t)((p.dim + 64 * CPL - 1) / (64 * CPL));
+  const int64_t row = blockIdx.x / cols;
+  const int64_t d = ((int64_t)(blockIdx.x % cols) * 64 + threadIdx.x) * CPL;
   if (d >= p.dim) return;
+  const int n = (int)min((int64_t)CPL, p.dim - d);
   const int64_t slot = p.state_indices ? p.state_indices[row] : row;
-  float h = 0.0f;
-  if (slot >= 0 && slot < p.slots) {
-    float a, beta;
-    const float k = DECAY ? decay_rate(p.decay[d], p.decay_scale) : 0.0f;
-    forget<T, DECAY, false>(k, sinh_tail(k), to_f32(static_cast<const T*>(p.gate)[row * p.gate_stride + d]), a, beta);
-    float u = beta * to_f32(static_cast<const T*>(p.x)[row * p.x_stride + d]);
-    if (p.input_gate)
-      u *= sigmoid<T>(to_f32(static_cast<const T*>(p.input_gate)[row * p.input_gate_stride + d]));
-    float* st = p.state + slot * p.state_stride + d;
-    h = fmaf(a, *st, u);
-    *st = h;
+  T* out = static_cast<T*>(p.out) + row * p.dim + d;
+  const bool in = slot >= 0 && slot < p.slots;
+  const T* xp = static_cast<const T*>(p.x) + row * p.x_stride + d;
+  const T* gp = static_cast<const T*>(p.gate) + row * p.gate_stride + d;
+  const T* ip = static_cast<const T*>(p.input_gate) + row * p.input_gate_stride + d;
+  float* sp = p.state + (in ? slot : 0) * p.state_stride + d;
+  float x[CPL] = {}, g[CPL] = {}, ig[CPL] = {}, h[CPL] = {}, decay[CPL] = {};
+  if (in) {
+    if (n == CPL) {
+      V::unpack(V::ld(xp), x);
+      V::unpack(V::ld(gp), g);
+      if (p.input_gate) V::unpack(V::ld(ip), ig);
+      S::unpack(S::ld(sp), h);
+      if constexpr (DECAY) S::unpack(S::ld(p.decay + d), decay);
+    } else {
+#pragma unroll
+      for (int i = 0; i < CPL; ++i)
+        if (i < n) {
+          x[i] = to_f32(xp[i]);
+          g[i] = to_f32(gp[i]);
+          if (p.input_gate) ig[i] = to_f32(ip[i]);
+          h[i] = sp[i];
+          if constexpr (DECAY) decay[i] = p.decay[d + i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < CPL; ++i) {
+      float a, beta;
+      const float k = DECAY ? decay_rate(decay[i], p.decay_scale) : 0.0f;
+      forget<T, DECAY, false>(k, sinh_tail(k), g[i], a, beta);
+      float u = beta * x[i];
+      if (p.input_gate) u *= sigmoid<T>(ig[i]);
+      h[i] = fmaf(a, h[i], u);
+    }
   }
-  static_cast<T*>(p.out)[row * p.dim + d] = static_cast<T>(h);
+  if (n == CPL) {
+    if (in) S::st(sp, S::pack(h));
+    V::st(out, V::pack(h));
+  } else {
+#pragma unroll
+    for (int i = 0; i < CPL; ++i)
+      if (i < n) {
+        if (in) sp[i] = h[i];
+        out[i] = to_store<T>(h[i]);
+      }
+  }
 }
 
-template <typename T>
+template <typename T, int CPL>
 hipError_t update_t(const ccv1d_rec_update_args& a, hipStream_t s) {
-  const dim3 grid((unsigned)(a.rows * ((a.dim + 63) / 64)));
-  if (a.decay) rec_update_kernel<T, true><<<grid, 64, 0, s>>>(a);
-  else rec_update_kernel<T, false><<<grid, 64, 0, s>>>(a);
+  const dim3 grid((unsigned)(a.rows * ((a.dim + 64 * CPL - 1) / (64 * CPL))));
+  if (a.decay) rec_update_kernel<T, true, CPL><<<grid, 64, 0, s>>>(a);
+  else rec_update_kernel<T, false, CPL><<<grid, 64, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -144,11 +183,17 @@ size_t rec_workspace(int64_t B, int64_t T, int64_t D, bool backward) {
 hipError_t rec_fwd(const ccv1d_rec_args& a, hipStream_t s) { return run(a, false, s); }
 hipError_t rec_bwd(const ccv1d_rec_args& a, hipStream_t s) { return run(a, true, s); }
 
+// Four channels a lane from 2^17 channels on, where that still leaves a wave for every CU and half.
+template <typename T>
+hipError_t update_wide(const ccv1d_rec_update_args& a, hipStream_t s) {
+  return a.rows * a.dim >= (1 << 17) ? update_t<T, 4>(a, s) : update_t<T, 1>(a, s);
+}
+
 hipError_t rec_update(const ccv1d_rec_update_args& a, hipStream_t s) {
   switch (a.dtype) {
-    case CCV1D_BF16: return update_t<__bf16>(a, s);
-    case CCV1D_F16: return update_t<_Float16>(a, s);
-    default: return update_t<float>(a, s);
+    case CCV1D_BF16: return update_wide<__bf16>(a, s);
+    case CCV1D_F16: return update_wide<_Float16>(a, s);
+    default: return update_wide<float>(a, s);
   }
 }
 
