@@ -133,7 +133,7 @@ def gated_recurrence_fn(
     if torch.compiler.is_compiling():
         out, final, _ = _fwd_op(x, gate, decay, input_gate, seq_idx, initial_states, decay_scale)
     elif torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad
+            getattr(t, "requires_grad", False)
             for t in (x, gate, decay, input_gate, initial_states)):
         out, final = _GatedRecurrenceFn.apply(x, gate, decay, input_gate, seq_idx, initial_states,
                                               return_final_states, decay_scale)

@@ -54,6 +54,7 @@ int check_rec(const ccv1d_rec_args* a, bool backward) {
   if (!a) return invalid("args is null");
   if (a->batch < 0 || a->seqlen < 0 || a->dim < 0) return invalid("negative size");
   if (!dtype_ok(a->dtype)) return invalid("dtype must be fp32, fp16 or bf16");
+  if (!(a->decay_scale >= 0.0f)) return invalid("decay_scale must not be negative");
   // Rows, row offsets and workgroup numbers are 32-bit, the product of all three 64-bit.
   if (a->seqlen > kMaxGrid || a->dim > kMaxGrid ||
       !product_within(a->batch, cdiv(a->dim, 64), kMaxGrid) ||
@@ -127,6 +128,7 @@ int ccv1d_rec_update(const struct ccv1d_rec_update_args* args) {
   const ccv1d_rec_update_args& a = *args;
   if (a.rows < 0 || a.slots < 0 || a.dim < 0) return invalid("negative size");
   if (!dtype_ok(a.dtype)) return invalid("dtype must be fp32, fp16 or bf16");
+  if (!(a.decay_scale >= 0.0f)) return invalid("decay_scale must not be negative");
   if (!a.state_indices && a.rows > a.slots) return invalid("more rows than slots");
   if (!product_within(a.rows, cdiv(a.dim, 64), kMaxGrid))
     return fail(CCV1D_ERR_UNSUPPORTED, "rows and dim too large for one launch");
