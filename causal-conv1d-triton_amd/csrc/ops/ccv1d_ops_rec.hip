@@ -126,7 +126,7 @@ unsigned fill_blocks(int64_t n) {
 }
 
 struct Plan {
-  int64_t chunks, groups, words, part;  // words of 8 bytes, cleared; floats after them
+  int64_t chunks, groups, tickets, words, part;  // words of 8 bytes, cleared; floats after them
 };
 
 Plan plan_of(int64_t B, int64_t T, int64_t D, bool backward) {
@@ -134,7 +134,9 @@ Plan plan_of(int64_t B, int64_t T, int64_t D, bool backward) {
   const int64_t rows = backward ? kBwdWaves * kBwdRows : kFwdWaves * kFwdRows;
   p.chunks = (T + rows - 1) / rows;
   p.groups = (p.chunks + kRecGroup - 1) / kRecGroup;
-  p.words = p.chunks > 1 ? B * D * (p.chunks + p.groups) + 1 : 0;  // and the ticket
+  // and a ticket of 4 bytes per wave column, of 64 channels at the least
+  p.tickets = B * ((D + kWave - 1) / kWave);
+  p.words = p.chunks > 1 ? B * D * (p.chunks + p.groups) + (p.tickets + 1) / 2 : 0;
   p.part = backward ? B * D * p.chunks : 0;
   return p;
 }
@@ -157,7 +159,7 @@ hipError_t run(const ccv1d_rec_args& a, bool backward, hipStream_t s) {
   p.part = reinterpret_cast<float*>(p.pairs + pl.words);
   if (pl.words) {
     p.states = p.pairs + a.batch * a.dim * pl.chunks;
-    p.ticket = reinterpret_cast<uint32_t*>(p.pairs + pl.words - 1);
+    p.tickets = reinterpret_cast<uint32_t*>(p.states + a.batch * a.dim * pl.groups);
     rec_clear_kernel<<<fill_blocks(pl.words), 256, 0, s>>>(p.pairs, pl.words);
     if (hipError_t err = hipGetLastError(); err != hipSuccess) return err;
   }

@@ -14,10 +14,11 @@
 //     most kRecGroup - 1, and combines them in order, so results do not depend on timing.
 // A word holds its own ready mark (the sign bit of A, which is never negative; the workspace is
 // cleared before), so an atomic load of 64 bits that shows the mark shows the whole word, and no fence
-// or flag is needed across the caches of the XCDs. Chunks are dealt by a ticket in order of time
-// (backward: from the end), not by workgroup number: a chunk waits only for words of chunks with lower
-// tickets, whose workgroups have therefore started, and these publish their pairs before they wait for
-// anything. The one wait on a wait is the state after a group, and by induction over tickets that ends too.
+// or flag is needed across the caches of the XCDs. The chunks of a wave column are dealt by a ticket in
+// order of time (backward: from the end), not by workgroup number: a chunk waits only for words of chunks
+// with lower tickets, whose workgroups have therefore started, and these publish their pairs before they
+// wait for anything. The one wait on a wait is the state after a group, and by induction over tickets
+// that ends too.
 //
 // A sequence's first row and padding cut the state: the row's factor is no number times zero but a
 // branch (an infinity of one sequence never meets the next), and A = 0 says that a stretch contains
@@ -47,7 +48,7 @@ struct RecParams {
   int32_t cols, chunks, groups;  // wave columns of 64 * CPL channels; chunks along time; their groups
   uint64_t* pairs;               // (batch, chunks, dim)
   uint64_t* states;              // (batch, groups, dim): word of the state after a group
-  uint32_t* ticket;
+  uint32_t* tickets;             // (batch * cols,): the next chunk of each wave column
   float* part;  // backward: (batch, chunks, dim) sums behind ddecay
   // Rows whose starts and ends lie on the 128-byte lines are read and written once and kept out of the
   // caches' way (forward and backward at B=4 T=8192 D=1024 bf16: 219 us with cached accesses, 213 with
@@ -169,18 +170,22 @@ __device__ __forceinline__ void forget_row(RAW& v) {
   }
 }
 
-// Deals a chunk to this workgroup: (batch row and wave column, chunk from the walk's start).
+// Deals a chunk to this workgroup: (batch row and wave column, chunk from the walk's start). A column's
+// chunks have a counter of their own: with one for all, the 512 workgroups that start together waited in
+// line for it (forward of B=16 T=256 D=2048 25 us, 18 so). Workgroups go to the 8 XCDs in turn; columns
+// move on by one from n to n workgroups, or with n a multiple of 8 an XCD would have the same columns
+// for good, and with rows of a power of two the same part of the memory's channels (forward and backward
+// at B=4 T=8192 D=1024 219 us, 198 so).
 __device__ __forceinline__ void deal(const RecParams& p, int& bc, int& chunk, uint32_t* s_ticket) {
   const uint32_t n = (uint32_t)(p.a.batch * p.cols);
-  uint32_t k = blockIdx.x;
+  bc = (int)((blockIdx.x % n + blockIdx.x / n) % n);
+  chunk = 0;
   if (p.chunks > 1) {
     if (threadIdx.x == 0)
-      *s_ticket = __hip_atomic_fetch_add(p.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      *s_ticket = __hip_atomic_fetch_add(p.tickets + bc, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    k = __builtin_amdgcn_readfirstlane(*s_ticket);
+    chunk = (int)__builtin_amdgcn_readfirstlane(*s_ticket);
   }
-  chunk = (int)(k / n);
-  bc = (int)(k % n);
 }
 
 // The pairs of the waves of a workgroup, and of the chunks before it, in LDS.

@@ -115,12 +115,13 @@ def test_rec_workspace(lib):
     ws = lib.ccv1d_rec_workspace_bytes
     assert ws(0, 10, 8, 0) == ws(1, 0, 8, 1) == ws(1, 10, 0, 1) == 0
     assert ws(3, 128, 70, 0) == 0  # one chunk: nothing to hand on
-    # beyond one chunk: a word per channel and chunk, one per channel and group, and the ticket
-    assert ws(2, 129, 70, 0) == 8 * (2 * 70 * (2 + 1) + 1)
+    # beyond one chunk: a word per channel and chunk, one per channel and group, and half a word, rounded
+    # up, per 64 channels of a batch row
+    assert ws(2, 129, 70, 0) == 8 * (2 * 70 * (2 + 1) + 2)
     assert ws(1, 128 * 17, 5, 0) == 8 * (5 * (17 + 2) + 1)
     # the backward's chunks are half as long, with a sum per channel and chunk
     assert ws(3, 64, 70, 1) == 4 * 3 * 70
-    assert ws(2, 65, 70, 1) == 8 * (2 * 70 * (2 + 1) + 1) + 4 * 2 * 70 * 2
+    assert ws(2, 65, 70, 1) == 8 * (2 * 70 * (2 + 1) + 2) + 4 * 2 * 70 * 2
 
 
 def update(**kw):
