@@ -175,10 +175,12 @@ __device__ __forceinline__ void forget_row(RAW& v) {
 // line for it (forward of B=16 T=256 D=2048 25 us, 18 so). Workgroups go to the 8 XCDs in turn; columns
 // move on by one from n to n workgroups, or with n a multiple of 8 an XCD would have the same columns
 // for good, and with rows of a power of two the same part of the memory's channels (forward and backward
-// at B=4 T=8192 D=1024 219 us, 198 so).
+// at B=4 T=8192 D=1024 219 us, 198 so). Where rows are not on cache lines, an XCD takes columns side by
+// side, whose lines overlap (B=3 T=5001 D=1501 fp32 273 us, 248 so; rows on lines 1 % slower).
 __device__ __forceinline__ void deal(const RecParams& p, int& bc, int& chunk, uint32_t* s_ticket) {
   const uint32_t n = (uint32_t)(p.a.batch * p.cols);
-  bc = (int)((blockIdx.x % n + blockIdx.x / n) % n);
+  const uint32_t i = blockIdx.x % n, at = p.stream ? i : (uint32_t)xcd_remap((int)i, (int)n);
+  bc = (int)((at + blockIdx.x / n) % n);
   chunk = 0;
   if (p.chunks > 1) {
     if (threadIdx.x == 0)
@@ -662,7 +664,10 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
 
   float sum[CPL];
 #pragma unroll
-  for (int i = 0; i < CPL; ++i) sum[i] = 0.0f;
+  for (int i = 0; i < CPL; ++i) {
+    sum[i] = 0.0f;
+    if constexpr (DECAY) k[i] *= kLn2;  // ln a = k r from here on
+  }
   const int64_t last = t0 + valid - 1;  // stored from the last row back
   RowWalk<T, CPL> dx(a.dx, T_ * D, D, b, last, at.c0), dg(a.dgate, T_ * D, D, b, last, at.c0);
   RowWalk<T, CPL> di(a.dinput_gate, T_ * D, D, b, last, at.c0);
@@ -704,15 +709,15 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
           oi[i] = ox[i] * kx[j][i];
         } else if constexpr (IG) {
           float in, not_in;
-          sigmoid_pair<T>(ig[i], in, not_in);
+          sigmoid_pair_of_number<T>(ig[i], in, not_in);
           oi[i] = ox[i] * (x[i] * not_in);
         }
         float r, not_r;
         if constexpr (kKeep) r = kr[j][i], not_r = kn[j][i];
-        else sigmoid_pair<T>(g[i], r, not_r);
+        else sigmoid_pair_of_number<T>(g[i], r, not_r);
         float q = dh * f[j][i] * w[j][i];
         if constexpr (DECAY) {
-          q *= kLn2 * k[i] * r;
+          q *= k[i] * r;
           sum[i] += pad ? 0.0f : q;
         }
         og[i] = q * not_r;

@@ -39,6 +39,15 @@ __device__ __forceinline__ void sigmoid_pair(float z, float& s, float& rest) {
   rest = e * s;
 }
 
+// The same where a NaN need not pass (a factor beside it carries it): one operation less in 16 bits.
+template <typename T>
+__device__ __forceinline__ void sigmoid_pair_of_number(float z, float& s, float& rest) {
+  if constexpr (sizeof(T) == 4) return sigmoid_pair<T>(z, s, rest);
+  const float e = __builtin_amdgcn_exp2f(fminf(-kLog2e * z, 126.0f));
+  s = __builtin_amdgcn_rcpf(1.0f + e);
+  rest = e * s;
+}
+
 // sigmoid(z) alone, where 2^t may pass the largest number and the result reach zero.
 template <typename T>
 __device__ __forceinline__ float sigmoid(float z) {
