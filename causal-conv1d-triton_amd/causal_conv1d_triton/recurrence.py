@@ -90,10 +90,11 @@ class _GatedRecurrenceFn(torch.autograd.Function):
         return out, final
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dout, dfinal):
         x, gate, decay, input_gate, seq_idx, init, saved = ctx.saved_tensors
         if dout is None:
-            dout = torch.zeros(1, 1, 1, device=x.device, dtype=x.dtype).expand(x.shape).contiguous()
+            dout = torch.zeros(x.shape, device=x.device, dtype=x.dtype)
         need = init is not None and ctx.needs_input_grad[5]
         dx, dgate, ddecay, dig, dinit = native().rec_bwd(
             x, gate, decay, input_gate, seq_idx, init, ctx.decay_scale, saved, dout, dfinal, need)

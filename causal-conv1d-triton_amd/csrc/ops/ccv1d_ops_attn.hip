@@ -115,14 +115,13 @@ hipError_t paged_attn(const ccv1d_paged_attn_args& a, hipStream_t s) {
     default: e = paged_attn_f32(p, mode, s); break;
   }
   if (e != hipSuccess || p.splits <= 1) return e;
-  const unsigned grid = (unsigned)(a.rows * a.q_heads);
-  const unsigned block = 64 * (p.splits < kJoinWaves ? p.splits : kJoinWaves);
+  const int64_t grid = a.rows * a.q_heads;
+  const int block = 64 * (p.splits < kJoinWaves ? p.splits : kJoinWaves);
   switch (a.dtype) {
-    case CCV1D_BF16: paged_join_kernel<__bf16><<<grid, block, 0, s>>>(p); break;
-    case CCV1D_F16: paged_join_kernel<_Float16><<<grid, block, 0, s>>>(p); break;
-    default: paged_join_kernel<float><<<grid, block, 0, s>>>(p); break;
+    case CCV1D_BF16: return start(&paged_join_kernel<__bf16>, grid, block, s, p);
+    case CCV1D_F16: return start(&paged_join_kernel<_Float16>, grid, block, s, p);
+    default: return start(&paged_join_kernel<float>, grid, block, s, p);
   }
-  return hipGetLastError();
 }
 
 }  // namespace ops

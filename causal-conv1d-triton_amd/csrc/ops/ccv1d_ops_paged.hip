@@ -200,17 +200,15 @@ hipError_t write_as(const ccv1d_paged_write_args& a, hipStream_t s) {
   const int64_t pieces = 2 * a.kv_heads * per_head;
   // Small tokens share a workgroup, two pieces a lane.
   const int tokens = pieces < 2 * kWriteThreads ? (int)(2 * kWriteThreads / pieces) : 1;
-  const unsigned grid = (unsigned)((a.tokens + tokens - 1) / tokens);
-  paged_write_kernel<V><<<grid, kWriteThreads, 0, s>>>(a, per_head, tokens);
-  return hipGetLastError();
+  return start(&paged_write_kernel<V>, (a.tokens + tokens - 1) / tokens, kWriteThreads, s, a, per_head,
+               tokens);
 }
 
 }  // namespace
 
 hipError_t paged_plan(const ccv1d_paged_plan_args& a, hipStream_t s) {
   const int64_t blocks = (a.max_tokens + kPlanTokens - 1) / kPlanTokens;
-  paged_plan_kernel<<<(unsigned)(blocks > 0 ? blocks : 1), kPlanThreads, 0, s>>>(a, divisor(a.page_size));
-  return hipGetLastError();
+  return start(&paged_plan_kernel, blocks > 0 ? blocks : 1, kPlanThreads, s, a, divisor(a.page_size));
 }
 
 hipError_t paged_write(const ccv1d_paged_write_args& a, hipStream_t s) {

@@ -114,15 +114,14 @@ __global__ __launch_bounds__(64) void rec_update_kernel(ccv1d_rec_update_args p)
 
 template <typename T, int CPL>
 hipError_t update_t(const ccv1d_rec_update_args& a, hipStream_t s) {
-  const dim3 grid((unsigned)(a.rows * ((a.dim + 64 * CPL - 1) / (64 * CPL))));
-  if (a.decay) rec_update_kernel<T, true, CPL><<<grid, 64, 0, s>>>(a);
-  else rec_update_kernel<T, false, CPL><<<grid, 64, 0, s>>>(a);
-  return hipGetLastError();
+  const int64_t grid = a.rows * ((a.dim + 64 * CPL - 1) / (64 * CPL));
+  return a.decay ? start(&rec_update_kernel<T, true, CPL>, grid, 64, s, a)
+                 : start(&rec_update_kernel<T, false, CPL>, grid, 64, s, a);
 }
 
-unsigned fill_blocks(int64_t n) {
+int64_t fill_blocks(int64_t n) {
   const int64_t b = (n + 1023) / 1024;
-  return (unsigned)(b < 1 ? 1 : b > 2048 ? 2048 : b);
+  return b < 1 ? 1 : b > 2048 ? 2048 : b;
 }
 
 struct Plan {
@@ -147,8 +146,8 @@ hipError_t run(const ccv1d_rec_args& a, bool backward, hipStream_t s) {
     const float* from = backward ? a.dfinal_states : a.initial_states;
     float* to = backward ? a.dinitial_states : a.final_states;
     float* zero = backward ? a.ddecay : nullptr;
-    if (to || zero) rec_empty_kernel<<<fill_blocks(n), 256, 0, s>>>(from, to, n, zero, a.dim);
-    return hipGetLastError();
+    if (!to && !zero) return hipSuccess;
+    return start(&rec_empty_kernel, fill_blocks(n), 256, s, from, to, n, zero, a.dim);
   }
   const Plan pl = plan_of(a.batch, a.seqlen, a.dim, backward);
   RecParams p{};
@@ -160,8 +159,8 @@ hipError_t run(const ccv1d_rec_args& a, bool backward, hipStream_t s) {
   if (pl.words) {
     p.states = p.pairs + a.batch * a.dim * pl.chunks;
     p.tickets = reinterpret_cast<uint32_t*>(p.states + a.batch * a.dim * pl.groups);
-    rec_clear_kernel<<<fill_blocks(pl.words), 256, 0, s>>>(p.pairs, pl.words);
-    if (hipError_t err = hipGetLastError(); err != hipSuccess) return err;
+    const hipError_t err = start(&rec_clear_kernel, fill_blocks(pl.words), 256, s, p.pairs, pl.words);
+    if (err != hipSuccess) return err;
   }
   hipError_t e;
   switch (a.dtype) {
@@ -170,9 +169,8 @@ hipError_t run(const ccv1d_rec_args& a, bool backward, hipStream_t s) {
     default: e = rec_launch_f32(p, backward, s); break;
   }
   if (e != hipSuccess || !backward || !a.decay) return e;
-  rec_reduce_kernel<<<(unsigned)((a.dim + 31) / 32), 1024, 0, s>>>(p.part, a.batch * pl.chunks, a.dim,
-                                                                   a.decay, a.ddecay);
-  return hipGetLastError();
+  return start(&rec_reduce_kernel, (a.dim + 31) / 32, 1024, s, (const float*)p.part, a.batch * pl.chunks,
+               a.dim, a.decay, a.ddecay);
 }
 
 }  // namespace

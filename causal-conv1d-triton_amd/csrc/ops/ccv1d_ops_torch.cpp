@@ -89,6 +89,18 @@ at::Tensor as_type(const at::Tensor& t, at::ScalarType type) {
 at::Tensor as_f32(const at::Tensor& t) { return as_type(t, at::kFloat); }
 at::Tensor as_i32(const at::Tensor& t) { return as_type(t, at::kInt); }
 
+// Whole numbers as int32; 64-bit ones outside its range stay outside any index or length.
+at::Tensor as_index(const at::Tensor& t) {
+  if (t.defined() && t.scalar_type() == at::kLong)
+    return t.clamp(INT32_MIN, INT32_MAX).to(at::kInt).contiguous();
+  return as_i32(t);
+}
+
+// Tells autograd that a tensor was written to.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // A contiguous tensor in the storage of `base`, from byte `at` on (a multiple of its element's size):
 // several small outputs share one allocation.
 at::Tensor inside(const at::Tensor& base, int64_t at, at::ScalarType type, int64_t n) {
@@ -309,7 +321,7 @@ PyObject* rec_update(PyObject* const* o) {
         "gate and input_gate must have the dtype of x");
   no_grad_through({&x, &gate, &decay, &igate, &state},
                   "gated_recurrence_update has no backward: call it under torch.no_grad()");
-  x = unit_last(x), gate = unit_last(gate), decay = as_f32(decay), idx = as_i32(idx);
+  x = unit_last(x), gate = unit_last(gate), decay = as_f32(decay), idx = as_index(idx);
   if (igate.defined()) {
     igate = unit_last(igate);
     a.input_gate = ptr(igate), a.input_gate_stride = igate.stride(0);
@@ -322,6 +334,7 @@ PyObject* rec_update(PyObject* const* o) {
   a.out = ptr(out);
   a.device = (int)dev, a.stream = stream_of(dev);
   call(ccv1d_rec_update, a);
+  written(state);
   return tuple_of({out});
 }
 
@@ -381,6 +394,7 @@ PyObject* paged_plan(PyObject* const* o) {
   a.slot_mapping = ptr<int64_t>(slots), a.num_free_out = ptr<int32_t>(left);
   a.device = (int)dev, a.stream = stream_of(dev);
   call(ccv1d_paged_plan, a);
+  written(tables);
   return tuple_of({lens, start, pos, ids, slots, left});
 }
 
@@ -428,6 +442,8 @@ PyObject* paged_cache_write(PyObject* const* o) {
   a.slot_mapping = ptr<int64_t>(s);
   a.device = (int)dev, a.stream = stream_of(dev);
   call(ccv1d_paged_write, a);
+  written(kc);
+  written(vc);
   Py_RETURN_NONE;
 }
 
@@ -475,7 +491,7 @@ PyObject* paged_attention(PyObject* const* o) {
         "the caches must have the dtype of q");
   no_grad_through({&q, &kc, &vc}, "paged_attention has no backward: call it under torch.no_grad()");
   a.scale = o[6] == Py_None ? 1.0f / std::sqrt((float)a.head_dim) : (float)number(o[6]);
-  q = unit_last(q), lens = as_i32(lens), ids = as_i32(ids);
+  q = unit_last(q), lens = as_index(lens), ids = as_index(ids);
   at::Tensor out = at::empty({a.rows, a.q_heads, a.head_dim}, q.options());
   at::Tensor lse = truth(o[9]) ? at::empty({a.rows, a.q_heads}, q.options().dtype(at::kFloat))
                                : at::Tensor();

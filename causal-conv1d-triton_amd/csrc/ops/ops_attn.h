@@ -422,13 +422,13 @@ hipError_t paged_attn_f32(const AttnParams& p, int mode, hipStream_t s);
 
 template <typename T, int DH>
 hipError_t paged_attn_mode(const AttnParams& p, int mode, hipStream_t s) {
-  const dim3 grid((unsigned)(p.a.rows * p.splits * p.a.kv_heads * p.tiles)), block(kAttnWaves * kWave);
+  const int64_t grid = p.a.rows * p.splits * p.a.kv_heads * p.tiles;
+  constexpr int kBlock = kAttnWaves * kWave;
   switch (mode) {
-    case kPageStep: paged_attn_kernel<T, DH, kPageStep><<<grid, block, 0, s>>>(p); break;
-    case kPageFour: paged_attn_kernel<T, DH, kPageFour><<<grid, block, 0, s>>>(p); break;
-    default: paged_attn_kernel<T, DH, kPageAny><<<grid, block, 0, s>>>(p); break;
+    case kPageStep: return start(&paged_attn_kernel<T, DH, kPageStep>, grid, kBlock, s, p);
+    case kPageFour: return start(&paged_attn_kernel<T, DH, kPageFour>, grid, kBlock, s, p);
+    default: return start(&paged_attn_kernel<T, DH, kPageAny>, grid, kBlock, s, p);
   }
-  return hipGetLastError();
 }
 
 // The kernels' row sizes: a head_dim takes the next one.

@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <tuple>
+
 #include "ccv1d_ops.h"
 
 namespace ccv1d {
@@ -37,6 +39,19 @@ inline Divisor divisor(int64_t d) {
 
 __device__ __forceinline__ uint32_t divide(uint32_t x, Divisor d) {
   return (uint32_t)(((uint64_t)x * d.magic) >> d.shift);
+}
+
+// Launches a kernel; the status is this launch's own.
+template <typename... P, typename... A>
+hipError_t start(void (*kernel)(P...), int64_t grid, int block, hipStream_t s, const A&... args) {
+  std::tuple<P...> held(static_cast<P>(args)...);
+  return std::apply(
+      [&](P&... a) {
+        void* at[] = {(void*)&a...};
+        return hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3((unsigned)grid),
+                               dim3((unsigned)block), at, 0, s);
+      },
+      held);
 }
 
 // Launchers (arguments checked, device current).

@@ -14,8 +14,8 @@ template <typename T, int CPL>
 hipError_t rec_launch(RecParams p, bool backward, hipStream_t s) {
   const ccv1d_rec_args& a = p.a;
   p.cols = (int32_t)((a.dim + kWave * CPL - 1) / (kWave * CPL));
-  const dim3 grid((unsigned)(a.batch * p.cols * p.chunks));
-  const dim3 block((backward ? kBwdWaves : kFwdWaves) * kWave);
+  const int64_t grid = a.batch * p.cols * p.chunks;
+  hipError_t status = hipErrorInvalidValue;
   const auto lines = [](const void* at, int64_t stride_b, int64_t stride_t) {
     return !at || (reinterpret_cast<uintptr_t>(at) % 128 == 0 && stride_b * (int64_t)sizeof(T) % 128 == 0 &&
                    stride_t * (int64_t)sizeof(T) % 128 == 0);
@@ -31,9 +31,11 @@ hipError_t rec_launch(RecParams p, bool backward, hipStream_t s) {
     constexpr bool kDecay = decltype(decay)::value, kGate = decltype(input_gate)::value;
     constexpr bool kSeq = decltype(seq)::value, kStream = decltype(stream)::value;
     if (backward)
-      rec_bwd_kernel<T, CPL, kDecay, kGate, kSeq, kStream, kBwdWaves, kBwdRows><<<grid, block, 0, s>>>(p);
+      status = start(&rec_bwd_kernel<T, CPL, kDecay, kGate, kSeq, kStream, kBwdWaves, kBwdRows>, grid,
+                     kBwdWaves * kWave, s, p);
     else
-      rec_fwd_kernel<T, CPL, kDecay, kGate, kSeq, kStream, kFwdWaves, kFwdRows><<<grid, block, 0, s>>>(p);
+      status = start(&rec_fwd_kernel<T, CPL, kDecay, kGate, kSeq, kStream, kFwdWaves, kFwdRows>, grid,
+                     kFwdWaves * kWave, s, p);
   };
   // A flag at a time becomes a type.
   auto choose = [](bool flag, auto&& then) {
@@ -50,7 +52,7 @@ hipError_t rec_launch(RecParams p, bool backward, hipStream_t s) {
       });
     });
   });
-  return hipGetLastError();
+  return status;
 }
 
 hipError_t rec_launch_bf16(const RecParams& p, bool backward, hipStream_t s);

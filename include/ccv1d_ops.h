@@ -6,7 +6,9 @@
  * enqueued on `stream` and nothing synchronised, the calling thread's device restored, a status from
  * enum ccv1d_status and a thread-local message (ccv1d_last_error). Arguments travel in one struct per
  * entry point, which the library reads during the call only. Element types are enum ccv1d_dtype
- * (F32, F16, BF16). Calls can be captured in a graph: no memset nodes, no allocation.
+ * (F32, F16, BF16), and pointers are aligned to an element; workspaces to 8 bytes, their contents on
+ * entry do not matter, and calls that may overlap in time need one each. Calls can be captured in a graph:
+ * no memset nodes, no allocation.
  */
 #ifndef CCV1D_OPS_H
 #define CCV1D_OPS_H

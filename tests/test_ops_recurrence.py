@@ -290,6 +290,25 @@ def test_after_the_convolution_compiled():
         assert torch.equal(a, b)
 
 
+def test_registered_operators():
+    """Schema, fake implementations, autograd registration and AOT dispatch of the two operators."""
+    from causal_conv1d_triton import recurrence
+    t = make(15, 2, 130, 66, BF, packed=True, init=True)
+    d = {k: None if v is None else v.to(DEV) for k, v in t.items()}
+    for k in ("x", "gate", "decay", "igate", "init"):
+        d[k].requires_grad_(True)
+    torch.library.opcheck(recurrence._fwd_op, (d["x"], d["gate"], d["decay"], d["igate"], d["seq"],
+                                               d["init"], 8.0))
+    torch.library.opcheck(recurrence._fwd_op, (d["x"], d["gate"], None, None, None, None, 8.0))
+
+
+def test_second_derivatives_are_refused():
+    x = torch.randn(1, 5, 8, device=DEV, requires_grad=True)
+    (g,) = torch.autograd.grad(gated_recurrence_fn(x, x).square().sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
 @pytest.mark.parametrize("R,D", [(1, 1), (1, 130), (5, 66), (16, 2048), (300, 97)])
 @pytest.mark.parametrize("dtype", [BF, HF, F])
 @pytest.mark.parametrize("decay", [True, False])
@@ -315,7 +334,7 @@ def test_update_skips_rows_outside_the_pool():
     t = make(1, 6, 1, 70, BF)
     pool = torch.randn(4, 2 * 70, generator=torch.Generator().manual_seed(1))
     state = pool.to(DEV)[:, 3:73]  # rows with a stride and an odd start
-    idx = torch.tensor([2, -1, 4, 0, 2 ** 31 - 1, -2 ** 31], dtype=torch.int64)
+    idx = torch.tensor([2, -1, 4, 0, 2 ** 32 + 1, -2 ** 32 + 1], dtype=torch.int64)
     out = gated_recurrence_update(t["x"][:, 0].to(DEV), t["gate"][:, 0].to(DEV), state,
                                   t["decay"].to(DEV), t["igate"][:, 0].to(DEV), idx.to(DEV))
     assert not out[[1, 2, 4, 5]].any()
@@ -325,6 +344,15 @@ def test_update_skips_rows_outside_the_pool():
     oracle.assert_close(out[sel], (want["out"][0][:, 0], want["out"][1][:, 0]))
     oracle.assert_close(state[[2, 0]], want["final"])
     assert torch.equal(state[[1, 3]].cpu(), pool[[1, 3], 3:73])
+    # every index that int32 can hold
+    edge = torch.tensor([-1, 4, 2 ** 31 - 1, -2 ** 31, 5, -2], dtype=torch.int32, device=DEV)
+    out = gated_recurrence_update(t["x"][:, 0].to(DEV), t["gate"][:, 0].to(DEV), state,
+                                  state_indices=edge)
+    assert not out.any() and torch.equal(state[[1, 3]].cpu(), pool[[1, 3], 3:73])
+    # a write in place is one to autograd too
+    version = state._version
+    gated_recurrence_update(t["x"][:, 0].to(DEV), t["gate"][:, 0].to(DEV), state, state_indices=edge)
+    assert state._version > version
     # without indices row r uses slot r
     state = pool.to(DEV)[:, :70].contiguous()
     gated_recurrence_update(t["x"][:4, 0].to(DEV), t["gate"][:4, 0].to(DEV), state)
