@@ -149,7 +149,8 @@ hipError_t run(const ccv1d_rec_args& a, bool backward, hipStream_t s) {
     if (!to && !zero) return hipSuccess;
     return start(&rec_empty_kernel, fill_blocks(n), 256, s, from, to, n, zero, a.dim);
   }
-  const Plan pl = plan_of(a.batch, a.seqlen, a.dim, backward);
+  Plan pl = plan_of(a.batch, a.seqlen, a.dim, backward);
+  if (rec_one_chunk(a, backward)) pl.chunks = 1, pl.words = 0;
   RecParams p{};
   p.a = a;
   p.chunks = (int32_t)pl.chunks;

@@ -474,6 +474,15 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
   __shared__ Pairs<NW, CPL> mine, got;
   __shared__ float s_h[NW][CPL][kWave];
   __shared__ float base[CPL][kWave];
+  // Kept per element from the coefficients to the gradients: in registers a, beta i and w (then m). One
+  // channel a lane also leaves room for r, 1 - r and x (1 - i). With two, 1 - i goes through LDS, and for
+  // the first kGate rows 1 - r, with r in registers (without decay r is a); the other rows' are made
+  // again from the gate. (B=4 T=8192 D=1024 bf16, kernel and its two small ones: all made again 125 us,
+  // 1 - i in LDS 122, 4 rows' r and 1 - r too 121, 6 rows' 122. Without decay, B=4 T=16384 D=4096: 523
+  // and 515.)
+  constexpr bool kKeep = CPL == 1;
+  constexpr int kGate = kKeep ? 0 : IG ? R / 2 : R, kRest = kKeep || !IG ? 0 : R;
+  __shared__ float s_rest[kKeep ? 1 : NW][kRest + kGate + kKeep][kWave][CPL];
   __shared__ uint32_t s_ticket;
   const ccv1d_rec_args& a = p.a;
   int bc, from_end;
@@ -507,11 +516,8 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
     h[i] = (a.saved + (b * p.chunks + chunk) * D + c0)[lane_c + i];
   }
 
-  // Kept per element: a, beta i and w (then m). With two channels a lane the gates' other factors are
-  // made again from the inputs in the last walk: keeping them too would leave half of the waves.
-  constexpr bool kKeep = CPL == 1;
   float f[R][CPL], bi[R][CPL], w[R][CPL];
-  float kr[R][CPL], kn[R][CPL], kx[R][CPL];  // kKeep: r, 1 - r, x (1 - i)
+  float kr[R][CPL], kn[R][CPL], kx[R][CPL];  // kKeep: r (and of kGate rows), 1 - r, x (1 - i)
   auto coefficients = [&](auto is_slow) {
     constexpr int kTogether = decltype(is_slow)::value ? 2 : 1;  // rows
     float tail[CPL];
@@ -533,16 +539,20 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
       if constexpr (IG) V::unpack(ir[j], ig);
 #pragma unroll
       for (int i = 0; i < CPL; ++i) {
-        float in = 1.0f, not_in, r;
+        float in = 1.0f, r;
         if constexpr (IG && kKeep) {
+          float not_in;
           sigmoid_pair<T>(ig[i], in, not_in);
           kx[j][i] = x[i] * not_in;
         } else if constexpr (IG) {
-          in = sigmoid<T>(ig[i]);
+          sigmoid_and_rest<T>(ig[i], in, s_rest[wave][j][lane][i]);
         }
         if constexpr (DECAY) {
           if constexpr (kKeep) {
             sigmoid_pair<T>(g[i], r, kn[j][i]);
+            kr[j][i] = r;
+          } else if (j < kGate) {
+            sigmoid_and_rest<T>(g[i], r, s_rest[wave][kRest + j][lane][i]);
             kr[j][i] = r;
           } else {
             r = sigmoid<T>(g[i]);
@@ -557,6 +567,7 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
           float beta;
           sigmoid_pair<T>(g[i], f[j][i], beta);
           if constexpr (kKeep) kn[j][i] = beta;
+          else if (j < kGate) s_rest[wave][kRest + j][lane][i] = beta;
           bi[j][i] = beta * in;
           w[j][i] = in * x[i];
         }
@@ -567,6 +578,7 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
           settle(f[n]);
           settle(bi[n]);
           settle(w[n]);
+          if (DECAY && n < kGate) settle(kr[n]);
         }
       }
     }
@@ -690,16 +702,14 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
       if (j >= valid) continue;
       if constexpr (!kKeep) {
         forget_row(xr[j]);
-        forget_row(gr[j]);
+        if (j >= kGate) forget_row(gr[j]);
         forget_row(yr[j]);
-        if constexpr (IG) forget_row(ir[j]);
       }
       const bool pad = kMasked && (rows.pad >> j & 1);
-      float y[CPL], x[CPL], g[CPL], ig[CPL], ox[CPL], og[CPL], oi[CPL];
+      float y[CPL], x[CPL], g[CPL], ox[CPL], og[CPL], oi[CPL];
       V::unpack(yr[j], y);
       V::unpack(xr[j], x);
       V::unpack(gr[j], g);
-      if constexpr (IG) V::unpack(ir[j], ig);
 #pragma unroll
       for (int i = 0; i < CPL; ++i) {
         const float dh = y[i] + cc[i];
@@ -708,12 +718,11 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
         if constexpr (IG && kKeep) {
           oi[i] = ox[i] * kx[j][i];
         } else if constexpr (IG) {
-          float in, not_in;
-          sigmoid_pair_of_number<T>(ig[i], in, not_in);
-          oi[i] = ox[i] * (x[i] * not_in);
+          oi[i] = ox[i] * (x[i] * s_rest[wave][j][lane][i]);
         }
         float r, not_r;
         if constexpr (kKeep) r = kr[j][i], not_r = kn[j][i];
+        else if (j < kGate) r = DECAY ? kr[j][i] : f[j][i], not_r = s_rest[wave][kRest + j][lane][i];
         else sigmoid_pair_of_number<T>(g[i], r, not_r);
         float q = dh * f[j][i] * w[j][i];
         if constexpr (DECAY) {

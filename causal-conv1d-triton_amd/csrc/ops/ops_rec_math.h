@@ -39,6 +39,16 @@ __device__ __forceinline__ void sigmoid_pair(float z, float& s, float& rest) {
   rest = e * s;
 }
 
+// The same where 1 - s is only used as a factor of s, so that it need not be right once s is zero: an
+// operation less. e is held below infinity in it, which would make no number of that zero.
+template <typename T>
+__device__ __forceinline__ void sigmoid_and_rest(float z, float& s, float& rest) {
+  if constexpr (sizeof(T) == 4) return sigmoid_pair<T>(z, s, rest);
+  const float e = __builtin_amdgcn_exp2f(-kLog2e * z);
+  s = __builtin_amdgcn_rcpf(1.0f + e);
+  rest = fminf(e, 8.507059e37f) * s;  // 2^126
+}
+
 // The same where a NaN need not pass (a factor beside it carries it): one operation less in 16 bits.
 template <typename T>
 __device__ __forceinline__ void sigmoid_pair_of_number(float z, float& s, float& rest) {

@@ -104,6 +104,22 @@ def test_wide_gates(decay):
     check(make(6, 2, 200, 66, F, decay=decay, spread=6.0, init=True))
 
 
+@pytest.mark.parametrize("decay", [True, False])
+@pytest.mark.parametrize("igate", [True, False])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_wide_gates_of_16_bits(decay, igate, dtype):
+    check(make(16, 2, 200, 66, dtype, decay, igate, spread=6.0, init=True))
+
+
+@pytest.mark.parametrize("B,T", [(128, 129), (128, 200), (130, 256), (127, 256), (128, 257)])
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("packed", [True, False])
+def test_around_one_chunk(B, T, dtype, packed):
+    """Lengths and batches on both sides of the rule that takes 256 rows in one chunk."""
+    t = make(17, B, T, 6, dtype, packed=packed, init=True)
+    check(t, final=True, dfinal=torch.randn(B, 6, generator=torch.Generator().manual_seed(2)))
+
+
 @pytest.mark.parametrize("D", [66, 129])
 def test_strides(D):
     """Slices of one projection, an upstream gradient and gates with strides of their own."""

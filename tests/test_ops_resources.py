@@ -1,8 +1,8 @@
 """Registers and waves of the kernels around the convolution, read from the built gfx950 code objects as
 tests/test_kernel_resources.py does (which also holds every kernel to no scratch memory):
 
-* the recurrence's main kernels hold 4 waves per SIMD, two workgroups of 8 a CU, which their chunks
-  are sized for, one instance of each for every combination of what a call has;
+* the recurrence's main kernels hold 4 waves per SIMD, two workgroups of 8 a CU (or one of 16), which
+  their chunks are sized for, one instance of each for every combination of what a call has;
 * the attention holds 2 waves per SIMD, heads of 256 in fp32 one.
 """
 
@@ -23,11 +23,12 @@ def test_recurrence_kernels_hold_four_waves(kernels):  # noqa: F811
         if _waves_per_simd(int(d["vgpr_count"])) < 4:
             bad.append((d["name"], d["vgpr_count"]))
     assert not bad, f"fewer waves than the chunks are sized for: {bad}"
-    for k in ("fwd", "bwd"):
-        # decay, input gate, packed, streamed; a 16-bit single channel is never streamed
+    for k, sizes in (("fwd", 2), ("bwd", 1)):
+        # decay, input gate, packed, streamed; a 16-bit single channel is never streamed. The forward also
+        # has workgroups of 16 waves.
         assert {t: len(found[k, t, c]) for t, c in (("DF16b", 2), ("DF16_", 2), ("f", 1))} == {
-            "DF16b": 16, "DF16_": 16, "f": 16}
-        assert len(found[k, "DF16b", 1]) == len(found[k, "DF16_", 1]) == 8
+            "DF16b": 16 * sizes, "DF16_": 16 * sizes, "f": 16 * sizes}
+        assert len(found[k, "DF16b", 1]) == len(found[k, "DF16_", 1]) == 8 * sizes
 
 
 def test_attention_kernels_hold_two_waves(kernels):  # noqa: F811
