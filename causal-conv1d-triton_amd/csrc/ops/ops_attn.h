@@ -374,7 +374,7 @@ __global__ __launch_bounds__(kAttnWaves* kWave, sizeof(T) * DH > 768 ? 1 : 2) vo
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
   __shared__ float s_m[kAttnWaves][16], s_l[kAttnWaves][16];
-  __shared__ float s_o[kAttnWaves][16][DH + 4];
+  __shared__ alignas(16) float s_o[kAttnWaves][16][DH + 4];
   if (g == 0) {
     s_m[wave][n] = m;
     s_l[wave][n] = l;
@@ -390,28 +390,45 @@ __global__ __launch_bounds__(kAttnWaves* kWave, sizeof(T) * DH > 768 ? 1 : 2) vo
           s_o[wave][n][16 * Pc::before(k) + (4 * g + i) * Pc::width(k) + j] = o[Pc::before(k) + j][i];
   }
   __syncthreads();
-  for (int w = threadIdx.x; w < heads * Dh; w += kAttnWaves * kWave) {
-    const int h = w / Dh, d = w - h * Dh;
-    float top = s_m[0][h];
+  // 16 to 64 lanes a head, which needs the waves' factors once, and 4 elements at a time (an element at a
+  // time, factors and all, 16 heads of 256 took 4 us).
+  const int lanes = heads > 8 ? 16 : heads > 4 ? 32 : 64;
+  const int h = threadIdx.x / lanes;
+  if (h >= heads) return;
+  float top = s_m[0][h], f[kAttnWaves], total = 0.0f;
 #pragma unroll
-    for (int v = 1; v < kAttnWaves; ++v) top = fmaxf(top, s_m[v][h]);
-    float sum = 0.0f, total = 0.0f;
+  for (int v = 1; v < kAttnWaves; ++v) top = fmaxf(top, s_m[v][h]);
+#pragma unroll
+  for (int v = 0; v < kAttnWaves; ++v) {
+    f[v] = __builtin_amdgcn_exp2f(s_m[v][h] - top);
+    total = fmaf(s_l[v][h], f[v], total);
+  }
+  const int64_t at = row * a.q_heads + head0 + h;
+  T* out = static_cast<T*>(a.out) + at * Dh;
+  float* part = p.part + (at * p.splits + split) * Dh;
+  const float by = 1.0f / total;
+  for (int d = threadIdx.x % lanes * 4; d < Dh; d += lanes * 4) {
+    float sum[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int v = 0; v < kAttnWaves; ++v) {
-      const float f = __builtin_amdgcn_exp2f(s_m[v][h] - top);
-      total = fmaf(s_l[v][h], f, total);
-      sum = fmaf(s_o[v][h][d], f, sum);
+      const f32x4 o4 = *reinterpret_cast<const f32x4*>(&s_o[v][h][d]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] = fmaf(o4[i], f[v], sum[i]);
     }
-    const int64_t at = row * a.q_heads + head0 + h;
     if (only) {
-      static_cast<T*>(a.out)[at * Dh + d] = static_cast<T>(total == 0.0f ? 0.0f : sum / total);
-      if (a.lse && d == 0) a.lse[at] = (top + __log2f(total)) * 0.69314718055994530942f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] = total == 0.0f ? 0.0f : sum[i] * by;
+      VecIO<T, 4>::st(out + d, VecIO<T, 4>::pack(sum));
     } else {
-      p.part[(at * p.splits + split) * Dh + d] = sum;
-      if (d == 0) {
-        p.part_ml[(at * p.splits + split) * 2] = top;
-        p.part_ml[(at * p.splits + split) * 2 + 1] = total;
-      }
+      VecIO<float, 4>::st(part + d, VecIO<float, 4>::pack(sum));
+    }
+  }
+  if (threadIdx.x % lanes == 0) {
+    if (only) {
+      if (a.lse) a.lse[at] = (top + __log2f(total)) * 0.69314718055994530942f;
+    } else {
+      p.part_ml[(at * p.splits + split) * 2] = top;
+      p.part_ml[(at * p.splits + split) * 2 + 1] = total;
     }
   }
 }
