@@ -75,15 +75,20 @@ AttnParams plan(const ccv1d_paged_attn_args& a) {
   int64_t limit = a.max_pages * a.page_size;
   if (a.max_seq_len && a.max_seq_len < limit) limit = a.max_seq_len;
   p.limit = (int32_t)limit;
-  // Spans: as many as make 2048 workgroups, of at least a step of every wave (128 positions) and at most
-  // 1024 positions, so that a long row beside short ones is spread too; at most 256 of them. (64
-  // requests of 512 to 8192 positions, 8 key heads of 128: spans of 2048 293 us, 1024 254, 512 253; two
-  // rows of 131072: 194, 202, 211; 256 rows of 1000 to 3000, heads of 64: 358, 278, 314. 16 rows of a
-  // 1024 window: spans of 256 20.1 us, 128 17.3.)
+  // Spans: as many as make `target` workgroups, twice what the card holds or more, of at least a step of
+  // every wave (128 positions) and at most 1024 positions, so that a long row beside short ones is spread
+  // too; at most 256 of them. The wider a head, the fewer workgroups hold as many bytes, and the more
+  // each writes for the join: 2^18 over the bytes of a row, i.e. 2048, 1024, 512 for 16-bit heads of 64,
+  // 128, 256. (Targets 512, 1024, 2048: 64 rows of 512 to 4096 positions, 16 query heads of 256 over 2
+  // key heads 77, 79, 88 us, over one 46, 53, 59; 128 rows of 300 to 700, 8 key heads of 128 64, 64, 70;
+  // 16 rows of 512 to 4096 of those 47, 43, 42; 32 rows of 1000 to 3000, heads of 64 46, 48, 44. Most
+  // positions: 64 requests of 512 to 8192, 8 key heads of 128: 2048 254 us, 1024 228; two rows of 131072:
+  // 197, 196. Least: 16 rows of a 1024 window, one key head of 256: 256 15.7 us, 128 13.1.)
+  const int64_t target = (int64_t(1) << 18) / (a.head_dim * (a.dtype == CCV1D_F32 ? 4 : 2));
   int64_t most = a.window && a.window + 31 < limit ? a.window + 31 : limit;
   if (most < 1) most = 1;
   const int64_t wgs = a.rows * a.kv_heads * p.tiles;
-  int64_t splits = (2048 + wgs - 1) / wgs;
+  int64_t splits = (target + wgs - 1) / wgs;
   int64_t span = (most + splits - 1) / splits;
   if (span > 1024) span = 1024;
   if (span < 128) span = 128;

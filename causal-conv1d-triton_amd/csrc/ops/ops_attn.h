@@ -221,28 +221,46 @@ __global__ __launch_bounds__(kAttnWaves* kWave, sizeof(T) * DH > 768 ? 1 : 2) vo
   };
 
   for (int p0 = begin + wave * kStep; p0 < end; p0 += kAttnWaves * kStep) {
-    // Where the keys and the values of this lane are.
-    const T* kp[kTiles];
+    // The keys are requested before the places of the values are worked out (64 rows of 512 to 8192
+    // positions, 8 key heads of 128: 230.7 us after them, 228.1 so).
+    uint32_t kw[kTiles][kChunks][4];
+    {
+      const T* kp[kTiles];
+      uint32_t page, off;
+      if constexpr (MODE == kPageStep) {
+        locate(p0, page, off);
+        const T* kb = kc + (int64_t)page * a.k_cache_stride_p + (int64_t)off * a.k_cache_stride_t;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) kp[t] = kb + (16 * t + n) * a.k_cache_stride_t;
+      } else {
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+          locate(p0 + 16 * t + n, page, off);
+          kp[t] = kc + (int64_t)page * a.k_cache_stride_p + (int64_t)off * a.k_cache_stride_t;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        const int d = (4 * c + g) * kE;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) load_words<4>(kp[t] + (d < Dh ? d : 0), kw[t][c]);
+      }
+    }
     const T* vp[kMine];
     uint32_t ok = 0;  // bit e: my position e counts
     if constexpr (MODE == kPageStep) {
       uint32_t page, off;
       const bool in = locate(p0, page, off);
-      const T* kb = kc + (int64_t)page * a.k_cache_stride_p + (int64_t)off * a.k_cache_stride_t;
       const T* vb = vc + (int64_t)page * a.v_cache_stride_p + (int64_t)off * a.v_cache_stride_t;
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        kp[t] = kb + (16 * t + n) * a.k_cache_stride_t;
+      for (int t = 0; t < kTiles; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) vp[4 * t + i] = vb + (16 * t + 4 * g + i) * a.v_cache_stride_t;
-      }
       ok = in ? ~0u : 0u;
     } else {
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
         uint32_t page, off;
-        locate(p0 + 16 * t + n, page, off);
-        kp[t] = kc + (int64_t)page * a.k_cache_stride_p + (int64_t)off * a.k_cache_stride_t;
         if constexpr (MODE == kPageFour) {
           const bool in = locate(p0 + 16 * t + 4 * g, page, off);
           const T* v0 = vc + (int64_t)page * a.v_cache_stride_p + (int64_t)off * a.v_cache_stride_t;
@@ -270,13 +288,6 @@ __global__ __launch_bounds__(kAttnWaves* kWave, sizeof(T) * DH > 768 ? 1 : 2) vo
     constexpr uint32_t kAll = kMine == 8 ? 255u : 15u;
     whole = __all((ok & kAll) == kAll);
 
-    uint32_t kw[kTiles][kChunks][4];
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      const int d = (4 * c + g) * kE;
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) load_words<4>(kp[t] + (d < Dh ? d : 0), kw[t][c]);
-    }
     uint32_t vw[kMine][kVW];
     auto load_values = [&]() {
 #pragma unroll
