@@ -17,10 +17,10 @@ template <typename T>
 __global__ __launch_bounds__(kJoinWaves * 64) void paged_join_kernel(AttnParams p) {
   __shared__ float s_sum[kJoinWaves][256], s_total[kJoinWaves];
   const ccv1d_paged_attn_args& a = p.a;
-  const int64_t at = blockIdx.x, row = at / a.q_heads;
+  const int64_t at = blockIdx.x, row = divide(blockIdx.x, p.by_q_heads);
   int64_t request;
   const Span sp = span_of(p, row, request);
-  const int spans = (sp.end - sp.base + p.span - 1) / p.span;
+  const int spans = (int)divide(sp.end - sp.base + p.span - 1, p.by_span);
   if (spans <= 1) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int Dh = (int)a.head_dim;
@@ -70,8 +70,8 @@ AttnParams plan(const ccv1d_paged_attn_args& a) {
   AttnParams p{};
   p.a = a;
   p.by_page = divisor(a.page_size);
-  const int64_t group = a.q_heads / a.kv_heads;
-  p.tiles = (int32_t)((group + kAttnHeads - 1) / kAttnHeads);
+  p.group = (int32_t)(a.q_heads / a.kv_heads);
+  p.tiles = (p.group + kAttnHeads - 1) / kAttnHeads;
   int64_t limit = a.max_pages * a.page_size;
   if (a.max_seq_len && a.max_seq_len < limit) limit = a.max_seq_len;
   p.limit = (int32_t)limit;
@@ -96,6 +96,13 @@ AttnParams plan(const ccv1d_paged_attn_args& a) {
   span = (span + 127) / 128 * 128;
   p.span = (int32_t)span;
   p.splits = (int32_t)((most + span - 1) / span);
+  p.block = (int32_t)(8 * a.kv_heads * p.tiles);
+  p.by_block = divisor(p.block);
+  p.by_tiles = divisor(p.tiles);
+  p.by_kv_heads = divisor(a.kv_heads);
+  p.by_splits = divisor(p.splits);
+  p.by_q_heads = divisor(a.q_heads);
+  p.by_span = divisor(p.span);
   return p;
 }
 

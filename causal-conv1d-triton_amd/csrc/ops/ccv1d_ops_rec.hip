@@ -55,12 +55,12 @@ __global__ __launch_bounds__(1024) void rec_reduce_kernel(const float* part, int
 // One token of a request: CPL channels a lane, the last lane of a row those that are left. Bound by
 // latency for a small batch (16 rows of 2048 channels: 3 us), by memory for a large one.
 template <typename T, bool DECAY, int CPL>
-__global__ __launch_bounds__(64) void rec_update_kernel(ccv1d_rec_update_args p) {
+__global__ __launch_bounds__(64) void rec_update_kernel(ccv1d_rec_update_args p,
+                                                               uint32_t cols, Divisor by_cols) {
   using V = VecIO<T, CPL>;
   using S = VecIO<float, CPL>;
-  const uint32_t cols = (uint32_t)((p.dim + 64 * CPL - 1) / (64 * CPL));
-  const int64_t row = blockIdx.x / cols;
-  const int64_t d = ((int64_t)(blockIdx.x % cols) * 64 + threadIdx.x) * CPL;
+  const uint32_t r = divide(blockIdx.x, by_cols);
+  const int64_t row = r, d = ((int64_t)(blockIdx.x - r * cols) * 64 + threadIdx.x) * CPL;
   if (d >= p.dim) return;
   const int n = (int)min((int64_t)CPL, p.dim - d);
   const int64_t slot = p.state_indices ? p.state_indices[row] : row;
@@ -114,9 +114,9 @@ __global__ __launch_bounds__(64) void rec_update_kernel(ccv1d_rec_update_args p)
 
 template <typename T, int CPL>
 hipError_t update_t(const ccv1d_rec_update_args& a, hipStream_t s) {
-  const int64_t grid = a.rows * ((a.dim + 64 * CPL - 1) / (64 * CPL));
-  return a.decay ? start(&rec_update_kernel<T, true, CPL>, grid, 64, s, a)
-                 : start(&rec_update_kernel<T, false, CPL>, grid, 64, s, a);
+  const int64_t cols = (a.dim + 64 * CPL - 1) / (64 * CPL), grid = a.rows * cols;
+  return a.decay ? start(&rec_update_kernel<T, true, CPL>, grid, 64, s, a, cols, divisor(cols))
+                 : start(&rec_update_kernel<T, false, CPL>, grid, 64, s, a, cols, divisor(cols));
 }
 
 int64_t fill_blocks(int64_t n) {

@@ -44,7 +44,9 @@ constexpr float kLowest = -3.402823466e38f;
 
 struct AttnParams {
   ccv1d_paged_attn_args a;
-  Divisor by_page;
+  Divisor by_page, by_block, by_tiles, by_kv_heads, by_splits, by_q_heads, by_span;
+  int32_t group;      // query heads of a key head
+  int32_t block;      // workgroups of 8 spans of a row, or of neighbouring rows
   int32_t tiles;      // workgroups of kAttnHeads query heads per key head
   int32_t span;       // positions of a workgroup, a multiple of a step of all waves
   int32_t splits;     // most spans of a row
@@ -161,21 +163,20 @@ __global__ __launch_bounds__(kAttnWaves* kWave, sizeof(T) * DH > 768 ? 1 : 2) vo
   const ccv1d_paged_attn_args& a = p.a;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int Dh = (int)a.head_dim, group = (int)(a.q_heads / a.kv_heads);
+  const int Dh = (int)a.head_dim, group = p.group;
   // Workgroups go to the 8 XCDs in turn: ids are dealt anew so that the key heads of one span, whose rows
   // lie side by side in memory, share an XCD's L2 at the same time (256 rows of 1000 to 3000 positions,
   // heads of 64: 278 -> 246 us). The spans move on by one XCD from 8 to 8, or with 8 spans a row one XCD
   // would get all the last ones, which short rows do not have.
   uint32_t id = blockIdx.x;
-  const uint32_t together = (uint32_t)(a.kv_heads * p.tiles), block = 8 * together;
-  const uint32_t in = id % block, start = id - in;
-  if (start + block <= gridDim.x) id = start + (in + start / block) % 8 * together + in / 8;
-  const int tile = (int)(id % p.tiles);
-  id /= p.tiles;
-  const int64_t kvh = id % (uint32_t)a.kv_heads;
-  id /= (uint32_t)a.kv_heads;
-  const int split = (int)(id % p.splits);
-  const int64_t row = id / p.splits;
+  const uint32_t nth = divide(id, p.by_block), start = nth * p.block, in = id - start;
+  if (start + p.block <= gridDim.x) id = start + (in + nth) % 8 * (p.block / 8) + in / 8;
+  // id = ((row * splits + split) * kv_heads + key head) * tiles + tile
+  const uint32_t kvs = divide(id, p.by_tiles), spans = divide(kvs, p.by_kv_heads);
+  const int tile = (int)(id - kvs * p.tiles);
+  const int64_t kvh = kvs - spans * (uint32_t)a.kv_heads;
+  const int64_t row = divide(spans, p.by_splits);
+  const int split = (int)(spans - (uint32_t)row * p.splits);
 
   int64_t request;
   const Span sp = span_of(p, row, request);

@@ -46,6 +46,7 @@ constexpr float kTiny = 1.17549435e-38f;
 struct RecParams {
   ccv1d_rec_args a;
   int32_t cols, chunks, groups;  // wave columns of 64 * CPL channels; chunks along time; their groups
+  Divisor by_cols, by_columns;   // cols; batch * cols
   uint64_t* pairs;               // (batch, chunks, dim)
   uint64_t* states;              // (batch, groups, dim): word of the state after a group
   uint32_t* tickets;             // (batch * cols,): the next chunk of each wave column
@@ -179,8 +180,9 @@ __device__ __forceinline__ void forget_row(RAW& v) {
 // side, whose lines overlap (B=3 T=5001 D=1501 fp32 273 us, 248 so; rows on lines 1 % slower).
 __device__ __forceinline__ void deal(const RecParams& p, int& bc, int& chunk, uint32_t* s_ticket) {
   const uint32_t n = (uint32_t)(p.a.batch * p.cols);
-  const uint32_t i = blockIdx.x % n, at = p.stream ? i : (uint32_t)xcd_remap((int)i, (int)n);
-  bc = (int)((at + blockIdx.x / n) % n);
+  const uint32_t turn = divide(blockIdx.x, p.by_columns), i = blockIdx.x - turn * n;
+  const uint32_t at = (p.stream ? i : (uint32_t)xcd_remap((int)i, (int)n)) + turn;
+  bc = (int)(at - divide(at, p.by_columns) * n);
   chunk = 0;
   if (p.chunks > 1) {
     if (threadIdx.x == 0)
@@ -279,11 +281,12 @@ struct Place {
   __device__ __forceinline__ Place(const RecParams& p, int bc, int chunk)
       : lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {
     const int64_t D = p.a.dim, T = p.a.seqlen;
-    b = bc / p.cols;
+    const uint32_t row = divide(bc, p.by_cols);
+    b = row;
     t0 = ((int64_t)chunk * NW + wave) * R;
     t1 = min(t0, T - 1);
     valid = (int)max((int64_t)0, min((int64_t)R, T - t0));
-    c0 = min((int64_t)(bc % p.cols) * (kWave * CPL), D - CPL);
+    c0 = min((int64_t)(bc - (int)row * p.cols) * (kWave * CPL), D - CPL);
     lane_c = (uint32_t)min((int64_t)lane * CPL, D - CPL - c0);
   }
 };

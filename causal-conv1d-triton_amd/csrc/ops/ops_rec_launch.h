@@ -27,6 +27,8 @@ template <typename T, int CPL>
 hipError_t rec_launch(RecParams p, bool backward, hipStream_t s) {
   const ccv1d_rec_args& a = p.a;
   p.cols = (int32_t)((a.dim + kWave * CPL - 1) / (kWave * CPL));
+  p.by_cols = divisor(p.cols);
+  p.by_columns = divisor(a.batch * p.cols);
   const int64_t grid = a.batch * p.cols * p.chunks;  // chunks: 1 where rec_one_chunk holds
   hipError_t status = hipErrorInvalidValue;
   const auto lines = [](const void* at, int64_t stride_b, int64_t stride_t) {
