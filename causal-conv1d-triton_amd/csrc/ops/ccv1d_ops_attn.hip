@@ -6,12 +6,14 @@ namespace ops {
 
 namespace {
 
-// Joins the spans of a row and query head: the workgroup's waves (kJoinWaves at most, one a span where
-// there are fewer) take the spans in turn, 64 lanes the elements, and the waves' sums meet in LDS.
+// Joins the spans of a row and query head: the workgroup's waves (kJoinWaves at most, one for
+// kJoinSpans spans where there are fewer) take the spans in turn, 64 lanes the elements, and the waves'
+// sums meet in LDS.
 // Rows of one span have been written by the main kernel. Bound by its two dependent reads (the length,
 // then maxima and sums together): two rows of 128 spans and 32 heads of 128 take 6 us (4 waves that read
-// the maxima first 17).
-constexpr int kJoinWaves = 16;
+// the maxima first 17); many rows by their workgroups' waves: with a wave a span, 64 rows of 8 spans made the
+// whole call 225 us, with one for 4 222, and 32 rows of 64 heads of 64 and 8 spans 43 and 39.
+constexpr int kJoinWaves = 16, kJoinSpans = 4;
 
 template <typename T>
 __global__ __launch_bounds__(kJoinWaves * 64) void paged_join_kernel(AttnParams p) {
@@ -128,7 +130,8 @@ hipError_t paged_attn(const ccv1d_paged_attn_args& a, hipStream_t s) {
   }
   if (e != hipSuccess || p.splits <= 1) return e;
   const int64_t grid = a.rows * a.q_heads;
-  const int block = 64 * (p.splits < kJoinWaves ? p.splits : kJoinWaves);
+  const int waves = (p.splits + kJoinSpans - 1) / kJoinSpans;
+  const int block = 64 * (waves < kJoinWaves ? waves : kJoinWaves);
   switch (a.dtype) {
     case CCV1D_BF16: return start(&paged_join_kernel<__bf16>, grid, block, s, p);
     case CCV1D_F16: return start(&paged_join_kernel<_Float16>, grid, block, s, p);

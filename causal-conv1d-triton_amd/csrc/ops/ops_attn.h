@@ -147,8 +147,8 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
 }
 
 // Measured, with the join: 64 rows of 512 to 8192 positions, 32 query over 8 key heads of 128, bf16, pages of
-// 16: 226 us, 5.0 TB/s of 1.14 GB, a copy's rate; two rows of 100001 to 131072, fp16, pages of 64: 195 us,
-// 4.85 TB/s. Wide heads with many query heads write and join more per position: 16 query heads of 256
+// 16: 222 us, 5.15 TB/s of 1.14 GB, a large copy's rate; two rows of 100001 to 131072, fp16, pages of 64: 195 us,
+// 4.9 TB/s. Wide heads with many query heads write and join more per position: 16 query heads of 256
 // over 2 key heads, 64 rows of 512 to 4096: 77 us, 3.9 TB/s. One step a wave is latency: 16 rows of a 1024
 // window, one key head of 256: 12.6 us, 4 of them the join. The matrix cores are idle most of the time
 // (below 10 % busy in the first).
