@@ -90,15 +90,23 @@ class _GatedRecurrenceFn(torch.autograd.Function):
         return out, final
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout, dfinal):
-        x, gate, decay, input_gate, seq_idx, init, saved = ctx.saved_tensors
-        if dout is None:
-            dout = torch.zeros(x.shape, device=x.device, dtype=x.dtype)
-        need = init is not None and ctx.needs_input_grad[5]
-        dx, dgate, ddecay, dig, dinit = native().rec_bwd(
-            x, gate, decay, input_gate, seq_idx, init, ctx.decay_scale, saved, dout, dfinal, need)
-        return dx, dgate, ddecay, dig, None, dinit, None, None
+        # Second derivatives are refused; without a graph to record, the wrapper that does so (6 us of
+        # the host) has nothing to do.
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, dout, dfinal)
+
+
+def _backward(ctx, dout, dfinal):
+    x, gate, decay, input_gate, seq_idx, init, saved = ctx.saved_tensors
+    if dout is None:
+        dout = torch.zeros(x.shape, device=x.device, dtype=x.dtype)
+    need = init is not None and ctx.needs_input_grad[5]
+    dx, dgate, ddecay, dig, dinit = native().rec_bwd(
+        x, gate, decay, input_gate, seq_idx, init, ctx.decay_scale, saved, dout, dfinal, need)
+    return dx, dgate, ddecay, dig, None, dinit, None, None
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 def gated_recurrence_fn(
