@@ -295,7 +295,7 @@ struct Place {
 //
 // Bound by memory without decay: B=4 T=16384 D=4096 bf16 without an input gate 297 us, 5.4 TB/s of its
 // 1.61 GB. With decay (6 of its 31 operations per element are transcendental, at half rate) memory and
-// arithmetic, the VALUs 57 % busy: B=4 T=8192 D=1024 bf16 68 us with the clearing, 4.0 TB/s; in fp32,
+// arithmetic, the VALUs 58 % busy: B=4 T=8192 D=1024 bf16 68 us with the clearing, 4.0 TB/s; in fp32,
 // B=3 T=5001 D=1501, 87 us, 4.1 TB/s. 8 waves of 16 rows at 4 waves per SIMD: 4 waves of 16 rows
 // took 1 % more with decay and 1 % less without, 8 waves of 8 rows 6 and 14 % more.
 
@@ -477,7 +477,7 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_fwd_kernel(RecParams p) {
 //   without decay:  w = i x,           dgate = dh a beta m
 //
 // Bound like the forward: without decay 503 us, 5.3 TB/s of 2.68 GB, at the size given there; with decay
-// (71 operations per element) the VALUs are 66 % busy: B=4 T=8192 D=1024 bf16 120 us with the clearing
+// (71 operations per element) the VALUs are 65 % busy: B=4 T=8192 D=1024 bf16 120 us with the clearing
 // and the decay's sum, 3.9 TB/s; in fp32, B=3 T=5001 D=1501, 159 us, 4.0 TB/s. Rows per wave are half of
 // the forward's, since twice as much is held per row; 4 waves of 8 rows: 128 us where 8 were 126, and
 // 4 % more without decay.
