@@ -89,20 +89,20 @@ struct Rows {
   uint32_t first, pad;  // a sequence's first row; padding
 };
 
+// Lane l looks at row t0 - 1 + l (a row inside): its id is requested before the inputs and looked at once
+// they are requested too (B=4 T=16384 D=4096 without decay, packed, forward and backward: looked at
+// first 833 us, 812 so).
+__device__ __forceinline__ int32_t id_of(const int32_t* seq, int64_t t0, int64_t T, int lane) {
+  return seq[min(max(t0 - 1 + lane, (int64_t)0), T - 1)];
+}
+
 template <int R>
-__device__ __forceinline__ Rows rows_of(const int32_t* seq, int64_t t0, int64_t T, int lane) {
-  Rows w{0, 0};
-  if (t0 < T) {  // lane l looks at row t0 - 1 + l
-    const int64_t t = t0 - 1 + lane;
-    const int32_t id = seq[min(max(t, (int64_t)0), T - 1)];
-    const int32_t prev = __shfl_up(id, 1);
-    const uint64_t pad = __ballot(id < 0);
-    const uint64_t first = __ballot(t > 0 && id != prev);
-    const uint32_t live = T - t0 < R ? (1u << (int)(T - t0)) - 1 : (1u << R) - 1;
-    w.pad = (uint32_t)(pad >> 1) & live;
-    w.first = (uint32_t)(first >> 1) & live;
-  }
-  return w;
+__device__ __forceinline__ Rows rows_of(int32_t id, int64_t t0, int valid, int lane) {
+  const int32_t prev = __shfl_up(id, 1);
+  const uint64_t pad = __ballot(id < 0);
+  const uint64_t first = __ballot(t0 + lane > 1 && id != prev);
+  const uint32_t live = (1u << valid) - 1;
+  return {(uint32_t)(first >> 1) & live, (uint32_t)(pad >> 1) & live};
 }
 
 // The rows of one tensor under a wave, from row t0 on: a uniform address (kept in scalar registers, which
@@ -171,25 +171,31 @@ __device__ __forceinline__ void forget_row(RAW& v) {
   }
 }
 
-// Deals a chunk to this workgroup: (batch row and wave column, chunk from the walk's start). A column's
-// chunks have a counter of their own: with one for all, the 512 workgroups that start together waited in
-// line for it (forward of B=16 T=256 D=2048 25 us, 18 so). Workgroups go to the 8 XCDs in turn; columns
+// The wave column (batch row and channels) of this workgroup. Workgroups go to the 8 XCDs in turn; columns
 // move on by one from n to n workgroups, or with n a multiple of 8 an XCD would have the same columns
 // for good, and with rows of a power of two the same part of the memory's channels (forward and backward
 // at B=4 T=8192 D=1024 219 us, 198 so). Where rows are not on cache lines, an XCD takes columns side by
 // side, whose lines overlap (B=3 T=5001 D=1501 fp32 273 us, 248 so; rows on lines 1 % slower).
-__device__ __forceinline__ void deal(const RecParams& p, int& bc, int& chunk, uint32_t* s_ticket) {
+__device__ __forceinline__ int column_of(const RecParams& p) {
   const uint32_t n = (uint32_t)(p.a.batch * p.cols);
   const uint32_t turn = divide(blockIdx.x, p.by_columns), i = blockIdx.x - turn * n;
   const uint32_t at = (p.stream ? i : (uint32_t)xcd_remap((int)i, (int)n)) + turn;
-  bc = (int)(at - divide(at, p.by_columns) * n);
-  chunk = 0;
-  if (p.chunks > 1) {
-    if (threadIdx.x == 0)
-      *s_ticket = __hip_atomic_fetch_add(p.tickets + bc, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    chunk = (int)__builtin_amdgcn_readfirstlane(*s_ticket);
-  }
+  return (int)(at - divide(at, p.by_columns) * n);
+}
+
+// Deals this workgroup a chunk of its column, counted from the walk's start. A column's chunks have a
+// counter of their own: with one for all, the 512 workgroups that start together waited in line for it
+// (forward of B=16 T=256 D=2048 25 us, 18 so). `meanwhile` is what can be done before the chunk is known.
+template <typename F>
+__device__ __forceinline__ int deal(const RecParams& p, int bc, uint32_t* s_ticket, F&& meanwhile) {
+  uint32_t ticket = 0;
+  if (p.chunks > 1 && threadIdx.x == 0)
+    ticket = __hip_atomic_fetch_add(p.tickets + bc, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  meanwhile();
+  if (p.chunks <= 1) return 0;
+  if (threadIdx.x == 0) *s_ticket = ticket;
+  __syncthreads();
+  return (int)__builtin_amdgcn_readfirstlane(*s_ticket);
 }
 
 // The pairs of the waves of a workgroup, and of the chunks before it, in LDS.
@@ -271,32 +277,75 @@ __device__ __forceinline__ float look_back_state(const Pairs<NW, CPL>& got,
   return h;
 }
 
-// What the kernels share at their start: which rows and channels a wave has.
-template <int CPL, int NW, int R>
-struct Place {
-  int lane, wave, valid;  // valid: rows inside the sequence
-  int64_t b, t0, t1, c0;  // batch row, first row (and a row inside), the wave column's first channel
-  uint32_t lane_c;        // the lane's first channel, from c0 on
-  // The last lanes of a row share its last CPL channels and compute the same values twice.
-  __device__ __forceinline__ Place(const RecParams& p, int bc, int chunk)
-      : lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {
-    const int64_t D = p.a.dim, T = p.a.seqlen;
+// A lane's channels. The last lanes of a row share its last CPL channels and compute the same values twice.
+template <int CPL>
+struct Channels {
+  int64_t b, c0;    // batch row, the wave column's first channel
+  uint32_t lane_c;  // the lane's first channel, from c0 on
+  __device__ __forceinline__ Channels(const RecParams& p, int bc, int lane) {
+    const int64_t D = p.a.dim;
     const uint32_t row = divide(bc, p.by_cols);
     b = row;
-    t0 = ((int64_t)chunk * NW + wave) * R;
-    t1 = min(t0, T - 1);
-    valid = (int)max((int64_t)0, min((int64_t)R, T - t0));
     c0 = min((int64_t)(bc - (int)row * p.cols) * (kWave * CPL), D - CPL);
     lane_c = (uint32_t)min((int64_t)lane * CPL, D - CPL - c0);
   }
 };
 
+// The rows of a wave.
+template <int NW, int R>
+struct Place {
+  int valid;       // rows inside the sequence
+  int64_t t0, t1;  // first row (and a row inside)
+  __device__ __forceinline__ Place(const RecParams& p, int chunk, int wave) {
+    const int64_t T = p.a.seqlen;
+    t0 = ((int64_t)chunk * NW + wave) * R;
+    t1 = min(t0, T - 1);
+    valid = (int)max((int64_t)0, min((int64_t)R, T - t0));
+  }
+};
+
+// The rates of a lane's channels; whether all of them are slow.
+template <int CPL, bool DECAY>
+__device__ __forceinline__ bool rates(const ccv1d_rec_args& a, const Channels<CPL>& ch, float (&k)[CPL]) {
+  bool slow = true;
+#pragma unroll
+  for (int i = 0; i < CPL; ++i) {
+    k[i] = DECAY ? decay_rate((a.decay + ch.c0)[ch.lane_c + i], a.decay_scale) : 0.0f;
+    slow = slow && slow_channel(k[i]);
+  }
+  return slow;
+}
+
+// Requests the inputs row by row, so that work on the first rows can begin while the rest is on its way
+// (loads complete in order; tensor by tensor, with the decay after them, B=4 T=8192 D=1024 bf16 took 188 us
+// forward and backward, 173 so, and 170 with the rates made while the ticket is on its way). Rows past the last one repeat it.
+template <bool STREAM, bool IG, typename T, int CPL, int R, int NW>
+__device__ __forceinline__ void load_inputs(const ccv1d_rec_args& a, const Channels<CPL>& ch,
+                                            const Place<NW, R>& at, uint32_t lane_bytes,
+                                            typename VecIO<T, CPL>::raw (&gr)[R],
+                                            typename VecIO<T, CPL>::raw (&xr)[R],
+                                            typename VecIO<T, CPL>::raw (&ir)[R]) {
+  RowWalk<T, CPL> g(a.gate, a.gate_stride_b, a.gate_stride_t, ch.b, at.t1, ch.c0);
+  RowWalk<T, CPL> x(a.x, a.x_stride_b, a.x_stride_t, ch.b, at.t1, ch.c0);
+  RowWalk<T, CPL> i(a.input_gate, a.input_gate_stride_b, a.input_gate_stride_t, ch.b, at.t1, ch.c0);
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    gr[j] = g.template load<STREAM>(lane_bytes);
+    xr[j] = x.template load<STREAM>(lane_bytes);
+    if constexpr (IG) ir[j] = i.template load<STREAM>(lane_bytes);
+    const bool more = j + 1 < at.valid;
+    g.move(more ? g.step : 0);
+    x.move(more ? x.step : 0);
+    if constexpr (IG) i.move(more ? i.step : 0);
+  }
+}
+
 // ------------------------------------------------------------------------------------- forward
 //
-// Bound by memory without decay: B=4 T=16384 D=4096 bf16 without an input gate 297 us, 5.4 TB/s of its
+// Bound by memory without decay: B=4 T=16384 D=4096 bf16 without an input gate 295 us, 5.5 TB/s of its
 // 1.61 GB. With decay (6 of its 31 operations per element are transcendental, at half rate) memory and
-// arithmetic, the VALUs 58 % busy: B=4 T=8192 D=1024 bf16 68 us with the clearing, 4.0 TB/s; in fp32,
-// B=3 T=5001 D=1501, 87 us, 4.1 TB/s. 8 waves of 16 rows at 4 waves per SIMD: 4 waves of 16 rows
+// arithmetic, the VALUs 58 % busy: B=4 T=8192 D=1024 bf16 62 us with the clearing, 4.3 TB/s; in fp32,
+// B=3 T=5001 D=1501, 86 us, 4.2 TB/s. 8 waves of 16 rows at 4 waves per SIMD: 4 waves of 16 rows
 // took 1 % more with decay and 1 % less without, 8 waves of 8 rows 6 and 14 % more.
 
 template <typename T, int CPL, bool DECAY, bool IG, bool SEQ, bool STREAM, int NW, int R>
@@ -307,32 +356,25 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_fwd_kernel(RecParams p) {
   __shared__ float base[CPL][kWave];
   __shared__ uint32_t s_ticket;
   const ccv1d_rec_args& a = p.a;
-  int bc, chunk;
-  deal(p, bc, chunk, &s_ticket);
-  const Place<CPL, NW, R> at(p, bc, chunk);
-  const int lane = at.lane, wave = at.wave, valid = at.valid;
-  const int64_t b = at.b, T_ = a.seqlen, D = a.dim, t0 = at.t0, c0 = at.c0;
-  const uint32_t lane_c = at.lane_c;
-  const uint32_t lane_bytes = at.lane_c * (uint32_t)sizeof(T);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int bc = column_of(p);
+  const Channels<CPL> ch(p, bc, lane);
+  float k[CPL];
+  bool slow;
+  const int chunk = deal(p, bc, &s_ticket, [&]() { slow = rates<CPL, DECAY>(a, ch, k); });
+  const Place<NW, R> at(p, chunk, wave);
+  const int valid = at.valid;
+  const int64_t b = ch.b, T_ = a.seqlen, D = a.dim, t0 = at.t0, c0 = ch.c0;
+  const uint32_t lane_c = ch.lane_c, lane_bytes = lane_c * (uint32_t)sizeof(T);
 
-  Rows rows{0, 0};
-  if constexpr (SEQ) rows = rows_of<R>(a.seq_idx + b * T_, t0, T_, lane);
-  const uint32_t cut = rows.first | rows.pad;
+  int32_t id = 0;
+  if constexpr (SEQ) id = id_of(a.seq_idx + b * T_, t0, T_, lane);
 
   typename V::raw xr[R], gr[R], ir[R];
-  load_rows<STREAM, T, CPL, R>({a.gate, a.gate_stride_b, a.gate_stride_t, b, at.t1, c0}, valid,
-                                lane_bytes, gr);
-  load_rows<STREAM, T, CPL, R>({a.x, a.x_stride_b, a.x_stride_t, b, at.t1, c0}, valid, lane_bytes, xr);
-  if constexpr (IG)
-    load_rows<STREAM, T, CPL, R>(
-        {a.input_gate, a.input_gate_stride_b, a.input_gate_stride_t, b, at.t1, c0}, valid, lane_bytes, ir);
-  float k[CPL];
-  bool slow = true;
-#pragma unroll
-  for (int i = 0; i < CPL; ++i) {
-    k[i] = DECAY ? decay_rate((a.decay + c0)[lane_c + i], a.decay_scale) : 0.0f;
-    slow = slow && slow_channel(k[i]);
-  }
+  load_inputs<STREAM, IG, T>(a, ch, at, lane_bytes, gr, xr, ir);
+  Rows rows{0, 0};
+  if constexpr (SEQ) rows = rows_of<R>(id, t0, valid, lane);
+  const uint32_t cut = rows.first | rows.pad;
 
   float f[R][CPL], u[R][CPL], A[CPL], H[CPL];
   auto coefficients = [&](auto is_slow) {
@@ -418,10 +460,10 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_fwd_kernel(RecParams p) {
           H0 = after(H0, mine.A[w][i][lane], mine.H[w][i][lane]);
           A0 = product(A0, mine.A[w][i][lane]);
         }
-        publish(word_row(p.pairs, b * p.chunks + chunk, D, at.c0) + at.lane_c + i, A0, H0);
+        publish(word_row(p.pairs, b * p.chunks + chunk, D, c0) + lane_c + i, A0, H0);
       }
     }
-    look_back<NW, CPL>(p, b, at.c0, at.lane_c, chunk, 1, a.initial_states, got, base, wave, lane);
+    look_back<NW, CPL>(p, b, c0, lane_c, chunk, 1, a.initial_states, got, base, wave, lane);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < CPL; ++i) h[i] = look_back_state<NW, CPL>(got, base, chunk, i, lane);
@@ -435,7 +477,7 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_fwd_kernel(RecParams p) {
   if (wave == NW - 1 && chunk % kRecGroup == kRecGroup - 1 && chunk + 1 < p.chunks) {
 #pragma unroll
     for (int i = 0; i < CPL; ++i)
-      publish(word_row(p.states, b * p.groups + chunk / kRecGroup, D, at.c0) + at.lane_c + i, 0.0f,
+      publish(word_row(p.states, b * p.groups + chunk / kRecGroup, D, c0) + lane_c + i, 0.0f,
               after(h[i], mine.A[wave][i][lane], mine.H[wave][i][lane]));
   }
   if (valid == 0) return;
@@ -445,7 +487,7 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_fwd_kernel(RecParams p) {
     for (int i = 0; i < CPL; ++i)
       (a.saved + (b * ns + t0 / CCV1D_REC_SAVED_ROWS) * D + c0)[lane_c + i] = h[i];
   }
-  RowWalk<T, CPL> out(a.out, T_ * D, D, b, t0, at.c0);
+  RowWalk<T, CPL> out(a.out, T_ * D, D, b, t0, c0);
   auto walk = [&](auto masked) {
 #pragma unroll
     for (int j = 0; j < R; ++j) {
@@ -477,8 +519,8 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_fwd_kernel(RecParams p) {
 //   without decay:  w = i x,           dgate = dh a beta m
 //
 // Bound like the forward: without decay 503 us, 5.3 TB/s of 2.68 GB, at the size given there; with decay
-// (71 operations per element) the VALUs are 65 % busy: B=4 T=8192 D=1024 bf16 120 us with the clearing
-// and the decay's sum, 3.9 TB/s; in fp32, B=3 T=5001 D=1501, 159 us, 4.0 TB/s. Rows per wave are half of
+// (71 operations per element) the VALUs are 65 % busy: B=4 T=8192 D=1024 bf16 108 us with the clearing
+// and the decay's sum, 4.3 TB/s; in fp32, B=3 T=5001 D=1501, 162 us, 3.9 TB/s. Rows per wave are half of
 // the forward's, since twice as much is held per row; 4 waves of 8 rows: 128 us where 8 were 126, and
 // 4 % more without decay.
 
@@ -500,36 +542,31 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
   __shared__ float s_rest[kKeep ? 1 : NW][kRest + kGate + kKeep][kWave][CPL];
   __shared__ uint32_t s_ticket;
   const ccv1d_rec_args& a = p.a;
-  int bc, from_end;
-  deal(p, bc, from_end, &s_ticket);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int bc = column_of(p);
+  const Channels<CPL> ch(p, bc, lane);
+  float k[CPL];
+  bool slow;
+  const int from_end = deal(p, bc, &s_ticket, [&]() { slow = rates<CPL, DECAY>(a, ch, k); });
   const int chunk = p.chunks - 1 - from_end;
-  const Place<CPL, NW, R> at(p, bc, chunk);
-  const int lane = at.lane, wave = at.wave, valid = at.valid;
-  const int64_t b = at.b, T_ = a.seqlen, D = a.dim, t0 = at.t0, c0 = at.c0;
-  const uint32_t lane_c = at.lane_c;
-  const uint32_t lane_bytes = at.lane_c * (uint32_t)sizeof(T);
+  const Place<NW, R> at(p, chunk, wave);
+  const int valid = at.valid;
+  const int64_t b = ch.b, T_ = a.seqlen, D = a.dim, t0 = at.t0, c0 = ch.c0;
+  const uint32_t lane_c = ch.lane_c, lane_bytes = lane_c * (uint32_t)sizeof(T);
 
-  Rows rows{0, 0};
-  if constexpr (SEQ) rows = rows_of<R>(a.seq_idx + b * T_, t0, T_, lane);
-  const uint32_t cut = rows.first | rows.pad;
+  int32_t id = 0;
+  if constexpr (SEQ) id = id_of(a.seq_idx + b * T_, t0, T_, lane);
 
   typename V::raw xr[R], gr[R], ir[R], yr[R];
-  load_rows<STREAM, T, CPL, R>({a.gate, a.gate_stride_b, a.gate_stride_t, b, at.t1, c0}, valid,
-                                lane_bytes, gr);
-  load_rows<STREAM, T, CPL, R>({a.x, a.x_stride_b, a.x_stride_t, b, at.t1, c0}, valid, lane_bytes, xr);
-  if constexpr (IG)
-    load_rows<STREAM, T, CPL, R>(
-        {a.input_gate, a.input_gate_stride_b, a.input_gate_stride_t, b, at.t1, c0}, valid, lane_bytes, ir);
+  load_inputs<STREAM, IG, T>(a, ch, at, lane_bytes, gr, xr, ir);
+  Rows rows{0, 0};
+  if constexpr (SEQ) rows = rows_of<R>(id, t0, valid, lane);
+  const uint32_t cut = rows.first | rows.pad;
   load_rows<STREAM, T, CPL, R>({a.dout, a.dout_stride_b, a.dout_stride_t, b, at.t1, c0}, valid,
                                 lane_bytes, yr);
-  float k[CPL], h[CPL];
-  bool slow = true;
+  float h[CPL];
 #pragma unroll
-  for (int i = 0; i < CPL; ++i) {
-    k[i] = DECAY ? decay_rate((a.decay + c0)[lane_c + i], a.decay_scale) : 0.0f;
-    slow = slow && slow_channel(k[i]);
-    h[i] = (a.saved + (b * p.chunks + chunk) * D + c0)[lane_c + i];
-  }
+  for (int i = 0; i < CPL; ++i) h[i] = (a.saved + (b * p.chunks + chunk) * D + c0)[lane_c + i];
 
   float f[R][CPL], bi[R][CPL], w[R][CPL];
   float kr[R][CPL], kn[R][CPL], kx[R][CPL];  // kKeep: r (and of kGate rows), 1 - r, x (1 - i)
@@ -665,10 +702,10 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
           G0 = after(G0, mine.A[v][i][lane], mine.H[v][i][lane]);
           A0 = product(A0, mine.A[v][i][lane]);
         }
-        publish(word_row(p.pairs, b * p.chunks + chunk, D, at.c0) + at.lane_c + i, A0, G0);
+        publish(word_row(p.pairs, b * p.chunks + chunk, D, c0) + lane_c + i, A0, G0);
       }
     }
-    look_back<NW, CPL>(p, b, at.c0, at.lane_c, from_end, -1, a.dfinal_states, got, base, wave, lane);
+    look_back<NW, CPL>(p, b, c0, lane_c, from_end, -1, a.dfinal_states, got, base, wave, lane);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < CPL; ++i) cc[i] = look_back_state<NW, CPL>(got, base, from_end, i, lane);
@@ -685,7 +722,7 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
   if (wave == 0 && from_end % kRecGroup == kRecGroup - 1 && chunk > 0) {
 #pragma unroll
     for (int i = 0; i < CPL; ++i)
-      publish(word_row(p.states, b * p.groups + from_end / kRecGroup, D, at.c0) + at.lane_c + i, 0.0f,
+      publish(word_row(p.states, b * p.groups + from_end / kRecGroup, D, c0) + lane_c + i, 0.0f,
               after(cc[i], mine.A[wave][i][lane], mine.H[wave][i][lane]));
   }
 
@@ -696,8 +733,8 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
     if constexpr (DECAY) k[i] *= kLn2;  // ln a = k r from here on
   }
   const int64_t last = t0 + valid - 1;  // stored from the last row back
-  RowWalk<T, CPL> dx(a.dx, T_ * D, D, b, last, at.c0), dg(a.dgate, T_ * D, D, b, last, at.c0);
-  RowWalk<T, CPL> di(a.dinput_gate, T_ * D, D, b, last, at.c0);
+  RowWalk<T, CPL> dx(a.dx, T_ * D, D, b, last, c0), dg(a.dgate, T_ * D, D, b, last, c0);
+  RowWalk<T, CPL> di(a.dinput_gate, T_ * D, D, b, last, c0);
   // The states again, row by row (w becomes m), then the gradients from the last row back.
   auto walk = [&](auto masked) {
     constexpr bool kMasked = decltype(masked)::value;

@@ -13,7 +13,7 @@ constexpr int kBwdWaves = 8, kBwdRows = 8;
 constexpr int kWideWaves = 16, kWideRows = kWideWaves * kFwdRows;
 
 // Forward of 129 to 256 rows in one chunk of twice the waves: no words to clear and no wait for another
-// chunk, but one workgroup a CU. B=16 T=256 D=2048 bf16 18.5 us in two chunks, 16.0 in one; D=1024
+// chunk, but one workgroup a CU. B=16 T=256 D=2048 bf16 18.5 us in two chunks, 16.0 in one (14.6 since); D=1024
 // without decay 9.9, 8.2; B=64 T=200 61.9, 58; few columns leave CUs idle (B=4 T=256 D=2048 12.2, 12.7;
 // B=2 D=512 11.4, 12.0), hence the bound of a wave column for every other CU. Shorter rows are one chunk as
 // it is (B=16 T=128 10 us in 8 waves, 14 in 16).
