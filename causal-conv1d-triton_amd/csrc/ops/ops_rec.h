@@ -76,12 +76,15 @@ __device__ __forceinline__ uint64_t await(const uint64_t* at, uint64_t v) {
   return v;
 }
 
-// The pair (A, H) after the pair (A0, H0), or after a state: A = 0 cuts.
+// The pair (A, H) after the pair (A0, H0), or after a state: A = 0 cuts, which only happens in packed
+// sequences (SEQ; elsewhere A is kTiny at the least).
+template <bool SEQ>
 __device__ __forceinline__ float after(float h, float A, float H) {
-  return A == 0.0f ? H : fmaf(A, h, H);
+  return SEQ && A == 0.0f ? H : fmaf(A, h, H);
 }
+template <bool SEQ>
 __device__ __forceinline__ float product(float A0, float A) {
-  return A == 0.0f || A0 == 0.0f ? 0.0f : fmaxf(A0 * A, kTiny);
+  return SEQ && (A == 0.0f || A0 == 0.0f) ? 0.0f : fmaxf(A0 * A, kTiny);
 }
 
 // The rows of one wave that are not plain: bit j of each mask is row t0 + j.
@@ -214,7 +217,7 @@ __device__ __forceinline__ uint64_t* word_row(uint64_t* words, int64_t row, int6
 template <int NW>
 constexpr int kLook = (kRecGroup - 2) / NW + 1;
 
-template <int NW, int CPL>
+template <bool SEQ, int NW, int CPL>
 __device__ __forceinline__ void look_back(const RecParams& p, int64_t b, int64_t c0, uint32_t lane_c,
                                           int chunk, int dir, const float* start,
                                           Pairs<NW, CPL>& got, float (&base)[CPL][kWave], int wave,
@@ -248,8 +251,8 @@ __device__ __forceinline__ void look_back(const RecParams& p, int64_t b, int64_t
           const uint64_t w = await(pair(j0 + n) + i, v[n][i]);
           const float A1 = __uint_as_float((uint32_t)w & ~kReady);
           const float H1 = __uint_as_float((uint32_t)(w >> 32));
-          H[i] = n == 0 ? H1 : after(H[i], A1, H1);
-          A[i] = n == 0 ? A1 : product(A[i], A1);
+          H[i] = n == 0 ? H1 : after<SEQ>(H[i], A1, H1);
+          A[i] = n == 0 ? A1 : product<SEQ>(A[i], A1);
         }
       }
 #pragma unroll
@@ -267,13 +270,13 @@ __device__ __forceinline__ void look_back(const RecParams& p, int64_t b, int64_t
 }
 
 // The state in front of the chunk from what look_back left, and the chunk's pair from its waves'.
-template <int NW, int CPL>
+template <bool SEQ, int NW, int CPL>
 __device__ __forceinline__ float look_back_state(const Pairs<NW, CPL>& got,
                                                  const float (&base)[CPL][kWave], int chunk, int i,
                                                  int lane) {
   float h = base[i][lane];
   const int n = chunk % kRecGroup;
-  for (int w = 0; w * kLook<NW> < n; ++w) h = after(h, got.A[w][i][lane], got.H[w][i][lane]);
+  for (int w = 0; w * kLook<NW> < n; ++w) h = after<SEQ>(h, got.A[w][i][lane], got.H[w][i][lane]);
   return h;
 }
 
@@ -457,28 +460,28 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_fwd_kernel(RecParams p) {
         float A0 = mine.A[0][i][lane], H0 = mine.H[0][i][lane];
 #pragma unroll
         for (int w = 1; w < NW; ++w) {
-          H0 = after(H0, mine.A[w][i][lane], mine.H[w][i][lane]);
-          A0 = product(A0, mine.A[w][i][lane]);
+          H0 = after<SEQ>(H0, mine.A[w][i][lane], mine.H[w][i][lane]);
+          A0 = product<SEQ>(A0, mine.A[w][i][lane]);
         }
         publish(word_row(p.pairs, b * p.chunks + chunk, D, c0) + lane_c + i, A0, H0);
       }
     }
-    look_back<NW, CPL>(p, b, c0, lane_c, chunk, 1, a.initial_states, got, base, wave, lane);
+    look_back<SEQ>(p, b, c0, lane_c, chunk, 1, a.initial_states, got, base, wave, lane);
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < CPL; ++i) h[i] = look_back_state<NW, CPL>(got, base, chunk, i, lane);
+    for (int i = 0; i < CPL; ++i) h[i] = look_back_state<SEQ>(got, base, chunk, i, lane);
   } else {
 #pragma unroll
     for (int i = 0; i < CPL; ++i) h[i] = a.initial_states ? (a.initial_states + b * D + c0)[lane_c + i] : 0.0f;
   }
   for (int w = 0; w < wave; ++w)
 #pragma unroll
-    for (int i = 0; i < CPL; ++i) h[i] = after(h[i], mine.A[w][i][lane], mine.H[w][i][lane]);
+    for (int i = 0; i < CPL; ++i) h[i] = after<SEQ>(h[i], mine.A[w][i][lane], mine.H[w][i][lane]);
   if (wave == NW - 1 && chunk % kRecGroup == kRecGroup - 1 && chunk + 1 < p.chunks) {
 #pragma unroll
     for (int i = 0; i < CPL; ++i)
       publish(word_row(p.states, b * p.groups + chunk / kRecGroup, D, c0) + lane_c + i, 0.0f,
-              after(h[i], mine.A[wave][i][lane], mine.H[wave][i][lane]));
+              after<SEQ>(h[i], mine.A[wave][i][lane], mine.H[wave][i][lane]));
   }
   if (valid == 0) return;
   if (a.saved && t0 % CCV1D_REC_SAVED_ROWS == 0) {
@@ -532,13 +535,13 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
   __shared__ float s_h[NW][CPL][kWave];
   __shared__ float base[CPL][kWave];
   // Kept per element from the coefficients to the gradients: in registers a, beta i and w (then m). One
-  // channel a lane also leaves room for r, 1 - r and x (1 - i). With two, 1 - i goes through LDS, and for
+  // channel a lane also leaves room for r, 1 - r and x (1 - i). With two, x (1 - i) goes through LDS, and for
   // the first kGate rows 1 - r, with r in registers (without decay r is a); the other rows' are made
   // again from the gate. (B=4 T=8192 D=1024 bf16, kernel and its two small ones: all made again 125 us,
-  // 1 - i in LDS 122, 4 rows' r and 1 - r too 121, 6 rows' 122. Without decay, B=4 T=16384 D=4096: 523
-  // and 515.)
+  // the first in LDS 122, 4 rows' r and 1 - r too 121, 6 rows' 122; without an input gate 8 rows' need a
+  // register more than there are. Without decay, B=4 T=16384 D=4096: 523 and 515.)
   constexpr bool kKeep = CPL == 1;
-  constexpr int kGate = kKeep ? 0 : IG ? R / 2 : R, kRest = kKeep || !IG ? 0 : R;
+  constexpr int kGate = kKeep ? 0 : IG ? R / 2 : DECAY ? R - 2 : R, kRest = kKeep || !IG ? 0 : R;
   __shared__ float s_rest[kKeep ? 1 : NW][kRest + kGate + kKeep][kWave][CPL];
   __shared__ uint32_t s_ticket;
   const ccv1d_rec_args& a = p.a;
@@ -597,7 +600,9 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
           sigmoid_pair<T>(ig[i], in, not_in);
           kx[j][i] = x[i] * not_in;
         } else if constexpr (IG) {
-          sigmoid_and_rest<T>(ig[i], in, s_rest[wave][j][lane][i]);
+          float not_in;
+          sigmoid_and_rest<T>(ig[i], in, not_in);
+          s_rest[wave][j][lane][i] = x[i] * not_in;
         }
         if constexpr (DECAY) {
           if constexpr (kKeep) {
@@ -613,8 +618,9 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
           f[j][i] = __builtin_amdgcn_exp2f(l);
           const float s = one_minus_square<decltype(is_slow)::value>(tail[i], l, f[j][i]);
           const float inv = __builtin_amdgcn_rsqf(fmaxf(s, kTiny));
-          bi[j][i] = s * inv * in;
-          w[j][i] = in * x[i] * (f[j][i] * inv);
+          const float ib = in * inv;
+          bi[j][i] = s * ib;
+          w[j][i] = x[i] * (f[j][i] * ib);
         } else {
           float beta;
           sigmoid_pair<T>(g[i], f[j][i], beta);
@@ -699,31 +705,31 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
         float A0 = mine.A[NW - 1][i][lane], G0 = mine.H[NW - 1][i][lane];
 #pragma unroll
         for (int v = NW - 2; v >= 0; --v) {
-          G0 = after(G0, mine.A[v][i][lane], mine.H[v][i][lane]);
-          A0 = product(A0, mine.A[v][i][lane]);
+          G0 = after<SEQ>(G0, mine.A[v][i][lane], mine.H[v][i][lane]);
+          A0 = product<SEQ>(A0, mine.A[v][i][lane]);
         }
         publish(word_row(p.pairs, b * p.chunks + chunk, D, c0) + lane_c + i, A0, G0);
       }
     }
-    look_back<NW, CPL>(p, b, c0, lane_c, from_end, -1, a.dfinal_states, got, base, wave, lane);
+    look_back<SEQ>(p, b, c0, lane_c, from_end, -1, a.dfinal_states, got, base, wave, lane);
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < CPL; ++i) cc[i] = look_back_state<NW, CPL>(got, base, from_end, i, lane);
+    for (int i = 0; i < CPL; ++i) cc[i] = look_back_state<SEQ>(got, base, from_end, i, lane);
   } else {
 #pragma unroll
     for (int i = 0; i < CPL; ++i) cc[i] = a.dfinal_states ? (a.dfinal_states + b * D + c0)[lane_c + i] : 0.0f;
   }
   for (int v = NW - 1; v > wave; --v)
 #pragma unroll
-    for (int i = 0; i < CPL; ++i) cc[i] = after(cc[i], mine.A[v][i][lane], mine.H[v][i][lane]);
+    for (int i = 0; i < CPL; ++i) cc[i] = after<SEQ>(cc[i], mine.A[v][i][lane], mine.H[v][i][lane]);
   for (int v = 0; v < wave; ++v)
 #pragma unroll
-    for (int i = 0; i < CPL; ++i) h[i] = after(h[i], mine.A[v][i][lane], s_h[v][i][lane]);
+    for (int i = 0; i < CPL; ++i) h[i] = after<SEQ>(h[i], mine.A[v][i][lane], s_h[v][i][lane]);
   if (wave == 0 && from_end % kRecGroup == kRecGroup - 1 && chunk > 0) {
 #pragma unroll
     for (int i = 0; i < CPL; ++i)
       publish(word_row(p.states, b * p.groups + from_end / kRecGroup, D, c0) + lane_c + i, 0.0f,
-              after(cc[i], mine.A[wave][i][lane], mine.H[wave][i][lane]));
+              after<SEQ>(cc[i], mine.A[wave][i][lane], mine.H[wave][i][lane]));
   }
 
   float sum[CPL];
@@ -753,14 +759,12 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
     for (int j = R - 1; j >= 0; --j) {
       if (j >= valid) continue;
       if constexpr (!kKeep) {
-        forget_row(xr[j]);
         if (j >= kGate) forget_row(gr[j]);
         forget_row(yr[j]);
       }
       const bool pad = kMasked && (rows.pad >> j & 1);
-      float y[CPL], x[CPL], g[CPL], ox[CPL], og[CPL], oi[CPL];
+      float y[CPL], g[CPL], ox[CPL], og[CPL], oi[CPL];
       V::unpack(yr[j], y);
-      V::unpack(xr[j], x);
       V::unpack(gr[j], g);
 #pragma unroll
       for (int i = 0; i < CPL; ++i) {
@@ -770,7 +774,7 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
         if constexpr (IG && kKeep) {
           oi[i] = ox[i] * kx[j][i];
         } else if constexpr (IG) {
-          oi[i] = ox[i] * (x[i] * s_rest[wave][j][lane][i]);
+          oi[i] = ox[i] * s_rest[wave][j][lane][i];
         }
         float r, not_r;
         if constexpr (kKeep) r = kr[j][i], not_r = kn[j][i];
