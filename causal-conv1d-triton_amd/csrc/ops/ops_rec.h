@@ -346,8 +346,8 @@ __device__ __forceinline__ void load_inputs(const ccv1d_rec_args& a, const Chann
 // ------------------------------------------------------------------------------------- forward
 //
 // Bound by memory without decay: B=4 T=16384 D=4096 bf16 without an input gate 295 us, 5.5 TB/s of its
-// 1.61 GB. With decay (6 of its 31 operations per element are transcendental, at half rate) memory and
-// arithmetic, the VALUs 58 % busy: B=4 T=8192 D=1024 bf16 62 us with the clearing, 4.3 TB/s; in fp32,
+// 1.61 GB. With decay (6 of its 30 operations per element are transcendental, at half rate) memory and
+// arithmetic, the VALUs 60 % busy: B=4 T=8192 D=1024 bf16 62 us with the clearing, 4.3 TB/s; in fp32,
 // B=3 T=5001 D=1501, 86 us, 4.2 TB/s. 8 waves of 16 rows at 4 waves per SIMD: 4 waves of 16 rows
 // took 1 % more with decay and 1 % less without, 8 waves of 8 rows 6 and 14 % more.
 
@@ -522,8 +522,8 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_fwd_kernel(RecParams p) {
 //   without decay:  w = i x,           dgate = dh a beta m
 //
 // Bound like the forward: without decay 503 us, 5.3 TB/s of 2.68 GB, at the size given there; with decay
-// (71 operations per element) the VALUs are 65 % busy: B=4 T=8192 D=1024 bf16 108 us with the clearing
-// and the decay's sum, 4.3 TB/s; in fp32, B=3 T=5001 D=1501, 162 us, 3.9 TB/s. Rows per wave are half of
+// (66 operations per element) the VALUs are 72 % busy: B=4 T=8192 D=1024 bf16 106 us with the clearing
+// and the decay's sum, 4.4 TB/s; in fp32, B=3 T=5001 D=1501, 161 us, 3.9 TB/s. Rows per wave are half of
 // the forward's, since twice as much is held per row; 4 waves of 8 rows: 128 us where 8 were 126, and
 // 4 % more without decay.
 
