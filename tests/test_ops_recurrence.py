@@ -374,3 +374,27 @@ def test_update_skips_rows_outside_the_pool():
     gated_recurrence_update(t["x"][:4, 0].to(DEV), t["gate"][:4, 0].to(DEV), state)
     want = oracle.recurrence(t["x"][:4], t["gate"][:4], None, None, None, pool[:, :70])
     oracle.assert_close(state, want["final"])
+
+
+def test_offsets_past_32_bits():
+    """Batch rows, time rows and slots further apart than 32 bits of elements."""
+    n = 2 ** 32 + 5 * 70
+    store = torch.zeros(n, dtype=BF, device=DEV)
+    t = make(18, 2, 5, 70, BF)
+    d = {k: None if v is None else v.to(DEV) for k, v in t.items()}
+    want = gated_recurrence_fn(d["x"], d["gate"], d["decay"], d["igate"])
+    x = store.as_strided((2, 5, 70), (2 ** 32, 70, 1))
+    x.copy_(d["x"])
+    assert torch.equal(gated_recurrence_fn(x, d["gate"], d["decay"], d["igate"]), want)
+    x = store.as_strided((1, 3, 70), (70, 2 ** 31, 1))
+    x.copy_(d["x"][:1, :3])
+    cut = [d[k][:1, :3] for k in ("gate", "igate")]
+    assert torch.equal(gated_recurrence_fn(x, cut[0], d["decay"], cut[1]), want[:1, :3])
+    pool = store[:2 ** 32].view(F).as_strided((2, 70), (2 ** 31 - 70, 1))
+    pool.copy_(torch.ones(2, 70))
+    small = pool.clone()
+    args = (d["x"][:, 0], d["gate"][:, 0])
+    idx = torch.tensor([1, 0], device=DEV)
+    out = gated_recurrence_update(*args, pool, d["decay"], state_indices=idx)
+    assert torch.equal(out, gated_recurrence_update(*args, small, d["decay"], state_indices=idx))
+    assert torch.equal(pool, small)
