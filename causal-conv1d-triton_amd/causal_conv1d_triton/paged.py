@@ -96,8 +96,8 @@ def paged_attention(
       softmax_scale: head_dim ** -0.5 by default.
       request_ids: optional (rows,) integers: the request of each row (row r is request r without), for
          the tokens of a prompt (seq_lens = positions + 1). A negative one makes a row empty.
-      max_seq_len: optional bound of seq_lens, which sizes the launch; the table's capacity by default.
-         Positions past it are left out.
+      max_seq_len: optional bound of seq_lens, which sizes the launch; the table's capacity by default,
+         and where it is 0. Positions past it are left out.
       return_lse: also return the log-sum-exp of the scores, (rows, q_heads) fp32, -inf for empty rows.
 
     Returns out (rows, q_heads, head_dim) in q's dtype, or (out, lse). Softmax and sums are fp32.
