@@ -76,39 +76,6 @@ def _op_backward(ctx, dout, dfinal, _):
 _fwd_op.register_autograd(_op_backward, setup_context=_op_setup)
 
 
-class _GatedRecurrenceFn(torch.autograd.Function):
-    """Eager autograd node. Kept for the backward: the inputs, and the state in front of every 64th
-    row in fp32, from which the backward makes the states between again."""
-
-    @staticmethod
-    def forward(ctx, x, gate, decay, input_gate, seq_idx, initial_states, return_final, decay_scale):
-        out, final, saved = native().rec_fwd(x, gate, decay, input_gate, seq_idx, initial_states,
-                                             decay_scale, return_final, True)
-        ctx.save_for_backward(x, gate, decay, input_gate, seq_idx, initial_states, saved)
-        ctx.decay_scale = decay_scale
-        ctx.set_materialize_grads(False)
-        return out, final
-
-    @staticmethod
-    def backward(ctx, dout, dfinal):
-        # Second derivatives are refused; without a graph to record, the wrapper that does so (6 us of
-        # the host) has nothing to do.
-        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, dout, dfinal)
-
-
-def _backward(ctx, dout, dfinal):
-    x, gate, decay, input_gate, seq_idx, init, saved = ctx.saved_tensors
-    if dout is None:
-        dout = torch.zeros(x.shape, device=x.device, dtype=x.dtype)
-    need = init is not None and ctx.needs_input_grad[5]
-    dx, dgate, ddecay, dig, dinit = native().rec_bwd(
-        x, gate, decay, input_gate, seq_idx, init, ctx.decay_scale, saved, dout, dfinal, need)
-    return dx, dgate, ddecay, dig, None, dinit, None, None
-
-
-_backward_once = torch.autograd.function.once_differentiable(_backward)
-
-
 def gated_recurrence_fn(
     x: Tensor,
     gate: Tensor,
@@ -144,8 +111,8 @@ def gated_recurrence_fn(
     elif torch.is_grad_enabled() and any(
             getattr(t, "requires_grad", False)
             for t in (x, gate, decay, input_gate, initial_states)):
-        out, final = _GatedRecurrenceFn.apply(x, gate, decay, input_gate, seq_idx, initial_states,
-                                              return_final_states, decay_scale)
+        out, final = native().rec_train(x, gate, decay, input_gate, seq_idx, initial_states,
+                                        decay_scale, return_final_states)
     else:
         out, final, _ = native().rec_fwd(x, gate, decay, input_gate, seq_idx, initial_states,
                                          decay_scale, return_final_states, False)

@@ -325,6 +325,34 @@ def test_second_derivatives_are_refused():
         g.sum().backward()
 
 
+def test_second_derivatives_are_refused_where_the_incoming_gradient_is_a_constant():
+    """The gradient still depends on x, so a sum with x must not leave that part out silently."""
+    x = torch.randn(1, 5, 8, device=DEV, requires_grad=True)
+    h0 = torch.randn(1, 8, device=DEV, requires_grad=True)
+    out, fin = gated_recurrence_fn(x, x, initial_states=h0, return_final_states=True)
+    g, gh = torch.autograd.grad(out.sum() + fin.sum(), [x, h0], create_graph=True)
+    with pytest.raises(RuntimeError):
+        ((g * x).sum() + gh.sum()).backward()
+
+
+def test_gradients_of_some_inputs_and_twice():
+    """A graph that is kept gives the same bits again; gradients of a part of the inputs are those of all."""
+    t = make(16, 2, 130, 66, BF, init=True)
+    d = {k: None if v is None else v.to(DEV) for k, v in t.items()}
+    names = ("x", "gate", "decay", "igate", "init")
+    for k in names:
+        d[k].requires_grad_(True)
+    out = gated_recurrence_fn(d["x"], d["gate"], d["decay"], d["igate"], None, d["init"])
+    every = torch.autograd.grad(out, [d[k] for k in names], d["dy"], retain_graph=True)
+    for k, g in zip(names, every):
+        (again,) = torch.autograd.grad(out, [d[k]], d["dy"], retain_graph=True)
+        assert again.dtype == d[k].dtype and torch.equal(again, g)
+    with torch.no_grad():
+        d["x"].mul_(2)
+    with pytest.raises(RuntimeError):  # an input that was changed since
+        torch.autograd.grad(out, [d["gate"]], d["dy"])
+
+
 @pytest.mark.parametrize("R,D", [(1, 1), (1, 130), (5, 66), (16, 2048), (300, 97)])
 @pytest.mark.parametrize("dtype", [BF, HF, F])
 @pytest.mark.parametrize("decay", [True, False])
