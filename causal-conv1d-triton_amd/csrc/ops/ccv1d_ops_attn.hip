@@ -86,7 +86,8 @@ AttnParams plan(const ccv1d_paged_attn_args& a) {
   // 16 rows of 512 to 4096 of those 47, 43, 42; 32 rows of 1000 to 3000, heads of 64 46, 48, 44. Most
   // positions: 64 requests of 512 to 8192, 8 key heads of 128: 2048 254 us, 1024 228; two rows of 131072:
   // 197, 196. Least: 16 rows of a 1024 window, one key head of 256: 256 15.7 us, 128 13.1.)
-  const int64_t target = (int64_t(1) << 18) / (a.head_dim * (a.dtype == CCV1D_F32 ? 4 : 2));
+  const int64_t row_bytes = a.head_dim * (a.dtype == CCV1D_F32 ? 4 : 2);
+  const int64_t target = (int64_t(1) << 18) / row_bytes;
   int64_t most = a.window && a.window + 31 < limit ? a.window + 31 : limit;
   if (most < 1) most = 1;
   const int64_t wgs = a.rows * a.kv_heads * p.tiles;
@@ -94,6 +95,14 @@ AttnParams plan(const ccv1d_paged_attn_args& a) {
   int64_t span = (most + splits - 1) / splits;
   if (span > 1024) span = 1024;
   if (span < 128) span = 128;
+  // One span, and with it no join, where that saves more than the split: with 256 workgroups, one a CU, up
+  // to 1024 positions (and a window's 31 of rounding), with fewer up to 512 positions of 100 KiB of keys.
+  // (Split and whole, us, every row of the stated length, then lengths from 1 to it: heads of 128 bf16, 512
+  // workgroups, 384 positions 30.2 and 22.9, 19.8 and 15.1; 1024 62.2 and 53.1, 40.2 and 38.4; 256
+  // workgroups, 1024 35.9 and 29.2, 24.3 and 25.3; 64 workgroups, 384 9.9 and 9.2, 9.5 and 8.9; 512 10.5
+  // and 11.0, 9.6 and 10.7; heads of 64, 64 workgroups, 512 9.0 and 8.9, 8.3 and 7.6; heads of 256, 64
+  // workgroups, 200 12.2 and 10.6, 11.7 and 10.0; 384 13.3 and 14.5.)
+  if (wgs >= 256 ? most <= 1024 + 31 : most <= 512 && most * row_bytes <= 100 << 10) span = most;
   if (span < (most + 255) / 256) span = (most + 255) / 256;
   span = (span + 127) / 128 * 128;
   p.span = (int32_t)span;

@@ -201,6 +201,23 @@ def test_attention_long(dtype):
     check_attn(3, [7000, 100, 6999], 16, 1, 256, 32, dtype, window=4000)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+@pytest.mark.parametrize("Dh", [8, 16, 40, 64, 72, 96, 120, 128, 136, 192, 200, 256])
+def test_attention_joined_head_sizes(dtype, Dh):
+    check_attn(Dh + 1, [1300, 5, 0, 131, 700], 4, 2, Dh, 16, dtype)
+
+
+@pytest.mark.parametrize("R,Dh,most", [(3, 128, 400), (3, 128, 401), (3, 64, 512), (3, 64, 513), (3, 256, 200),
+                                       (3, 256, 201), (127, 64, 513), (128, 64, 513), (128, 64, 1055),
+                                       (128, 64, 1056)])
+def test_attention_whole_and_split_rows(R, Dh, most):
+    """Either side of the sizes at which rows are split over workgroups."""
+    lens = [most, 0, most - 1] + [n * 37 % 140 for n in range(R - 4)] + [most] * (R > 3)
+    check_attn(most, lens, 4, 2, Dh, 16, BF, max_seq_len=most)
+    if R > 3:
+        check_attn(most + 1, lens, 4, 2, Dh, 20, HF, window=most - 300)
+
+
 def test_attention_many_rows():
     check_attn(4, [n % 97 for n in range(700)], 4, 2, 64, 16, BF)
 
