@@ -323,8 +323,9 @@ struct Interpreter {
 
 /* The autograd node of gated_recurrence_fn. Kept for the backward: the inputs, and the state in front of
  * every 64th row in fp32, from which the backward makes the states between again. In C++ because a
- * training call of little work is bound by the host, and a Python node is a part of that (B=11 T=38 D=3693
- * bf16 without decay, forward and backward: Python 72 us, C++ 60; B=3 T=159 D=320 with decay 97 and 83). */
+ * training call of little work is bound by the host, and a Python node is a part of that (forward and backward
+ * on one machine, runs in turn, which differ by when the engine's thread wakes: B=11 T=38 D=3693 bf16 without
+ * decay Python 78 to 81 us, C++ 38 to 65; B=3 T=159 D=320 with decay 105 to 109 and 56 to 93). */
 struct RecNode : torch::autograd::Function<RecNode> {
   using Maybe = std::optional<at::Tensor>;
   using Context = torch::autograd::AutogradContext;
