@@ -71,6 +71,9 @@ __global__ __launch_bounds__(kJoinWaves * 64) void paged_join_kernel(AttnParams 
 AttnParams plan(const ccv1d_paged_attn_args& a) {
   AttnParams p{};
   p.a = a;
+  // A window that no int32 length passes is none (and sums with it stay in range).
+  if (a.window >= INT32_MAX) p.a.window = 0;
+  const int64_t window = p.a.window;
   p.by_page = divisor(a.page_size);
   p.group = (int32_t)(a.q_heads / a.kv_heads);
   p.tiles = (p.group + kAttnHeads - 1) / kAttnHeads;
@@ -88,7 +91,7 @@ AttnParams plan(const ccv1d_paged_attn_args& a) {
   // 197, 196. Least: 16 rows of a 1024 window, one key head of 256: 256 15.7 us, 128 13.1.)
   const int64_t row_bytes = a.head_dim * (a.dtype == CCV1D_F32 ? 4 : 2);
   const int64_t target = (int64_t(1) << 18) / row_bytes;
-  int64_t most = a.window && a.window + 31 < limit ? a.window + 31 : limit;
+  int64_t most = window && window + 31 < limit ? window + 31 : limit;
   if (most < 1) most = 1;
   const int64_t wgs = a.rows * a.kv_heads * p.tiles;
   int64_t splits = (target + wgs - 1) / wgs;

@@ -233,6 +233,21 @@ def test_paged_attn_workspace(lib):
     assert ws(max_pages=1 << 20, window=97) == 0
 
 
+def test_paged_attn_windows_past_every_length(lib):
+    """A window that no length reaches is none, up to the largest that the argument holds: the launch is
+    sized for the table, and the sums of its spans have a place."""
+    for kw in (dict(max_pages=1000), dict(rows=64, requests=64, q_heads=32, head_dim=128, max_pages=512),
+               dict(max_pages=1000, max_seq_len=9000)):
+        none = lib.ccv1d_paged_attn_workspace_bytes(C.byref(attn(**kw)))
+        assert none > 0
+        for window in (kw["max_pages"] * 16, 2 ** 31 - 32, 2 ** 31 - 1, 2 ** 31, 2 ** 63 - 32, 2 ** 63 - 31,
+                       2 ** 63 - 1):
+            a = attn(**kw, window=window)
+            assert lib.ccv1d_paged_attn_workspace_bytes(C.byref(a)) == none, window
+        a = attn(**kw, window=2 ** 63 - 1, workspace=0, workspace_bytes=0)
+        _refused(lib, lib.ccv1d_paged_attn, a, 3, "workspace")
+
+
 def test_empty_requests_are_no_ops(lib):
     assert lib.ccv1d_rec_fwd(C.byref(rec(batch=0))) == 0
     assert lib.ccv1d_rec_fwd(C.byref(rec(dim=0))) == 0

@@ -193,6 +193,18 @@ def test_attention_window(window, ps):
     check_attn(window, LENS[::3], 4, 1, 128, ps, F, window=window)
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 32, 2 ** 31 - 1, 2 ** 31, 2 ** 63 - 31, 2 ** 63 - 1])
+def test_attention_window_past_every_length(window):
+    """Rows that are split, with a window that reaches past every length: the bits of no window."""
+    lens = [1, 0, 5000, 129]
+    kc, vc, tables = caches(8, lens, 2, 64, 16, BF)
+    q = torch.randn(4, 4, 64, generator=torch.Generator().manual_seed(2)).to(BF).to(DEV)
+    args = (q, kc.to(DEV), vc.to(DEV), tables.to(DEV), torch.tensor(lens, device=DEV))
+    want = paged_attention(*args, return_lse=True)
+    got = paged_attention(*args, window=window, return_lse=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 @pytest.mark.parametrize("dtype", [BF, HF, F])
 def test_attention_long(dtype):
     """Lengths that are split over workgroups and joined, beside short ones."""
