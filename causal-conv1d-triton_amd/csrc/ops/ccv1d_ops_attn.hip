@@ -106,7 +106,13 @@ AttnParams plan(const ccv1d_paged_attn_args& a) {
   // and 11.0, 9.6 and 10.7; heads of 64, 64 workgroups, 512 9.0 and 8.9, 8.3 and 7.6; heads of 256, 64
   // workgroups, 200 12.2 and 10.6, 11.7 and 10.0; 384 13.3 and 14.5.)
   if (wgs >= 256 ? most <= 1024 + 31 : most <= 512 && most * row_bytes <= 100 << 10) span = most;
-  if (span < (most + 255) / 256) span = (most + 255) / 256;
+  // The sums of the spans take at most 512 MiB: many rows (a prompt's, say) beside a long table fill the card
+  // with fewer spans each. It bounds the workgroups too: below 2^24, as a launch of 256 threads each has to be.
+  const int64_t sums = a.rows * a.q_heads * (a.head_dim + 2) * 4;
+  int64_t spans = (int64_t(512) << 20) / (sums > 0 ? sums : 1);
+  if (spans > 256) spans = 256;
+  if (spans < 1) spans = 1;
+  if (span < (most + spans - 1) / spans) span = (most + spans - 1) / spans;
   span = (span + 127) / 128 * 128;
   p.span = (int32_t)span;
   p.splits = (int32_t)((most + span - 1) / span);

@@ -248,6 +248,25 @@ def test_paged_attn_windows_past_every_length(lib):
         _refused(lib, lib.ccv1d_paged_attn, a, 3, "workspace")
 
 
+@pytest.mark.parametrize("rows,q_heads,kv_heads,head_dim,positions", [
+    (2048, 32, 8, 128, 131072), (8192, 32, 8, 128, 131072), (8192, 32, 8, 128, 262144),
+    (16384, 32, 8, 128, 131072), (1000, 64, 64, 256, 1 << 20), (100000, 8, 8, 8, 1 << 20),
+    (8388607, 1, 1, 8, 1 << 20), (131071, 64, 1, 64, 1 << 30)])
+def test_paged_attn_many_rows_of_a_long_table(lib, rows, q_heads, kv_heads, head_dim, positions):
+    """Where the rows alone fill the card, the table's capacity does not size the workspace, and no launch
+    has 2^32 threads (256 a workgroup; the join: 64 for four spans, at most 1024)."""
+    a = attn(rows=rows, requests=rows, q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim,
+             max_pages=positions // 16, num_pages=positions)
+    need = lib.ccv1d_paged_attn_workspace_bytes(C.byref(a))
+    assert need <= 512 << 20
+    each = rows * q_heads * (head_dim + 2) * 4
+    assert need % each == 0
+    splits = max(1, need // each)
+    tiles = -(-(q_heads // kv_heads) // 16)
+    assert rows * splits * kv_heads * tiles * 256 < 2 ** 32
+    assert splits == 1 or rows * q_heads * min(1024, 64 * -(-splits // 4)) < 2 ** 32
+
+
 def test_empty_requests_are_no_ops(lib):
     assert lib.ccv1d_rec_fwd(C.byref(rec(batch=0))) == 0
     assert lib.ccv1d_rec_fwd(C.byref(rec(dim=0))) == 0
