@@ -9,6 +9,7 @@ using namespace ccv1d;
 namespace {
 
 constexpr int64_t kMaxGrid = (int64_t(1) << 31) - 1;
+constexpr int64_t kMaxThreads = (int64_t(1) << 32) - 1;  // of a launch
 
 int fail(int code, const char* fmt, ...) {
   char buf[256];
@@ -60,6 +61,8 @@ int check_rec(const ccv1d_rec_args* a, bool backward) {
       !product_within(a->batch, cdiv(a->dim, 64), kMaxGrid) ||
       !product_within(a->batch * cdiv(a->dim, 64), cdiv(a->seqlen, CCV1D_REC_SAVED_ROWS), kMaxGrid))
     return fail(CCV1D_ERR_UNSUPPORTED, "batch, seqlen and dim too large for one launch");
+  if (ops::rec_threads(*a, backward) > kMaxThreads)
+    return fail(CCV1D_ERR_UNSUPPORTED, "batch, seqlen and dim too large for one launch");
   if (a->batch == 0 || a->dim == 0) return CCV1D_OK;
   if (a->seqlen > 0) {
     if (!a->x || !a->gate) return invalid("x or gate is null");
@@ -94,6 +97,7 @@ int check_attn(const ccv1d_paged_attn_args* a) {
     return invalid("q_heads must be a multiple of kv_heads");
   if (a->page_size > (int64_t(1) << 30) || !product_within(a->max_pages, a->page_size, int64_t(1) << 30))
     return fail(CCV1D_ERR_UNSUPPORTED, "max_pages * page_size must be at most 2^30");
+  // The spans are planned for fewer than 2^32 threads where this holds.
   if (!product_within(a->rows, a->q_heads, kMaxGrid / 256))
     return fail(CCV1D_ERR_UNSUPPORTED, "rows * q_heads too large for one launch");
   return CCV1D_OK;
@@ -130,7 +134,7 @@ int ccv1d_rec_update(const struct ccv1d_rec_update_args* args) {
   if (!dtype_ok(a.dtype)) return invalid("dtype must be fp32, fp16 or bf16");
   if (!(a.decay_scale >= 0.0f)) return invalid("decay_scale must not be negative");
   if (!a.state_indices && a.rows > a.slots) return invalid("more rows than slots");
-  if (!product_within(a.rows, cdiv(a.dim, 64), kMaxGrid))
+  if (!product_within(a.rows, cdiv(a.dim, 64), kMaxGrid) || ops::rec_update_threads(a) > kMaxThreads)
     return fail(CCV1D_ERR_UNSUPPORTED, "rows and dim too large for one launch");
   if (a.rows == 0 || a.dim == 0) return CCV1D_OK;
   if (!a.x || !a.gate || !a.out || (a.slots && !a.state))
@@ -171,6 +175,8 @@ int ccv1d_paged_write(const struct ccv1d_paged_write_args* args) {
     return fail(CCV1D_ERR_UNSUPPORTED, "tokens or kv_heads * head_dim too large for one launch");
   if (!product_within(a.num_pages, a.page_size, INT64_MAX)) return invalid("cache too large");
   if (a.tokens == 0 || a.kv_heads == 0 || a.head_dim == 0 || a.num_pages == 0) return CCV1D_OK;
+  if (ops::paged_write_threads(a) > kMaxThreads)
+    return fail(CCV1D_ERR_UNSUPPORTED, "tokens too large for one launch");
   if (!a.k || !a.v || !a.k_cache || !a.v_cache || !a.slot_mapping)
     return invalid("k, v, a cache or slot_mapping is null");
   return launch(a, ops::paged_write);

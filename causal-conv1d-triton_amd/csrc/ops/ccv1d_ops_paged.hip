@@ -193,15 +193,27 @@ __global__ __launch_bounds__(kWriteThreads) void paged_write_kernel(ccv1d_paged_
   }
 }
 
+// Whether heads are whole numbers of 16-byte pieces.
+bool write_wide(const ccv1d_paged_write_args& a) { return a.head_dim % (a.dtype == CCV1D_F32 ? 4 : 8) == 0; }
+
+int write_per_head(const ccv1d_paged_write_args& a) {
+  return (int)(a.head_dim * (a.dtype == CCV1D_F32 ? 4 : 2) / (write_wide(a) ? 16 : 2));
+}
+
+// Tokens of a workgroup: small ones share it, two pieces a lane.
+int write_tokens(const ccv1d_paged_write_args& a) {
+  const int64_t pieces = 2 * a.kv_heads * write_per_head(a);
+  return pieces < 2 * kWriteThreads ? (int)(2 * kWriteThreads / pieces) : 1;
+}
+
+int64_t write_grid(const ccv1d_paged_write_args& a) {
+  const int tokens = write_tokens(a);
+  return (a.tokens + tokens - 1) / tokens;
+}
+
 template <typename V>
 hipError_t write_as(const ccv1d_paged_write_args& a, hipStream_t s) {
-  const int64_t es = a.dtype == CCV1D_F32 ? 4 : 2;
-  const int per_head = (int)(a.head_dim * es / (int64_t)sizeof(V));
-  const int64_t pieces = 2 * a.kv_heads * per_head;
-  // Small tokens share a workgroup, two pieces a lane.
-  const int tokens = pieces < 2 * kWriteThreads ? (int)(2 * kWriteThreads / pieces) : 1;
-  return start(&paged_write_kernel<V>, (a.tokens + tokens - 1) / tokens, kWriteThreads, s, a, per_head,
-               tokens);
+  return start(&paged_write_kernel<V>, write_grid(a), kWriteThreads, s, a, write_per_head(a), write_tokens(a));
 }
 
 }  // namespace
@@ -213,9 +225,10 @@ hipError_t paged_plan(const ccv1d_paged_plan_args& a, hipStream_t s) {
 
 hipError_t paged_write(const ccv1d_paged_write_args& a, hipStream_t s) {
   typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
-  const bool wide = a.head_dim % (a.dtype == CCV1D_F32 ? 4 : 8) == 0;
-  return wide ? write_as<u4>(a, s) : write_as<uint16_t>(a, s);
+  return write_wide(a) ? write_as<u4>(a, s) : write_as<uint16_t>(a, s);
 }
+
+int64_t paged_write_threads(const ccv1d_paged_write_args& a) { return write_grid(a) * kWriteThreads; }
 
 }  // namespace ops
 }  // namespace ccv1d

@@ -118,10 +118,14 @@ __global__ __launch_bounds__(64) void rec_update_kernel(ccv1d_rec_update_args p,
   }
 }
 
+int64_t update_cols(const ccv1d_rec_update_args& a) {
+  constexpr int kColumn = 64 * kUpdateChannels;
+  return (a.dim + kColumn - 1) / kColumn;
+}
+
 template <typename T>
 hipError_t update_t(const ccv1d_rec_update_args& a, hipStream_t s) {
-  constexpr int kColumn = 64 * kUpdateChannels;
-  const int64_t cols = (a.dim + kColumn - 1) / kColumn, grid = a.rows * cols;
+  const int64_t cols = update_cols(a), grid = a.rows * cols;
   return a.decay ? start(&rec_update_kernel<T, true>, grid, 64, s, a, cols, divisor(cols))
                  : start(&rec_update_kernel<T, false>, grid, 64, s, a, cols, divisor(cols));
 }
@@ -187,6 +191,19 @@ size_t rec_workspace(int64_t B, int64_t T, int64_t D, bool backward) {
   const Plan p = plan_of(B, T, D, backward);
   return (size_t)p.words * 8 + (size_t)p.part * 4;
 }
+
+int64_t rec_threads(const ccv1d_rec_args& a, bool backward) {
+  const int64_t width = kWave * (a.dtype == CCV1D_F32 || a.dim == 1 ? 1 : 2);  // as the launches take it
+  const int64_t columns = a.batch * ((a.dim + width - 1) / width);
+  const int64_t main = rec_one_chunk(a, backward)
+                           ? columns * kWideWaves * kWave
+                           : columns * plan_of(a.batch, a.seqlen, a.dim, backward).chunks *
+                                 (backward ? kBwdWaves : kFwdWaves) * kWave;
+  const int64_t sum = backward && a.decay ? (a.dim + 31) / 32 * 1024 : 0;
+  return main > sum ? main : sum;
+}
+
+int64_t rec_update_threads(const ccv1d_rec_update_args& a) { return a.rows * update_cols(a) * 64; }
 
 hipError_t rec_fwd(const ccv1d_rec_args& a, hipStream_t s) { return run(a, false, s); }
 hipError_t rec_bwd(const ccv1d_rec_args& a, hipStream_t s) { return run(a, true, s); }

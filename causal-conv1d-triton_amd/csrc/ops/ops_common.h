@@ -54,6 +54,11 @@ hipError_t start(void (*kernel)(P...), int64_t grid, int block, hipStream_t s, c
       held);
 }
 
+// Threads of a call's largest launch, which have to be fewer than 2^32.
+int64_t rec_threads(const ccv1d_rec_args& a, bool backward);
+int64_t rec_update_threads(const ccv1d_rec_update_args& a);
+int64_t paged_write_threads(const ccv1d_paged_write_args& a);
+
 // Launchers (arguments checked, device current).
 hipError_t rec_fwd(const ccv1d_rec_args& a, hipStream_t s);
 hipError_t rec_bwd(const ccv1d_rec_args& a, hipStream_t s);

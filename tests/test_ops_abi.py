@@ -267,6 +267,34 @@ def test_paged_attn_many_rows_of_a_long_table(lib, rows, q_heads, kv_heads, head
     assert splits == 1 or rows * q_heads * min(1024, 64 * -(-splits // 4)) < 2 ** 32
 
 
+@pytest.mark.parametrize("fn,args", [
+    # 512 threads for 64 channels (16 bits: 128, but for a single one) and 128 rows, backward 64 rows
+    ("rec_fwd", dict(batch=1, dim=1, seqlen=(1 << 30) + 1)),
+    ("rec_fwd", dict(batch=1 << 23, dim=1)),
+    ("rec_fwd", dict(batch=1 << 22, dim=130, seqlen=1)),
+    ("rec_fwd", dict(batch=1 << 22, dim=65, seqlen=1, dtype=F32)),
+    # one chunk of 1024 threads
+    ("rec_fwd", dict(batch=1 << 22, dim=128, seqlen=200)),
+    ("rec_bwd", dict(batch=1, dim=1, seqlen=(1 << 29) + 1)),
+    ("rec_bwd", dict(batch=1 << 23, dim=1)),
+    # 1024 threads for 32 channels of the decay's sum
+    ("rec_bwd", dict(batch=1, dim=1 << 27, seqlen=1, decay=4096, ddecay=4096)),
+])
+def test_recurrence_of_2_32_threads_is_refused(lib, fn, args):
+    _refused(lib, getattr(lib, "ccv1d_" + fn), rec(**args), 2, "too large for one launch")
+
+
+def test_other_launches_of_2_32_threads_are_refused(lib):
+    # 64 threads for 256 channels of a row
+    n = 1 << 26
+    _refused(lib, lib.ccv1d_rec_update, update(rows=n, slots=n), 2, "too large for one launch")
+    _refused(lib, lib.ccv1d_rec_update, update(rows=n // 2, slots=n // 2, dim=257), 2, "too large for one")
+    # 256 threads for one token, or for as many as have 512 pieces between them
+    _refused(lib, lib.ccv1d_paged_write, write(tokens=1 << 24, kv_heads=16, head_dim=128), 2, "too large for one")
+    _refused(lib, lib.ccv1d_paged_write, write(tokens=(1 << 31) - 1, kv_heads=2, head_dim=8, dtype=F32), 2,
+             "too large for one")
+
+
 def test_empty_requests_are_no_ops(lib):
     assert lib.ccv1d_rec_fwd(C.byref(rec(batch=0))) == 0
     assert lib.ccv1d_rec_fwd(C.byref(rec(dim=0))) == 0
