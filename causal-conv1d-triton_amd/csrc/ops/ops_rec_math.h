@@ -19,14 +19,15 @@ constexpr float kLn2 = 0.69314718055994530942f;
 // exp(-z) = 2^t, t = -z log2 e. The rounding of t, |t| 2^-24, is a relative error of the result that
 // grows with |z|. For fp32 inputs its residue is added back (4 operations, and twice the bytes per
 // element to hide them); for 16-bit ones it lies far below the rounding of what is stored. t is held
-// at 126, so that 1 / (1 + 2^t) stays a normal number; a NaN passes.
+// at 126, so that 1 / (1 + 2^t) stays a normal number. Past 2^-126 and 2^126 the residue, which is no
+// number for an infinite t, is left out; a NaN passes through it.
 template <typename T>
 __device__ __forceinline__ float exp_minus(float z) {
   float t = -kLog2e * z;
   if constexpr (sizeof(T) == 4) {
     const float rest = fmaf(z, -kLog2eLow, fmaf(z, -kLog2e, -t));
-    const float e = __builtin_amdgcn_exp2f(t > 126.0f ? 126.0f : t);
-    return t > 126.0f ? e : fmaf(e, kLn2 * rest, e);
+    const float e = __builtin_amdgcn_exp2f(fminf(t, 126.0f));
+    return fabsf(t) > 126.0f ? e : fmaf(e, kLn2 * rest, e);
   }
   return __builtin_amdgcn_exp2f(t > 126.0f ? 126.0f : t);
 }

@@ -111,6 +111,61 @@ def test_wide_gates_of_16_bits(decay, igate, dtype):
     check(make(16, 2, 200, 66, dtype, decay, igate, spread=6.0, init=True))
 
 
+# A gate far below zero counts as 2^-126 in some of the forms, and the root of that, 2^-63, is the largest
+# trace of it in beta and the gradients; the other factors here (states, x, dout, the decay's exponent)
+# stay below 2^5 each, three of them in a product.
+CLOSED = 2.0 ** -48
+
+
+@pytest.mark.parametrize("decay", [True, False])
+@pytest.mark.parametrize("igate", [True, False])
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+def test_gates_at_the_ends_of_their_type(decay, igate, dtype):
+    """Gates that are infinite or their type's largest and lowest value, as masks are: sigmoid is 1 or 0
+    there, forward and backward, and in the form for one token."""
+    ends = torch.tensor([float("inf"), float("-inf"), torch.finfo(dtype).max, torch.finfo(dtype).min])
+    t = make(19, 2, 150, 70, dtype, decay, igate, init=True)
+    g = torch.Generator().manual_seed(4)
+    for k in ("gate", "igate"):
+        if t[k] is not None:
+            at = torch.rand(t[k].shape, generator=g) < 0.2
+            t[k][at] = ends[torch.randint(0, 4, (int(at.sum()),), generator=g)].to(dtype)
+    dfin = torch.randn(2, 70, generator=g)
+    want = oracle.recurrence(t["x"], t["gate"], t["decay"], t["igate"], None, t["init"], dy=t["dy"], dfinal=dfin)
+    for k, v in run(t, final=True, dfinal=dfin).items():
+        if v is not None:
+            oracle.assert_close(v, (want[k][0], want[k][1] + CLOSED), k)
+    state = t["init"].to(DEV)
+    d = {k: None if v is None else v.to(DEV) for k, v in t.items()}
+    for j in range(20):
+        out = gated_recurrence_update(d["x"][:, j], d["gate"][:, j], state, d["decay"],
+                                      None if d["igate"] is None else d["igate"][:, j])
+        oracle.assert_close(out, (want["out"][0][:, j], want["out"][1][:, j] + CLOSED))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+def test_decay_that_never_forgets(dtype):
+    """A decay of -infinity or the lowest number: softplus is 0, a is 1, beta 0 and so is its gradient."""
+    t = make(20, 2, 150, 70, dtype, init=True)
+    ends = [0, 1, 33, 69]
+    t["decay"][ends] = torch.tensor([float("-inf"), torch.finfo(F).min, float("-inf"), -200.0])
+    got = run(t, final=True)
+    want = oracle.recurrence(t["x"], t["gate"], t["decay"], t["igate"], None, t["init"], dy=t["dy"])
+    live = torch.ones(70, dtype=torch.bool)
+    live[ends] = False
+    assert not got["decay"].cpu()[~live].any()
+    for k, v in got.items():
+        value, bound = want[k]
+        if k == "decay":  # the oracle divides by the softplus
+            oracle.assert_close(v.cpu()[live], (value[live], bound[live]), k)
+        else:
+            oracle.assert_close(v, (value, bound + CLOSED), k)
+    state = t["init"].to(DEV)
+    out = gated_recurrence_update(t["x"][:, 0].to(DEV), t["gate"][:, 0].to(DEV), state, t["decay"].to(DEV),
+                                  t["igate"][:, 0].to(DEV))
+    oracle.assert_close(out, (want["out"][0][:, 0], want["out"][1][:, 0] + CLOSED))
+
+
 @pytest.mark.parametrize("B,T", [(128, 129), (128, 200), (130, 256), (127, 256), (128, 257)])
 @pytest.mark.parametrize("dtype", [BF, F])
 @pytest.mark.parametrize("packed", [True, False])
