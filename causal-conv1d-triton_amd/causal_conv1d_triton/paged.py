@@ -92,7 +92,8 @@ def paged_attention(
       block_tables: (requests, max_pages) int32 with contiguous rows. Pages outside the cache are
          left out.
       seq_lens: (rows,) integers: row r attends to the positions before seq_lens[r], with `window`
-         to the last `window` of them. A row with none (a length of zero) gets zeros.
+         to the last `window` of them, counted from seq_lens[r] also where that passes the table or
+         max_seq_len. A row with none (a length of zero) gets zeros.
       softmax_scale: head_dim ** -0.5 by default.
       request_ids: optional (rows,) integers: the request of each row (row r is request r without), for
          the tokens of a prompt (seq_lens = positions + 1). A negative one makes a row empty.

@@ -60,12 +60,16 @@ struct Span {
   int32_t first, end, base;
 };
 
+// The window is the last of the row's length, also where that passes the table or the bound of the lengths,
+// which cut the end off; a window wholly past them leaves nothing.
 __device__ __forceinline__ Span span_of(const AttnParams& p, int64_t row, int64_t& request) {
   request = p.a.request_ids ? p.a.request_ids[row] : row;
   Span s{0, 0, 0};
-  if (request >= 0 && request < p.a.requests && p.a.num_pages > 0)
-    s.end = max(0, min(p.a.seq_lens[row], p.limit));
-  if (p.a.window && s.end > p.a.window) s.first = s.end - (int32_t)p.a.window;
+  int32_t length = 0;
+  if (request >= 0 && request < p.a.requests && p.a.num_pages > 0) length = max(0, p.a.seq_lens[row]);
+  s.end = min(length, p.limit);
+  if (p.a.window && length > p.a.window) s.first = length - (int32_t)p.a.window;
+  if (s.first >= s.end) s.first = s.end = 0;
   s.base = s.first & ~31;
   return s;
 }

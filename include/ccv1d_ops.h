@@ -156,7 +156,8 @@ int ccv1d_paged_write(const struct ccv1d_paged_write_args* args);
  * [max(0, L - window), L), L = seq_lens[r], of request request_ids[r] (r without request_ids):
  *   out[r, h] = sum_p softmax_p(scale * q[r, h] . k[p, h / group]) v[p, h / group],  group = q_heads / kv_heads
  * A row with no position (L <= 0, a request outside the table) gets zeros and a log-sum-exp of -inf.
- * Positions past max_pages * page_size, or in pages outside the cache, are left out. */
+ * Positions past max_pages * page_size or max_seq_len, or in pages outside the cache, are left out; L is not
+ * cut by them. */
 struct ccv1d_paged_attn_args {
   const void* q; /* (rows, q_heads, head_dim), unit last stride */
   int64_t q_stride_r, q_stride_h;
@@ -174,7 +175,7 @@ struct ccv1d_paged_attn_args {
   float scale;
   int64_t window; /* 0: none */
   int64_t rows, requests, q_heads, kv_heads, head_dim, num_pages, page_size, max_pages;
-  int64_t max_seq_len; /* no seq_len is larger (0: max_pages * page_size): sizes the launch */
+  int64_t max_seq_len; /* no position at or past it (0: max_pages * page_size): sizes the launch */
   void* workspace;
   size_t workspace_bytes;
   int device;

@@ -205,6 +205,34 @@ def test_attention_window_past_every_length(window):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("window", [1, 20, 31, 100, 700])
+@pytest.mark.parametrize("cut", ["table", "max_seq_len"])
+def test_attention_window_of_lengths_past_the_end(window, cut):
+    """The window is the last of the length, not of what the table or max_seq_len leaves of it: a row sees
+    [length - window, end), which is nothing where the window starts past the end."""
+    end, ps = 480, 16
+    lens = [n for o in (-1, 0, 1, 10, 19, 20, 21, 99, 100, 101, 699, 701, 2 ** 31 - 1 - end) for n in [end + o]]
+    kc, vc, tables = caches(9, [end] * len(lens), 2, 64, ps, BF)
+    kw = dict(window=window)
+    if cut == "table":
+        tables = tables[:, :end // ps].contiguous()
+    else:
+        kw["max_seq_len"] = end
+    q = torch.randn(len(lens), 4, 64, generator=torch.Generator().manual_seed(2)).to(BF)
+    out, lse = paged_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), tables.to(DEV),
+                               torch.tensor(lens, device=DEV), return_lse=True, **kw)
+    for r, n in enumerate(lens):
+        stop = min(n, end)
+        start = max(0, n - window)
+        if start >= stop:
+            assert not out[r].any() and (lse[r] == float("-inf")).all(), n
+            continue
+        one = slice(r, r + 1)
+        want, want_lse = oracle.attention(q[one], kc, vc, tables[one], torch.tensor([stop]), window=stop - start)
+        oracle.assert_close(out[one], want, n)
+        oracle.assert_close(lse[one], want_lse, n)
+
+
 @pytest.mark.parametrize("dtype", [BF, HF, F])
 def test_attention_long(dtype):
     """Lengths that are split over workgroups and joined, beside short ones."""
