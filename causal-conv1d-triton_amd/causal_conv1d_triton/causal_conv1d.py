@@ -270,7 +270,8 @@ def causal_conv1d_fn(
       bias: optional (dim,).
       seq_idx: optional (batch, seqlen) integer ids marking packed sequences: a tap only reaches
          rows with the same id as the output row, and rows with a negative id are padding, whose
-         outputs (and input gradients) are zero. initial_states are treated as rows of
+         outputs (and input gradients) are zero (ids are taken as int32: of 64-bit ones the low 32
+         bits count). initial_states are treated as rows of
          seq_idx[:, 0]'s sequence. Not allowed together with return_final_states.
       initial_states: optional (batch, width - 1, dim), the width - 1 rows that precede x[:, 0].
       return_final_states: also return the last width - 1 rows of cat(initial_states, x), which

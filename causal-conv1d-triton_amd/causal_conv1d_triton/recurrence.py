@@ -94,7 +94,8 @@ def gated_recurrence_fn(
          stride along dim (other strides are free, so slices of one projection go in as they are; a
          tensor without a unit stride is copied first). gate and input_gate are pre-activations.
       decay: optional (dim,), any float type; its gradient comes back in that type.
-      seq_idx: optional (batch, seqlen) integer ids marking packed sequences: the state starts at zero
+      seq_idx: optional (batch, seqlen) integer ids below 2^63 (causal_conv1d_fn tells its ids apart by
+         their low 32 bits) marking packed sequences: the state starts at zero
          in each row whose id differs from the row before; rows with a negative id are padding, whose
          outputs and gradients are zero whatever x and the gates hold there. initial_states belong to
          the sequence of seq_idx[:, 0].

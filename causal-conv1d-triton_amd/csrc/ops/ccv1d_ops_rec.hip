@@ -166,6 +166,7 @@ hipError_t run(const ccv1d_rec_args& a, bool backward, hipStream_t s) {
   p.a = a;
   p.chunks = (int32_t)pl.chunks;
   p.groups = (int32_t)pl.groups;
+  p.wide_ids = a.seq_idx_64 != 0;
   p.pairs = static_cast<uint64_t*>(a.workspace);
   p.part = reinterpret_cast<float*>(p.pairs + pl.words);
   if (pl.words) {

@@ -100,6 +100,13 @@ at::Tensor as_index(const at::Tensor& t) {
   return as_i32(t);
 }
 
+// Sequence ids as they are in 32 or 64 bits: a shorter one could join two sequences or turn one to padding.
+at::Tensor as_ids(const at::Tensor& t) {
+  const bool wide = t.defined() && (t.scalar_type() == at::kLong || t.scalar_type() == at::kUInt32 ||
+                                    t.scalar_type() == at::kUInt64);
+  return as_type(t, wide ? at::kLong : at::kInt);
+}
+
 // Tells autograd that a tensor was written to.
 void written(const at::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -215,7 +222,7 @@ void rec_check(Rec& r) {
   if (r.init.defined()) r.init_type = r.init.scalar_type();
   r.decay = as_f32(r.decay);
   r.init = as_f32(r.init);
-  r.seq = as_i32(r.seq);
+  r.seq = as_ids(r.seq);
   a.x = ptr(r.x), a.x_stride_b = r.x.stride(0), a.x_stride_t = r.x.stride(1);
   a.gate = ptr(r.gate), a.gate_stride_b = r.gate.stride(0), a.gate_stride_t = r.gate.stride(1);
   if (r.igate.defined()) {
@@ -223,7 +230,8 @@ void rec_check(Rec& r) {
     a.input_gate_stride_b = r.igate.stride(0), a.input_gate_stride_t = r.igate.stride(1);
   }
   a.decay = ptr<float>(r.decay);
-  a.seq_idx = ptr<int32_t>(r.seq);
+  a.seq_idx = ptr(r.seq);
+  a.seq_idx_64 = r.seq.defined() && r.seq.scalar_type() == at::kLong;
   a.initial_states = ptr<float>(r.init);
   a.device = (int)dev;
   a.stream = stream_of(dev);

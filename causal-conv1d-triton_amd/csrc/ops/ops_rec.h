@@ -46,6 +46,7 @@ constexpr float kTiny = 1.17549435e-38f;
 struct RecParams {
   ccv1d_rec_args a;
   int32_t cols, chunks, groups;  // wave columns of 64 * CPL channels; chunks along time; their groups
+  int32_t wide_ids;              // 1: seq_idx holds 64-bit ids, else 0
   Divisor by_cols, by_columns;   // cols; batch * cols
   uint64_t* pairs;               // (batch, chunks, dim)
   uint64_t* states;              // (batch, groups, dim): word of the state after a group
@@ -92,18 +93,25 @@ struct Rows {
   uint32_t first, pad;  // a sequence's first row; padding
 };
 
+// A row's id: two words of 64 bits, or one of 32 twice.
+struct Id {
+  int32_t low, high;
+};
+
 // Lane l looks at row t0 - 1 + l (a row inside): its id is requested before the inputs and looked at once
 // they are requested too (B=4 T=16384 D=4096 without decay, packed, forward and backward: looked at
 // first 833 us, 812 so).
-__device__ __forceinline__ int32_t id_of(const int32_t* seq, int64_t t0, int64_t T, int lane) {
-  return seq[min(max(t0 - 1 + lane, (int64_t)0), T - 1)];
+__device__ __forceinline__ Id id_of(const RecParams& p, int64_t b, int64_t t0, int lane) {
+  const int64_t T = p.a.seqlen, t = min(max(t0 - 1 + lane, (int64_t)0), T - 1);
+  const int32_t* at = static_cast<const int32_t*>(p.a.seq_idx) + ((b * T + t) << p.wide_ids);
+  return {at[0], at[p.wide_ids]};
 }
 
 template <int R>
-__device__ __forceinline__ Rows rows_of(int32_t id, int64_t t0, int valid, int lane) {
-  const int32_t prev = __shfl_up(id, 1);
-  const uint64_t pad = __ballot(id < 0);
-  const uint64_t first = __ballot(t0 + lane > 1 && id != prev);
+__device__ __forceinline__ Rows rows_of(Id id, int64_t t0, int valid, int lane) {
+  const int32_t low = __shfl_up(id.low, 1), high = __shfl_up(id.high, 1);
+  const uint64_t pad = __ballot(id.high < 0);
+  const uint64_t first = __ballot(t0 + lane > 1 && (id.low != low || id.high != high));
   const uint32_t live = (1u << valid) - 1;
   return {(uint32_t)(first >> 1) & live, (uint32_t)(pad >> 1) & live};
 }
@@ -370,8 +378,8 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_fwd_kernel(RecParams p) {
   const int64_t b = ch.b, T_ = a.seqlen, D = a.dim, t0 = at.t0, c0 = ch.c0;
   const uint32_t lane_c = ch.lane_c, lane_bytes = lane_c * (uint32_t)sizeof(T);
 
-  int32_t id = 0;
-  if constexpr (SEQ) id = id_of(a.seq_idx + b * T_, t0, T_, lane);
+  Id id{0, 0};
+  if constexpr (SEQ) id = id_of(p, b, t0, lane);
 
   typename V::raw xr[R], gr[R], ir[R];
   load_inputs<STREAM, IG, T>(a, ch, at, lane_bytes, gr, xr, ir);
@@ -557,8 +565,8 @@ __global__ __launch_bounds__(NW* kWave, 4) void rec_bwd_kernel(RecParams p) {
   const int64_t b = ch.b, T_ = a.seqlen, D = a.dim, t0 = at.t0, c0 = ch.c0;
   const uint32_t lane_c = ch.lane_c, lane_bytes = lane_c * (uint32_t)sizeof(T);
 
-  int32_t id = 0;
-  if constexpr (SEQ) id = id_of(a.seq_idx + b * T_, t0, T_, lane);
+  Id id{0, 0};
+  if constexpr (SEQ) id = id_of(p, b, t0, lane);
 
   typename V::raw xr[R], gr[R], ir[R], yr[R];
   load_inputs<STREAM, IG, T>(a, ch, at, lane_bytes, gr, xr, ir);

@@ -40,7 +40,8 @@
 extern "C" {
 #endif
 
-#define CCV1D_ABI_VERSION 1
+/* 2: ccv1d_rec_args (ccv1d_ops.h) has seq_idx_64 in what was padding. */
+#define CCV1D_ABI_VERSION 2
 
 /* Element types. x, out, final_states, dout, dfinal_states and dx may be F32, F16 or BF16 (F64 is
  * accepted on the generic path). weight, bias and initial_states may each have any of the four types;

@@ -50,7 +50,8 @@ struct ccv1d_rec_args {
   int dtype;
   const float* decay; /* (dim,) or NULL */
   float decay_scale; /* not negative */
-  const int32_t* seq_idx;      /* (batch, seqlen) contiguous, or NULL */
+  int seq_idx_64;              /* 0: seq_idx holds int32_t, else int64_t */
+  const void* seq_idx;         /* (batch, seqlen) contiguous, or NULL */
   const float* initial_states; /* (batch, dim) or NULL */
   int64_t batch, seqlen, dim;
   /* forward */

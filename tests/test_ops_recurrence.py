@@ -280,6 +280,48 @@ def test_values_in_padding_and_other_sequences_stay_there(decay):
     assert torch.equal(dx[~hit], ref[~hit])
 
 
+@pytest.mark.parametrize("T", [9, 150, 1200])
+@pytest.mark.parametrize("decay", [True, False])
+def test_ids_of_64_bits(T, decay):
+    """Ids that 32 bits cannot hold or tell apart: the bits of the same sequences under small ids."""
+    t = make(21, 2, T, 70, BF, decay=decay, init=True)
+    big = [2 ** 31, 2 ** 32 + 2 ** 31, 5, 5 + 2 ** 32, 5 + 2 ** 33, -1, 2 ** 32 - 1, -2 ** 32, 2 ** 62, 0, -2 ** 63]
+    small = torch.full((2, T), 0, dtype=torch.int32)
+    wide = torch.full((2, T), big[0], dtype=torch.int64)
+    for b in range(2):
+        cuts = [0, *(torch.randint(1, T, (len(big) - 1,), generator=torch.Generator().manual_seed(b)).sort()
+                     .values.tolist())]
+        for j, (c, n) in enumerate(zip(cuts, big)):
+            wide[b, c:] = n
+            small[b, c:] = j if n >= 0 else -1
+    dfin = torch.randn(2, 70, generator=torch.Generator().manual_seed(3))
+    t["seq"] = small
+    want = run(t, final=True, dfinal=dfin)
+    t["seq"] = wide
+    got = run(t, final=True, dfinal=dfin)
+    for k, v in want.items():
+        assert v is None or torch.equal(got[k], v), k
+    t["seq"] = wide.repeat(1, 2)[:, ::2].contiguous()  # the forward alone, from ids with strides
+    wide2 = torch.stack([t["seq"], t["seq"] + 1], 2).to(DEV)[..., 0]
+    t["seq"] = None
+    d = {k: None if v is None else v.to(DEV) for k, v in t.items()}
+    args = (d["x"], d["gate"], d["decay"], d["igate"])
+    assert torch.equal(gated_recurrence_fn(*args, wide2, d["init"]),
+                       gated_recurrence_fn(*args, wide2.contiguous(), d["init"]))
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.uint32])
+def test_ids_of_other_types(dtype):
+    t = make(22, 2, 150, 70, BF)
+    ids = torch.tensor([100, 3, 0, 127, 4])[torch.arange(150) // 32].expand(2, 150)
+    t["seq"] = ids.int()
+    want = run(t, train=False)["out"]
+    if dtype == torch.uint32:
+        ids = ids + 2 ** 31
+    t["seq"] = ids.to(dtype)
+    assert torch.equal(run(t, train=False)["out"], want)
+
+
 def test_all_padding():
     t = make(11, 2, 100, 64, BF, init=True)
     t["seq"] = torch.full((2, 100), -1, dtype=torch.int32)
