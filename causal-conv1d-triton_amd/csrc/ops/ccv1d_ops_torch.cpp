@@ -93,18 +93,21 @@ at::Tensor as_type(const at::Tensor& t, at::ScalarType type) {
 at::Tensor as_f32(const at::Tensor& t) { return as_type(t, at::kFloat); }
 at::Tensor as_i32(const at::Tensor& t) { return as_type(t, at::kInt); }
 
-// Whole numbers as int32; 64-bit ones outside its range stay outside any index or length.
+// Whether int32 cannot hold all whole numbers of a tensor's type.
+bool past_i32(const at::Tensor& t) {
+  return t.scalar_type() == at::kLong || t.scalar_type() == at::kUInt32 || t.scalar_type() == at::kUInt64;
+}
+
+// Whole numbers as int32; those outside its range stay outside any index or length.
 at::Tensor as_index(const at::Tensor& t) {
-  if (t.defined() && t.scalar_type() == at::kLong)
-    return t.clamp(INT32_MIN, INT32_MAX).to(at::kInt).contiguous();
+  if (t.defined() && past_i32(t))
+    return t.to(at::kLong).clamp(INT32_MIN, INT32_MAX).to(at::kInt).contiguous();
   return as_i32(t);
 }
 
 // Sequence ids as they are in 32 or 64 bits: a shorter one could join two sequences or turn one to padding.
 at::Tensor as_ids(const at::Tensor& t) {
-  const bool wide = t.defined() && (t.scalar_type() == at::kLong || t.scalar_type() == at::kUInt32 ||
-                                    t.scalar_type() == at::kUInt64);
-  return as_type(t, wide ? at::kLong : at::kInt);
+  return as_type(t, t.defined() && past_i32(t) ? at::kLong : at::kInt);
 }
 
 // Tells autograd that a tensor was written to.

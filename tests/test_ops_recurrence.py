@@ -501,6 +501,20 @@ def test_update_skips_rows_outside_the_pool():
     oracle.assert_close(state, want["final"])
 
 
+@pytest.mark.parametrize("dtype", [torch.uint32, torch.uint64])
+def test_update_with_unsigned_indices(dtype):
+    """Those that int32 cannot hold lie outside the pool, whatever their low bits."""
+    t = make(1, 4, 1, 70, BF)
+    pool = torch.randn(4, 70, generator=torch.Generator().manual_seed(1))
+    state = pool.to(DEV)
+    far = 2 ** 32 - 1 if dtype == torch.uint32 else 2 ** 32 + 1
+    idx = torch.tensor([2, far, 0, 2 ** 31], dtype=torch.int64).to(dtype).to(DEV)
+    out = gated_recurrence_update(t["x"][:, 0].to(DEV), t["gate"][:, 0].to(DEV), state, state_indices=idx)
+    want = oracle.recurrence(t["x"][[0, 2]], t["gate"][[0, 2]], None, None, None, pool[[2, 0]])
+    oracle.assert_close(out[[0, 2]], (want["out"][0][:, 0], want["out"][1][:, 0]))
+    assert not out[[1, 3]].any() and torch.equal(state[[1, 3]].cpu(), pool[[1, 3]])
+
+
 def test_offsets_past_32_bits():
     """Batch rows, time rows and slots further apart than 32 bits of elements."""
     n = 2 ** 32 + 5 * 70
