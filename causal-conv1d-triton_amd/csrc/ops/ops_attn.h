@@ -22,10 +22,12 @@
 // So neither keys, values, scores nor weights pass through LDS.
 //
 // fp32 throughout except the operands: q, K and V as they are stored; a weight goes in as two 16-bit
-// pieces whose sum is the fp32 weight to 2^-16 (bf16) or 2^-22 (fp16) of it, since one piece's
-// rounding would be as large as that of the result (fp32 caches: as it is). The running
+// pieces, since one piece's rounding would be as large as that of the result (fp32 caches: as it is). Their
+// sum is the fp32 weight to 2^-16 of it in bf16. In fp16 it is to 2^-22 of it, or to 2^-25 where that is more,
+// the type's smallest step: so a maximum's weight is 2^7 there, and what is lost of a weight stays below
+// 2^-32 of the wave's largest (with 1, positions at 2^-25 of a wave's largest fell out of the sum). The running
 // maximum is raised only when a score passes it by more than 2^8 in weight, which spares most steps the
-// reduction across lanes and the scaling of O; the sums hold 2^8 without loss.
+// reduction across lanes and the scaling of O; the sums hold 2^8, and fp16 pieces 2^15, without loss.
 //
 // Positions outside [first, end), or in pages outside the cache, have weight zero: their scores are
 // dropped, and their values replaced by zeros, since a cache's unused rows may hold anything and zero
@@ -214,6 +216,8 @@ __global__ __launch_bounds__(kAttnWaves* kWave, sizeof(T) * DH > 768 ? 1 : 2) vo
   f32x4 o[Pc::kElems];
 #pragma unroll
   for (int j = 0; j < Pc::kElems; ++j) o[j] = (f32x4){0, 0, 0, 0};
+  // The weight of a position is 2^(x - m); m is 7 below the maximum in fp16.
+  constexpr float kHead = __is_same(T, _Float16) ? 7.0f : 0.0f;
   float m = kLowest, l = 0.0f;
   const float to2 = a.scale * 1.44269504088896340736f;
   const int32_t* table = a.block_tables + request * a.block_table_stride;
@@ -354,20 +358,24 @@ __global__ __launch_bounds__(kAttnWaves* kWave, sizeof(T) * DH > 768 ? 1 : 2) vo
     float top = x[0];
 #pragma unroll
     for (int e = 1; e < kMine; ++e) top = fmaxf(top, x[e]);
-    if (__any(top > m + 8.0f)) {
+    if (__any(top > m + (8.0f + kHead))) {
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
-      const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - mn);
+      const float mn = fmaxf(m, top - kHead), f = __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       l *= f;
 #pragma unroll
       for (int j = 0; j < Pc::kElems; ++j) o[j] *= f;
     }
+    // A step's weights are summed before they meet the others': one by one, small ones beside a large sum
+    // would all be rounded away.
+    float sum = 0.0f;
 #pragma unroll
     for (int e = 0; e < kMine; ++e) {
       x[e] = __builtin_amdgcn_exp2f(x[e] - m);
-      l += x[e];
+      sum += x[e];
     }
+    l += sum;
 
     // Values.
     if constexpr (sizeof(T) == 4) {
@@ -393,7 +401,7 @@ __global__ __launch_bounds__(kAttnWaves* kWave, sizeof(T) * DH > 768 ? 1 : 2) vo
     }
   }
 
-  // Join the waves. Query head n's maximum is the same in all g; its sum is over them.
+  // Join the waves. Query head n's m is the same in all g; its sum is over them.
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
   __shared__ float s_m[kAttnWaves][16], s_l[kAttnWaves][16];

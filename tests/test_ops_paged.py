@@ -268,6 +268,37 @@ def test_attention_scale_and_large_scores():
     check_attn(7, [200, 33, 0], 4, 2, 64, 16, HF, scale=0.0)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+@pytest.mark.parametrize("low", [16.4, 20.4, 24.4, 25.3, 27.4])
+def test_attention_beside_a_dominant_position(low, dtype):
+    """Positions that take most of the weight and have values of zero, one in each wave, beside a tail at
+    2^-low: the result is the tail's. Room: what the pieces of a weight leave out (2^-16 of it in bf16, 2^-22 of it or
+    2^-32 of the largest in fp16, nothing in fp32) and a score's rounding, 2^-22 of 32 at most in its exponent."""
+    ps, n, Dh = 16, 400, 64
+    g = torch.Generator().manual_seed(int(low))
+    kc, vc = torch.zeros(25, ps, 1, Dh).to(dtype), torch.zeros(25, ps, 1, Dh).to(dtype)
+    score = -low + (torch.rand(n, generator=g) - 0.5) / 8
+    sinks = torch.zeros(n, dtype=torch.bool)
+    sinks[[0, 33, 70, 100]] = True
+    score[sinks] = 0
+    kc.view(n, Dh)[:, 0] = score.to(dtype)
+    vc.view(n, Dh)[:] = (256 + 700 * torch.rand(n, Dh, generator=g)).to(dtype)
+    vc.view(n, Dh)[sinks] = 0
+    q = torch.zeros(1, 4, Dh, dtype=dtype)
+    q[..., 0] = 1
+    ln2 = 0.6931471805599453
+    tables = torch.arange(25, dtype=torch.int32)[None]
+    out, lse = paged_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), tables.to(DEV), torch.tensor([n], device=DEV),
+                               softmax_scale=ln2, return_lse=True)
+    w = torch.exp2(kc.view(n, Dh)[:, 0].double())
+    v = vc.view(n, Dh).double()
+    lost = {BF: 2.0 ** -16 * w, HF: torch.clamp(2.0 ** -22 * w, min=2.0 ** -32), F: 0 * w}[dtype]
+    want = (w @ v / w.sum()).expand(1, 4, Dh)
+    room = ((lost + 2.0 ** -17 * w) @ v / w.sum()).expand(1, 4, Dh)
+    oracle.assert_close(out, (want, room))
+    oracle.assert_close(lse, (torch.log(w.sum()).expand(1, 4), torch.full((1, 4), 2.0 ** -20, dtype=torch.float64)))
+
+
 @pytest.mark.parametrize("dtype", [BF, F])
 def test_attention_strides(dtype):
     """Heads before tokens in one tensor of keys and values, odd starts, a strided table and query."""
