@@ -67,7 +67,8 @@ def paged_cache_write(
 ) -> None:
     """Writes k and v, (tokens, kv_heads, head_dim) with a unit last stride, to the slots that
     slot_mapping (tokens,) names, in place. Tokens whose slot lies outside the cache (-1: padding) are
-    left out. Caches and tokens have one type. No backward."""
+    left out. Caches and tokens have one type; rows of the caches must not overlap, nor the caches each
+    other. Two tokens of one slot leave one of them there, or pieces of both. No backward."""
     native().paged_cache_write(k, v, k_cache, v_cache, slot_mapping)
 
 

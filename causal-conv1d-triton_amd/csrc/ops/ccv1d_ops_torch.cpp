@@ -16,10 +16,13 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+#include <array>
 #include <cmath>
 #include <exception>
 #include <initializer_list>
 #include <optional>
+#include <utility>
 
 #include "ccv1d_ops.h"
 
@@ -531,6 +534,22 @@ void check_cache(const at::Tensor& t, const at::Tensor& like, const char* shape)
   check(t.size(3) <= 1 || t.stride(3) == 1, "the caches must have a unit last stride");
 }
 
+// Whether no two elements of a cache share memory: each stride, from the smallest on, passes all that those
+// before it reach. (Strides that interleave without meeting are taken to meet.)
+bool distinct(const at::Tensor& t) {
+  if (t.is_contiguous()) return true;
+  std::array<std::pair<int64_t, int64_t>, 4> dims;  // strides and sizes; of one element: (0, 1)
+  for (int d = 0; d < 4; ++d)
+    dims[d] = t.size(d) > 1 ? std::pair(t.stride(d), t.size(d)) : std::pair(int64_t(0), int64_t(1));
+  std::sort(dims.begin(), dims.end());
+  int64_t reach = 0;
+  for (const auto& [stride, size] : dims) {
+    if (size > 1 && stride <= reach) return false;
+    reach += (size - 1) * stride;
+  }
+  return true;
+}
+
 /* paged_cache_write(k, v, k_cache, v_cache, slot_mapping) */
 PyObject* paged_cache_write(PyObject* const* o) {
   at::Tensor k = tensor(o[0], "k must be a tensor"), v = tensor(o[1], "v must be a tensor");
@@ -543,6 +562,7 @@ PyObject* paged_cache_write(PyObject* const* o) {
   check(a.page_size >= 1, "page_size must be at least 1");
   check_cache(kc, kc, "");
   check_cache(vc, kc, "v_cache must have the shape of k_cache");
+  check(kc.numel() == 0 || (distinct(kc) && distinct(vc)), "rows of the caches must not overlap");
   check(k.dim() == 3 && k.size(1) == a.kv_heads && k.size(2) == a.head_dim,
         "k must be (tokens, kv_heads, head_dim)");
   check(v.sizes() == k.sizes(), "v must have the shape of k");

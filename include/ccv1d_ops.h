@@ -135,7 +135,7 @@ struct ccv1d_paged_plan_args {
 int ccv1d_paged_plan(const struct ccv1d_paged_plan_args* args);
 
 /* Writes keys and values (tokens, kv_heads, head_dim) to their slots; slots outside the cache are left
- * out. */
+ * out. The caches' rows do not overlap; two tokens of one slot leave one of them there, or pieces of both. */
 struct ccv1d_paged_write_args {
   const void* k; /* unit last stride */
   int64_t k_stride_t, k_stride_h;

@@ -113,6 +113,27 @@ def test_write_refuses(args, msg):
     assert msg in str(e.value)
 
 
+@pytest.mark.parametrize("cache", [
+    Z(1, 4, 2, 8).expand(3, 4, 2, 8), Z(3, 1, 2, 8).expand(3, 4, 2, 8), Z(3, 4, 1, 8).expand(3, 4, 2, 8),
+    Z(200).as_strided((3, 4, 2, 8), (60, 16, 8, 1)), Z(200).as_strided((3, 4, 2, 8), (64, 16, 7, 1)),
+    Z(200).as_strided((3, 4, 2, 8), (16, 16, 8, 1))])
+def test_write_refuses_caches_that_overlap(cache):
+    """Rows written by two workgroups at once would hold whichever came last."""
+    for caches in ((cache, C4), (C4, cache)):
+        with pytest.raises(AssertionError) as e:
+            paged_cache_write(Z(5, 2, 8), Z(5, 2, 8), *caches, I(5))
+        assert "must not overlap" in str(e.value)
+
+
+@pytest.mark.parametrize("cache", [
+    C4, Z(3, 2, 4, 8).transpose(1, 2), Z(3, 4, 4, 8)[:, :, 1:3], Z(3, 4, 2, 11)[..., 2:10], Z(4, 3, 2, 8).transpose(0, 1),
+    Z(3, 2, 2, 4, 11)[:, 1].transpose(1, 2)[..., :8], Z(9, 4, 2, 8)[::3]])
+def test_write_takes_caches_with_strides(cache):
+    with pytest.raises(AssertionError) as e:
+        paged_cache_write(Z(5, 2, 8), Z(5, 2, 8), cache, C4, I(5))
+    assert "k must be on a GPU" in str(e.value)
+
+
 @pytest.mark.parametrize("args,kw,msg", [
     ((Z(2, 8), C4, C4, I(2, 3), I(2)), {}, "q must be (rows, q_heads, head_dim)"),
     ((Z(2, 4, 9), C4, C4, I(2, 3), I(2)), {}, "the caches must have the head_dim of q"),
