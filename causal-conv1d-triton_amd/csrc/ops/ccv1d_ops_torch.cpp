@@ -128,9 +128,15 @@ at::Tensor inside(const at::Tensor& base, int64_t at, at::ScalarType type, int64
   return t;
 }
 
+// The address of a tensor, null where there is none. One without memory of its own (a subclass that wraps
+// other tensors, a fake tensor) is refused: to the library its null would mean that the tensor is absent.
 template <typename P = void>
 P* ptr(const at::Tensor& t) {
-  return t.defined() ? static_cast<P*>(t.data_ptr()) : nullptr;
+  if (!t.defined()) return nullptr;
+  void* p = t.data_ptr();
+  if (!p && t.numel() > 0)
+    raise(PyExc_TypeError, "a tensor without memory of its own (a wrapper subclass, say) is not supported");
+  return static_cast<P*>(p);
 }
 
 void* stream_of(int64_t dev) {

@@ -179,6 +179,19 @@ def test_fake_shapes(decay, igate, init):
         assert not init or g[4].dtype == torch.float16
 
 
+def test_tensors_without_memory_are_refused():
+    """An address of null means an absent tensor to the library."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x = torch.empty(2, 13, 8, device="cuda")
+        with pytest.raises(TypeError) as e:
+            gated_recurrence_fn(x, x)
+        assert "memory of its own" in str(e.value)
+        with pytest.raises(TypeError) as e:
+            gated_recurrence_update(x[0], x[0], x[0])
+        assert "memory of its own" in str(e.value)
+
+
 # ------------------------------------------------------------------------------ the oracle
 
 

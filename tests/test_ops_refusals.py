@@ -102,6 +102,45 @@ def test_attention(make, msg):
     assert msg in str(e.value)
 
 
+class Wrapper(torch.Tensor):
+    """A subclass that holds another tensor and has no memory of its own."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, strides=inner.stride(), dtype=inner.dtype,
+                                                   device=inner.device)
+
+    def __init__(self, inner):
+        self.inner = inner
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        plain = torch.utils._pytree.tree_map(lambda t: t.inner if isinstance(t, cls) else t, (args, kwargs or {}))
+        return torch.utils._pytree.tree_map(lambda t: cls(t) if isinstance(t, torch.Tensor) else t,
+                                            func(*plain[0], **plain[1]))
+
+
+@pytest.mark.parametrize("call", [
+    lambda: gated_recurrence_fn(z(1, 2, 3), z(1, 2, 3), Wrapper(z(3, dtype=F))),
+    lambda: gated_recurrence_fn(z(1, 2, 3), z(1, 2, 3), None, Wrapper(z(1, 2, 3))),
+    lambda: gated_recurrence_fn(z(1, 2, 3), z(1, 2, 3), None, None, Wrapper(i32(1, 2))),
+    lambda: gated_recurrence_fn(z(1, 2, 3), z(1, 2, 3), None, None, None, Wrapper(z(1, 3, dtype=F))),
+    lambda: gated_recurrence_fn(z(1, 2, 3).requires_grad_(), z(1, 2, 3), None, None, Wrapper(i32(1, 2))),
+    lambda: gated_recurrence_update(z(2, 3), z(2, 3), z(2, 3, dtype=F), None, None, Wrapper(i32(2))),
+    lambda: gated_recurrence_update(z(2, 3), z(2, 3), z(2, 3, dtype=F), Wrapper(z(3, dtype=F))),
+    lambda: paged_attention(z(2, 4, 8), z(3, 4, 2, 8), z(3, 4, 2, 8), i32(2, 3), i32(2),
+                            request_ids=Wrapper(i32(2))),
+    lambda: paged_attention(Wrapper(z(2, 4, 8)), z(3, 4, 2, 8), z(3, 4, 2, 8), i32(2, 3), i32(2)),
+    lambda: paged_plan(Wrapper(i32(2)), i32(2), i32(2, 4), i32(9), i32(1), 16, 4),
+    lambda: paged_cache_write(z(5, 2, 8), z(5, 2, 8), Wrapper(z(3, 4, 2, 8)), z(3, 4, 2, 8), i32(5)),
+])
+def test_wrappers(call):
+    """Taken for their null address, an optional one would count as absent."""
+    with pytest.raises(TypeError) as e:
+        call()
+    assert "memory of its own" in str(e.value)
+
+
 def test_backward_gradients_of_another_shape():
     """The library reads as many elements of the incoming gradients as x has."""
     from causal_conv1d_triton._ops import native
