@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -42,9 +43,13 @@ void check(bool ok, const char* msg) {
   if (!ok) raise(PyExc_AssertionError, msg);
 }
 
+// A tangent of forward-mode differentiation would be lost without a word.
 const at::Tensor& tensor(PyObject* o, const char* msg) {
   if (!THPVariable_Check(o)) raise(PyExc_TypeError, msg);
-  return THPVariable_Unpack(o);
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    raise(PyExc_NotImplementedError, "the operators have no forward-mode derivatives");
+  return t;
 }
 
 // An optional tensor; undefined for None.

@@ -179,6 +179,27 @@ def test_fake_shapes(decay, igate, init):
         assert not init or g[4].dtype == torch.float16
 
 
+@pytest.mark.parametrize("call", [
+    lambda d: gated_recurrence_fn(d(1, 2, 3), Z(1, 2, 3)),
+    lambda d: gated_recurrence_fn(Z(1, 2, 3), Z(1, 2, 3), d(3)),
+    lambda d: gated_recurrence_fn(Z(1, 2, 3).requires_grad_(), d(1, 2, 3)),
+    lambda d: gated_recurrence_update(Z(2, 3), Z(2, 3), d(2, 3)),
+    lambda d: paged_cache_write(Z(5, 2, 8), d(5, 2, 8), C4, C4, I(5)),
+    lambda d: paged_attention(d(2, 4, 8), C4, C4, I(2, 3), I(2)),
+])
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(call, grad):
+    """Autograd is off for one-token calls, which leaves tangents on."""
+    import torch.autograd.forward_ad as ad
+    with ad.dual_level(), torch.set_grad_enabled(grad):
+        with pytest.raises(NotImplementedError) as e:
+            call(lambda *s: ad.make_dual(Z(*s), torch.ones(*s)))
+        assert "forward-mode" in str(e.value)
+        with ad._set_fwd_grad_enabled(False), pytest.raises(AssertionError) as e:  # as if there were none
+            call(lambda *s: ad.make_dual(Z(*s), torch.ones(*s)))
+        assert "must be on a GPU" in str(e.value)
+
+
 def test_tensors_without_memory_are_refused():
     """An address of null means an absent tensor to the library."""
     from torch._subclasses.fake_tensor import FakeTensorMode
