@@ -679,8 +679,11 @@ PyObject* native_call(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return IMPL(a);
   } catch (const Raised&) {
     return nullptr;
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (const std::exception&) {  // torch's, with their types: out of memory among them
+    torch::translate_exception_to_python(std::current_exception());
+    return nullptr;
+  } catch (...) {
+    PyErr_SetString(PyExc_RuntimeError, "unknown error");
     return nullptr;
   }
 }

@@ -102,6 +102,22 @@ def test_attention(make, msg):
     assert msg in str(e.value)
 
 
+@pytest.mark.parametrize("train", [False, True])
+def test_out_of_memory_keeps_its_type(train):
+    """Serving loops catch torch.OutOfMemoryError. The process's share of the card is made small: the output,
+    of a row that the input's strides repeat, does not fit it."""
+    x = z(1, 1, 64).requires_grad_(train).expand(1, 1 << 26, 64)
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(0).total_memory
+    try:
+        torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (1 << 30)) / total)
+        with pytest.raises(torch.OutOfMemoryError):
+            gated_recurrence_fn(x, x)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert gated_recurrence_fn(x[:, :100], x[:, :100]).shape == (1, 100, 64)
+
+
 class Wrapper(torch.Tensor):
     """A subclass that holds another tensor and has no memory of its own."""
 
