@@ -152,6 +152,64 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
   lo = __builtin_bit_cast(uint32_t, l);
 }
 
+// An infinite value times a second piece of zero or below is no number or the other infinity. So an element
+// that is no number, though the weights are, is looked at again: it is infinite where all its infinite
+// values of a weight above zero have one sign, and none of its values is no number (else 0 is returned). For
+// one element, by its lane, in the span of a workgroup; `top` is what its weights are relative to. The launch's
+// parameters are read anew, so that the kernel holds none of them for this: held, 10 scalar registers spilled,
+// and 16 rows of a 1024 window, one key head of 256, took 13.1 us, 12.9 so (12.7 without this). Values with an
+// infinite channel take 6 times as long, infinite throughout 20 times (64 rows of 4096, 8 heads of 128).
+template <typename T>
+__device__ __forceinline__ float infinite(int64_t row, int split, int head, int d, float top) {
+  const AttnParams* args = (const AttnParams*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(args));
+  const AttnParams& p = *args;
+  const ccv1d_paged_attn_args& a = p.a;
+  int64_t request;
+  const Span sp = span_of(p, row, request);
+  const int begin = sp.base + split * p.span, end = min(sp.end, begin + p.span), first = max(begin, sp.first);
+  const int kvh = head / p.group, Dh = (int)a.head_dim;
+  const float to2 = a.scale * 1.44269504088896340736f;
+  const T* qp = static_cast<const T*>(a.q) + row * a.q_stride_r + head * a.q_stride_h;
+  const T* kc = static_cast<const T*>(a.k_cache) + kvh * a.k_cache_stride_h;
+  const T* vc = static_cast<const T*>(a.v_cache) + kvh * a.v_cache_stride_h + d;
+  const int32_t* table = a.block_tables + request * a.block_table_stride;
+  constexpr int kBatch = 8;  // positions whose values are requested together
+  bool plus = false, minus = false;
+#pragma unroll 1
+  for (int p0 = first; p0 < end; p0 += kBatch) {
+    uint32_t up = 0, down = 0;  // bit i: the value of position p0 + i is infinite
+    bool none = false;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int pos = min(p0 + i, end - 1), at = (int)divide(pos, p.by_page);
+      const uint32_t page = (uint32_t)table[at];
+      const bool in = page < (uint64_t)a.num_pages;
+      const float v = to_f32(vc[(in ? page : 0) * a.v_cache_stride_p +
+                                (pos - at * a.page_size) * a.v_cache_stride_t]);
+      up |= (in && v == INFINITY ? 1u : 0u) << i;
+      down |= (in && v == -INFINITY ? 1u : 0u) << i;
+      none = none || (in && v != v);
+    }
+    if (none) return 0.0f;
+#pragma unroll 1
+    for (uint32_t left = up | down; left; left &= left - 1) {
+      const int i = __builtin_ctz(left), pos = min(p0 + i, end - 1), at = (int)divide(pos, p.by_page);
+      const bool sign = up >> i & 1;
+      if (sign ? plus : minus) continue;
+      const T* kp = kc + (int64_t)table[at] * a.k_cache_stride_p + (pos - at * a.page_size) * a.k_cache_stride_t;
+      float score = 0.0f;
+#pragma unroll 1
+      for (int e = 0; e < Dh; ++e) score = fmaf(to_f32(qp[e]), to_f32(kp[e]), score);
+      const bool weighs = __builtin_amdgcn_exp2f(score * to2 - top) > 0.0f;
+      plus = plus || (sign && weighs);
+      minus = minus || (!sign && weighs);
+    }
+    if (plus && minus) return 0.0f;
+  }
+  return plus ? INFINITY : minus ? -INFINITY : 0.0f;
+}
+
 // Measured, with the join: 64 rows of 512 to 8192 positions, 32 query over 8 key heads of 128, bf16, pages of
 // 16: 222 us, 5.15 TB/s of 1.14 GB, a large copy's rate; two rows of 100001 to 131072, fp16, pages of 64: 195 us,
 // 4.9 TB/s. Wide heads with many query heads write and join more per position: 16 query heads of 256
@@ -438,6 +496,7 @@ __global__ __launch_bounds__(kAttnWaves* kWave, sizeof(T) * DH > 768 ? 1 : 2) vo
   T* out = static_cast<T*>(a.out) + at * Dh;
   float* part = p.part + (at * p.splits + split) * Dh;
   const float by = 1.0f / total;
+  bool odd = false;  // one of my elements is no number (or infinite beside another of the other sign)
   for (int d = threadIdx.x % lanes * 4; d < Dh; d += lanes * 4) {
     float sum[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -446,6 +505,8 @@ __global__ __launch_bounds__(kAttnWaves* kWave, sizeof(T) * DH > 768 ? 1 : 2) vo
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[i] = fmaf(o4[i], f[v], sum[i]);
     }
+    const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    odd = odd || all != all;
     if (only) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[i] = total == 0.0f ? 0.0f : sum[i] * by;
@@ -460,6 +521,19 @@ __global__ __launch_bounds__(kAttnWaves* kWave, sizeof(T) * DH > 768 ? 1 : 2) vo
     } else {
       p.part_ml[(at * p.splits + split) * 2] = top;
       p.part_ml[(at * p.splits + split) * 2 + 1] = total;
+    }
+  }
+  if (sizeof(T) == 2 && odd && total == total) {
+#pragma unroll 1
+    for (int j = 0, d = threadIdx.x % lanes * 4; d < Dh; d += ++j % 4 ? 1 : lanes * 4 - 3) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int v = 0; v < kAttnWaves; ++v) sum = fmaf(s_o[v][h][d], f[v], sum);
+      if (sum == sum) continue;
+      const float value = infinite<T>(row, split, (int)head0 + h, d, top);
+      if (value == 0.0f) continue;
+      if (only) out[d] = static_cast<T>(value);
+      else part[d] = value;
     }
   }
 }

@@ -385,6 +385,31 @@ def test_attention_of_scores_without_a_finite_maximum(dtype):
     assert not out[1].any() and lse[1, 0] == float("-inf")
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+@pytest.mark.parametrize("Dh", [64, 40, 256])
+@pytest.mark.parametrize("lens", [[40, 1, 33], [3000, 7, 1500]])
+def test_attention_of_infinite_values(dtype, Dh, lens):
+    """An infinite value that a row sees is its element's result, two of both signs or a NaN make it no number;
+    the other elements, heads and rows keep their bits."""
+    kc, vc, tables = caches(11, lens, 2, Dh, 16, dtype)
+    q = (0.3 * torch.randn(len(lens), 4, Dh, generator=torch.Generator().manual_seed(2))).to(dtype)
+    args = (q.to(DEV), kc.to(DEV))
+    rest = (tables.to(DEV), torch.tensor(lens, device=DEV))
+    clean = paged_attention(*args, vc.to(DEV), *rest).cpu()
+    want = clean.float()
+    inf, nan = float("inf"), float("nan")
+    bad = vc.clone()
+    for r, p, h, d, v, res in ((0, 0, 0, 3, inf, inf), (0, lens[0] - 1, 0, 7, -inf, -inf), (0, 5, 1, 8, inf, nan),
+                               (0, 37, 1, 8, -inf, nan), (0, 20, 1, 11, nan, nan), (1, 0, 1, 0, -inf, -inf),
+                               (2, 30, 0, Dh - 1, inf, inf), (2, 31, 0, Dh - 1, inf, inf),
+                               (2, 32, 0, 2, inf, nan), (2, 9, 0, 2, nan, nan)):
+        bad[tables[r, p // 16], p % 16, h, d] = v
+        want[r, 2 * h:2 * h + 2, d] = res
+    got = paged_attention(*args, bad.to(DEV), *rest).cpu().float()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got.nan_to_num(123.0, inf, -inf), want.nan_to_num(123.0, inf, -inf))
+
+
 def test_attention_offsets_past_32_bits():
     """A cache of more than 2^32 elements, its last pages in use."""
     ps, H, Dh = 64, 8, 128
