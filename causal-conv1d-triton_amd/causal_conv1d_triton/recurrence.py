@@ -6,6 +6,7 @@ in a recurrent block, with forward and backward. Per channel d, in fp32 whatever
     a = r,                                           beta = 1 - r             without
     h[t] = a[t] * h[t - 1] + beta[t] * i[t] * x[t]
 
+A sequence's first row has the beta of any other (some models of this family take 1 there).
 `gated_recurrence_fn` runs whole sequences, training included; `gated_recurrence_update` one token of
 each request of a serving batch, the states in a pool. Layout, packing (`seq_idx`) and states follow
 causal_conv1d_fn, so that one block hands the same tensors to both. The kernels are hand-written HIP
@@ -137,7 +138,7 @@ def gated_recurrence_update(
       state: (slots, dim) fp32 with a unit channel stride, a pool of states, updated in place.
       state_indices: optional (rows,) integers, the slot of each row (row r uses slot r without). Rows
          whose index lies outside the pool, -1 above all, are left out: their output is zero. Two rows
-         of one slot leave one of their results there.
+         of one slot race: what they leave there and return is not defined.
 
     Returns out (rows, dim).
     """

@@ -108,6 +108,9 @@ AttnParams plan(const ccv1d_paged_attn_args& a) {
   if (wgs >= 256 ? most <= 1024 + 31 : most <= 512 && most * row_bytes <= 100 << 10) span = most;
   // The sums of the spans take at most 512 MiB: many rows (a prompt's, say) beside a long table fill the card
   // with fewer spans each. It bounds the workgroups too: below 2^24, as a launch of 256 threads each has to be.
+  // (Spans of 1024 and so, 32 query over 8 key heads of 128 bf16, a table of 131072 positions: 1024 rows of 1 to 600
+  // 1555 and 311 us, 1023 rows of 300 beside one of 131072 1628 and 487, the 2048 rows of one prompt 4387 and 751;
+  // a prompt of 8192 with its own table 17.6 and 11.0 ms.)
   const int64_t sums = a.rows * a.q_heads * (a.head_dim + 2) * 4;
   int64_t spans = (int64_t(512) << 20) / (sums > 0 ? sums : 1);
   if (spans > 256) spans = 256;

@@ -18,7 +18,9 @@ constexpr float kLn2 = 0.69314718055994530942f;
 
 // exp(-z) = 2^t, t = -z log2 e. The rounding of t, |t| 2^-24, is a relative error of the result that
 // grows with |z|. For fp32 inputs its residue is added back (4 operations, and twice the bytes per
-// element to hide them); for 16-bit ones it lies far below the rounding of what is stored. t is held
+// element to hide them). For 16-bit ones it is left in: a sigmoid takes at most |z| 2^-24 of itself from it,
+// and that only far below zero, where it is small; so it lies far below the rounding of what is stored in 16
+// bits, and is of the size of fp32's own in the fp32 results (states, the gradients of decay and states). t is held
 // at 126, so that 1 / (1 + 2^t) stays a normal number. Past 2^-126 and 2^126 the residue, which is no
 // number for an infinite t, is left out; a NaN passes through it.
 template <typename T>

@@ -30,7 +30,8 @@ extern "C" {
  *   without decay:  a = r,                                           beta = 1 - r
  *   h[t] = a[t] * h[t-1] + beta[t] * i[t] * x[t],   h[-1] = initial_states (zero without)
  *
- * computed in fp32 whatever the element type. With seq_idx the state starts at zero in each row whose
+ * computed in fp32 whatever the element type. A sequence's first row has the beta of any other (some models
+ * of this family take 1 there). With seq_idx the state starts at zero in each row whose
  * id differs from the row before it; initial_states belong to the sequence of seq_idx[:, 0]; rows of a
  * negative id are padding: their h is zero, whatever x and the gates hold there, and no gradient
  * leaves them.
@@ -81,8 +82,8 @@ int ccv1d_rec_fwd(const struct ccv1d_rec_args* args);
 int ccv1d_rec_bwd(const struct ccv1d_rec_args* args);
 
 /* One token of each request: h = a * state + beta * i * x, the states in a pool of slots, in place.
- * A row whose index is outside [0, slots) is left out: its out is zero. An index that occurs twice
- * leaves one of its results in the slot. */
+ * A row whose index is outside [0, slots) is left out: its out is zero. Two rows of one slot race: what they
+ * leave there and return is not defined. */
 struct ccv1d_rec_update_args {
   const void* x; /* (rows, dim) of type dtype, unit channel stride; so gate and input_gate */
   int64_t x_stride;
@@ -114,7 +115,7 @@ int ccv1d_rec_update(const struct ccv1d_rec_update_args* args);
  * their rows) are free; an admitted request's new pages come from the end of the free list, in order
  * of request and position, and are noted in block_tables. The tokens of all requests lie one after the
  * other in max_tokens places; places past the last token, and those of requests that were not admitted,
- * get -1. */
+ * get -1. No output shares memory with an input, block_tables apart, which is both. */
 struct ccv1d_paged_plan_args {
   const int32_t* cached_lens; /* (requests,) */
   const int32_t* new_lens;    /* (requests,) */
