@@ -143,6 +143,28 @@ def test_gates_at_the_ends_of_their_type(decay, igate, dtype):
         oracle.assert_close(out, (want["out"][0][:, j], want["out"][1][:, j] + CLOSED))
 
 
+@pytest.mark.parametrize("decay", [True, False])
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+def test_gates_that_are_no_numbers(dtype, decay):
+    """They reach the rows that the formulas lead to, forward and backward, and the rest keeps its bits."""
+    t = make(23, 2, 150, 70, dtype, decay, init=True)
+    t["seq"] = (torch.arange(150) // 40).int().expand(2, 150).contiguous()
+    clean = run(t)
+    t["gate"][0, 20, 5] = t["igate"][1, 30, 6] = float("nan")
+    got = run(t)
+    where = {k: torch.zeros(2, 150, 70, dtype=torch.bool) for k in ("out", "x", "gate", "igate")}
+    where["out"][0, 20:40, 5] = where["out"][1, 30:40, 6] = True  # the state from the row on
+    where["x"][0, :21, 5] = True  # the incoming gradient up to the row, and beta in it
+    where["x"][1, 30, 6] = where["igate"][1, 30, 6] = True  # i alone
+    where["gate"][0, :40, 5] = where["gate"][1, 30:40, 6] = True  # the state before, or the gradient
+    where["igate"][0, :21, 5] = True
+    for k, bad in where.items():
+        v, ref = got[k].cpu(), clean[k].cpu()
+        assert v[bad].isnan().all(), k
+        assert torch.equal(v[~bad], ref[~bad]), k
+    assert got["init"][0, 5].isnan() and got["init"].isnan().sum() == 1
+
+
 @pytest.mark.parametrize("dtype", [BF, HF, F])
 def test_decay_that_never_forgets(dtype):
     """A decay of -infinity or the lowest number: softplus is 0, a is 1, beta 0 and so is its gradient."""
