@@ -21,11 +21,13 @@
 //             when the result is stored.)
 // So neither keys, values, scores nor weights pass through LDS.
 //
-// fp32 throughout except the operands: q, K and V as they are stored; a weight goes in as two 16-bit
-// pieces, since one piece's rounding would be as large as that of the result (fp32 caches: as it is). Their
-// sum is the fp32 weight to 2^-16 of it in bf16. In fp16 it is to 2^-22 of it, or to 2^-25 where that is more,
-// the type's smallest step: so a maximum's weight is 2^7 there, and what is lost of a weight stays below
-// 2^-32 of the wave's largest (with 1, positions at 2^-25 of a wave's largest fell out of the sum). The running
+// fp32 throughout except the operands: q, K and V as they are stored; a weight goes in as 16-bit pieces, since
+// one piece's rounding would be as large as that of the result (fp32 caches: as it is). In bf16 the sum of
+// three is the fp32 weight (of two 2^-16 of it away, which moves one result in 500 to the next bf16 number; the
+// third takes no time: 64 rows of 512 to 8192 positions 229.7 and 228.8 us). In fp16 the sum of two is the weight
+// to 2^-22 of it, or to 2^-25 where that is more, the type's smallest step: so a maximum's weight is 2^7 there,
+// and what is lost of a weight stays below 2^-32 of the wave's largest (with 1, positions at 2^-25 of a wave's
+// largest fell out of the sum). The running
 // maximum is raised only when a score passes it by more than 2^8 in weight, which spares most steps the
 // reduction across lanes and the scaling of O; the sums hold 2^8, and fp16 pieces 2^15, without loss.
 //
@@ -140,19 +142,21 @@ __device__ __forceinline__ f32x4 product32(const uint32_t* a, const uint32_t* b,
   }
 }
 
-// Two fp32 values to one dword of T, and what the rounding left over to another.
-template <typename T>
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+// Two fp32 values to a dword of T, what the rounding left over to the next, and so on.
+template <typename T, int N>
+__device__ __forceinline__ void pieces_of(float a, float b, uint32_t (&to)[N]) {
   typedef T t2 __attribute__((ext_vector_type(2)));
   typedef float f2 __attribute__((ext_vector_type(2)));
-  const t2 h = __builtin_convertvector((f2){a, b}, t2);
-  const f2 back = __builtin_convertvector(h, f2);
-  const t2 l = __builtin_convertvector((f2){a - back.x, b - back.y}, t2);
-  hi = __builtin_bit_cast(uint32_t, h);
-  lo = __builtin_bit_cast(uint32_t, l);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const t2 piece = __builtin_convertvector((f2){a, b}, t2);
+    const f2 back = __builtin_convertvector(piece, f2);
+    a -= back.x, b -= back.y;
+    to[i] = __builtin_bit_cast(uint32_t, piece);
+  }
 }
 
-// An infinite value times a second piece of zero or below is no number or the other infinity. So an element
+// An infinite value times a later piece of zero or below is no number or the other infinity. So an element
 // that is no number, though the weights are, is looked at again: it is infinite where all its infinite
 // values of a weight above zero have one sign, and none of its values is no number (else 0 is returned). For
 // one element, by its lane, in the span of a workgroup; `top` is what its weights are relative to. The launch's
@@ -443,9 +447,15 @@ __global__ __launch_bounds__(kAttnWaves* kWave, sizeof(T) * DH > 768 ? 1 : 2) vo
         for (int e = 0; e < kMine; ++e)
           o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vw[e][j]), x[e], o[j], 0, 0, 0);
     } else {
-      uint32_t hi[4], lo[4];
+      constexpr int kPieces = __is_same(T, __bf16) ? 3 : 2;
+      uint32_t w[kPieces][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) split2<T>(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
+      for (int i = 0; i < 4; ++i) {
+        uint32_t piece[kPieces];
+        pieces_of<T>(x[2 * i], x[2 * i + 1], piece);
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c) w[c][i] = piece[c];
+      }
 #pragma unroll
       for (int j = 0; j < Pc::kElems; ++j) {
         uint32_t v[4];
@@ -453,8 +463,8 @@ __global__ __launch_bounds__(kAttnWaves* kWave, sizeof(T) * DH > 768 ? 1 : 2) vo
         for (int i = 0; i < 4; ++i)  // the 16-bit half j % 2 of two positions
           v[i] = __builtin_amdgcn_perm(vw[2 * i + 1][j / 2], vw[2 * i][j / 2],
                                        j % 2 ? 0x07060302u : 0x05040100u);
-        o[j] = product32<T>(v, lo, o[j]);
-        o[j] = product32<T>(v, hi, o[j]);
+#pragma unroll
+        for (int c = kPieces - 1; c >= 0; --c) o[j] = product32<T>(v, w[c], o[j]);
       }
     }
   }

@@ -299,6 +299,30 @@ def test_attention_beside_a_dominant_position(low, dtype):
     oracle.assert_close(lse, (torch.log(w.sum()).expand(1, 4), torch.full((1, 4), 2.0 ** -20, dtype=torch.float64)))
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+def test_attention_weights_keep_their_bits(dtype):
+    """Six positions whose weighted values nearly cancel, so that the result shows how far the weights are off.
+    Room, of the sum of the products' sizes: a score's rounding in its exponent (2 * 2^-23), the exponential's,
+    the pieces' (2^-22 in fp16), the sums' and the division's, together below 2^-20."""
+    R, n, Dh, ps = 40, 6, 64, 16
+    g = torch.Generator().manual_seed(5)
+    score = -torch.randint(0, 65, (R, n), generator=g) / 32
+    w = torch.exp2(score.double())
+    v = ((0.5 + 1.5 * torch.rand(R, n, Dh, generator=g)) * torch.sign(torch.randn(R, n, Dh, generator=g))).to(dtype)
+    for j in (4, 5):  # the last two take back what the others sum to
+        v[:, j] = 0
+        v[:, j] = (-(w[:, :, None] * v.double())[:, :j].sum(1) / w[:, j, None]).to(dtype)
+    kc, vc = torch.zeros(R, ps, 1, Dh).to(dtype), torch.zeros(R, ps, 1, Dh).to(dtype)
+    kc[:, :n, 0, 0], vc[:, :n, 0] = score.to(dtype), v
+    q = torch.zeros(R, 2, Dh, dtype=dtype)
+    q[..., 0] = 1
+    out = paged_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), torch.arange(R, dtype=torch.int32, device=DEV)[:, None],
+                          torch.full((R,), n, device=DEV), softmax_scale=0.6931471805599453)
+    p = (w / w.sum(1, keepdim=True))[:, :, None]
+    want, size = (p * v.double()).sum(1), (p * v.double().abs()).sum(1)
+    oracle.assert_close(out, (want[:, None].expand(R, 2, Dh), 2.0 ** -20 * size[:, None].expand(R, 2, Dh)))
+
+
 @pytest.mark.parametrize("dtype", [BF, F])
 def test_attention_strides(dtype):
     """Heads before tokens in one tensor of keys and values, odd starts, a strided table and query."""
