@@ -215,11 +215,11 @@ __device__ __forceinline__ float infinite(int64_t row, int split, int head, int 
 }
 
 // Measured, with the join: 64 rows of 512 to 8192 positions, 32 query over 8 key heads of 128, bf16, pages of
-// 16: 222 us, 5.15 TB/s of 1.14 GB, a large copy's rate; two rows of 100001 to 131072, fp16, pages of 64: 195 us,
-// 4.9 TB/s. Wide heads with many query heads write and join more per position: 16 query heads of 256
+// 16: 223 to 230 us on different cards, 5.0 to 5.1 TB/s of 1.14 GB, a large copy's rate; two rows of 100001 to
+// 131072, fp16, pages of 64: 196 us, 4.8 TB/s. Wide heads with many query heads write and join more per position: 16 query heads of 256
 // over 2 key heads, 64 rows of 512 to 4096: 77 us, 3.9 TB/s. One step a wave is latency: 16 rows of a 1024
 // window, one key head of 256: 12.9 us, 4 of them the join. fp32: the first with 2.28 GB 388 us, 5.9 TB/s. The
-// matrix cores are idle most of the time (5 % busy in the first).
+// matrix cores are idle most of the time (6.5 % busy in the first).
 
 // How pages meet steps: one page holds a whole step (page_size a multiple of it); a page holds
 // whole groups of 4 positions; anything else.
