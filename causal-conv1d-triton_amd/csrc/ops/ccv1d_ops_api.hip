@@ -1,4 +1,4 @@
-// C ABI of include/ccv1d_ops.h: argument checks before anything is launched, then the launchers.
+// C ABI of include/ccv1d_ops.h and include/ccv1d_layer.h: argument checks before anything is launched, then the launchers.
 #include <cstdarg>
 #include <cstdio>
 
@@ -103,6 +103,57 @@ int check_attn(const ccv1d_paged_attn_args* a) {
   return CCV1D_OK;
 }
 
+int check_delta(const ccv1d_delta_args* a) {
+  if (!a) return invalid("args is null");
+  if (a->batch < 0 || a->seqlen < 0) return invalid("negative size");
+  if (!dtype_ok(a->dtype) || !dtype_ok(a->log_decay_dtype) || !dtype_ok(a->beta_dtype))
+    return invalid("dtypes must be fp32, fp16 or bf16");
+  if (a->key_heads < 1 || a->heads < 1 || a->heads % a->key_heads)
+    return invalid("heads must be a multiple of key_heads");
+  if (a->key_dim < 1 || a->key_dim > CCV1D_DELTA_MAX_KEY_DIM)
+    return fail(CCV1D_ERR_INVALID, "key_dim must be 1 to %d", CCV1D_DELTA_MAX_KEY_DIM);
+  if (a->value_dim < 1) return invalid("value_dim must be at least 1");
+  if (!ops::delta_fits(*a)) return fail(CCV1D_ERR_UNSUPPORTED, "batch, seqlen, heads and dims too large for one launch");
+  return CCV1D_OK;
+}
+
+int check_delta_call(const ccv1d_delta_args* a, bool backward) {
+  if (int rc = check_delta(a)) return rc;
+  if (a->batch == 0 || a->seqlen == 0) return CCV1D_OK;
+  if (!a->q || !a->k || !a->v || !a->log_decay || !a->beta) return invalid("q, k, v, log_decay or beta is null");
+  if (backward) {
+    if (!a->dout || !a->dq || !a->dk || !a->dv || !a->dlog_decay || !a->dbeta)
+      return invalid("dout, dq, dk, dv, dlog_decay or dbeta is null");
+    if (!a->saved) return invalid("saved is null");
+  } else if (!a->out) {
+    return invalid("out is null");
+  }
+  const size_t need = ops::delta_workspace(*a, backward);
+  if (!a->workspace || a->workspace_bytes < need)
+    return fail(CCV1D_ERR_WORKSPACE, "workspace of %zu bytes needed", need);
+  return CCV1D_OK;
+}
+
+int check_norm(const ccv1d_norm_args* a) {
+  if (!a) return invalid("args is null");
+  if (a->outer < 0 || a->inner < 0) return invalid("negative size");
+  if (a->dim < 1 || a->dim > CCV1D_NORM_MAX_DIM)
+    return fail(CCV1D_ERR_INVALID, "dim must be 1 to %d", CCV1D_NORM_MAX_DIM);
+  if (!dtype_ok(a->dtype)) return invalid("dtype must be fp32, fp16 or bf16");
+  if (a->residual_dtype != a->dtype && a->residual_dtype != CCV1D_F32)
+    return invalid("residual_dtype must be dtype or fp32");
+  if (a->residual_dtype != a->dtype && !a->residual) return invalid("residual_dtype is dtype without residual");
+  if (!a->post_weight && !a->pre_weight) return invalid("post_weight and pre_weight are null");
+  if ((a->post_weight && !dtype_ok(a->post_dtype)) || (a->scale_weight && !dtype_ok(a->scale_dtype)) ||
+      (a->pre_weight && !dtype_ok(a->pre_dtype)))
+    return invalid("the weights' dtypes must be fp32, fp16 or bf16");
+  if (!(a->eps >= 0.0f)) return invalid("eps must not be negative");
+  if (a->activation < CCV1D_NORM_IDENTITY || a->activation > CCV1D_NORM_SIGMOID) return invalid("unknown activation");
+  if (!product_within(a->outer, a->inner, kMaxGrid) || ops::norm_threads(*a) > kMaxThreads)
+    return fail(CCV1D_ERR_UNSUPPORTED, "too many rows for one launch");
+  return CCV1D_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -200,6 +251,87 @@ int ccv1d_paged_attn(const struct ccv1d_paged_attn_args* args) {
   if (need && (!a.workspace || a.workspace_bytes < need))
     return fail(CCV1D_ERR_WORKSPACE, "workspace of %zu bytes needed", need);
   return launch(a, ops::paged_attn);
+}
+
+size_t ccv1d_delta_saved_floats(const struct ccv1d_delta_args* args) {
+  if (check_delta(args) || args->batch == 0 || args->seqlen == 0) return 0;
+  return ops::delta_saved(*args);
+}
+
+size_t ccv1d_delta_workspace_bytes(const struct ccv1d_delta_args* args, int backward) {
+  if (check_delta(args) || args->batch == 0 || args->seqlen == 0) return 0;
+  return ops::delta_workspace(*args, backward != 0);
+}
+
+int ccv1d_delta_fwd(const struct ccv1d_delta_args* args) {
+  clear_error();
+  if (int rc = check_delta_call(args, false)) return rc;
+  if (args->batch == 0) return CCV1D_OK;
+  return launch(*args, ops::delta_fwd);
+}
+
+int ccv1d_delta_bwd(const struct ccv1d_delta_args* args) {
+  clear_error();
+  if (int rc = check_delta_call(args, true)) return rc;
+  if (args->batch == 0) return CCV1D_OK;
+  return launch(*args, ops::delta_bwd);
+}
+
+int ccv1d_delta_update(const struct ccv1d_delta_update_args* args) {
+  clear_error();
+  if (!args) return invalid("args is null");
+  const ccv1d_delta_update_args& a = *args;
+  if (a.rows < 0 || a.slots < 0) return invalid("negative size");
+  if (!dtype_ok(a.dtype) || !dtype_ok(a.log_decay_dtype) || !dtype_ok(a.beta_dtype))
+    return invalid("dtypes must be fp32, fp16 or bf16");
+  if (a.key_heads < 1 || a.heads < 1 || a.heads % a.key_heads) return invalid("heads must be a multiple of key_heads");
+  if (a.key_dim < 1 || a.key_dim > CCV1D_DELTA_MAX_KEY_DIM)
+    return fail(CCV1D_ERR_INVALID, "key_dim must be 1 to %d", CCV1D_DELTA_MAX_KEY_DIM);
+  if (a.value_dim < 1) return invalid("value_dim must be at least 1");
+  if (!a.state_indices && a.rows > a.slots) return invalid("more rows than slots");
+  if (!product_within(a.rows, a.heads, kMaxGrid) || !product_within(a.rows * a.heads, cdiv(a.value_dim, 64), kMaxGrid) ||
+      ops::delta_update_threads(a) > kMaxThreads)
+    return fail(CCV1D_ERR_UNSUPPORTED, "rows, heads and value_dim too large for one launch");
+  if (a.rows == 0) return CCV1D_OK;
+  if (!a.q || !a.k || !a.v || !a.log_decay || !a.beta || !a.out || (a.slots && !a.state))
+    return invalid("q, k, v, log_decay, beta, state or out is null");
+  return launch(a, ops::delta_update);
+}
+
+size_t ccv1d_norm_workspace_bytes(const struct ccv1d_norm_args* args) {
+  if (check_norm(args)) return 0;
+  return ops::norm_workspace(*args);
+}
+
+int ccv1d_norm_fwd(const struct ccv1d_norm_args* args) {
+  clear_error();
+  if (int rc = check_norm(args)) return rc;
+  const ccv1d_norm_args& a = *args;
+  if (a.outer * a.inner == 0) return CCV1D_OK;
+  if (!a.x) return invalid("x is null");
+  if ((a.pre_weight != nullptr) != (a.y != nullptr)) return invalid("y goes with pre_weight");
+  if (!a.pre_weight && !a.r) return invalid("r is null");
+  return launch(a, ops::norm_fwd);
+}
+
+int ccv1d_norm_bwd(const struct ccv1d_norm_args* args) {
+  clear_error();
+  if (int rc = check_norm(args)) return rc;
+  const ccv1d_norm_args& a = *args;
+  if ((a.post_weight != nullptr) != (a.dpost_weight != nullptr) ||
+      (a.scale_weight != nullptr) != (a.dscale_weight != nullptr) ||
+      (a.pre_weight != nullptr) != (a.dpre_weight != nullptr))
+    return invalid("the weights' gradients go with the weights");
+  if (a.dy && !a.pre_weight) return invalid("dy goes with pre_weight");
+  if (a.outer * a.inner > 0) {
+    if (!a.x || !a.dx) return invalid("x or dx is null");
+    if ((a.gate != nullptr) != (a.dgate != nullptr)) return invalid("dgate goes with gate");
+    if (a.dresidual && !a.residual) return invalid("dresidual goes with residual");
+    const size_t need = ops::norm_workspace(a);
+    if (!a.workspace || a.workspace_bytes < need)
+      return fail(CCV1D_ERR_WORKSPACE, "workspace of %zu bytes needed", need);
+  }
+  return launch(a, ops::norm_bwd);
 }
 
 }  // extern "C"

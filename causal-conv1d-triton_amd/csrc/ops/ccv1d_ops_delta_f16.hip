@@ -1,0 +1,10 @@
+// The gated delta rule over whole sequences, f16 elements.
+#include "ops_delta.h"
+
+namespace ccv1d {
+namespace ops {
+hipError_t delta_launch_f16(const DeltaParams& p, bool backward, hipStream_t s) {
+  return delta_launch<_Float16>(p, backward, s);
+}
+}  // namespace ops
+}  // namespace ccv1d

@@ -1,0 +1,11 @@
+// Norms around a block, bf16 elements.
+#include "ops_norm.h"
+
+namespace ccv1d {
+namespace ops {
+hipError_t norm_launch_bf16(const NormParams& p, bool backward, hipStream_t s) {
+  if (p.a.residual_dtype != p.a.dtype) return norm_types<__bf16, float>(p, backward, s);
+  return norm_types<__bf16, __bf16>(p, backward, s);
+}
+}  // namespace ops
+}  // namespace ccv1d

@@ -7,6 +7,7 @@
 
 #include <tuple>
 
+#include "ccv1d_layer.h"
 #include "ccv1d_ops.h"
 
 namespace ccv1d {
@@ -68,6 +69,17 @@ hipError_t paged_plan(const ccv1d_paged_plan_args& a, hipStream_t s);
 hipError_t paged_write(const ccv1d_paged_write_args& a, hipStream_t s);
 hipError_t paged_attn(const ccv1d_paged_attn_args& a, hipStream_t s);
 size_t paged_attn_workspace(const ccv1d_paged_attn_args& a);
+bool delta_fits(const ccv1d_delta_args& a);  // whether its launches and sizes are in range
+size_t delta_saved(const ccv1d_delta_args& a);
+size_t delta_workspace(const ccv1d_delta_args& a, bool backward);
+hipError_t delta_fwd(const ccv1d_delta_args& a, hipStream_t s);
+hipError_t delta_bwd(const ccv1d_delta_args& a, hipStream_t s);
+int64_t delta_update_threads(const ccv1d_delta_update_args& a);
+hipError_t delta_update(const ccv1d_delta_update_args& a, hipStream_t s);
+int64_t norm_threads(const ccv1d_norm_args& a);
+size_t norm_workspace(const ccv1d_norm_args& a);
+hipError_t norm_fwd(const ccv1d_norm_args& a, hipStream_t s);
+hipError_t norm_bwd(const ccv1d_norm_args& a, hipStream_t s);
 
 }  // namespace ops
 }  // namespace ccv1d
