@@ -34,7 +34,7 @@ Sizes sizes_of(const ccv1d_delta_args& a) {
   return z;
 }
 
-constexpr int64_t kRowFloats = 5 * CCV1D_DELTA_CHUNK;
+constexpr int64_t kRowFloats = 8 * CCV1D_DELTA_CHUNK;
 
 struct Places {  // in bytes
   int64_t kf, qf, kt, qt, tf, pf, rows, ds, dr, gates, all;
@@ -58,8 +58,8 @@ Places places_of(const ccv1d_delta_args& a, const Sizes& z, bool backward) {
   p.rows = next(hc * kRowFloats * 4);
   p.ds = next(backward ? hc * z.dk * z.dvp * 4 : 0);
   p.dr = next(backward ? hc * CCV1D_DELTA_CHUNK * z.dvp * 4 : 0);
-  // a key's elements lie in workgroups of 128, in fp16 and fp32 of 64
-  const int64_t parts = z.dk / (a.dtype == CCV1D_BF16 ? 128 : 64);
+  // of keys whose elements lie in several workgroups, 128 in each, in fp32 64
+  const int64_t parts = z.dk / (a.dtype == CCV1D_F32 ? 64 : 128);
   p.gates = next(backward && parts > 1 ? hc * parts * 4 * CCV1D_DELTA_CHUNK * 4 : 0);
   p.all = at;
   return p;

@@ -196,13 +196,13 @@ __device__ __forceinline__ void frag_of(const T* p, u4 (&o)[kPieces<T>]) {
   }
 }
 
-// Element e of a fragment, from its pieces.
+// Element e of the half `half` of a fragment, from its pieces.
 template <int N>
-__device__ __forceinline__ float piece_sum(const u4 (&f)[N], int e) {
+__device__ __forceinline__ float piece_sum(const u4 (&f)[N], int half, int e) {
   float s = 0.0f;
 #pragma unroll
   for (int n = N - 1; n >= 0; --n) {
-    const uint32_t w = f[n][e >> 1];
+    const uint32_t w = half ? f[n][2 + (e >> 1)] : f[n][e >> 1];
     s += __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
   }
   return s;
@@ -216,8 +216,8 @@ constexpr int kTri = 6;
 
 // What a chunk's rows have, per head: [0] e^G where the carried state reaches the row, [1] e^(G_C - G) where the
 // row reaches the chunk's end, [2] beta, [3] one for a row that is there and no padding, [4][0] e^G_C where
-// the carried state reaches the end; zero elsewhere.
-constexpr int kRowFields = 5;
+// the carried state reaches the end; zero elsewhere; [5] and [6] G log2 e in 64 bits, [7] the number of resets.
+constexpr int kRowFields = 8;
 
 struct ChunkRows {
   double sum;   // G log2 e, from the row's sequence's start in the chunk
@@ -289,6 +289,8 @@ __device__ __forceinline__ ChunkRows share_rows(const ccv1d_delta_args& a, int64
     rows[2 * kC + lane] = r.beta;
     rows[3 * kC + lane] = r.live ? 1.0f : 0.0f;
     rows[4 * kC + lane] = lane == 0 && last == 0 ? exp2_of(end) : 0.0f;
+    reinterpret_cast<double*>(rows + 5 * kC)[lane] = r.sum;
+    reinterpret_cast<int*>(rows + 7 * kC)[lane] = r.run;
   }
   return r;
 }
@@ -486,460 +488,667 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
   }
 }
 
-// Which head and which 16 value columns a workgroup of a chain has: workgroups go to the XCDs in turn, and all
+// Which head and which CT tiles of 16 value columns a workgroup of a chain has: workgroups go to the XCDs in turn, and all
 // columns of a head to one, whose L2 then holds the head's fragments once.
 struct ChainPlace {
   int64_t head;  // batch * heads + head
   int64_t dv0;
   bool any;
 };
+template <int CT>
 __device__ __forceinline__ ChainPlace chain_place(const DeltaParams& p) {
   const int64_t xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
   ChainPlace r;
-  r.head = xcd + 8 * (slot / p.tiles);
-  r.dv0 = slot % p.tiles * 16;
+  const int64_t groups = p.tiles / CT;
+  r.head = xcd + 8 * (slot / groups);
+  r.dv0 = slot % groups * (16 * CT);
   r.any = r.head < p.a.batch * p.a.heads;
   return r;
 }
 
-// Waves of a chain: 32 of the keys' elements each, 64 for the largest heads, whose operands need the registers.
+// How a chain's eight waves share the work. Four carry the states, 32 or 64 of the keys' elements each (keys of up to
+// 64 elements twice over, with half of the chunk's rows each in the first product), and 16 of the chunk's rows
+// in the products between rows; the other four do what no later chunk waits for.
 template <int DK>
-constexpr int kChainWaves = DK / 32 < 4 ? DK / 32 : 4;
-
-// Whether a chain requests the next chunk's operands of k and q while it works on this one's: not for the largest
-// heads in fp32, whose operands alone are 300 registers.
-template <typename T, int DK>
-constexpr bool kLoadAhead = !(sizeof(T) == 4 && DK == 256);
-
-// The tiles of 16 rows that a wave has of the products between rows: four over the waves.
-template <int NW>
-struct RowTiles {
-  static constexpr int kN = 4 / NW;
-  static __device__ __forceinline__ int at(int wave, int q) { return NW == 2 && q ? 3 - wave : wave; }
+struct Chain {
+  static constexpr int kKS = DK / 32;                     // steps of the sum over the keys' elements
+  static constexpr int kKB = kKS < 4 ? 1 : kKS / 4;       // of a wave
+  static constexpr int kParts = kKS < 4 ? kKS : 4;        // partial sums of the first product
+  static constexpr int kRows = kKS < 4 ? 2 : 4;           // tiles of rows of a wave in it
+  static __device__ __forceinline__ int part(int w) { return w % kParts; }
+  static __device__ __forceinline__ int rows0(int w) { return kKS < 4 ? w / 2 * 2 : 0; }
 };
 
-// The chain of states forward. A workgroup has 16 value columns of a head, a wave 32 or 64 of the keys'
-// elements of their states (in the accumulators' layout), and 16 or 32 of a chunk's rows.
-// Bound by latency: three products after one another a chunk, each behind a barrier.
-template <typename T, int DK, bool SAVE>
-__global__ __launch_bounds__(kChainWaves<DK> * 64) void delta_fwd_kernel(DeltaParams p) {
-  constexpr int NI = kPieces<T>, KS = DK / 32, NW = kChainWaves<DK>, KB = KS / NW, MT = RowTiles<NW>::kN;
-  constexpr int NO = kOutPieces<T>, LO = NO - 1;
+// Whether a chain requests the next chunk's operands of k while it works on this one's: not for the largest heads
+// in fp16 and fp32, whose operands alone are 130 and 200 registers.
+template <typename T, int DK>
+constexpr bool kLoadAhead = kPieces<T> * DK < 512;
+
+// A wave's number, known to be the same in all lanes.
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+template <int N>
+__device__ __forceinline__ void load_frag(const u4* p, uint32_t lane, u4 (&o)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) o[n] = p[n * 64 + lane];
+}
+
+// An element as it lies in memory, in a register of its own: two 16-bit ones packed into one would be waited for
+// where they are packed.
+template <typename T>
+__device__ __forceinline__ uint32_t load_raw(const T* p) {
+  if constexpr (sizeof(T) == 4) return __builtin_bit_cast(uint32_t, *p);
+  else return *reinterpret_cast<const uint16_t*>(p);
+}
+template <typename T>
+__device__ __forceinline__ float raw_to_f32(uint32_t x) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(x);
+  else if constexpr (kPieces<T> == 1) return __uint_as_float(x << 16);
+  else return (float)__builtin_bit_cast(T, (uint16_t)x);
+}
+
+// The four rows of a lane in a tile of 16, of one column of a tensor, read one by one. Past the last row or column
+// another is read, and not used.
+template <typename T>
+struct ColumnReader {
+  const T* p;  // row 4 (lane / 16) of the tile of the first chunk
+  int64_t stride;
+  __device__ __forceinline__ void at(const void* base, int64_t offset, int64_t stride_t, int64_t dv, int64_t dim, int row) {
+    p = static_cast<const T*>(base) + offset + min(dv, dim - 1) + row * stride_t;
+    stride = stride_t;
+  }
+  __device__ __forceinline__ void load(int64_t c, int64_t seqlen, int row, uint32_t (&o)[4]) const {
+    const T* at = p + c * (kC * stride);
+    if ((c + 1) * kC <= seqlen) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = load_raw(at + e * stride);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t over = c * kC + row + e - (seqlen - 1);
+        o[e] = load_raw(at + (e - max((int64_t)0, over)) * stride);
+      }
+    }
+  }
+};
+
+// The chain of states forward: a workgroup has CT tiles of 16 value columns of a head. Bound by latency: three
+// products after one another a chunk, each behind a barrier; the waves that make the outputs run beside them.
+template <typename T, int DK, int CT, bool SAVE>
+__global__ __launch_bounds__(512) void delta_fwd_kernel(DeltaParams p) {
+  using L = Chain<DK>;
+  constexpr int NI = kPieces<T>, KS = L::kKS, KB = L::kKB, NO = kOutPieces<T>, LO = NO - 1;
   constexpr bool AHEAD = kLoadAhead<T, DK>;
-  __shared__ f4 red[2][NW][4][64];
-  __shared__ u4 rb[2][3][64], ub[2][3][64], uo[2][NO][64];
+  __shared__ f4 red[CT][L::kParts][4][64];
+  __shared__ u4 sp[CT][KS][NO][64], rb[CT][2][3][64], ub[CT][2][3][64], uo[CT][2][NO][64];
   const ccv1d_delta_args& a = p.a;
-  const ChainPlace at = chain_place(p);
+  const ChainPlace at = chain_place<CT>(p);
   if (!at.any) return;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+  const uint32_t lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int wave = wave_index(), w = wave & 3;
   const int64_t b = at.head / a.heads, h = at.head - b * a.heads, kh = h / p.group;
   const int64_t dv = at.dv0 + col;
-  const bool column = dv < a.value_dim;
-  const int64_t N = p.chunks, kc0 = (b * a.key_heads + kh) * N, hc0 = at.head * N;
+  const bool all_columns = at.dv0 + 16 * CT <= a.value_dim;
+  const int64_t N = p.chunks;
+  const int row = 16 * w + 4 * g;  // the lane's first row of the wave's tile of rows
+  const u4* kf = p.kf + (b * a.key_heads + kh) * N * (4 * KS * NI * 64);
+  const u4* qf = p.qf + (b * a.key_heads + kh) * N * (4 * KS * NI * 64);
+  const u4* kt = p.kt + (b * a.key_heads + kh) * N * (DK / 16 * 2 * NI * 64);
+  const u4* tf = p.tf + at.head * N * (kTri * 3 * 64);
+  const u4* pf = p.pf + at.head * N * (kTri * NO * 64);
+  const float* rows = p.rows + at.head * N * (kRowFields * kC);
 
-  u4 kf[KB][4][NI], qf[KB][4][NI], kt[2 * KB][2][NI], tf[MT][2][3], pf[MT][2][NO];
-  float v[MT][4];
-  f4 into[MT], rest[MT], beta[MT], live[MT];
-  float whole = 0.0f;
-  auto load_kq = [&](int64_t c) {
+  if (wave >= 4) {  // outputs: O = scale e^G Q S0 + P U of a tile of rows
+    u4 qx[KS][NI], px[2][NO];
+    f4 into, live;
+    auto load_q = [&](int64_t c) {
 #pragma unroll
-    for (int i = 0; i < KB; ++i)
+      for (int s = 0; s < KS; ++s) load_frag(qf + c * (4 * KS * NI * 64) + (w * KS + s) * (NI * 64), lane, qx[s]);
+      into = *reinterpret_cast<const f4*>(rows + c * (kRowFields * kC) + row);
+    };
+    auto load_p = [&](int64_t c) {
+      live = *reinterpret_cast<const f4*>(rows + c * (kRowFields * kC) + 3 * kC + row);
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const int64_t o = (kc0 + c) * (4 * KS * NI * 64) + (m * KS + w * KB + i) * (NI * 64) + lane;
-        load_frag(p.kf + o, kf[i][m]);
-        load_frag(p.qf + o, qf[i][m]);
+      for (int s = 0; s < 2; ++s)
+        if (s <= w / 2) load_frag(pf + c * (kTri * NO * 64) + lower_frag(w, s) * (NO * 64), lane, px[s]);
+    };
+    const int64_t stride = a.heads * a.value_dim;
+    T* out = static_cast<T*>(a.out) + (b * a.seqlen + row) * stride + h * a.value_dim + dv;
+    load_q(0);
+    load_p(0);
+    for (int64_t c = 0; c < N; ++c) {
+      const int64_t next = c + 1 < N ? c + 1 : c;
+      lds_barrier();
+      f4 o[CT];
+#pragma unroll
+      for (int n = 0; n < CT; ++n) {
+        f4 y[2] = {};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          u4 so[NO];
+          load_frag(&sp[n][s][0][0], lane, so);
+          y[s & 1] = mac<LO>(qx[s], so, y[s & 1]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          o[n][e] = a.scale * into[e] * (y[0][e] + y[1][e]);
+          if (into[e] == 0.0f) o[n][e] = 0.0f;  // not a product with zero: the state may hold no number
+        }
       }
+      load_q(next);
+      lds_barrier();
+      lds_barrier();
+#pragma unroll
+      for (int n = 0; n < CT; ++n)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+          if (s <= w / 2) {
+            u4 u[NO];
+            load_frag(&uo[n][s][0][0], lane, u);
+            o[n] = mac<LO>(px[s], u, o[n]);
+          }
+      T* to = out + c * (kC * stride);
+#pragma unroll
+      for (int n = 0; n < CT; ++n)
+        if (dv + 16 * n < a.value_dim)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c * kC + row + e < a.seqlen) to[e * stride + 16 * n] = (T)(live[e] != 0.0f ? o[n][e] : 0.0f);
+      load_p(next);
+    }
+    return;
+  }
+
+  const int part = L::part(w), rows0 = L::rows0(w);
+  const bool keeper = L::kParts == 4 || w < L::kParts;  // of two waves with the same states, the first
+  u4 kx[KB][L::kRows][NI], kc[2 * KB][2][NI], tx[2][3];
+  uint32_t v[CT][4];
+  f4 into, rest, beta, live;
+  float whole = 0.0f, whole_now;
+  ColumnReader<T> vr[CT];
+#pragma unroll
+  for (int n = 0; n < CT; ++n)
+    vr[n].at(a.v, b * a.v_stride_b + h * a.v_stride_h, a.v_stride_t, dv + 16 * n, a.value_dim, row);
+  auto load_k_of = [&](int64_t c, int i) {
+#pragma unroll
+    for (int m = 0; m < L::kRows; ++m)
+      load_frag(kf + c * (4 * KS * NI * 64) + ((rows0 + m) * KS + part * KB + i) * (NI * 64), lane, kx[i][m]);
   };
-  auto load_kt = [&](int64_t c) {
-    whole = p.rows[(hc0 + c) * (kRowFields * kC) + 4 * kC];
+  auto load_kc_of = [&](int64_t c, int s) {
+#pragma unroll
+    for (int t = 0; t < 2 * KB; ++t)
+      load_frag(kt + c * (DK / 16 * 2 * NI * 64) + ((2 * KB * part + t) * 2 + s) * (NI * 64), lane, kc[t][s]);
+  };
+  auto load_k = [&](int64_t c) {
+#pragma unroll
+    for (int i = 0; i < KB; ++i) load_k_of(c, i);
+  };
+  auto load_kc = [&](int64_t c) {
+    load_kc_of(c, 0);
+    load_kc_of(c, 1);
+  };
+  auto load_v = [&](int64_t c) {
+    const float* r = rows + c * (kRowFields * kC);
+    whole = r[4 * kC];
+    into = *reinterpret_cast<const f4*>(r + row);
+    beta = *reinterpret_cast<const f4*>(r + 2 * kC + row);
+    live = *reinterpret_cast<const f4*>(r + 3 * kC + row);
+#pragma unroll
+    for (int n = 0; n < CT; ++n) vr[n].load(c, a.seqlen, row, v[n]);
+  };
+  auto load_t = [&](int64_t c) {
+    rest = *reinterpret_cast<const f4*>(rows + c * (kRowFields * kC) + kC + row);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      if (s <= w / 2) load_frag(tf + c * (kTri * 3 * 64) + lower_frag(w, s) * (3 * 64), lane, tx[s]);
+  };
+
+  f4 state[CT][2 * KB];
+#pragma unroll
+  for (int n = 0; n < CT; ++n)
 #pragma unroll
     for (int t = 0; t < 2 * KB; ++t)
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        load_frag(p.kt + (kc0 + c) * (DK / 16 * 2 * NI * 64) + ((2 * KB * w + t) * 2 + s) * (NI * 64) + lane, kt[t][s]);
-  };
-  auto load_rows_of = [&](int64_t c) {  // of the wave's row tiles, T and V
-#pragma unroll
-    for (int q = 0; q < MT; ++q) {
-      const int m = RowTiles<NW>::at(w, q);
-      const float* rows = p.rows + (hc0 + c) * (kRowFields * kC) + 16 * m + 4 * g;
-      into[q] = *reinterpret_cast<const f4*>(rows);
-      rest[q] = *reinterpret_cast<const f4*>(rows + kC);
-      beta[q] = *reinterpret_cast<const f4*>(rows + 2 * kC);
-      live[q] = *reinterpret_cast<const f4*>(rows + 3 * kC);
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-        if (s <= m / 2) load_frag(p.tf + (hc0 + c) * (kTri * 3 * 64) + lower_frag(m, s) * (3 * 64) + lane, tf[q][s]);
-#pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int64_t t = c * kC + 16 * m + 4 * g + e;
-        v[q][e] = column && t < a.seqlen
-                      ? to_f32(static_cast<const T*>(a.v)[b * a.v_stride_b + t * a.v_stride_t + h * a.v_stride_h + dv])
-                      : 0.0f;
+        const int64_t d = 32 * KB * part + 16 * t + 4 * g + e;
+        state[n][t][e] = a.initial_states && dv + 16 * n < a.value_dim && d < a.key_dim
+                             ? a.initial_states[(at.head * a.key_dim + d) * a.value_dim + dv + 16 * n]
+                             : 0.0f;
       }
-    }
-  };
-  auto load_p = [&](int64_t c) {
-#pragma unroll
-    for (int q = 0; q < MT; ++q) {
-      const int m = RowTiles<NW>::at(w, q);
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-        if (s <= m / 2) load_frag(p.pf + (hc0 + c) * (kTri * NO * 64) + lower_frag(m, s) * (NO * 64) + lane, pf[q][s]);
-    }
-  };
-
-  f4 state[2 * KB];
-#pragma unroll
-  for (int t = 0; t < 2 * KB; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t d = 32 * KB * w + 16 * t + 4 * g + e;
-      state[t][e] = a.initial_states && column && d < a.key_dim
-                        ? a.initial_states[(at.head * a.key_dim + d) * a.value_dim + dv]
-                        : 0.0f;
-    }
+  float* s0 = SAVE ? p.s0 + at.head * N * (DK * (int64_t)p.dvp) + (32 * KB * part + 4 * g) * p.dvp + dv : nullptr;
+  float* us = SAVE ? p.u + at.head * N * (kC * (int64_t)p.dvp) + row * p.dvp + dv : nullptr;
   if constexpr (AHEAD) {
-    load_kq(0);
-    load_kt(0);
+    load_k(0);
+    load_kc(0);
   }
-  load_rows_of(0);
-  load_p(0);
+  load_v(0);
+  load_t(0);
   for (int64_t c = 0; c < N; ++c) {
     const int64_t next = c + 1 < N ? c + 1 : c;
-    if constexpr (SAVE) {
-      float* to = p.s0 + (hc0 + c) * ((int64_t)DK * p.dvp) + at.dv0 + col;
-#pragma unroll
-      for (int t = 0; t < 2 * KB; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) to[(32 * KB * w + 16 * t + 4 * g + e) * p.dvp] = state[t][e];
-    }
     {
-      if constexpr (!AHEAD) load_kq(c);
-      f4 x[4] = {}, y[4] = {};
+      f4 x[CT][L::kRows] = {};
 #pragma unroll
       for (int i = 0; i < KB; ++i) {
-        u4 sb[3], so[NO];
-        split8<3>(state[2 * i], state[2 * i + 1], sb);
+        if constexpr (!AHEAD) load_k_of(c, i);
 #pragma unroll
-        for (int n = 0; n < NO; ++n) so[n] = sb[n];
+        for (int n = 0; n < CT; ++n) {
+          u4 sb[3];
+          split8<3>(state[n][2 * i], state[n][2 * i + 1], sb);
+          if (keeper)
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          x[m] = mac<2>(kf[i][m], sb, x[m]);
-          y[m] = mac<LO>(qf[i][m], so, y[m]);
+            for (int j = 0; j < NO; ++j) sp[n][part * KB + i][j][lane] = sb[j];
+#pragma unroll
+          for (int m = 0; m < L::kRows; ++m) x[n][m] = mac<2>(kx[i][m], sb, x[n][m]);
         }
       }
 #pragma unroll
-      for (int m = 0; m < 4; ++m) red[0][w][m][lane] = x[m], red[1][w][m][lane] = y[m];
+      for (int n = 0; n < CT; ++n)
+#pragma unroll
+        for (int m = 0; m < L::kRows; ++m) red[n][part][rows0 + m][lane] = x[n][m];
     }
-    if constexpr (AHEAD) load_kq(next);
+    if constexpr (SAVE)
+      if (keeper) {
+        float* to = s0 + c * (DK * (int64_t)p.dvp);
+#pragma unroll
+        for (int t = 0; t < 2 * KB; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int n = 0; n < CT; ++n) to[(16 * t + e) * p.dvp + 16 * n] = state[n][t][e];
+      }
+    if constexpr (AHEAD) load_k(next);
+    // A chunk that the carried state goes through has no reset and no padding but past the last row, where beta and
+    // the keys are zero: only the others need selections in place of products with zero.
+    whole_now = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(whole)));
+    const bool plain = whole_now != 0.0f && all_columns;
     lds_barrier();
-    f4 o[MT], now_live[MT];
 #pragma unroll
-    for (int q = 0; q < MT; ++q) {
-      const int m = RowTiles<NW>::at(w, q);
-      f4 x = red[0][0][m][lane], y = red[1][0][m][lane];
+    for (int n = 0; n < CT; ++n) {
+      f4 x = red[n][0][w][lane];
 #pragma unroll
-      for (int n = 1; n < NW; ++n) x += red[0][n][m][lane], y += red[1][n][m][lane];
+      for (int j = 1; j < L::kParts; ++j) x += red[n][j][w][lane];
       f4 r;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool carried = into[q][e] != 0.0f;  // not a product with zero: the state may hold no number
-        const float ve = live[q][e] != 0.0f ? v[q][e] : 0.0f;
-        r[e] = beta[q][e] * (ve - (carried ? into[q][e] * x[e] : 0.0f));
-        o[q][e] = carried ? a.scale * into[q][e] * y[e] : 0.0f;
-      }
+      for (int e = 0; e < 4; ++e) r[e] = beta[e] * (raw_to_f32<T>(v[n][e]) - into[e] * x[e]);
+      if (!plain)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          r[e] = beta[e] * ((live[e] != 0.0f && dv + 16 * n < a.value_dim ? raw_to_f32<T>(v[n][e]) : 0.0f) -
+                            (into[e] != 0.0f ? into[e] * x[e] : 0.0f));
       u2 half[3];
       split4<3>(r, half);
-      store_half<3>(&rb[m / 2][0][lane], m & 1, half);
+      store_half<3>(&rb[n][w / 2][0][lane], w & 1, half);
     }
+    load_v(next);
     lds_barrier();
+    f4 u[CT];
 #pragma unroll
-    for (int q = 0; q < MT; ++q) {
-      const int m = RowTiles<NW>::at(w, q);
-      f4 u = {0, 0, 0, 0};
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-        if (s <= m / 2) {
-          u4 r[3];
-          load_frag(&rb[s][0][lane], r);
-          u = mac<2>(tf[q][s], r, u);
-        }
-      if constexpr (SAVE) {
-        float* to = p.u + (hc0 + c) * (kC * p.dvp) + at.dv0 + col;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) to[(16 * m + 4 * g + e) * p.dvp] = u[e];
+    for (int n = 0; n < CT; ++n) {
+      f4 u1 = {0, 0, 0, 0};
+      u4 rx[3];
+      u[n] = f4{0, 0, 0, 0};
+      load_frag(&rb[n][0][0][0], lane, rx);
+      u[n] = mac<2>(tx[0], rx, u[n]);
+      if (w >= 2) {
+        load_frag(&rb[n][1][0][0], lane, rx);
+        u1 = mac<2>(tx[1], rx, u1);
       }
+      u[n] += u1;
+    }
+#pragma unroll
+    for (int n = 0; n < CT; ++n) {
+      f4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = rest[e] * u[n][e];
+      if (!plain)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = rest[e] != 0.0f ? y[e] : 0.0f;
       u2 half[3], out[NO];
-      split4<NO>(u, out);
-      store_half<NO>(&uo[m / 2][0][lane], m & 1, out);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) u[e] = rest[q][e] != 0.0f ? rest[q][e] * u[e] : 0.0f;
-      split4<3>(u, half);
-      store_half<3>(&ub[m / 2][0][lane], m & 1, half);
-      now_live[q] = live[q];
+      split4<3>(y, half);
+      store_half<3>(&ub[n][w / 2][0][lane], w & 1, half);
+      split4<NO>(u[n], out);
+      store_half<NO>(&uo[n][w / 2][0][lane], w & 1, out);
     }
-    load_rows_of(next);
-    if constexpr (!AHEAD) load_kt(c);
+    if constexpr (SAVE) {
+      float* to = us + c * (kC * (int64_t)p.dvp);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int n = 0; n < CT; ++n) to[e * p.dvp + 16 * n] = u[n][e];
+    }
+    load_t(next);
+#pragma unroll
+    for (int n = 0; n < CT; ++n)
+#pragma unroll
+      for (int t = 0; t < 2 * KB; ++t) {
+        state[n][t] *= whole_now;
+        if (whole_now == 0.0f) state[n][t] = f4{0, 0, 0, 0};
+      }
     lds_barrier();
 #pragma unroll
-    for (int t = 0; t < 2 * KB; ++t) {
+    for (int s = 0; s < 2; ++s) {
+      if constexpr (!AHEAD) load_kc_of(c, s);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) state[t][e] = whole != 0.0f ? whole * state[t][e] : 0.0f;
+      for (int n = 0; n < CT; ++n) {
+        u4 ux[3];
+        load_frag(&ub[n][s][0][0], lane, ux);
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        u4 u[3];
-        load_frag(&ub[s][0][lane], u);
-        state[t] = mac<2>(kt[t][s], u, state[t]);
+        for (int t = 0; t < 2 * KB; ++t) state[n][t] = mac<2>(kc[t][s], ux, state[n][t]);
       }
     }
-    if constexpr (AHEAD) load_kt(next);
-#pragma unroll
-    for (int q = 0; q < MT; ++q) {
-      const int m = RowTiles<NW>::at(w, q);
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-        if (s <= m / 2) {
-          u4 u[NO];
-          load_frag(&uo[s][0][lane], u);
-          o[q] = mac<LO>(pf[q][s], u, o[q]);
-        }
-      T* out = static_cast<T*>(a.out);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t t = c * kC + 16 * m + 4 * g + e;
-        if (column && t < a.seqlen)
-          out[((b * a.seqlen + t) * a.heads + h) * a.value_dim + dv] = (T)(now_live[q][e] != 0.0f ? o[q][e] : 0.0f);
-      }
-    }
-    load_p(next);
+    if constexpr (AHEAD) load_kc(next);
   }
-  if (a.final_states && column)
+  if (a.final_states && keeper)
 #pragma unroll
-    for (int t = 0; t < 2 * KB; ++t)
+    for (int n = 0; n < CT; ++n)
+      if (dv + 16 * n < a.value_dim)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t d = 32 * KB * w + 16 * t + 4 * g + e;
-        if (d < a.key_dim) a.final_states[(at.head * a.key_dim + d) * a.value_dim + dv] = state[t][e];
-      }
+        for (int t = 0; t < 2 * KB; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int64_t d = 32 * KB * part + 16 * t + 4 * g + e;
+            if (d < a.key_dim) a.final_states[(at.head * a.key_dim + d) * a.value_dim + dv + 16 * n] = state[n][t][e];
+          }
 }
 
 // The chain of the states' gradients, from the last chunk to the first; divided like the forward's. Leaves dS1 of
-// every chunk and dR, and writes dV.
-template <typename T, int DK>
-__global__ __launch_bounds__(kChainWaves<DK> * 64) void delta_bwd_kernel(DeltaParams p) {
-  constexpr int NI = kPieces<T>, KS = DK / 32, NW = kChainWaves<DK>, KB = KS / NW, MT = RowTiles<NW>::kN;
+// every chunk and dR, and writes dV. The waves beside the chain make P^T dO and scale Q^T (e^G dO) a chunk ahead.
+template <typename T, int DK, int CT>
+__global__ __launch_bounds__(512) void delta_bwd_kernel(DeltaParams p) {
+  using L = Chain<DK>;
+  constexpr int NI = kPieces<T>, KS = L::kKS, KB = L::kKB, TQ = DK / 64;  // tiles of the keys' elements beside the chain
   constexpr bool AHEAD = kLoadAhead<T, DK>;
-  __shared__ f4 red[NW][4][64];
-  __shared__ u4 ob[2][NI][64], oq[2][3][64], ub[2][3][64], rb[2][3][64];
+  __shared__ f4 red[CT][L::kParts][4][64], pd[CT][4][64], qd[CT][DK / 16][64];
+  __shared__ u4 ob[CT][2][NI][64], oq[CT][2][3][64], ub[CT][2][3][64], rb[CT][2][3][64];
   const ccv1d_delta_args& a = p.a;
-  const ChainPlace at = chain_place(p);
+  const ChainPlace at = chain_place<CT>(p);
   if (!at.any) return;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+  const uint32_t lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int wave = wave_index(), w = wave & 3;
   const int64_t b = at.head / a.heads, h = at.head - b * a.heads, kh = h / p.group;
   const int64_t dv = at.dv0 + col;
-  const bool column = dv < a.value_dim;
-  const int64_t N = p.chunks, kc0 = (b * a.key_heads + kh) * N, hc0 = at.head * N;
+  const int64_t N = p.chunks;
+  const int row = 16 * w + 4 * g;
+  const u4* kf = p.kf + (b * a.key_heads + kh) * N * (4 * KS * NI * 64);
+  const u4* kt = p.kt + (b * a.key_heads + kh) * N * (DK / 16 * 2 * NI * 64);
+  const u4* qt = p.qt + (b * a.key_heads + kh) * N * (DK / 16 * 2 * NI * 64);
+  const u4* tf = p.tf + at.head * N * (kTri * 3 * 64);
+  const u4* pf = p.pf + at.head * N * (kTri * 3 * 64);
+  const float* rows = p.rows + at.head * N * (kRowFields * kC);
 
-  u4 kf[KB][4][NI], kt[2 * KB][2][NI], qt[2 * KB][2][NI], tf[MT][2][3], pf[MT][2][3];
-  float dy[MT][4];
-  f4 into[MT], rest[MT], beta[MT];
-  float whole = 0.0f;
+  if (wave >= 4) {
+    u4 px[2][3], qx[TQ][2][NI];
+    f4 into, live, sum[CT][TQ];
+    uint32_t dy[CT][4];
+    ColumnReader<T> yr[CT];
+#pragma unroll
+    for (int n = 0; n < CT; ++n)
+      yr[n].at(a.dout, b * a.dout_stride_b + h * a.dout_stride_h, a.dout_stride_t, dv + 16 * n, a.value_dim, row);
+    auto load_dy = [&](int64_t c) {
+      into = *reinterpret_cast<const f4*>(rows + c * (kRowFields * kC) + row);
+      live = *reinterpret_cast<const f4*>(rows + c * (kRowFields * kC) + 3 * kC + row);
+#pragma unroll
+      for (int n = 0; n < CT; ++n) yr[n].load(c, a.seqlen, row, dy[n]);
+    };
+    auto load_pq = [&](int64_t c) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (s >= w / 2) load_frag(pf + c * (kTri * 3 * 64) + upper_frag(w, s) * (3 * 64), lane, px[s]);
+      if constexpr (AHEAD)
+#pragma unroll
+        for (int t = 0; t < TQ; ++t)
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+            load_frag(qt + c * (DK / 16 * 2 * NI * 64) + ((TQ * w + t) * 2 + s) * (NI * 64), lane, qx[t][s]);
+    };
+    auto share = [&](int64_t c) {  // dO of the wave's rows, and scale e^G dO
+#pragma unroll
+      for (int n = 0; n < CT; ++n) {
+        f4 d, s;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          d[e] = live[e] != 0.0f && dv + 16 * n < a.value_dim ? raw_to_f32<T>(dy[n][e]) : 0.0f;
+          s[e] = a.scale * into[e] * d[e];
+        }
+        u2 half[NI], third[3];
+        split4<NI>(d, half);
+        store_half<NI>(&ob[n][w / 2][0][lane], w & 1, half);
+        split4<3>(s, third);
+        store_half<3>(&oq[n][w / 2][0][lane], w & 1, third);
+      }
+      load_dy(c ? c - 1 : 0);
+    };
+    auto products = [&](int64_t c) {
+#pragma unroll
+      for (int n = 0; n < CT; ++n) {
+        f4 y[2] = {};
+#pragma unroll
+        for (int t = 0; t < TQ; ++t) sum[n][t] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          u4 o[NI], x[3];
+          if (s >= w / 2) {
+            load_frag(&ob[n][s][0][0], lane, o);
+            y[s] = mac<2>(px[s], o, y[s]);
+          }
+          load_frag(&oq[n][s][0][0], lane, x);
+#pragma unroll
+          for (int t = 0; t < TQ; ++t) {
+            if constexpr (!AHEAD)
+              load_frag(qt + c * (DK / 16 * 2 * NI * 64) + ((TQ * w + t) * 2 + s) * (NI * 64), lane, qx[t][s]);
+            sum[n][t] = mac<2>(qx[t][s], x, sum[n][t]);
+          }
+        }
+        pd[n][w][lane] = y[0] + y[1];
+      }
+      load_pq(c ? c - 1 : 0);
+    };
+    load_dy(N - 1);
+    load_pq(N - 1);
+    share(N - 1);
+    lds_barrier();
+    products(N - 1);
+    for (int64_t c = N - 1; c >= 0; --c) {
+      lds_barrier();
+#pragma unroll
+      for (int n = 0; n < CT; ++n)
+#pragma unroll
+        for (int t = 0; t < TQ; ++t) qd[n][TQ * w + t][lane] = sum[n][t];
+      share(c ? c - 1 : 0);
+      lds_barrier();
+      products(c ? c - 1 : 0);
+      lds_barrier();
+    }
+    return;
+  }
+
+  const int part = L::part(w), rows0 = L::rows0(w);
+  const bool keeper = L::kParts == 4 || w < L::kParts;
+  u4 kx[KB][L::kRows][NI], kc[2 * KB][2][NI], tx[2][3];
+  f4 into, rest, beta;
+  float whole = 0.0f, whole_now;
+  auto load_k_of = [&](int64_t c, int i) {
+#pragma unroll
+    for (int m = 0; m < L::kRows; ++m)
+      load_frag(kf + c * (4 * KS * NI * 64) + ((rows0 + m) * KS + part * KB + i) * (NI * 64), lane, kx[i][m]);
+  };
+  auto load_kc_of = [&](int64_t c, int s) {
+#pragma unroll
+    for (int t = 0; t < 2 * KB; ++t)
+      load_frag(kt + c * (DK / 16 * 2 * NI * 64) + ((2 * KB * part + t) * 2 + s) * (NI * 64), lane, kc[t][s]);
+  };
   auto load_k = [&](int64_t c) {
 #pragma unroll
-    for (int i = 0; i < KB; ++i)
-#pragma unroll
-      for (int m = 0; m < 4; ++m)
-        load_frag(p.kf + (kc0 + c) * (4 * KS * NI * 64) + (m * KS + w * KB + i) * (NI * 64) + lane, kf[i][m]);
+    for (int i = 0; i < KB; ++i) load_k_of(c, i);
+  };
+  auto load_kc = [&](int64_t c) {
+    load_kc_of(c, 0);
+    load_kc_of(c, 1);
+  };
+  auto load_rest = [&](int64_t c) {
+    const float* r = rows + c * (kRowFields * kC);
+    whole = r[4 * kC];
+    rest = *reinterpret_cast<const f4*>(r + kC + row);
   };
   auto load_t = [&](int64_t c) {
-    whole = p.rows[(hc0 + c) * (kRowFields * kC) + 4 * kC];
+    const float* r = rows + c * (kRowFields * kC);
+    into = *reinterpret_cast<const f4*>(r + row);
+    beta = *reinterpret_cast<const f4*>(r + 2 * kC + row);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      if (s >= w / 2) load_frag(tf + c * (kTri * 3 * 64) + upper_frag(w, s) * (3 * 64), lane, tx[s]);
+  };
+
+  f4 ds[CT][2 * KB];
+#pragma unroll
+  for (int n = 0; n < CT; ++n)
 #pragma unroll
     for (int t = 0; t < 2 * KB; ++t)
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int64_t o = (kc0 + c) * (DK / 16 * 2 * NI * 64) + ((2 * KB * w + t) * 2 + s) * (NI * 64) + lane;
-        load_frag(p.kt + o, kt[t][s]);
-        load_frag(p.qt + o, qt[t][s]);
-      }
-  };
-  auto load_dy = [&](int64_t c) {
-#pragma unroll
-    for (int q = 0; q < MT; ++q) {
-      const int m = RowTiles<NW>::at(w, q);
-      const float* rows = p.rows + (hc0 + c) * (kRowFields * kC) + 16 * m + 4 * g;
-      into[q] = *reinterpret_cast<const f4*>(rows);
-      const f4 live = *reinterpret_cast<const f4*>(rows + 3 * kC);
-#pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int64_t t = c * kC + 16 * m + 4 * g + e;
-        dy[q][e] = column && t < a.seqlen && live[e] != 0.0f
-                       ? to_f32(static_cast<const T*>(
-                             a.dout)[b * a.dout_stride_b + t * a.dout_stride_t + h * a.dout_stride_h + dv])
-                       : 0.0f;
+        const int64_t d = 32 * KB * part + 16 * t + 4 * g + e;
+        ds[n][t][e] = a.dfinal_states && dv + 16 * n < a.value_dim && d < a.key_dim
+                          ? a.dfinal_states[(at.head * a.key_dim + d) * a.value_dim + dv + 16 * n]
+                          : 0.0f;
       }
-    }
-  };
-  auto load_p = [&](int64_t c) {
-#pragma unroll
-    for (int q = 0; q < MT; ++q) {
-      const int m = RowTiles<NW>::at(w, q);
-      rest[q] = *reinterpret_cast<const f4*>(p.rows + (hc0 + c) * (kRowFields * kC) + kC + 16 * m + 4 * g);
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-        if (s >= m / 2) load_frag(p.pf + (hc0 + c) * (kTri * 3 * 64) + upper_frag(m, s) * (3 * 64) + lane, pf[q][s]);
-    }
-  };
-  auto load_tri = [&](int64_t c) {
-#pragma unroll
-    for (int q = 0; q < MT; ++q) {
-      const int m = RowTiles<NW>::at(w, q);
-      beta[q] = *reinterpret_cast<const f4*>(p.rows + (hc0 + c) * (kRowFields * kC) + 2 * kC + 16 * m + 4 * g);
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-        if (s >= m / 2) load_frag(p.tf + (hc0 + c) * (kTri * 3 * 64) + upper_frag(m, s) * (3 * 64) + lane, tf[q][s]);
-    }
-  };
-
-  f4 ds[2 * KB];
-#pragma unroll
-  for (int t = 0; t < 2 * KB; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t d = 32 * KB * w + 16 * t + 4 * g + e;
-      ds[t][e] = a.dfinal_states && column && d < a.key_dim
-                     ? a.dfinal_states[(at.head * a.key_dim + d) * a.value_dim + dv]
-                     : 0.0f;
-    }
+  float* dsp = p.ds + at.head * N * (DK * (int64_t)p.dvp) + (32 * KB * part + 4 * g) * p.dvp + dv;
+  float* drp = p.dr + at.head * N * (kC * (int64_t)p.dvp) + row * p.dvp + dv;
+  const int64_t stride = a.heads * a.value_dim;
+  T* dvo = static_cast<T*>(a.dv) + (b * a.seqlen + row) * stride + h * a.value_dim + dv;
   if constexpr (AHEAD) {
     load_k(N - 1);
-    load_t(N - 1);
+    load_kc(N - 1);
   }
-  load_dy(N - 1);
-  load_p(N - 1);
-  load_tri(N - 1);
+  load_rest(N - 1);
+  load_t(N - 1);
+  lds_barrier();  // the waves beside the chain begin with the last chunk's dO
   for (int64_t c = N - 1; c >= 0; --c) {
     const int64_t next = c ? c - 1 : 0;
     {
-      float* to = p.ds + (hc0 + c) * ((int64_t)DK * p.dvp) + at.dv0 + col;
+      f4 x[CT][L::kRows] = {};
+#pragma unroll
+      for (int i = 0; i < KB; ++i) {
+        if constexpr (!AHEAD) load_k_of(c, i);
+#pragma unroll
+        for (int n = 0; n < CT; ++n) {
+          u4 sb[3];
+          split8<3>(ds[n][2 * i], ds[n][2 * i + 1], sb);
+#pragma unroll
+          for (int m = 0; m < L::kRows; ++m) x[n][m] = mac<2>(kx[i][m], sb, x[n][m]);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < CT; ++n)
+#pragma unroll
+        for (int m = 0; m < L::kRows; ++m) red[n][part][rows0 + m][lane] = x[n][m];
+    }
+    if (keeper) {
+      float* to = dsp + c * (DK * (int64_t)p.dvp);
 #pragma unroll
       for (int t = 0; t < 2 * KB; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) to[(32 * KB * w + 16 * t + 4 * g + e) * p.dvp] = ds[t][e];
-      if constexpr (!AHEAD) load_k(c);
-      f4 x[4] = {};
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int i = 0; i < KB; ++i) {
-        u4 sb[3];
-        split8<3>(ds[2 * i], ds[2 * i + 1], sb);
-#pragma unroll
-        for (int m = 0; m < 4; ++m) x[m] = mac<2>(kf[i][m], sb, x[m]);
-      }
-#pragma unroll
-      for (int m = 0; m < 4; ++m) red[w][m][lane] = x[m];
+          for (int n = 0; n < CT; ++n) to[(16 * t + e) * p.dvp + 16 * n] = ds[n][t][e];
     }
     if constexpr (AHEAD) load_k(next);
-    f4 now_into[MT];
-#pragma unroll
-    for (int q = 0; q < MT; ++q) {
-      const int m = RowTiles<NW>::at(w, q);
-      const f4 d = {dy[q][0], dy[q][1], dy[q][2], dy[q][3]};
-      f4 s;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[e] = a.scale * into[q][e] * d[e];
-      u2 half[NI], third[3];
-      split4<NI>(d, half);
-      store_half<NI>(&ob[m / 2][0][lane], m & 1, half);
-      split4<3>(s, third);
-      store_half<3>(&oq[m / 2][0][lane], m & 1, third);
-      now_into[q] = into[q];
-    }
-    load_dy(next);
+    whole_now = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(whole)));
     lds_barrier();
 #pragma unroll
-    for (int q = 0; q < MT; ++q) {
-      const int m = RowTiles<NW>::at(w, q);
-      f4 y = red[0][m][lane];
+    for (int n = 0; n < CT; ++n) {
+      f4 y = red[n][0][w][lane];
 #pragma unroll
-      for (int n = 1; n < NW; ++n) y += red[n][m][lane];
+      for (int j = 1; j < L::kParts; ++j) y += red[n][j][w][lane];
+      const f4 o = pd[n][w][lane];
+      f4 z;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = rest[q][e] != 0.0f ? rest[q][e] * y[e] : 0.0f;
+      for (int e = 0; e < 4; ++e) z[e] = fmaf(rest[e], y[e], o[e]);
+      if (whole_now == 0.0f)  // a reset or padding: rows that do not reach the end
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        if (s >= m / 2) {
-          u4 o[NI];
-          load_frag(&ob[s][0][lane], o);
-          y = mac<2>(pf[q][s], o, y);
-        }
+        for (int e = 0; e < 4; ++e) z[e] = rest[e] != 0.0f ? z[e] : o[e];
       u2 half[3];
-      split4<3>(y, half);
-      store_half<3>(&ub[m / 2][0][lane], m & 1, half);
+      split4<3>(z, half);
+      store_half<3>(&ub[n][w / 2][0][lane], w & 1, half);
     }
-    load_p(next);
+    load_rest(next);
     lds_barrier();
 #pragma unroll
-    for (int q = 0; q < MT; ++q) {
-      const int m = RowTiles<NW>::at(w, q);
-      f4 r = {0, 0, 0, 0};
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-        if (s >= m / 2) {
-          u4 u[3];
-          load_frag(&ub[s][0][lane], u);
-          r = mac<2>(tf[q][s], u, r);
-        }
-      float* to = p.dr + (hc0 + c) * (kC * p.dvp) + at.dv0 + col;
-      T* out = static_cast<T*>(a.dv);
-      u2 half[3];
+    for (int n = 0; n < CT; ++n) {
+      f4 r = {0, 0, 0, 0}, r1 = {0, 0, 0, 0};
+      u4 u[3];
+      load_frag(&ub[n][1][0][0], lane, u);
+      r = mac<2>(tx[1], u, r);
+      if (w < 2) {
+        load_frag(&ub[n][0][0][0], lane, u);
+        r1 = mac<2>(tx[0], u, r1);
+      }
+      r += r1;
       f4 x;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t t = c * kC + 16 * m + 4 * g + e;
-        to[(16 * m + 4 * g + e) * p.dvp] = r[e];
-        if (column && t < a.seqlen)
-          out[((b * a.seqlen + t) * a.heads + h) * a.value_dim + dv] =
-              (T)(beta[q][e] != 0.0f ? beta[q][e] * r[e] : 0.0f);
-        x[e] = now_into[q][e] != 0.0f ? -beta[q][e] * now_into[q][e] * r[e] : 0.0f;
-      }
+      for (int e = 0; e < 4; ++e) x[e] = -beta[e] * into[e] * r[e];
+      if (whole_now == 0.0f)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = into[e] != 0.0f ? x[e] : 0.0f;
+      u2 half[3];
       split4<3>(x, half);
-      store_half<3>(&rb[m / 2][0][lane], m & 1, half);
+      store_half<3>(&rb[n][w / 2][0][lane], w & 1, half);
+      float* to = drp + c * (kC * (int64_t)p.dvp) + 16 * n;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) to[e * p.dvp] = r[e];
+      if (dv + 16 * n < a.value_dim) {
+        T* out = dvo + c * (kC * stride) + 16 * n;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c * kC + row + e < a.seqlen) out[e * stride] = (T)(beta[e] != 0.0f ? beta[e] * r[e] : 0.0f);
+      }
     }
-    load_tri(next);
-    if constexpr (!AHEAD) load_t(c);
+    load_t(next);
+#pragma unroll
+    for (int n = 0; n < CT; ++n)
+#pragma unroll
+      for (int t = 0; t < 2 * KB; ++t) {
+        ds[n][t] *= whole_now;
+        if (whole_now == 0.0f) ds[n][t] = f4{0, 0, 0, 0};
+      }
     lds_barrier();
 #pragma unroll
-    for (int t = 0; t < 2 * KB; ++t) {
+    for (int n = 0; n < CT; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) ds[t][e] = whole != 0.0f ? whole * ds[t][e] : 0.0f;
+      for (int t = 0; t < 2 * KB; ++t) ds[n][t] += qd[n][2 * KB * part + t][lane];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < 2; ++s) {
+      if constexpr (!AHEAD) load_kc_of(c, s);
+#pragma unroll
+      for (int n = 0; n < CT; ++n) {
         u4 x[3];
-        load_frag(&oq[s][0][lane], x);
-        ds[t] = mac<2>(qt[t][s], x, ds[t]);
-        load_frag(&rb[s][0][lane], x);
-        ds[t] = mac<2>(kt[t][s], x, ds[t]);
+        load_frag(&rb[n][s][0][0], lane, x);
+#pragma unroll
+        for (int t = 0; t < 2 * KB; ++t) ds[n][t] = mac<2>(kc[t][s], x, ds[n][t]);
       }
     }
-    if constexpr (AHEAD) load_t(next);
-    lds_barrier();  // ob and oq are written again before the next barrier
+    if constexpr (AHEAD) load_kc(next);
   }
-  if (a.dinitial_states && column)
+  if (a.dinitial_states && keeper)
 #pragma unroll
-    for (int t = 0; t < 2 * KB; ++t)
+    for (int n = 0; n < CT; ++n)
+      if (dv + 16 * n < a.value_dim)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t d = 32 * KB * w + 16 * t + 4 * g + e;
-        if (d < a.key_dim) a.dinitial_states[(at.head * a.key_dim + d) * a.value_dim + dv] = ds[t][e];
-      }
+        for (int t = 0; t < 2 * KB; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int64_t d = 32 * KB * part + 16 * t + 4 * g + e;
+            if (d < a.key_dim) a.dinitial_states[(at.head * a.key_dim + d) * a.value_dim + dv + 16 * n] = ds[n][t][e];
+          }
 }
 
 // All chunks: dq, dk and, as sums over the keys' elements, what dbeta and dlog_decay need, from S0, U, dS1 and dR. A
-// workgroup has a chunk of a key head, up to 128 of the keys' elements, and goes through the heads that share
+// workgroup has a chunk of a key head, 64 or 128 of the keys' elements, and goes through the heads that share
 // the key, so that their gradients are added in fp32 and in order. A wave has 16 of the elements as rows and the
-// chunk's rows as columns. (In fp16 and fp32 64 elements, for the registers of one wave per SIMD.)
+// chunk's rows as columns. The sum over the value columns goes by 32: their operands are requested while the products
+// of those before are made; dR, U and dO pass LDS as fragments, S0 and dS1 go to the wave that has their rows.
+// Eight waves a workgroup, but four for small heads, of which a CU holds two workgroups, and in fp32, for the registers.
 template <typename T, int DK>
-constexpr int kGradWaves = DK < 128 || kPieces<T> > 1 ? 4 : 8;
+constexpr int kGradWaves = DK < 128 || sizeof(T) == 4 ? 4 : 8;
 template <typename T, int DK>
 constexpr int kGradParts = DK / 16 / kGradWaves<T, DK>;
 
@@ -949,31 +1158,49 @@ struct GateSums {
 };
 constexpr int kGateFields = 4;
 
-// dbeta and dlog_decay of row `lane` of a head's chunk, in a wave.
-__device__ __forceinline__ void finish_gates(const ccv1d_delta_args& a, int64_t b, int64_t c, int64_t h, int lane,
+// What the kernels of the gradients take: 32-bit sizes and no more than they use, for the scalar registers.
+struct GradArgs {
+  const u4 *kf, *qf, *kt, *qt;
+  const float *rows, *s0, *u, *ds, *dr;
+  float* gates;
+  const void *v, *dout;
+  int64_t v_stride_b, v_stride_t, v_stride_h, dout_stride_b, dout_stride_t, dout_stride_h;
+  void *dq, *dk, *dlog_decay, *dbeta;
+  float scale;
+  int32_t units, chunks, group, key_heads, heads, seqlen, key_dim, value_dim, dvp, log_decay_dtype, beta_dtype;
+};
+
+// dbeta and dlog_decay of row `lane` of a head's chunk, in a wave. A row that resets the state has no gradient of
+// its decay.
+__device__ __forceinline__ void finish_gates(const GradArgs& p, int64_t b, int c, int h, int lane, const float* rows,
                                              const GateSums& x) {
-  const ChunkRows r = chunk_row(a, b, c, h, lane);
-  double s = (double)x.other - (double)r.beta * (double)x.kz + (lane == 63 ? (double)x.end : 0.0);
+  const float beta = rows[2 * kC + lane];
+  const bool live = rows[3 * kC + lane] != 0.0f;
+  const int run = reinterpret_cast<const int*>(rows + 7 * kC)[lane];
+  const int before = __shfl_up(run, 1);
+  const bool reset = run != (lane ? before : 0);
+  double s = (double)x.other - (double)beta * (double)x.kz + (lane == 63 ? (double)x.end : 0.0);
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
     const double o = __shfl_down(s, d);
-    const int run = __shfl_down(r.run, d);
-    if (lane + d < 64 && run == r.run) s += o;
+    const int r = __shfl_down(run, d);
+    if (lane + d < 64 && r == run) s += o;
   }
-  const int64_t t = c * kC + lane, o = (b * a.seqlen + t) * a.heads + h;
-  if (t < a.seqlen) {
-    store_as(a.dlog_decay, o, a.log_decay_dtype, r.live && !r.reset ? (float)s : 0.0f);
-    store_as(a.dbeta, o, a.beta_dtype, r.live ? x.rv - x.kz : 0.0f);
+  const int t = c * kC + lane;
+  const int64_t o = (b * p.seqlen + t) * p.heads + h;
+  if (t < p.seqlen) {
+    store_as(p.dlog_decay, o, p.log_decay_dtype, live && !reset ? (float)s : 0.0f);
+    store_as(p.dbeta, o, p.beta_dtype, live ? x.rv - x.kz : 0.0f);
   }
 }
 
 // The same where the keys' elements lie in several workgroups; a wave has a head's chunk.
 template <int PARTS>
-__global__ __launch_bounds__(256) void delta_gates_kernel(DeltaParams p) {
+__global__ __launch_bounds__(256) void delta_gates_kernel(GradArgs p) {
   const int lane = threadIdx.x & 63;
   const int64_t hc = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (hc >= p.a.batch * p.a.heads * p.chunks) return;
-  const int64_t head = hc / p.chunks, b = head / p.a.heads;
+  if (hc >= (int64_t)p.units * p.group) return;
+  const int64_t head = hc / p.chunks, b = head / p.heads;
   GateSums x{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int i = 0; i < PARTS; ++i) {
@@ -981,149 +1208,189 @@ __global__ __launch_bounds__(256) void delta_gates_kernel(DeltaParams p) {
     x.kz += from[0], x.other += from[kC], x.end += from[3 * kC];
     if (i == 0) x.rv = from[2 * kC];  // each part has it
   }
-  finish_gates(p.a, b, hc - head * p.chunks, head - b * p.a.heads, lane, x);
+  finish_gates(p, b, (int)(hc - head * p.chunks), (int)(head - b * p.heads), lane, p.rows + hc * (kRowFields * kC), x);
 }
 
-template <typename T, int DK>
-__global__ __launch_bounds__((kGradWaves<T, DK>) * 64) void delta_grad_kernel(DeltaParams p) {
-  constexpr int NI = kPieces<T>, KS = DK / 32, NW = kGradWaves<T, DK>, LG = 68;
-  constexpr int PAIRS = (10 + NW - 1) / NW;
-  __shared__ u4 fr[12][3][64];  // fragments: dR, U, dO of 32 value columns, then those of the products between rows
-  __shared__ float gl[kC * LG];
-  __shared__ ChunkShared sh;
-  __shared__ float sums[NW][2][kC], vsum[kC], tail[NW];
-  const ccv1d_delta_args& a = p.a;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  const int part = blockIdx.x % kGradParts<T, DK>, tile = part * NW + w;  // the wave's elements: 16 tile ...
-  const int64_t kc = blockIdx.x / kGradParts<T, DK>, c = kc % p.chunks, bk = kc / p.chunks, b = bk / a.key_heads, kh = bk - b * a.key_heads;
-  const int64_t t0 = c * kC;
-  const u4* kf = p.kf + kc * (4 * KS * NI * 64);
-  const u4* qf = p.qf + kc * (4 * KS * NI * 64);
-  const u4* kt = p.kt + kc * (DK / 16 * 2 * NI * 64);
-  const u4* qt = p.qt + kc * (DK / 16 * 2 * NI * 64);
-  f4 dq[4] = {}, dk[4] = {};
-  // The tiles of the products between rows that a wave has: n <= m.
-  int tm[PAIRS], tn[PAIRS];
+// Eight elements of a row, at `p` and 16 further on, as they lie in memory.
+template <typename T>
+struct RawRow {
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  v4 lo, hi;
+  __device__ __forceinline__ void load(const T* p, int left) {  // so many elements from p on
+    if (left >= 32) {
+      __builtin_memcpy(&lo, p, sizeof lo);
+      __builtin_memcpy(&hi, p + 16, sizeof hi);
+    } else {
 #pragma unroll
-  for (int i = 0; i < PAIRS; ++i) {
-    const int x = w + NW * i;
-    tm[i] = x < 1 ? 0 : x < 3 ? 1 : x < 6 ? 2 : 3;
-    tn[i] = x < 10 ? x - tm[i] * (tm[i] + 1) / 2 : -1;
+      for (int e = 0; e < 4; ++e) {
+        lo[e] = e < left ? p[e] : (T)0.0f;
+        hi[e] = e + 16 < left ? p[e + 16] : (T)0.0f;
+      }
+    }
   }
+  __device__ __forceinline__ f4 low() const { return f4{to_f32(lo[0]), to_f32(lo[1]), to_f32(lo[2]), to_f32(lo[3])}; }
+  __device__ __forceinline__ f4 high() const { return f4{to_f32(hi[0]), to_f32(hi[1]), to_f32(hi[2]), to_f32(hi[3])}; }
+};
 
-  for (int64_t h = kh * p.group; h < (kh + 1) * p.group; ++h) {
-    const int64_t head = b * a.heads + h, hc = head * p.chunks + c;
-    const float* rows = p.rows + hc * (kRowFields * kC);
-    const float* s0 = p.s0 + hc * ((int64_t)DK * p.dvp);
-    const float* ds = p.ds + hc * ((int64_t)DK * p.dvp);
-    const float* u = p.u + hc * (kC * p.dvp);
-    const float* dr = p.dr + hc * (kC * p.dvp);
-    if (w == 0) share_rows(a, b, c, h, lane, sh, nullptr);
+template <typename T, int DK>
+__global__ __launch_bounds__((kGradWaves<T, DK>) * 64, kPieces<T> > 1 ? 1 : 2) void delta_grad_kernel(GradArgs p) {
+  constexpr int NI = kPieces<T>, KS = DK / 32, NW = kGradWaves<T, DK>, LG = 68, PAIRS = (10 + NW - 1) / NW;
+  // fragments: dR, U, dO of 32 value columns; then those of the products between rows
+  __shared__ u4 f[12][3][64];
+  __shared__ float gl[kC * LG], rows[kRowFields * kC];
+  __shared__ float sums[NW][2][kC], vsum[kC], tail[NW];
+  const int w = wave_index(), wr = w & 3;
+  // The parts of a chunk go to one XCD, whose L2 they share.
+  const int slot = blockIdx.x >> 3, kc = slot / kGradParts<T, DK> * 8 + (blockIdx.x & 7);
+  if (kc >= p.units) return;
+  const int part = slot % kGradParts<T, DK>, tile = part * NW + w;  // the wave's elements: 16 tile ...
+  const int bk = kc / p.chunks, c = kc - bk * p.chunks, b = bk / p.key_heads, kh = bk - b * p.key_heads;
+  const int t0 = c * kC;
+  const u4* kf = p.kf + (int64_t)kc * (4 * KS * NI * 64);
+  const u4* qf = p.qf + (int64_t)kc * (4 * KS * NI * 64);
+  const u4* kt = p.kt + (int64_t)kc * (DK / 16 * 2 * NI * 64);
+  const u4* qt = p.qt + (int64_t)kc * (DK / 16 * 2 * NI * 64);
+  const double* sum = reinterpret_cast<const double*>(rows + 5 * kC);
+  const int* run = reinterpret_cast<const int*>(rows + 7 * kC);
+  f4 dq[4] = {}, dk[4] = {};
+  // The tiles (m, n) of the products between rows that a wave has, n <= m: of ten, those of its number and every NW
+  // further.
+  struct Pair {
+    int m, n;
+    __device__ __forceinline__ Pair(int x) {
+      asm volatile("" : "+s"(x));  // made where it is used: scalar registers
+      m = x < 1 ? 0 : x < 3 ? 1 : x < 6 ? 2 : 3;
+      n = x - m * (m + 1) / 2;
+    }
+  };
+
+  for (int h = kh * p.group; h < (kh + 1) * p.group; ++h) {
+    const int64_t hc = (int64_t)(b * p.heads + h) * p.chunks + c;
+    // Addresses are made and k's and q's fragments read anew for every head: kept, they would spill.
+    uint32_t lane = threadIdx.x & 63;
+    asm volatile("" : "+s"(kf), "+s"(qf), "+s"(kt), "+s"(qt), "+v"(lane));
+    const uint32_t col = lane & 15, g = lane >> 4;
+    const int mine = 16 * wr + col;  // the row whose dR and V, or U and dO, the lane reads (four waves: all)
+    const int64_t mine_t = min(t0 + mine, p.seqlen - 1);
+    const float* s0 = p.s0 + hc * ((int64_t)DK * p.dvp) + (16 * tile + col) * p.dvp + 4 * g;
+    const float* ds = p.ds + hc * ((int64_t)DK * p.dvp) + (16 * tile + col) * p.dvp + 4 * g;
+    const float* up = p.u + hc * (kC * (int64_t)p.dvp) + mine * p.dvp + 4 * g;
+    const float* rp = p.dr + hc * (kC * (int64_t)p.dvp) + mine * p.dvp + 4 * g;
+    const T* vp = static_cast<const T*>(p.v) + b * p.v_stride_b + mine_t * p.v_stride_t + h * p.v_stride_h + 4 * g;
+    const T* op = static_cast<const T*>(p.dout) + b * p.dout_stride_b + mine_t * p.dout_stride_t + h * p.dout_stride_h +
+                  4 * g;
+    f4 xr[2], xu[2], xs[2], xd[2];
+    RawRow<T> xo, xv;
+    auto load = [&](int d0) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (NW == 4 || w < 4) xr[i] = *reinterpret_cast<const f4*>(rp + d0 + 16 * i);
+        if (NW == 4 || w >= 4) xu[i] = *reinterpret_cast<const f4*>(up + d0 + 16 * i);
+        xs[i] = *reinterpret_cast<const f4*>(s0 + d0 + 16 * i);
+        xd[i] = *reinterpret_cast<const f4*>(ds + d0 + 16 * i);
+      }
+      const int left = p.value_dim - d0 >= 32 ? 32 : p.value_dim - d0 - 4 * (int)g;
+      if (NW == 4 || w >= 4) xo.load(op + d0, left);
+      if (NW == 4 || w < 4) xv.load(vp + d0, left);
+    };
+    load(0);
+    if (threadIdx.x < kRowFields * kC / 4)
+      reinterpret_cast<f4*>(rows)[threadIdx.x] =
+          reinterpret_cast<const f4*>(p.rows + hc * (kRowFields * kC))[threadIdx.x];
+    lds_barrier();
+    const bool live = rows[3 * kC + mine] != 0.0f;
     f4 aq[4] = {}, az[4] = {}, ac[4] = {}, go[PAIRS] = {}, gr[PAIRS] = {};
     float through = 0.0f, along = 0.0f;  // <dS1, S0> and dR.V of the lane's elements
-    lds_barrier();
     for (int d0 = 0; d0 < p.dvp; d0 += 32) {
-      // dR, U and dO of 32 value columns as fragments, one tile of rows and one of the three a turn
-      for (int job = w; job < 12; job += NW) {
-        const int kind = job >> 2, m = job & 3, i = 16 * m + col;
-        const int64_t x = i * p.dvp + d0 + 4 * g;
-        if (kind < 2) {
-          const float* from = kind ? u : dr;
-          const f4 lo = *reinterpret_cast<const f4*>(from + x), hi = *reinterpret_cast<const f4*>(from + x + 16);
-          u4 f[3];
-          split8<3>(lo, hi, f);
-#pragma unroll
-          for (int n = 0; n < 3; ++n) fr[kind * 4 + m][n][lane] = f[n];
-          if (kind == 0 && sh.live[i]) {
-            const T* vp = static_cast<const T*>(a.v) + b * a.v_stride_b + (t0 + i) * a.v_stride_t + h * a.v_stride_h;
-            const int64_t d = d0 + 4 * g;
-            f4 y = {0, 0, 0, 0}, z = {0, 0, 0, 0};
-            if (d < a.value_dim) y = load4(vp + d, a.value_dim - d);
-            if (d + 16 < a.value_dim) z = load4(vp + d + 16, a.value_dim - d - 16);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) along = fmaf(lo[e], y[e], fmaf(hi[e], z[e], along));
-          }
-        } else {
-          f4 y = {0, 0, 0, 0}, z = {0, 0, 0, 0};
-          if (sh.live[i]) {
-            const T* op = static_cast<const T*>(a.dout) + b * a.dout_stride_b + (t0 + i) * a.dout_stride_t +
-                          h * a.dout_stride_h;
-            const int64_t d = d0 + 4 * g;
-            if (d < a.value_dim) y = load4(op + d, a.value_dim - d);
-            if (d + 16 < a.value_dim) z = load4(op + d + 16, a.value_dim - d - 16);
-          }
-          u4 f[NI];
-          split8<NI>(y, z, f);
-#pragma unroll
-          for (int n = 0; n < NI; ++n) fr[8 + m][n][lane] = f[n];
-        }
-      }
       lds_barrier();
-      const int64_t x = (int64_t)(16 * tile + col) * p.dvp + d0 + 4 * g;
-      const f4 slo = *reinterpret_cast<const f4*>(s0 + x), shi = *reinterpret_cast<const f4*>(s0 + x + 16);
-      const f4 dlo = *reinterpret_cast<const f4*>(ds + x), dhi = *reinterpret_cast<const f4*>(ds + x + 16);
       u4 sf[3], df[3];
-      split8<3>(slo, shi, sf);
-      split8<3>(dlo, dhi, df);
+      if (NW == 4 || w < 4) {
+        u4 x[3];
+        split8<3>(xr[0], xr[1], x);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) through = fmaf(slo[e], dlo[e], fmaf(shi[e], dhi[e], through));
+        for (int n = 0; n < 3; ++n) f[wr][n][lane] = x[n];
+        const f4 lo = xv.low(), hi = xv.high();
+        if (live)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) along = fmaf(xr[0][e], lo[e], fmaf(xr[1][e], hi[e], along));
+      }
+      if (NW == 4 || w >= 4) {
+        u4 x[3], y[NI];
+        split8<3>(xu[0], xu[1], x);
+#pragma unroll
+        for (int n = 0; n < 3; ++n) f[4 + wr][n][lane] = x[n];
+        f4 lo = xo.low(), hi = xo.high();
+        if (!live) lo = hi = f4{0, 0, 0, 0};
+        split8<NI>(lo, hi, y);
+#pragma unroll
+        for (int n = 0; n < NI; ++n) f[8 + wr][n][lane] = y[n];
+      }
+      split8<3>(xs[0], xs[1], sf);
+      split8<3>(xd[0], xd[1], df);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) through = fmaf(xs[0][e], xd[0][e], fmaf(xs[1][e], xd[1][e], through));
+      if (d0 + 32 < p.dvp) load(d0 + 32);
+      lds_barrier();
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
-        u4 x3[3], xo[NI];
-        load_frag(&fr[m][0][lane], x3);
+        __builtin_amdgcn_sched_barrier(0);  // a tile's operands at a time: registers
+        u4 x3[3], y[NI];
+        load_frag(&f[m][0][0], lane, x3);
         az[m] = mac<2>(sf, x3, az[m]);
-        load_frag(&fr[8 + m][0][lane], xo);
-        aq[m] = mac<2>(sf, xo, aq[m]);
-        load_frag(&fr[4 + m][0][lane], x3);
+        load_frag(&f[8 + m][0][0], lane, y);
+        aq[m] = mac<2>(sf, y, aq[m]);
+        load_frag(&f[4 + m][0][0], lane, x3);
         ac[m] = mac<2>(df, x3, ac[m]);
       }
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i)
-        if (tn[i] >= 0) {
-          u4 un[3], x3[3], xo[NI];
-          load_frag(&fr[4 + tn[i]][0][lane], un);
-          load_frag(&fr[8 + tm[i]][0][lane], xo);
-          go[i] = mac<2>(un, xo, go[i]);
-          load_frag(&fr[tm[i]][0][lane], x3);
+        if (w + NW * i < 10) {
+          const Pair t(w + NW * i);
+          __builtin_amdgcn_sched_barrier(0);
+          u4 un[3], x3[3], y[NI];
+          load_frag(&f[4 + t.n][0][0], lane, un);
+          load_frag(&f[8 + t.m][0][0], lane, y);
+          go[i] = mac<2>(un, y, go[i]);
+          load_frag(&f[t.m][0][0], lane, x3);
           gr[i] = mac<2>(un, x3, gr[i]);
         }
-      lds_barrier();
     }
     // The factors of the columns, and k.(state's part of c).
     float state_part = 0.0f;
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
       const float into = rows[16 * m + col], rest = rows[kC + 16 * m + col];
+      u4 kv[NI];
+      load_frag(kf + (m * KS + tile / 2) * (NI * 64), lane, kv);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        aq[m][e] = into != 0.0f ? a.scale * into * aq[m][e] : 0.0f;
+        aq[m][e] = into != 0.0f ? p.scale * into * aq[m][e] : 0.0f;
         az[m][e] = into != 0.0f ? into * az[m][e] : 0.0f;
         ac[m][e] = rest != 0.0f ? rest * ac[m][e] : 0.0f;
+        state_part = fmaf(piece_sum(kv, tile & 1, e), ac[m][e], state_part);
       }
-      u4 kv[NI];
-      load_frag(kf + (m * KS + tile / 2) * (NI * 64) + lane, kv);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) state_part = fmaf(piece_sum(kv, (tile & 1) * 4 + e), ac[m][e], state_part);
     }
     // Two rounds over the products between rows: scale D dO.U^T for dq and dk, D dR.U^T for z and dk.
 #pragma unroll
     for (int round = 0; round < 2; ++round) {
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i)
-        if (tn[i] >= 0) {
-          const int row = 16 * tm[i] + col;
+        if (w + NW * i < 10) {
+          const Pair t(w + NW * i);
+          const int r = 16 * t.m + col;
           f4 x;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int j = 16 * tn[i] + 4 * g + e;
-            const bool seen = (round ? j < row : j <= row) && sh.run[row] == sh.run[j];
-            const float d = seen ? exp2_of(sh.sum[row] - sh.sum[j]) : 0.0f;
-            x[e] = seen ? (round ? d * gr[i][e] : a.scale * d * go[i][e]) : 0.0f;
+            const int j = 16 * t.n + 4 * g + e;
+            const bool seen = (round ? j < r : j <= r) && run[r] == run[j];
+            const float d = seen ? exp2_of(sum[r] - sum[j]) : 0.0f;
+            x[e] = seen ? (round ? d * gr[i][e] : p.scale * d * go[i][e]) : 0.0f;
           }
-          *reinterpret_cast<f4*>(&gl[row * LG + 16 * tn[i] + 4 * g]) = x;
+          *reinterpret_cast<f4*>(&gl[r * LG + 16 * t.n + 4 * g]) = x;
         }
       lds_barrier();
       // fragments 0..5: sum over j, columns i (lower); 6..11: sum over i, columns j (upper)
+#pragma unroll 1
       for (int job = w; job < 12; job += NW) {
         const int x = job < 6 ? job : job - 6;
         const int m = job < 6 ? (x < 2 ? x : x < 4 ? 2 : 3) : (x < 2 ? 0 : x < 4 ? 1 : x - 2);
@@ -1139,47 +1406,49 @@ __global__ __launch_bounds__((kGradWaves<T, DK>) * 64) void delta_grad_kernel(De
             const int i = 32 * s + 4 * g + e;
             if (2 * s >= m) lo[e] = gl[i * LG + 16 * m + col];
             hi[e] = gl[(i + 16) * LG + 16 * m + col];
-            if (round) lo[e] *= -sh.beta[i], hi[e] *= -sh.beta[i + 16];
+            if (round) lo[e] *= -rows[2 * kC + i], hi[e] *= -rows[2 * kC + i + 16];
           }
         }
-        u4 f[3];
-        split8<3>(lo, hi, f);
+        u4 y[3];
+        split8<3>(lo, hi, y);
 #pragma unroll
-        for (int n = 0; n < 3; ++n) fr[job][n][lane] = f[n];
+        for (int n = 0; n < 3; ++n) f[job][n][lane] = y[n];
       }
       lds_barrier();
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        u4 kx[NI], qx[NI], x3[3];
-        load_frag(kt + (tile * 2 + s) * (NI * 64) + lane, kx);
-        if (round == 0) load_frag(qt + (tile * 2 + s) * (NI * 64) + lane, qx);
+        u4 kx[NI], qx[NI];
+        load_frag(kt + (tile * 2 + s) * (NI * 64), lane, kx);
+        if (round == 0) load_frag(qt + (tile * 2 + s) * (NI * 64), lane, qx);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
+          __builtin_amdgcn_sched_barrier(0);
+          u4 x3[3];
           if (s <= m / 2) {
-            load_frag(&fr[lower_frag(m, s)][0][lane], x3);
+            load_frag(&f[lower_frag(m, s)][0][0], lane, x3);
             if (round == 0) aq[m] = mac<2>(kx, x3, aq[m]);
             else az[m] = mac<2>(kx, x3, az[m]);
           }
           if (s >= m / 2) {
-            load_frag(&fr[6 + upper_frag(m, s)][0][lane], x3);
+            load_frag(&f[6 + upper_frag(m, s)][0][0], lane, x3);
             if (round == 0) ac[m] = mac<2>(qx, x3, ac[m]);
             else ac[m] = mac<2>(kx, x3, ac[m]);
           }
         }
       }
-      lds_barrier();
+      if (round == 0) lds_barrier();
     }
     // Sums over the keys' elements: k.z, and q.dq - k.c.
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
       float kz = 0.0f, rest = 0.0f;
-      const float beta = sh.beta[16 * m + col];
+      const float beta = rows[2 * kC + 16 * m + col];
       u4 kv[NI], qv[NI];
-      load_frag(kf + (m * KS + tile / 2) * (NI * 64) + lane, kv);
-      load_frag(qf + (m * KS + tile / 2) * (NI * 64) + lane, qv);
+      load_frag(kf + (m * KS + tile / 2) * (NI * 64), lane, kv);
+      load_frag(qf + (m * KS + tile / 2) * (NI * 64), lane, qv);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float k = piece_sum(kv, (tile & 1) * 4 + e), q = piece_sum(qv, (tile & 1) * 4 + e);
+        const float k = piece_sum(kv, tile & 1, e), q = piece_sum(qv, tile & 1, e);
         kz = fmaf(k, az[m][e], kz);
         rest = fmaf(q, aq[m][e], fmaf(-k, ac[m][e], rest));
         dk[m][e] += ac[m][e] - beta * az[m][e];
@@ -1189,11 +1458,9 @@ __global__ __launch_bounds__((kGradWaves<T, DK>) * 64) void delta_grad_kernel(De
       kz += __shfl_xor(kz, 32), rest += __shfl_xor(rest, 32);
       if (g == 0) sums[w][0][16 * m + col] = kz, sums[w][1][16 * m + col] = rest;
     }
-    if (w < 4) {  // dR.V: the wave's jobs were the tile of rows of its number
-      along += __shfl_xor(along, 16);
-      along += __shfl_xor(along, 32);
-      if (g == 0) vsum[16 * w + col] = along;
-    }
+    along += __shfl_xor(along, 16);
+    along += __shfl_xor(along, 32);
+    if (g == 0 && w < 4) vsum[mine] = along;
     const float whole = rows[4 * kC];
     float end = state_part + (whole != 0.0f ? whole * through : 0.0f);
 #pragma unroll
@@ -1205,7 +1472,7 @@ __global__ __launch_bounds__((kGradWaves<T, DK>) * 64) void delta_grad_kernel(De
 #pragma unroll
       for (int n = 0; n < NW; ++n) x.kz += sums[n][0][lane], x.other += sums[n][1][lane], x.end += tail[n];
       if constexpr (kGradParts<T, DK> == 1) {
-        finish_gates(a, b, c, h, lane, x);
+        finish_gates(p, b, c, h, lane, rows, x);
       } else {
         float* to = p.gates + (hc * kGradParts<T, DK> + part) * (kGateFields * kC) + lane;
         to[0] = x.kz, to[kC] = x.other, to[2 * kC] = x.rv, to[3 * kC] = x.end;
@@ -1213,37 +1480,51 @@ __global__ __launch_bounds__((kGradWaves<T, DK>) * 64) void delta_grad_kernel(De
     }
     lds_barrier();
   }
+  const uint32_t col = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
 #pragma unroll
   for (int m = 0; m < 4; ++m) {
     const int i = 16 * m + col;
-    if (t0 + i >= a.seqlen) continue;
-    const bool live = sh.live[i];
-    const int64_t row = ((b * a.seqlen + t0 + i) * a.key_heads + kh) * a.key_dim;
-    const int64_t d = 16 * tile + 4 * g;
-    if (d >= a.key_dim) continue;
+    if (t0 + i >= p.seqlen) continue;
+    const bool live = rows[3 * kC + i] != 0.0f;
+    const int64_t row = (((int64_t)b * p.seqlen + t0 + i) * p.key_heads + kh) * p.key_dim;
+    const int d = 16 * tile + 4 * g;
+    if (d >= p.key_dim) continue;
     const f4 none = {0, 0, 0, 0};
-    store4(static_cast<T*>(a.dq) + row + d, live ? dq[m] : none, a.key_dim - d);
-    store4(static_cast<T*>(a.dk) + row + d, live ? dk[m] : none, a.key_dim - d);
+    store4(static_cast<T*>(p.dq) + row + d, live ? dq[m] : none, p.key_dim - d);
+    store4(static_cast<T*>(p.dk) + row + d, live ? dk[m] : none, p.key_dim - d);
   }
+}
+
+// Two tiles of columns a workgroup where one each would be more workgroups than CUs, and the registers hold them:
+// a chunk then takes 1.4 times as long, but half of the workgroups would wait for the others.
+template <typename T, int DK, int CT>
+hipError_t delta_chain(const DeltaParams& p, bool backward, hipStream_t s) {
+  const int64_t grid = delta_chains(p.a, p.tiles / CT);
+  if (backward) return start(&delta_bwd_kernel<T, DK, CT>, grid, 512, s, p);
+  return p.s0 ? start(&delta_fwd_kernel<T, DK, CT, true>, grid, 512, s, p)
+              : start(&delta_fwd_kernel<T, DK, CT, false>, grid, 512, s, p);
 }
 
 template <typename T, int DK>
 hipError_t delta_launch_dk(const DeltaParams& p, bool backward, hipStream_t s) {
   const ccv1d_delta_args& a = p.a;
-  const int64_t chunks = a.batch * a.key_heads * p.chunks, chains = delta_chains(a, p.tiles);
-  hipError_t e;
-  if (!backward) {
-    e = start(&delta_prep_kernel<T, DK, false>, chunks, 256, s, p);
-    if (e != hipSuccess) return e;
-    return p.s0 ? start(&delta_fwd_kernel<T, DK, true>, chains, kChainWaves<DK> * 64, s, p)
-                : start(&delta_fwd_kernel<T, DK, false>, chains, kChainWaves<DK> * 64, s, p);
-  }
-  e = start(&delta_prep_kernel<T, DK, true>, chunks, 256, s, p);
-  if (e == hipSuccess) e = start(&delta_bwd_kernel<T, DK>, chains, kChainWaves<DK> * 64, s, p);
-  if (e == hipSuccess) e = start(&delta_grad_kernel<T, DK>, chunks * kGradParts<T, DK>, kGradWaves<T, DK> * 64, s, p);
+  const int64_t chunks = a.batch * a.key_heads * p.chunks;
+  hipError_t e = backward ? start(&delta_prep_kernel<T, DK, true>, chunks, 256, s, p)
+                          : start(&delta_prep_kernel<T, DK, false>, chunks, 256, s, p);
+  if (e != hipSuccess) return e;
+  constexpr int CT = kPieces<T> * DK <= 128 ? 2 : 1;
+  e = CT > 1 && a.batch * a.heads * p.tiles > 256 ? delta_chain<T, DK, CT>(p, backward, s)
+                                                  : delta_chain<T, DK, 1>(p, backward, s);
+  if (e != hipSuccess || !backward) return e;
+  const GradArgs ga = {p.kf, p.qf, p.kt, p.qt, p.rows, p.s0, p.u, p.ds, p.dr, p.gates, a.v, a.dout,
+                       a.v_stride_b, a.v_stride_t, a.v_stride_h, a.dout_stride_b, a.dout_stride_t, a.dout_stride_h,
+                       a.dq, a.dk, a.dlog_decay, a.dbeta, a.scale, (int32_t)chunks, p.chunks, p.group,
+                       (int32_t)a.key_heads, (int32_t)a.heads, (int32_t)a.seqlen, (int32_t)a.key_dim,
+                       (int32_t)a.value_dim, p.dvp, a.log_decay_dtype, a.beta_dtype};
+  e = start(&delta_grad_kernel<T, DK>, (chunks + 7) / 8 * 8 * kGradParts<T, DK>, kGradWaves<T, DK> * 64, s, ga);
   if constexpr (kGradParts<T, DK> > 1)
     if (e == hipSuccess)
-      e = start(&delta_gates_kernel<(kGradParts<T, DK>)>, (a.batch * a.heads * p.chunks + 3) / 4, 256, s, p);
+      e = start(&delta_gates_kernel<(kGradParts<T, DK>)>, (a.batch * a.heads * p.chunks + 3) / 4, 256, s, ga);
   return e;
 }
 

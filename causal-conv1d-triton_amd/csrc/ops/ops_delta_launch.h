@@ -12,7 +12,7 @@ struct DeltaParams {
   ccv1d_delta_args a;
   int32_t chunks, group;  // of a sequence; heads of a key head
   int32_t dk;             // key_dim as the kernels have it: 64, 128 or 256
-  int32_t dvp, tiles;     // value_dim up to a multiple of 32; its tiles of 16
+  int32_t dvp, tiles;     // value_dim up to a multiple of 32; its groups of 64
   // Workspace, in 16-byte units a lane: fragments of k and q by rows, k and q by elements (per key head's chunk),
   // T and P (per head's chunk), the rows' factors
   u4 *kf, *qf, *kt, *qt, *tf, *pf;
