@@ -80,6 +80,8 @@ hipError_t run(const ccv1d_delta_args& a, bool backward, hipStream_t s) {
   p.a = a;
   p.chunks = (int32_t)z.chunks;
   p.group = (int32_t)(a.heads / a.key_heads);
+  // Up to 512 workgroups run at once with some room: below that a head each is quicker, though each reads q and k anew.
+  p.prep_heads = a.batch * a.key_heads * z.chunks < 512 ? 1 : p.group;
   p.dk = (int32_t)z.dk, p.dvp = (int32_t)z.dvp, p.tiles = (int32_t)z.tiles;
   char* ws = static_cast<char*>(a.workspace);
   auto unit = [&](int64_t o) { return reinterpret_cast<u4*>(ws + o); };

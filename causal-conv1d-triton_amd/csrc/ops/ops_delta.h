@@ -319,17 +319,23 @@ __device__ __forceinline__ void load_rows(T* to, const T* from, int64_t stride_t
 }
 
 // All chunks: the operands of the chains as fragments, T and P (forward) or their transposes (backward).
-// Bound by memory: reads q and k, writes them three (four) times as fragments and 30 KiB a head's chunk.
+// A workgroup has a chunk of a key head and all heads of it, or, where that is too few workgroups, one of them each
+// (p.prep_heads). Reads q and k, writes them three (four) times as fragments and 30 KiB a head's chunk; bound by
+// latency within a workgroup, so three of them a CU: at B=4 T=4096, 16 heads of 128 128 -> 106 us forward.
 template <typename T, int DK, bool BWD>
-__global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
+__global__ __launch_bounds__(256, 3) void delta_prep_kernel(DeltaParams p) {
   constexpr int NI = kPieces<T>, KS = DK / 32, LD = DK + 16 / sizeof(T), LA = 68;
   constexpr int NP = BWD ? 3 : kOutPieces<T>;
-  __shared__ T kl[kC * LD], ql[kC * LD];
-  __shared__ float al[kC * LA], td[4 * 16 * 20];
+  // q and k, and once the fragments are made, A (then T) and T's tiles on the diagonal
+  constexpr size_t kRowsBytes = 2 * kC * LD * sizeof(T), kMatrixBytes = (kC * LA + 4 * 16 * 20) * sizeof(float);
+  __shared__ __attribute__((aligned(16))) char room[kRowsBytes > kMatrixBytes ? kRowsBytes : kMatrixBytes];
   __shared__ ChunkShared sh;
+  T *kl = reinterpret_cast<T*>(room), *ql = kl + kC * LD;
+  float *al = reinterpret_cast<float*>(room), *td = al + kC * LA;
   const ccv1d_delta_args& a = p.a;
   const int lane = threadIdx.x & 63, m = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  const int64_t kc = blockIdx.x;  // (batch, key head, chunk)
+  const int shares = p.group / p.prep_heads, share = blockIdx.x % shares;
+  const int64_t kc = blockIdx.x / shares;  // (batch, key head, chunk)
   const int64_t c = kc % p.chunks, bk = kc / p.chunks, b = bk / a.key_heads, kh = bk - b * a.key_heads;
   const int64_t t0 = c * kC;
   if (m == 0) share_rows(a, b, c, kh * p.group, lane, sh, nullptr);
@@ -350,11 +356,12 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
     u4 km[NI], qm[NI];
     frag_of(kl + (16 * m + col) * LD + 32 * s + 4 * g, km);
     frag_of(ql + (16 * m + col) * LD + 32 * s + 4 * g, qm);
+    if (share == 0)
 #pragma unroll
-    for (int n = 0; n < NI; ++n) {
-      kf[((m * KS + s) * NI + n) * 64 + lane] = km[n];
-      qf[((m * KS + s) * NI + n) * 64 + lane] = qm[n];
-    }
+      for (int n = 0; n < NI; ++n) {
+        kf[((m * KS + s) * NI + n) * 64 + lane] = km[n];
+        qf[((m * KS + s) * NI + n) * 64 + lane] = qm[n];
+      }
 #pragma unroll
     for (int n = 0; n < 4; ++n)
       if (n <= m) {
@@ -365,28 +372,30 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
       }
   }
   // Transposed: a lane has one element of 8 rows.
+  if (share == 0)
 #pragma unroll
-  for (int i = 0; i < DK / 16 / 4; ++i)
+    for (int i = 0; i < DK / 16 / 4; ++i)
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int t = m + 4 * i;
-      auto column = [&](const T* from, u4* to) {
-        u4 f[NI];
-        f4 x, y;
+      for (int s = 0; s < 2; ++s) {
+        const int t = m + 4 * i;
+        auto column = [&](const T* from, u4* to) {
+          u4 f[NI];
+          f4 x, y;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[e] = to_f32(from[(32 * s + 4 * g + e) * LD + 16 * t + col]);
-          y[e] = to_f32(from[(32 * s + 16 + 4 * g + e) * LD + 16 * t + col]);
-        }
-        split8<NI>(x, y, f);
+          for (int e = 0; e < 4; ++e) {
+            x[e] = to_f32(from[(32 * s + 4 * g + e) * LD + 16 * t + col]);
+            y[e] = to_f32(from[(32 * s + 16 + 4 * g + e) * LD + 16 * t + col]);
+          }
+          split8<NI>(x, y, f);
 #pragma unroll
-        for (int n = 0; n < NI; ++n) to[((t * 2 + s) * NI + n) * 64 + lane] = f[n];
-      };
-      column(kl, p.kt + kc * (DK / 16 * 2 * NI * 64));
-      if constexpr (BWD) column(ql, p.qt + kc * (DK / 16 * 2 * NI * 64));
-    }
+          for (int n = 0; n < NI; ++n) to[((t * 2 + s) * NI + n) * 64 + lane] = f[n];
+        };
+        column(kl, p.kt + kc * (DK / 16 * 2 * NI * 64));
+        if constexpr (BWD) column(ql, p.qt + kc * (DK / 16 * 2 * NI * 64));
+      }
 
-  for (int64_t h = kh * p.group; h < (kh + 1) * p.group; ++h) {
+  const int64_t h0 = kh * p.group + share * p.prep_heads;
+  for (int64_t h = h0; h < h0 + p.prep_heads; ++h) {
     const int64_t hc = (b * a.heads + h) * p.chunks + c;
     u4* tf = p.tf + hc * (kTri * 3 * 64);
     u4* pf = p.pf + hc * (kTri * NP * 64);
@@ -427,7 +436,12 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
       for (int i = 0; i < 16; ++i) {
         float s = i == col ? 1.0f : 0.0f;
 #pragma unroll
-        for (int j = 0; j < i; ++j) s = fmaf(-al[(16 * g + i) * LA + 16 * g + j], x[j], s);
+        for (int j = 0; j < i; j += 4) {
+          const f4 av = *reinterpret_cast<const f4*>(&al[(16 * g + i) * LA + 16 * g + j]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (j + e < i) s = fmaf(-av[e], x[j + e], s);
+        }
         x[i] = s;
         td[(g * 16 + i) * 20 + col] = s;
       }
@@ -1509,8 +1523,9 @@ template <typename T, int DK>
 hipError_t delta_launch_dk(const DeltaParams& p, bool backward, hipStream_t s) {
   const ccv1d_delta_args& a = p.a;
   const int64_t chunks = a.batch * a.key_heads * p.chunks;
-  hipError_t e = backward ? start(&delta_prep_kernel<T, DK, true>, chunks, 256, s, p)
-                          : start(&delta_prep_kernel<T, DK, false>, chunks, 256, s, p);
+  const int64_t prep = chunks * (p.group / p.prep_heads);
+  hipError_t e = backward ? start(&delta_prep_kernel<T, DK, true>, prep, 256, s, p)
+                          : start(&delta_prep_kernel<T, DK, false>, prep, 256, s, p);
   if (e != hipSuccess) return e;
   constexpr int CT = kPieces<T> * DK <= 128 ? 2 : 1;
   e = CT > 1 && a.batch * a.heads * p.tiles > 256 ? delta_chain<T, DK, CT>(p, backward, s)

@@ -11,6 +11,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 struct DeltaParams {
   ccv1d_delta_args a;
   int32_t chunks, group;  // of a sequence; heads of a key head
+  int32_t prep_heads;     // of a key head in one workgroup of the first kernel
   int32_t dk;             // key_dim as the kernels have it: 64, 128 or 256
   int32_t dvp, tiles;     // value_dim up to a multiple of 32; its groups of 64
   // Workspace, in 16-byte units a lane: fragments of k and q by rows, k and q by elements (per key head's chunk),
