@@ -219,7 +219,7 @@ bool within(int64_t a, int64_t b, int64_t limit) { return a == 0 || b <= limit /
 bool delta_fits(const ccv1d_delta_args& a) {
   if (a.seqlen > kMaxGrid || a.value_dim > (1 << 20) || !within(a.batch, a.heads, kMaxGrid)) return false;
   const Sizes z = sizes_of(a);
-  if (!within(a.batch * a.heads, z.chunks, kMaxGrid / 512)) return false;
+  if (!within(a.batch * a.heads, z.chunks, kMaxGrid / 1024 - 8)) return false;
   return within((a.batch * a.heads + 7) / 8 * 8, z.tiles, kMaxThreads / 512);
 }
 

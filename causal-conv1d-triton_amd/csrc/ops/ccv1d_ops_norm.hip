@@ -18,8 +18,19 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(NormParams p, int32_t
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
   const int64_t d = (int64_t)(blockIdx.x / 3) * 32 + x;
   float s = 0.0f;
-  if (d < a.dim)
-    for (int n = y; n < lines; n += 32) s += p.lines[((int64_t)n * 3 + which) * a.dim + d];
+  if (d < a.dim) {
+    const float* at = p.lines + which * a.dim + d;
+    const int64_t line = 3 * a.dim;
+    int n = y;
+    for (; n + 7 * 32 < lines; n += 8 * 32) {  // eight requested at a time
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = at[(n + 32 * j) * line];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += v[j];
+    }
+    for (; n < lines; n += 32) s += at[n * line];
+  }
   sums[y][x] = s;
   __syncthreads();
   if (y == 0 && d < a.dim) {
