@@ -27,6 +27,11 @@
 // two pieces, 2^-15 or better. By the rates of the instructions (16x16x32 in 16 bits 16 cycles, 16x16x4 in fp32
 // 32) three pieces against a bf16 input take 3/16 of fp32's time, against three pieces 6/16.
 //
+// A row that holds an infinity or NaN spoils its sequence from there on and nothing else, though the products run over all
+// of a chunk's rows and zero times infinity is no number: keys and rates of such a row enter A as zero and its R is
+// made NaN (chunk_row), and where a product over rows comes out as no number it is made again without those rows
+// (sum_apart). A and T are numbers then, unless finite keys overflow them.
+//
 // Layout: "fragment" is the operand of one such instruction, 16 rows (A) or columns (B) by 32 of the summed index,
 // 8 elements for each of 64 lanes: lane l has row l % 16 and, of the sum, 4 (l / 16) + 0..3 and 16 + 4 (l / 16) + 0..3.
 // The order of a sum is free as long as both operands have the same, and by this one a product's result (lane l has
@@ -223,12 +228,14 @@ struct ChunkRows {
   double sum;   // G log2 e, from the row's sequence's start in the chunk
   int run;      // resets in the chunk up to the row
   bool live, reset;
+  bool spoilt;  // holds an infinity or NaN; its decay and rate are then zero here
   float beta;
 };
 
 // Row `lane` of chunk c. A row that starts a sequence, padding, and a decay that is zero in fp32 reset the state: its
 // log-decay, which multiplies nothing, counts as zero, so that no sequence's sums meet another's.
-__device__ __forceinline__ ChunkRows chunk_row(const ccv1d_delta_args& a, int64_t b, int64_t c, int64_t h, int lane) {
+__device__ __forceinline__ ChunkRows chunk_row(const ccv1d_delta_args& a, int64_t b, int64_t c, int64_t h, int lane,
+                                               bool bad_key) {
   ChunkRows r;
   const int64_t t = c * kC + lane;
   const bool in = t < a.seqlen;
@@ -253,7 +260,10 @@ __device__ __forceinline__ ChunkRows chunk_row(const ccv1d_delta_args& a, int64_
                 a.log_decay_dtype);
     r.beta = load_as(a.beta, b * a.beta_stride_b + t * a.beta_stride_t + h * a.beta_stride_h, a.beta_dtype);
   }
+  r.spoilt = r.live && (bad_key || g != g || g == INFINITY || !__builtin_isfinite(r.beta));
   if (g < -104.0f) r.reset = true;
+  if (r.spoilt) r.beta = 0.0f;
+  if (g != g || g == INFINITY) g = 0.0f;
   const uint64_t resets = __ballot(r.reset);
   r.run = __popcll(resets & (~uint64_t(0) >> (63 - lane)));
   double s = r.reset ? 0.0 : (double)g * kLog2eDouble;
@@ -274,19 +284,20 @@ struct ChunkShared {
   int run[kC];
   float beta[kC];
   int live[kC];
+  int bad_k[kC], bad_q[kC];  // whether a row's k, q hold an infinity or NaN
 };
 
 // A wave makes a chunk's rows and leaves them in LDS and, in the workspace, what the chain needs of them.
 __device__ __forceinline__ ChunkRows share_rows(const ccv1d_delta_args& a, int64_t b, int64_t c, int64_t h, int lane,
-                                                ChunkShared& sh, float* rows) {
-  const ChunkRows r = chunk_row(a, b, c, h, lane);
+                                                ChunkShared& sh, float* rows, bool bad_key) {
+  const ChunkRows r = chunk_row(a, b, c, h, lane, bad_key);
   sh.sum[lane] = r.sum, sh.run[lane] = r.run, sh.beta[lane] = r.beta, sh.live[lane] = r.live;
   if (rows) {
     const double end = __shfl(r.sum, 63);
     const int last = __shfl(r.run, 63);
     rows[lane] = r.live && r.run == 0 ? exp2_of(r.sum) : 0.0f;
     rows[kC + lane] = r.live && r.run == last ? exp2_of(end - r.sum) : 0.0f;
-    rows[2 * kC + lane] = r.beta;
+    rows[2 * kC + lane] = r.spoilt ? __builtin_nanf("") : r.beta;
     rows[3 * kC + lane] = r.live ? 1.0f : 0.0f;
     rows[4 * kC + lane] = lane == 0 && last == 0 ? exp2_of(end) : 0.0f;
     reinterpret_cast<double*>(rows + 5 * kC)[lane] = r.sum;
@@ -295,10 +306,11 @@ __device__ __forceinline__ ChunkRows share_rows(const ccv1d_delta_args& a, int64
   return r;
 }
 
-// A chunk's rows of q or k into LDS, zero where there is none, past the last element, and in padding.
+// A chunk's rows of q or k into LDS, zero where there is none, past the last element, and in padding; `bad` says
+// which rows hold an infinity or NaN.
 template <typename T, int DK, int LD, int THREADS>
 __device__ __forceinline__ void load_rows(T* to, const T* from, int64_t stride_t, int64_t dk, int64_t t0, int64_t seqlen,
-                                          const int* live) {
+                                          const int* live, int* bad) {
   typedef T v4 __attribute__((ext_vector_type(4)));
 #pragma unroll
   for (int i = 0; i < kC * DK / 4 / THREADS; ++i) {
@@ -313,6 +325,10 @@ __device__ __forceinline__ void load_rows(T* to, const T* from, int64_t stride_t
         for (int e = 0; e < 3; ++e)
           if (d + e < dk) v[e] = p[e];
       }
+      bool finite = true;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) finite &= __builtin_isfinite(to_f32(v[e]));
+      if (!finite) bad[row] = 1;
     }
     *reinterpret_cast<v4*>(to + row * LD + d) = v;
   }
@@ -338,13 +354,22 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(DeltaParams p) {
   const int64_t kc = blockIdx.x / shares;  // (batch, key head, chunk)
   const int64_t c = kc % p.chunks, bk = kc / p.chunks, b = bk / a.key_heads, kh = bk - b * a.key_heads;
   const int64_t t0 = c * kC;
-  if (m == 0) share_rows(a, b, c, kh * p.group, lane, sh, nullptr);
+  if (m == 0) {
+    share_rows(a, b, c, kh * p.group, lane, sh, nullptr, false);
+    sh.bad_k[lane] = sh.bad_q[lane] = 0;
+  }
   lds_barrier();
   load_rows<T, DK, LD, 256>(kl, static_cast<const T*>(a.k) + b * a.k_stride_b + kh * a.k_stride_h, a.k_stride_t,
-                            a.key_dim, t0, a.seqlen, sh.live);
+                            a.key_dim, t0, a.seqlen, sh.live, sh.bad_k);
   load_rows<T, DK, LD, 256>(ql, static_cast<const T*>(a.q) + b * a.q_stride_b + kh * a.q_stride_h, a.q_stride_t,
-                            a.key_dim, t0, a.seqlen, sh.live);
+                            a.key_dim, t0, a.seqlen, sh.live, sh.bad_q);
   lds_barrier();
+  const uint64_t bad_k = __ballot(sh.bad_k[lane] != 0), bad_q = __ballot(sh.bad_q[lane] != 0);
+  if (bad_k) {  // the same in all waves
+    for (int i = threadIdx.x; i < kC * DK; i += 256)
+      if (bad_k >> (i / DK) & 1) kl[i / DK * LD + i % DK] = (T)0.0f;
+    lds_barrier();
+  }
 
   // Tiles (n, m) of k.k and q.k, n <= m: keys j of tile n as rows and i of tile m as columns, backward the other
   // way round, so that a lane's results are halves of P's (P^T's) fragments.
@@ -378,7 +403,7 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(DeltaParams p) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const int t = m + 4 * i;
-        auto column = [&](const T* from, u4* to) {
+        auto column = [&](const T* from, uint64_t bad, u4* to) {
           u4 f[NI];
           f4 x, y;
 #pragma unroll
@@ -386,12 +411,18 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(DeltaParams p) {
             x[e] = to_f32(from[(32 * s + 4 * g + e) * LD + 16 * t + col]);
             y[e] = to_f32(from[(32 * s + 16 + 4 * g + e) * LD + 16 * t + col]);
           }
+          if (bad)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (bad >> (32 * s + 4 * g + e) & 1) x[e] = 0.0f;
+              if (bad >> (32 * s + 16 + 4 * g + e) & 1) y[e] = 0.0f;
+            }
           split8<NI>(x, y, f);
 #pragma unroll
           for (int n = 0; n < NI; ++n) to[((t * 2 + s) * NI + n) * 64 + lane] = f[n];
         };
-        column(kl, p.kt + kc * (DK / 16 * 2 * NI * 64));
-        if constexpr (BWD) column(ql, p.qt + kc * (DK / 16 * 2 * NI * 64));
+        column(kl, 0, p.kt + kc * (DK / 16 * 2 * NI * 64));
+        if constexpr (BWD) column(ql, bad_q, p.qt + kc * (DK / 16 * 2 * NI * 64));
       }
 
   const int64_t h0 = kh * p.group + share * p.prep_heads;
@@ -400,7 +431,7 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(DeltaParams p) {
     u4* tf = p.tf + hc * (kTri * 3 * 64);
     u4* pf = p.pf + hc * (kTri * NP * 64);
     lds_barrier();
-    if (m == 0) share_rows(a, b, c, h, lane, sh, p.rows + hc * (kRowFields * kC));
+    if (m == 0) share_rows(a, b, c, h, lane, sh, p.rows + hc * (kRowFields * kC), bad_k >> lane & 1);
     lds_barrier();
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
@@ -586,6 +617,61 @@ struct ColumnReader {
   }
 };
 
+template <int N>
+__device__ __forceinline__ bool any_not_finite(const f4 (&x)[N]) {
+  float none = 0.0f;  // stays zero beside numbers
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) none = fmaf(x[n][e], 0.0f, none);
+  return __ballot(none != 0.0f) != 0;
+}
+
+// A product over the chunk's rows, a[0] f[0] + a[1] f[1] from `base` on, where it came out as no number: rows of f that hold
+// none are left out, and the result's rows (the lane's four, from `row` on) of their sequences made NaN, those behind
+// them or, UPPER, before them. What is a number has the bits that it has beside numbers. IN_TURN: one sum
+// for both, else one each. f is [2][NB][64] units in LDS; FROM..TO of it are read.
+template <bool UPPER, bool IN_TURN, int LIM, int NA, int NB>
+__device__ __forceinline__ f4 sum_apart(const u4 (&a)[2][NA], const u4 (*f)[NB][64], uint32_t lane, int from, int to, f4 base,
+                                        const int* run, int row) {
+  asm volatile("" : "+v"(lane), "+v"(row));  // what is made of them here is made here: registers
+  const uint32_t g = lane >> 4;
+  uint32_t bad[2] = {0, 0};
+  f4 r = base, other = {0, 0, 0, 0};
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    if (s < from || s > to) continue;
+    __builtin_amdgcn_sched_barrier(0);
+    u4 x[NB];
+    load_frag(&f[s][0][0], lane, x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+        if ((x[0][i] >> (16 * half) & 0x7f80u) == 0x7f80u) {
+          bad[s] |= 1u << ((i < 2 ? 0 : 16) + 4 * g + 2 * (i & 1) + half);
+#pragma unroll
+          for (int n = 0; n < NB; ++n) x[n][i] &= half ? 0x0000ffffu : 0xffff0000u;
+        }
+    if (IN_TURN || s == from) r = mac<LIM>(a[s], x, r);
+    else other = mac<LIM>(a[s], x, other);
+    bad[s] |= __shfl_xor(bad[s], 16);
+    bad[s] |= __shfl_xor(bad[s], 32);
+  }
+  r += other;
+  const uint64_t starts = __ballot(lane && run[lane] != run[lane ? lane - 1 : 0]), rows = bad[0] | (uint64_t)bad[1] << 32;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    __builtin_amdgcn_sched_barrier(0);
+    const int i = row + e;
+    const uint64_t up_to = ~uint64_t(0) >> (63 - i), later = starts & ~up_to;
+    const uint64_t own = UPPER ? ~(up_to >> 1) & (later ? (later & -later) - 1 : ~uint64_t(0))
+                               : up_to & (~uint64_t(0) << (63 - __clzll((starts & up_to) | 1)));
+    if (rows & own) r[e] = __builtin_nanf("");
+  }
+  return r;
+}
+
 // The chain of states forward: a workgroup has CT tiles of 16 value columns of a head. Bound by latency: three
 // products after one another a chunk, each behind a barrier; the waves that make the outputs run beside them.
 template <typename T, int DK, int CT, bool SAVE>
@@ -611,6 +697,9 @@ __global__ __launch_bounds__(512) void delta_fwd_kernel(DeltaParams p) {
   const u4* tf = p.tf + at.head * N * (kTri * 3 * 64);
   const u4* pf = p.pf + at.head * N * (kTri * NO * 64);
   const float* rows = p.rows + at.head * N * (kRowFields * kC);
+  auto runs_of = [&](int64_t c) {
+    return reinterpret_cast<const int*>(rows + c * (kRowFields * kC) + 7 * kC);
+  };
 
   if (wave >= 4) {  // outputs: O = scale e^G Q S0 + P U of a tile of rows
     u4 qx[KS][NI], px[2][NO];
@@ -633,7 +722,7 @@ __global__ __launch_bounds__(512) void delta_fwd_kernel(DeltaParams p) {
     for (int64_t c = 0; c < N; ++c) {
       const int64_t next = c + 1 < N ? c + 1 : c;
       lds_barrier();
-      f4 o[CT];
+      f4 o[CT], base[CT];
 #pragma unroll
       for (int n = 0; n < CT; ++n) {
         f4 y[2] = {};
@@ -653,7 +742,8 @@ __global__ __launch_bounds__(512) void delta_fwd_kernel(DeltaParams p) {
       lds_barrier();
       lds_barrier();
 #pragma unroll
-      for (int n = 0; n < CT; ++n)
+      for (int n = 0; n < CT; ++n) {
+        base[n] = o[n];
 #pragma unroll
         for (int s = 0; s < 2; ++s)
           if (s <= w / 2) {
@@ -661,6 +751,11 @@ __global__ __launch_bounds__(512) void delta_fwd_kernel(DeltaParams p) {
             load_frag(&uo[n][s][0][0], lane, u);
             o[n] = mac<LO>(px[s], u, o[n]);
           }
+      }
+      if (any_not_finite(o))
+#pragma unroll
+        for (int n = 0; n < CT; ++n)
+          o[n] = sum_apart<false, true, LO>(px, uo[n], lane, 0, w / 2, base[n], runs_of(c), row);
       T* to = out + c * (kC * stride);
 #pragma unroll
       for (int n = 0; n < CT; ++n)
@@ -729,8 +824,11 @@ __global__ __launch_bounds__(512) void delta_fwd_kernel(DeltaParams p) {
                              ? a.initial_states[(at.head * a.key_dim + d) * a.value_dim + dv + 16 * n]
                              : 0.0f;
       }
-  float* s0 = SAVE ? p.s0 + at.head * N * (DK * (int64_t)p.dvp) + (32 * KB * part + 4 * g) * p.dvp + dv : nullptr;
-  float* us = SAVE ? p.u + at.head * N * (kC * (int64_t)p.dvp) + row * p.dvp + dv : nullptr;
+  // Addresses of what is kept: a part that is the same in all lanes, and 32 bits a lane.
+  float* s0 = SAVE ? p.s0 + at.head * N * (DK * (int64_t)p.dvp) + 32 * KB * part * (int64_t)p.dvp + at.dv0 : nullptr;
+  float* us = SAVE ? p.u + at.head * N * (kC * (int64_t)p.dvp) + 16 * w * (int64_t)p.dvp + at.dv0 : nullptr;
+  const uint32_t kept = 4 * g * p.dvp + col;
+  uint32_t ld = p.dvp;
   if constexpr (AHEAD) {
     load_k(0);
     load_kc(0);
@@ -739,6 +837,7 @@ __global__ __launch_bounds__(512) void delta_fwd_kernel(DeltaParams p) {
   load_t(0);
   for (int64_t c = 0; c < N; ++c) {
     const int64_t next = c + 1 < N ? c + 1 : c;
+    asm volatile("" : "+s"(ld));  // offsets are made anew for each chunk: registers
     {
       f4 x[CT][L::kRows] = {};
 #pragma unroll
@@ -766,9 +865,11 @@ __global__ __launch_bounds__(512) void delta_fwd_kernel(DeltaParams p) {
 #pragma unroll
         for (int t = 0; t < 2 * KB; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int e = 0; e < 4; ++e) {
+            float* line = to + (16 * t + e) * ld;
 #pragma unroll
-            for (int n = 0; n < CT; ++n) to[(16 * t + e) * p.dvp + 16 * n] = state[n][t][e];
+            for (int n = 0; n < CT; ++n) (line + 16 * n)[kept] = state[n][t][e];
+          }
       }
     if constexpr (AHEAD) load_k(next);
     // A chunk that the carried state goes through has no reset and no padding but past the last row, where beta and
@@ -809,6 +910,10 @@ __global__ __launch_bounds__(512) void delta_fwd_kernel(DeltaParams p) {
       }
       u[n] += u1;
     }
+    if (any_not_finite(u))
+#pragma unroll
+      for (int n = 0; n < CT; ++n)
+        u[n] = sum_apart<false, false, 2>(tx, rb[n], lane, 0, w / 2, f4{0, 0, 0, 0}, runs_of(c), row);
 #pragma unroll
     for (int n = 0; n < CT; ++n) {
       f4 y;
@@ -826,9 +931,11 @@ __global__ __launch_bounds__(512) void delta_fwd_kernel(DeltaParams p) {
     if constexpr (SAVE) {
       float* to = us + c * (kC * (int64_t)p.dvp);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 4; ++e) {
+        float* line = to + e * ld;
 #pragma unroll
-        for (int n = 0; n < CT; ++n) to[e * p.dvp + 16 * n] = u[n][e];
+        for (int n = 0; n < CT; ++n) (line + 16 * n)[kept] = u[n][e];
+      }
     }
     load_t(next);
 #pragma unroll
@@ -880,49 +987,52 @@ __global__ __launch_bounds__(512) void delta_bwd_kernel(DeltaParams p) {
   const uint32_t lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int wave = wave_index(), w = wave & 3;
   const int64_t b = at.head / a.heads, h = at.head - b * a.heads, kh = h / p.group;
-  const int64_t dv = at.dv0 + col;
-  const int64_t N = p.chunks;
+  const int32_t dv = (int32_t)at.dv0 + col, dim = (int32_t)a.value_dim, seqlen = (int32_t)a.seqlen;
+  const int32_t N = p.chunks;
   const int row = 16 * w + 4 * g;
-  const u4* kf = p.kf + (b * a.key_heads + kh) * N * (4 * KS * NI * 64);
-  const u4* kt = p.kt + (b * a.key_heads + kh) * N * (DK / 16 * 2 * NI * 64);
-  const u4* qt = p.qt + (b * a.key_heads + kh) * N * (DK / 16 * 2 * NI * 64);
-  const u4* tf = p.tf + at.head * N * (kTri * 3 * 64);
-  const u4* pf = p.pf + at.head * N * (kTri * 3 * 64);
-  const float* rows = p.rows + at.head * N * (kRowFields * kC);
+  const u4* kf = p.kf + (b * a.key_heads + kh) * (int64_t)N * (4 * KS * NI * 64);
+  const u4* kt = p.kt + (b * a.key_heads + kh) * (int64_t)N * (DK / 16 * 2 * NI * 64);
+  const u4* qt = p.qt + (b * a.key_heads + kh) * (int64_t)N * (DK / 16 * 2 * NI * 64);
+  const u4* tf = p.tf + at.head * (int64_t)N * (kTri * 3 * 64);
+  const u4* pf = p.pf + at.head * (int64_t)N * (kTri * 3 * 64);
+  const float* rows = p.rows + at.head * (int64_t)N * (kRowFields * kC);
+  auto runs_of = [&](int32_t c) {
+    return reinterpret_cast<const int*>(rows + c * (int64_t)(kRowFields * kC) + 7 * kC);
+  };
 
   if (wave >= 4) {
     u4 px[2][3], qx[TQ][2][NI];
-    f4 into, live, sum[CT][TQ];
+    f4 into, live, sum[CT][TQ], z[CT];
     uint32_t dy[CT][4];
     ColumnReader<T> yr[CT];
 #pragma unroll
     for (int n = 0; n < CT; ++n)
-      yr[n].at(a.dout, b * a.dout_stride_b + h * a.dout_stride_h, a.dout_stride_t, dv + 16 * n, a.value_dim, row);
-    auto load_dy = [&](int64_t c) {
-      into = *reinterpret_cast<const f4*>(rows + c * (kRowFields * kC) + row);
-      live = *reinterpret_cast<const f4*>(rows + c * (kRowFields * kC) + 3 * kC + row);
+      yr[n].at(a.dout, b * a.dout_stride_b + h * a.dout_stride_h, a.dout_stride_t, dv + 16 * n, dim, row);
+    auto load_dy = [&](int32_t c) {
+      into = *reinterpret_cast<const f4*>(rows + c * (int64_t)(kRowFields * kC) + row);
+      live = *reinterpret_cast<const f4*>(rows + c * (int64_t)(kRowFields * kC) + 3 * kC + row);
 #pragma unroll
-      for (int n = 0; n < CT; ++n) yr[n].load(c, a.seqlen, row, dy[n]);
+      for (int n = 0; n < CT; ++n) yr[n].load(c, seqlen, row, dy[n]);
     };
-    auto load_pq = [&](int64_t c) {
+    auto load_pq = [&](int32_t c) {
 #pragma unroll
       for (int s = 0; s < 2; ++s)
-        if (s >= w / 2) load_frag(pf + c * (kTri * 3 * 64) + upper_frag(w, s) * (3 * 64), lane, px[s]);
+        if (s >= w / 2) load_frag(pf + c * (int64_t)(kTri * 3 * 64) + upper_frag(w, s) * (3 * 64), lane, px[s]);
       if constexpr (AHEAD)
 #pragma unroll
         for (int t = 0; t < TQ; ++t)
 #pragma unroll
           for (int s = 0; s < 2; ++s)
-            load_frag(qt + c * (DK / 16 * 2 * NI * 64) + ((TQ * w + t) * 2 + s) * (NI * 64), lane, qx[t][s]);
+            load_frag(qt + c * (int64_t)(DK / 16 * 2 * NI * 64) + ((TQ * w + t) * 2 + s) * (NI * 64), lane, qx[t][s]);
     };
-    auto share = [&](int64_t c) {  // dO of the wave's rows, and scale e^G dO
+    auto share = [&](int32_t c) {  // dO of the wave's rows, and scale e^G dO
 #pragma unroll
       for (int n = 0; n < CT; ++n) {
         f4 d, s;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          d[e] = live[e] != 0.0f && dv + 16 * n < a.value_dim ? raw_to_f32<T>(dy[n][e]) : 0.0f;
-          s[e] = a.scale * into[e] * d[e];
+          d[e] = live[e] != 0.0f && dv + 16 * n < dim ? raw_to_f32<T>(dy[n][e]) : 0.0f;
+          s[e] = into[e] != 0.0f ? a.scale * into[e] * d[e] : 0.0f;
         }
         u2 half[NI], third[3];
         split4<NI>(d, half);
@@ -932,7 +1042,7 @@ __global__ __launch_bounds__(512) void delta_bwd_kernel(DeltaParams p) {
       }
       load_dy(c ? c - 1 : 0);
     };
-    auto products = [&](int64_t c) {
+    auto products = [&](int32_t c) {
 #pragma unroll
       for (int n = 0; n < CT; ++n) {
         f4 y[2] = {};
@@ -949,12 +1059,20 @@ __global__ __launch_bounds__(512) void delta_bwd_kernel(DeltaParams p) {
 #pragma unroll
           for (int t = 0; t < TQ; ++t) {
             if constexpr (!AHEAD)
-              load_frag(qt + c * (DK / 16 * 2 * NI * 64) + ((TQ * w + t) * 2 + s) * (NI * 64), lane, qx[t][s]);
+              load_frag(qt + c * (int64_t)(DK / 16 * 2 * NI * 64) + ((TQ * w + t) * 2 + s) * (NI * 64), lane, qx[t][s]);
             sum[n][t] = mac<2>(qx[t][s], x, sum[n][t]);
           }
         }
-        pd[n][w][lane] = y[0] + y[1];
+        z[n] = y[0] + y[1];
       }
+    };
+    auto leave = [&](int32_t c) {
+      if (any_not_finite(z))
+#pragma unroll
+        for (int n = 0; n < CT; ++n)
+          z[n] = sum_apart<true, false, 2>(px, ob[n], lane, w / 2, 1, f4{0, 0, 0, 0}, runs_of(c), row);
+#pragma unroll
+      for (int n = 0; n < CT; ++n) pd[n][w][lane] = z[n];
       load_pq(c ? c - 1 : 0);
     };
     load_dy(N - 1);
@@ -962,7 +1080,8 @@ __global__ __launch_bounds__(512) void delta_bwd_kernel(DeltaParams p) {
     share(N - 1);
     lds_barrier();
     products(N - 1);
-    for (int64_t c = N - 1; c >= 0; --c) {
+    leave(N - 1);
+    for (int32_t c = N - 1; c >= 0; --c) {
       lds_barrier();
 #pragma unroll
       for (int n = 0; n < CT; ++n)
@@ -972,45 +1091,50 @@ __global__ __launch_bounds__(512) void delta_bwd_kernel(DeltaParams p) {
       lds_barrier();
       products(c ? c - 1 : 0);
       lds_barrier();
+      leave(c ? c - 1 : 0);
     }
     return;
   }
 
+  // A zero that the compiler does not know: these addresses are not kept for both kinds of waves (scalar registers).
+  int32_t zero = 0;
+  asm volatile("" : "+s"(zero));
+  rows += zero, tf += zero;
   const int part = L::part(w), rows0 = L::rows0(w);
   const bool keeper = L::kParts == 4 || w < L::kParts;
   u4 kx[KB][L::kRows][NI], kc[2 * KB][2][NI], tx[2][3];
   f4 into, rest, beta;
   float whole = 0.0f, whole_now;
-  auto load_k_of = [&](int64_t c, int i) {
+  auto load_k_of = [&](int32_t c, int i) {
 #pragma unroll
     for (int m = 0; m < L::kRows; ++m)
-      load_frag(kf + c * (4 * KS * NI * 64) + ((rows0 + m) * KS + part * KB + i) * (NI * 64), lane, kx[i][m]);
+      load_frag(kf + c * (int64_t)(4 * KS * NI * 64) + ((rows0 + m) * KS + part * KB + i) * (NI * 64), lane, kx[i][m]);
   };
-  auto load_kc_of = [&](int64_t c, int s) {
+  auto load_kc_of = [&](int32_t c, int s) {
 #pragma unroll
     for (int t = 0; t < 2 * KB; ++t)
-      load_frag(kt + c * (DK / 16 * 2 * NI * 64) + ((2 * KB * part + t) * 2 + s) * (NI * 64), lane, kc[t][s]);
+      load_frag(kt + c * (int64_t)(DK / 16 * 2 * NI * 64) + ((2 * KB * part + t) * 2 + s) * (NI * 64), lane, kc[t][s]);
   };
-  auto load_k = [&](int64_t c) {
+  auto load_k = [&](int32_t c) {
 #pragma unroll
     for (int i = 0; i < KB; ++i) load_k_of(c, i);
   };
-  auto load_kc = [&](int64_t c) {
+  auto load_kc = [&](int32_t c) {
     load_kc_of(c, 0);
     load_kc_of(c, 1);
   };
-  auto load_rest = [&](int64_t c) {
-    const float* r = rows + c * (kRowFields * kC);
+  auto load_rest = [&](int32_t c) {
+    const float* r = rows + c * (int64_t)(kRowFields * kC);
     whole = r[4 * kC];
     rest = *reinterpret_cast<const f4*>(r + kC + row);
   };
-  auto load_t = [&](int64_t c) {
-    const float* r = rows + c * (kRowFields * kC);
+  auto load_t = [&](int32_t c) {
+    const float* r = rows + c * (int64_t)(kRowFields * kC);
     into = *reinterpret_cast<const f4*>(r + row);
     beta = *reinterpret_cast<const f4*>(r + 2 * kC + row);
 #pragma unroll
     for (int s = 0; s < 2; ++s)
-      if (s >= w / 2) load_frag(tf + c * (kTri * 3 * 64) + upper_frag(w, s) * (3 * 64), lane, tx[s]);
+      if (s >= w / 2) load_frag(tf + c * (int64_t)(kTri * 3 * 64) + upper_frag(w, s) * (3 * 64), lane, tx[s]);
   };
 
   f4 ds[CT][2 * KB];
@@ -1021,12 +1145,14 @@ __global__ __launch_bounds__(512) void delta_bwd_kernel(DeltaParams p) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int64_t d = 32 * KB * part + 16 * t + 4 * g + e;
-        ds[n][t][e] = a.dfinal_states && dv + 16 * n < a.value_dim && d < a.key_dim
+        ds[n][t][e] = a.dfinal_states && dv + 16 * n < dim && d < a.key_dim
                           ? a.dfinal_states[(at.head * a.key_dim + d) * a.value_dim + dv + 16 * n]
                           : 0.0f;
       }
-  float* dsp = p.ds + at.head * N * (DK * (int64_t)p.dvp) + (32 * KB * part + 4 * g) * p.dvp + dv;
-  float* drp = p.dr + at.head * N * (kC * (int64_t)p.dvp) + row * p.dvp + dv;
+  float* dsp = p.ds + at.head * (int64_t)N * (DK * (int64_t)p.dvp) + 32 * KB * part * (int64_t)p.dvp + at.dv0;
+  float* drp = p.dr + at.head * (int64_t)N * (kC * (int64_t)p.dvp) + 16 * w * (int64_t)p.dvp + at.dv0;
+  const uint32_t kept = 4 * g * p.dvp + col;
+  uint32_t ld = p.dvp;
   const int64_t stride = a.heads * a.value_dim;
   T* dvo = static_cast<T*>(a.dv) + (b * a.seqlen + row) * stride + h * a.value_dim + dv;
   if constexpr (AHEAD) {
@@ -1036,8 +1162,9 @@ __global__ __launch_bounds__(512) void delta_bwd_kernel(DeltaParams p) {
   load_rest(N - 1);
   load_t(N - 1);
   lds_barrier();  // the waves beside the chain begin with the last chunk's dO
-  for (int64_t c = N - 1; c >= 0; --c) {
-    const int64_t next = c ? c - 1 : 0;
+  for (int32_t c = N - 1; c >= 0; --c) {
+    const int32_t next = c ? c - 1 : 0;
+    asm volatile("" : "+s"(ld));
     {
       f4 x[CT][L::kRows] = {};
 #pragma unroll
@@ -1061,9 +1188,11 @@ __global__ __launch_bounds__(512) void delta_bwd_kernel(DeltaParams p) {
 #pragma unroll
       for (int t = 0; t < 2 * KB; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < 4; ++e) {
+          float* line = to + (16 * t + e) * ld;
 #pragma unroll
-          for (int n = 0; n < CT; ++n) to[(16 * t + e) * p.dvp + 16 * n] = ds[n][t][e];
+          for (int n = 0; n < CT; ++n) (line + 16 * n)[kept] = ds[n][t][e];
+        }
     }
     if constexpr (AHEAD) load_k(next);
     whole_now = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(whole)));
@@ -1086,20 +1215,29 @@ __global__ __launch_bounds__(512) void delta_bwd_kernel(DeltaParams p) {
     }
     load_rest(next);
     lds_barrier();
+    f4 r[CT];
 #pragma unroll
     for (int n = 0; n < CT; ++n) {
-      f4 r = {0, 0, 0, 0}, r1 = {0, 0, 0, 0};
+      f4 r1 = {0, 0, 0, 0};
       u4 u[3];
+      r[n] = f4{0, 0, 0, 0};
       load_frag(&ub[n][1][0][0], lane, u);
-      r = mac<2>(tx[1], u, r);
+      r[n] = mac<2>(tx[1], u, r[n]);
       if (w < 2) {
         load_frag(&ub[n][0][0][0], lane, u);
         r1 = mac<2>(tx[0], u, r1);
       }
-      r += r1;
+      r[n] += r1;
+    }
+    if (any_not_finite(r))
+#pragma unroll
+      for (int n = 0; n < CT; ++n)
+        r[n] = sum_apart<true, false, 2>(tx, ub[n], lane, w / 2, 1, f4{0, 0, 0, 0}, runs_of(c), row);
+#pragma unroll
+    for (int n = 0; n < CT; ++n) {
       f4 x;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = -beta[e] * into[e] * r[e];
+      for (int e = 0; e < 4; ++e) x[e] = -beta[e] * into[e] * r[n][e];
       if (whole_now == 0.0f)
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = into[e] != 0.0f ? x[e] : 0.0f;
@@ -1108,12 +1246,12 @@ __global__ __launch_bounds__(512) void delta_bwd_kernel(DeltaParams p) {
       store_half<3>(&rb[n][w / 2][0][lane], w & 1, half);
       float* to = drp + c * (kC * (int64_t)p.dvp) + 16 * n;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) to[e * p.dvp] = r[e];
-      if (dv + 16 * n < a.value_dim) {
+      for (int e = 0; e < 4; ++e) (to + e * ld)[kept] = r[n][e];
+      if (dv + 16 * n < dim) {
         T* out = dvo + c * (kC * stride) + 16 * n;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (c * kC + row + e < a.seqlen) out[e * stride] = (T)(beta[e] != 0.0f ? beta[e] * r[e] : 0.0f);
+          if (c * kC + row + e < seqlen) out[e * stride] = (T)(beta[e] != 0.0f ? beta[e] * r[n][e] : 0.0f);
       }
     }
     load_t(next);
@@ -1145,7 +1283,7 @@ __global__ __launch_bounds__(512) void delta_bwd_kernel(DeltaParams p) {
   if (a.dinitial_states && keeper)
 #pragma unroll
     for (int n = 0; n < CT; ++n)
-      if (dv + 16 * n < a.value_dim)
+      if (dv + 16 * n < dim)
 #pragma unroll
         for (int t = 0; t < 2 * KB; ++t)
 #pragma unroll
@@ -1260,10 +1398,10 @@ __global__ __launch_bounds__((kGradWaves<T, DK>) * 64, kPieces<T> > 1 ? 1 : 2) v
   const int part = slot % kGradParts<T, DK>, tile = part * NW + w;  // the wave's elements: 16 tile ...
   const int bk = kc / p.chunks, c = kc - bk * p.chunks, b = bk / p.key_heads, kh = bk - b * p.key_heads;
   const int t0 = c * kC;
-  const u4* kf = p.kf + (int64_t)kc * (4 * KS * NI * 64);
-  const u4* qf = p.qf + (int64_t)kc * (4 * KS * NI * 64);
-  const u4* kt = p.kt + (int64_t)kc * (DK / 16 * 2 * NI * 64);
-  const u4* qt = p.qt + (int64_t)kc * (DK / 16 * 2 * NI * 64);
+  const u4* kf0 = p.kf + (int64_t)kc * (4 * KS * NI * 64);
+  const u4* qf0 = p.qf + (int64_t)kc * (4 * KS * NI * 64);
+  const u4* kt0 = p.kt + (int64_t)kc * (DK / 16 * 2 * NI * 64);
+  const u4* qt0 = p.qt + (int64_t)kc * (DK / 16 * 2 * NI * 64);
   const double* sum = reinterpret_cast<const double*>(rows + 5 * kC);
   const int* run = reinterpret_cast<const int*>(rows + 7 * kC);
   f4 dq[4] = {}, dk[4] = {};
@@ -1282,7 +1420,10 @@ __global__ __launch_bounds__((kGradWaves<T, DK>) * 64, kPieces<T> > 1 ? 1 : 2) v
     const int64_t hc = (int64_t)(b * p.heads + h) * p.chunks + c;
     // Addresses are made and k's and q's fragments read anew for every head: kept, they would spill.
     uint32_t lane = threadIdx.x & 63;
-    asm volatile("" : "+s"(kf), "+s"(qf), "+s"(kt), "+s"(qt), "+v"(lane));
+    // (Not the pointers themselves, of which it would not know then that they are no LDS: flat loads.)
+    int32_t zero = 0;
+    asm volatile("" : "+s"(zero), "+v"(lane));
+    const u4 *kf = kf0 + zero, *qf = qf0 + zero, *kt = kt0 + zero, *qt = qt0 + zero;
     const uint32_t col = lane & 15, g = lane >> 4;
     const int mine = 16 * wr + col;  // the row whose dR and V, or U and dO, the lane reads (four waves: all)
     const int64_t mine_t = min(t0 + mine, p.seqlen - 1);
@@ -1420,7 +1561,10 @@ __global__ __launch_bounds__((kGradWaves<T, DK>) * 64, kPieces<T> > 1 ? 1 : 2) v
             const int i = 32 * s + 4 * g + e;
             if (2 * s >= m) lo[e] = gl[i * LG + 16 * m + col];
             hi[e] = gl[(i + 16) * LG + 16 * m + col];
-            if (round) lo[e] *= -rows[2 * kC + i], hi[e] *= -rows[2 * kC + i + 16];
+            if (round) {  // not zero times the rate of a spoilt row, which is NaN
+              lo[e] = lo[e] != 0.0f ? lo[e] * -rows[2 * kC + i] : 0.0f;
+              hi[e] = hi[e] != 0.0f ? hi[e] * -rows[2 * kC + i + 16] : 0.0f;
+            }
           }
         }
         u4 y[3];

@@ -13,7 +13,7 @@ struct DeltaParams {
   int32_t chunks, group;  // of a sequence; heads of a key head
   int32_t prep_heads;     // of a key head in one workgroup of the first kernel
   int32_t dk;             // key_dim as the kernels have it: 64, 128 or 256
-  int32_t dvp, tiles;     // value_dim up to a multiple of 32; its groups of 64
+  int32_t dvp, tiles;     // value_dim up to a multiple of 32; its groups of 16
   // Workspace, in 16-byte units a lane: fragments of k and q by rows, k and q by elements (per key head's chunk),
   // T and P (per head's chunk), the rows' factors
   u4 *kf, *qf, *kt, *qt, *tf, *pf;

@@ -32,7 +32,9 @@ extern "C" {
  * Sums and states are fp32 whatever the element type. A log-decay below -104 (whose exponential is zero in
  * fp32) empties the state. With seq_idx the state starts at zero in each row whose id differs from the row
  * before it; initial_states belong to the sequence of seq_idx[:, 0]; rows of a negative id are padding:
- * their output is zero, the state behind them zero, whatever they hold, and no gradient leaves them.
+ * their output is zero, the state behind them zero, whatever they hold, and no gradient leaves them. An
+ * infinity or NaN in another row spoils its own sequence alone: outputs from that row on (in q: that row's; in v:
+ * its column's), gradients. Only finite keys so long that 64 rows' products overflow fp32 can spoil more.
  * ------------------------------------------------------------------------------------------- */
 
 /* Rows of a chunk: the forward hands the backward the state in front of every chunk, and the corrections u

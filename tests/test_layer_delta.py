@@ -227,6 +227,54 @@ def test_other_sequences_in_other_chunks(dtype):
     assert torch.equal(got["final"], clean["final"])
 
 
+SPOILT = [("q", math.nan), ("k", math.inf), ("v", -math.inf), ("v", math.nan), ("g", math.inf), ("g", math.nan),
+          ("beta", math.inf), ("beta", math.nan), ("do", math.inf)]
+
+
+@pytest.mark.parametrize("row", [50, 70])
+@pytest.mark.parametrize("name,bad", SPOILT)
+@pytest.mark.parametrize("dtype,Dk", [(BF, 64), (BF, 130), (HF, 40), (F, 100)])
+def test_other_sequences_in_the_same_chunk(dtype, Dk, name, bad, row):
+    """A row that holds an infinity or NaN spoils its sequence from there on (gradients: up to there, too), and
+    no bit of any other, wherever in the 64 rows these begin and end."""
+    t = make(16, B=1, T=270, Hk=1, H=2, Dk=Dk, Dv=40, dtype=dtype, init=True)
+    starts = torch.tensor([0, 17, 40, 75, 90, 150, 192, 263])
+    t["seq"] = (torch.arange(270)[:, None] >= starts).sum(1).int()[None]
+    clean = run(t)
+    t[name] = t[name].clone()
+    t[name][:, row] = bad
+    got = run(t)
+    own = (torch.arange(270) >= 40) & (torch.arange(270) < 75)
+    for n in ("out", "q", "k", "v", "g", "beta"):
+        assert torch.equal(got[n][:, ~own], clean[n][:, ~own]), n
+    for n in ("final", "init"):
+        assert torch.equal(got[n], clean[n]), n
+    assert torch.equal(got["out"][:, 40:row], clean["out"][:, 40:row])
+    if name == "do":
+        assert torch.equal(got["out"], clean["out"])
+        for n in ("q", "k", "v", "g", "beta"):
+            assert torch.equal(got[n][:, row + 1:75], clean[n][:, row + 1:75]), n
+            if n != "q":
+                assert not torch.isfinite(got[n][:, 40:row]).all(), n
+    else:
+        assert not torch.isfinite(got["out"][:, row]).any()
+        if name == "q":
+            assert torch.equal(got["out"][:, row + 1:], clean["out"][:, row + 1:])
+        else:
+            assert not torch.isfinite(got["out"][:, row:75]).any()
+
+
+def test_a_spoilt_initial_state_and_a_start_within_the_chunk():
+    t = make(17, B=1, T=130, Hk=1, H=1, init=True, grad=False)
+    t["seq"] = (torch.arange(130) >= 21).int()[None]
+    t["init"] = t["init"] * math.inf
+    got = run(t)
+    t["init"] = None
+    want = run(t)
+    assert torch.equal(got["out"][:, 21:], want["out"][:, 21:]) and torch.equal(got["final"], want["final"])
+    assert not torch.isfinite(got["out"][:, :21]).any()
+
+
 def test_a_spoiled_initial_state_ends_with_its_sequence():
     t = make(15, B=1, T=130, Hk=1, H=1, init=True, grad=False)
     t["seq"] = (torch.arange(130) >= 64).int()[None]
