@@ -255,7 +255,7 @@ __global__ __launch_bounds__(kThreads<LANES>) void norm_bwd_kernel(NormParams p)
 #pragma unroll
         for (int e = 0; e < kVec; ++e) s[0] = fmaf(x[i][e], x[i][e], s[0]);
       row_sums<LANES, 1>(s, lds1, 2 * turn);
-      inv1 = inverse(s[0], p.by_dim, a.eps);
+      inv1 = in ? inverse(s[0], p.by_dim, a.eps) : 0.0f;  // of no row, with eps 0, it would be infinite
     }
     // dr of all, in fp32, and m where a gradient needs it again
     float g[STEPS][kVec];
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(kThreads<LANES>) void norm_bwd_kernel(NormParams p)
         }
       }
       row_sums<LANES, 2>(s, lds2, turn);
-      const float inv2 = inverse(s[0], p.by_dim, a.eps), mean = s[1] * p.by_dim * inv2;  // of h2 t2
+      const float inv2 = in ? inverse(s[0], p.by_dim, a.eps) : 0.0f, mean = s[1] * p.by_dim * inv2;  // of h2 t2
 #pragma unroll
       for (int i = 0; i < STEPS; ++i) {
         const int d = column<LANES>(i) + shift, n = dim - d;

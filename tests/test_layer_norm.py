@@ -169,6 +169,12 @@ def test_rows_do_not_meet(bad):
         assert torch.equal(got[n][rest], clean[n][rest]), n
 
 
+@pytest.mark.parametrize("shape", [(1, 8), (5, 64), (17, 128), (3, 512), (3, 1024)])
+def test_no_eps_and_rows_that_fill_no_workgroup(shape):
+    """Weights' sums take nothing of the rows behind the last, whose inverse norm would be infinite."""
+    check(make(12, shape, F, F, True, True, "tensor", True), eps=0.0)
+
+
 def test_eps():
     for eps in (0.0, 1e-3, 1.0):
         check(make(11, (5, 77), F, F, True, True, None, True), eps=eps)
