@@ -58,6 +58,9 @@ constexpr int kPieces = std::is_same_v<T, __bf16> ? 1 : std::is_same_v<T, _Float
 template <typename T>
 constexpr int kOutPieces = sizeof(T) == 4 ? 3 : 2;
 
+// A wave's number, known to be the same in all lanes.
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 // A barrier for LDS alone: loads from memory that are on their way stay on it.
 __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -232,34 +235,49 @@ struct ChunkRows {
   float beta;
 };
 
+// What a row's factors are made of, as it lies in memory: requested together, before anything is looked at. Past the last
+// row another is read, and not used.
+struct RawGates {
+  uint32_t g, beta;
+  int64_t id, before;
+  __device__ __forceinline__ void load(const ccv1d_delta_args& a, int64_t b, int64_t c, int64_t h, int lane) {
+    const int64_t t = min(c * kC + lane, a.seqlen - 1);
+    auto raw = [](const void* p, int64_t at, int dtype) -> uint32_t {
+      if (dtype == CCV1D_F32) return static_cast<const uint32_t*>(p)[at];
+      return static_cast<const uint16_t*>(p)[at];
+    };
+    g = raw(a.log_decay, b * a.log_decay_stride_b + t * a.log_decay_stride_t + h * a.log_decay_stride_h,
+            a.log_decay_dtype);
+    beta = raw(a.beta, b * a.beta_stride_b + t * a.beta_stride_t + h * a.beta_stride_h, a.beta_dtype);
+    id = before = 0;
+    if (a.seq_idx) {
+      const int64_t at = b * a.seqlen + t, ahead = at - (t > 0);
+      if (a.seq_idx_64) {
+        const int64_t* s = static_cast<const int64_t*>(a.seq_idx);
+        id = s[at], before = s[ahead];
+      } else {
+        const int32_t* s = static_cast<const int32_t*>(a.seq_idx);
+        id = s[at], before = s[ahead];
+      }
+    }
+  }
+  static __device__ __forceinline__ float number(uint32_t x, int dtype) {
+    return dtype == CCV1D_F32   ? __uint_as_float(x)
+           : dtype == CCV1D_F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)x)
+                                : __uint_as_float(x << 16);
+  }
+};
+
 // Row `lane` of chunk c. A row that starts a sequence, padding, and a decay that is zero in fp32 reset the state: its
 // log-decay, which multiplies nothing, counts as zero, so that no sequence's sums meet another's.
-__device__ __forceinline__ ChunkRows chunk_row(const ccv1d_delta_args& a, int64_t b, int64_t c, int64_t h, int lane,
+__device__ __forceinline__ ChunkRows chunk_row(const ccv1d_delta_args& a, const RawGates& raw, int64_t c, int lane,
                                                bool bad_key) {
   ChunkRows r;
-  const int64_t t = c * kC + lane;
-  const bool in = t < a.seqlen;
-  r.live = in, r.reset = false;
-  if (a.seq_idx && in) {
-    const int64_t at = b * a.seqlen + t;
-    int64_t id, before;
-    if (a.seq_idx_64) {
-      const int64_t* s = static_cast<const int64_t*>(a.seq_idx);
-      id = s[at], before = t ? s[at - 1] : id;
-    } else {
-      const int32_t* s = static_cast<const int32_t*>(a.seq_idx);
-      id = s[at], before = t ? s[at - 1] : id;
-    }
-    r.live = id >= 0;
-    r.reset = id < 0 || id != before;
-  }
-  float g = 0.0f;
-  r.beta = 0.0f;
-  if (r.live) {
-    g = load_as(a.log_decay, b * a.log_decay_stride_b + t * a.log_decay_stride_t + h * a.log_decay_stride_h,
-                a.log_decay_dtype);
-    r.beta = load_as(a.beta, b * a.beta_stride_b + t * a.beta_stride_t + h * a.beta_stride_h, a.beta_dtype);
-  }
+  const bool in = c * kC + lane < a.seqlen;
+  r.live = in && raw.id >= 0;
+  r.reset = in && (raw.id < 0 || raw.id != raw.before);
+  float g = r.live ? RawGates::number(raw.g, a.log_decay_dtype) : 0.0f;
+  r.beta = r.live ? RawGates::number(raw.beta, a.beta_dtype) : 0.0f;
   r.spoilt = r.live && (bad_key || g != g || g == INFINITY || !__builtin_isfinite(r.beta));
   if (g < -104.0f) r.reset = true;
   if (r.spoilt) r.beta = 0.0f;
@@ -283,61 +301,71 @@ struct ChunkShared {
   double sum[kC];
   int run[kC];
   float beta[kC];
-  int live[kC];
-  int bad_k[kC], bad_q[kC];  // whether a row's k, q hold an infinity or NaN
 };
 
-// A wave makes a chunk's rows and leaves them in LDS and, in the workspace, what the chain needs of them.
-__device__ __forceinline__ ChunkRows share_rows(const ccv1d_delta_args& a, int64_t b, int64_t c, int64_t h, int lane,
-                                                ChunkShared& sh, float* rows, bool bad_key) {
-  const ChunkRows r = chunk_row(a, b, c, h, lane, bad_key);
-  sh.sum[lane] = r.sum, sh.run[lane] = r.run, sh.beta[lane] = r.beta, sh.live[lane] = r.live;
-  if (rows) {
-    const double end = __shfl(r.sum, 63);
-    const int last = __shfl(r.run, 63);
-    rows[lane] = r.live && r.run == 0 ? exp2_of(r.sum) : 0.0f;
-    rows[kC + lane] = r.live && r.run == last ? exp2_of(end - r.sum) : 0.0f;
-    rows[2 * kC + lane] = r.spoilt ? __builtin_nanf("") : r.beta;
-    rows[3 * kC + lane] = r.live ? 1.0f : 0.0f;
-    rows[4 * kC + lane] = lane == 0 && last == 0 ? exp2_of(end) : 0.0f;
-    reinterpret_cast<double*>(rows + 5 * kC)[lane] = r.sum;
-    reinterpret_cast<int*>(rows + 7 * kC)[lane] = r.run;
-  }
-  return r;
+// A wave makes a chunk's rows of a head and leaves them in LDS and, in the workspace, what the chain needs of them.
+__device__ __forceinline__ bool share_rows(const ccv1d_delta_args& a, const RawGates& raw, int64_t c, int lane,
+                                           ChunkShared& sh, float* rows, bool bad_key) {
+  const ChunkRows r = chunk_row(a, raw, c, lane, bad_key);
+  sh.sum[lane] = r.sum, sh.run[lane] = r.run, sh.beta[lane] = r.beta;
+  const double end = __shfl(r.sum, 63);
+  const int last = __shfl(r.run, 63);
+  rows[lane] = r.live && r.run == 0 ? exp2_of(r.sum) : 0.0f;
+  rows[kC + lane] = r.live && r.run == last ? exp2_of(end - r.sum) : 0.0f;
+  rows[2 * kC + lane] = r.spoilt ? __builtin_nanf("") : r.beta;
+  rows[3 * kC + lane] = r.live ? 1.0f : 0.0f;
+  rows[4 * kC + lane] = lane == 0 && last == 0 ? exp2_of(end) : 0.0f;
+  reinterpret_cast<double*>(rows + 5 * kC)[lane] = r.sum;
+  reinterpret_cast<int*>(rows + 7 * kC)[lane] = r.run;
+  return r.live;
 }
 
-// A chunk's rows of q or k into LDS, zero where there is none, past the last element, and in padding; `bad` says
-// which rows hold an infinity or NaN.
+// A chunk's rows of q or k on their way to LDS: requested all at once, past the last row or element others, and not used.
 template <typename T, int DK, int LD, int THREADS>
-__device__ __forceinline__ void load_rows(T* to, const T* from, int64_t stride_t, int64_t dk, int64_t t0, int64_t seqlen,
-                                          const int* live, int* bad) {
+struct RowLoader {
   typedef T v4 __attribute__((ext_vector_type(4)));
+  static constexpr int kUnits = kC * DK / 4 / THREADS;
+  v4 v[kUnits];
+  // A thread has the same four elements of rows THREADS / (DK / 4) apart.
+  static __device__ __forceinline__ int row_of(int i) { return i * (THREADS / (DK / 4)) + threadIdx.x / (DK / 4); }
+  static __device__ __forceinline__ int first() { return threadIdx.x % (DK / 4) * 4; }
+  __device__ __forceinline__ void load(const T* from, int64_t stride_t, int dk, int64_t t0, int64_t seqlen) {
+    const int last = (int)min((int64_t)kC, seqlen - t0) - 1;
+    from += t0 * stride_t;
+    const int d = first();
+    if (dk == DK) {
 #pragma unroll
-  for (int i = 0; i < kC * DK / 4 / THREADS; ++i) {
-    const int u = i * THREADS + threadIdx.x, row = u / (DK / 4), d = u % (DK / 4) * 4;
-    v4 v = {};
-    if (t0 + row < seqlen && live[row]) {
-      const T* p = from + (t0 + row) * stride_t + d;
-      if (d + 4 <= dk) {
-        __builtin_memcpy(&v, p, sizeof v);
-      } else {
+      for (int i = 0; i < kUnits; ++i) __builtin_memcpy(&v[i], from + min(row_of(i), last) * stride_t + d, sizeof v[i]);
+    } else {
 #pragma unroll
-        for (int e = 0; e < 3; ++e)
-          if (d + e < dk) v[e] = p[e];
-      }
-      bool finite = true;
+      for (int i = 0; i < kUnits; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) finite &= __builtin_isfinite(to_f32(v[e]));
-      if (!finite) bad[row] = 1;
+        for (int e = 0; e < 4; ++e) v[i][e] = from[min(row_of(i), last) * stride_t + min(d + e, dk - 1)];
     }
-    *reinterpret_cast<v4*>(to + row * LD + d) = v;
   }
-}
+  // Zero where `live` has no row and past the last element; `bad` says which rows hold an infinity or NaN.
+  __device__ __forceinline__ void store(T* to, int dk, uint64_t live, int* bad) {
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      const int row = row_of(i), d = first(), left = live >> row & 1 ? dk - d : 0;
+      float none = 0.0f;  // stays zero beside numbers
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (e >= left) v[i][e] = (T)0.0f;
+        none = fmaf(to_f32(v[i][e]), 0.0f, none);
+      }
+      if (none != 0.0f) bad[row] = 1;
+      *reinterpret_cast<v4*>(to + row * LD + d) = v[i];
+    }
+  }
+};
 
 // All chunks: the operands of the chains as fragments, T and P (forward) or their transposes (backward).
 // A workgroup has a chunk of a key head and all heads of it, or, where that is too few workgroups, one of them each
 // (p.prep_heads). Reads q and k, writes them three (four) times as fragments and 30 KiB a head's chunk; bound by
-// latency within a workgroup, so three of them a CU: at B=4 T=4096, 16 heads of 128 128 -> 106 us forward.
+// latency within a workgroup, so three of them a CU: at B=4 T=4096, 16 heads of 128 82 us forward and 89 backward, of
+// which the 0.31 and 0.36 GB take 60 and 71 at a copy's rate. With q and k requested row by row behind the rows'
+// factors, and those a head at a time, it took 108 and 116; with two workgroups a CU 128 before that.
 template <typename T, int DK, bool BWD>
 __global__ __launch_bounds__(256, 3) void delta_prep_kernel(DeltaParams p) {
   constexpr int NI = kPieces<T>, KS = DK / 32, LD = DK + 16 / sizeof(T), LA = 68;
@@ -345,7 +373,9 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(DeltaParams p) {
   // q and k, and once the fragments are made, A (then T) and T's tiles on the diagonal
   constexpr size_t kRowsBytes = 2 * kC * LD * sizeof(T), kMatrixBytes = (kC * LA + 4 * 16 * 20) * sizeof(float);
   __shared__ __attribute__((aligned(16))) char room[kRowsBytes > kMatrixBytes ? kRowsBytes : kMatrixBytes];
-  __shared__ ChunkShared sh;
+  __shared__ ChunkShared shared[4];  // of four heads at a time, one a wave
+  __shared__ int bad_rows[2][kC];    // whether a row's k, q hold an infinity or NaN
+  __shared__ uint64_t live_rows;
   T *kl = reinterpret_cast<T*>(room), *ql = kl + kC * LD;
   float *al = reinterpret_cast<float*>(room), *td = al + kC * LA;
   const ccv1d_delta_args& a = p.a;
@@ -354,20 +384,34 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(DeltaParams p) {
   const int64_t kc = blockIdx.x / shares;  // (batch, key head, chunk)
   const int64_t c = kc % p.chunks, bk = kc / p.chunks, b = bk / a.key_heads, kh = bk - b * a.key_heads;
   const int64_t t0 = c * kC;
-  if (m == 0) {
-    share_rows(a, b, c, kh * p.group, lane, sh, nullptr, false);
-    sh.bad_k[lane] = sh.bad_q[lane] = 0;
+  const int h0 = (int)kh * p.group + share * p.prep_heads, heads = h0 + p.prep_heads;
+  auto rows_of = [&](int h) { return p.rows + ((b * a.heads + h) * p.chunks + c) * (kRowFields * kC); };
+  // The rows' gates first, then q and k: the rows' factors are made while these are on their way.
+  RawGates raw;
+  RowLoader<T, DK, LD, 256> kr, qr;
+  raw.load(a, b, c, min(h0 + m, heads - 1), lane);
+  kr.load(static_cast<const T*>(a.k) + b * a.k_stride_b + kh * a.k_stride_h, a.k_stride_t, (int)a.key_dim, t0, a.seqlen);
+  constexpr bool BOTH = kPieces<T> * DK <= 256;  // else q's are requested when k's are there: registers
+  if (BOTH)
+    qr.load(static_cast<const T*>(a.q) + b * a.q_stride_b + kh * a.q_stride_h, a.q_stride_t, (int)a.key_dim, t0, a.seqlen);
+  if (h0 + m < heads) {
+    const bool live = share_rows(a, raw, c, lane, shared[m], rows_of(h0 + m), false);
+    const uint64_t all = __ballot(live);
+    if (m == 0 && lane == 0) live_rows = all;
   }
+  if (m == 3) bad_rows[0][lane] = bad_rows[1][lane] = 0;
   lds_barrier();
-  load_rows<T, DK, LD, 256>(kl, static_cast<const T*>(a.k) + b * a.k_stride_b + kh * a.k_stride_h, a.k_stride_t,
-                            a.key_dim, t0, a.seqlen, sh.live, sh.bad_k);
-  load_rows<T, DK, LD, 256>(ql, static_cast<const T*>(a.q) + b * a.q_stride_b + kh * a.q_stride_h, a.q_stride_t,
-                            a.key_dim, t0, a.seqlen, sh.live, sh.bad_q);
+  kr.store(kl, (int)a.key_dim, live_rows, bad_rows[0]);
+  if (!BOTH)
+    qr.load(static_cast<const T*>(a.q) + b * a.q_stride_b + kh * a.q_stride_h, a.q_stride_t, (int)a.key_dim, t0, a.seqlen);
+  qr.store(ql, (int)a.key_dim, live_rows, bad_rows[1]);
   lds_barrier();
-  const uint64_t bad_k = __ballot(sh.bad_k[lane] != 0), bad_q = __ballot(sh.bad_q[lane] != 0);
+  const uint64_t bad_k = __ballot(bad_rows[0][lane] != 0), bad_q = __ballot(bad_rows[1][lane] != 0);
   if (bad_k) {  // the same in all waves
     for (int i = threadIdx.x; i < kC * DK; i += 256)
       if (bad_k >> (i / DK) & 1) kl[i / DK * LD + i % DK] = (T)0.0f;
+    raw.load(a, b, c, min(h0 + m, heads - 1), lane);
+    if (h0 + m < heads) share_rows(a, raw, c, lane, shared[m], rows_of(h0 + m), bad_k >> lane & 1);
     lds_barrier();
   }
 
@@ -425,27 +469,48 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(DeltaParams p) {
         if constexpr (BWD) column(ql, bad_q, p.qt + kc * (DK / 16 * 2 * NI * 64));
       }
 
-  const int64_t h0 = kh * p.group + share * p.prep_heads;
-  for (int64_t h = h0; h < h0 + p.prep_heads; ++h) {
+  for (int h = h0; h < heads; ++h) {
     const int64_t hc = (b * a.heads + h) * p.chunks + c;
     u4* tf = p.tf + hc * (kTri * 3 * 64);
     u4* pf = p.pf + hc * (kTri * NP * 64);
+    const int turn = (h - h0) & 3;
     lds_barrier();
-    if (m == 0) share_rows(a, b, c, h, lane, sh, p.rows + hc * (kRowFields * kC), bad_k >> lane & 1);
-    lds_barrier();
+    if (turn == 0 && h > h0) {  // four more heads
+      if (h + m < heads) {
+        raw.load(a, b, c, h + m, lane);
+        share_rows(a, raw, c, lane, shared[m], rows_of(h + m), bad_rows[0][lane]);
+      }
+      lds_barrier();
+    }
+    const ChunkShared& sh = shared[turn];
+    // Of tile (n, m) a lane has one i and four j, backward four i and one j.
+    double sum_m[BWD ? 4 : 1];
+    int run_m[BWD ? 4 : 1];
+    float beta_m[BWD ? 4 : 1];
+#pragma unroll
+    for (int e = 0; e < (BWD ? 4 : 1); ++e) {
+      const int i = 16 * m + (BWD ? 4 * g + e : col);
+      sum_m[e] = sh.sum[i], run_m[e] = sh.run[i], beta_m[e] = sh.beta[i];
+    }
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       if (n > m + 1) continue;
-      // tile (n, m): of the lane's four results, i and j
       f4 pv = {0, 0, 0, 0};
       if (n <= m) {
+        f4 av;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int i = 16 * m + (BWD ? 4 * g + e : col), j = 16 * n + (BWD ? col : 4 * g + e);
-          const bool seen = j <= i && sh.run[i] == sh.run[j];
-          const float d = seen ? exp2_of(sh.sum[i] - sh.sum[j]) : 0.0f;
-          al[i * LA + j] = seen && j < i ? sh.beta[i] * d * kk[n][e] : 0.0f;
+          const int x = BWD ? e : 0, i = 16 * m + (BWD ? 4 * g + e : col), j = 16 * n + (BWD ? col : 4 * g + e);
+          const bool seen = j <= i && run_m[x] == sh.run[j];
+          const float d = seen ? exp2_of(sum_m[x] - sh.sum[j]) : 0.0f;
+          av[e] = seen && j < i ? beta_m[x] * d * kk[n][e] : 0.0f;
           pv[e] = seen ? a.scale * d * qk[n][e] : 0.0f;
+        }
+        if constexpr (BWD) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) al[(16 * m + 4 * g + e) * LA + 16 * n + col] = av[e];
+        } else {
+          *reinterpret_cast<f4*>(&al[(16 * m + col) * LA + 16 * n + 4 * g]) = av;
         }
       } else if (m & 1) {
         continue;  // no half of a fragment that is read
@@ -568,9 +633,6 @@ struct Chain {
 // in fp16 and fp32, whose operands alone are 130 and 200 registers.
 template <typename T, int DK>
 constexpr bool kLoadAhead = kPieces<T> * DK < 512;
-
-// A wave's number, known to be the same in all lanes.
-__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 template <int N>
 __device__ __forceinline__ void load_frag(const u4* p, uint32_t lane, u4 (&o)[N]) {
