@@ -363,7 +363,7 @@ struct RowLoader {
 // All chunks: the operands of the chains as fragments, T and P (forward) or their transposes (backward).
 // A workgroup has a chunk of a key head and all heads of it, or, where that is too few workgroups, one of them each
 // (p.prep_heads). Reads q and k, writes them three (four) times as fragments and 30 KiB a head's chunk; bound by
-// latency within a workgroup, so three of them a CU: at B=4 T=4096, 16 heads of 128 82 us forward and 89 backward, of
+// latency within a workgroup, so three of them a CU: at B=4 T=4096, 16 heads of 128 72 us forward and 82 backward, of
 // which the 0.31 and 0.36 GB take 60 and 71 at a copy's rate. With q and k requested row by row behind the rows'
 // factors, and those a head at a time, it took 108 and 116; with two workgroups a CU 128 before that.
 template <typename T, int DK, bool BWD>
@@ -380,9 +380,10 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(DeltaParams p) {
   float *al = reinterpret_cast<float*>(room), *td = al + kC * LA;
   const ccv1d_delta_args& a = p.a;
   const int lane = threadIdx.x & 63, m = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  const int shares = p.group / p.prep_heads, share = blockIdx.x % shares;
-  const int64_t kc = blockIdx.x / shares;  // (batch, key head, chunk)
-  const int64_t c = kc % p.chunks, bk = kc / p.chunks, b = bk / a.key_heads, kh = bk - b * a.key_heads;
+  const uint32_t shares = p.group / p.prep_heads, share = blockIdx.x % shares;
+  const uint32_t unit = blockIdx.x / shares;  // (batch, key head, chunk); 32 bits, in which divisions are short
+  const uint32_t bkh = unit / (uint32_t)p.chunks, batch = bkh / (uint32_t)a.key_heads;
+  const int64_t kc = unit, c = unit - bkh * p.chunks, b = batch, kh = bkh - batch * (uint32_t)a.key_heads;
   const int64_t t0 = c * kC;
   const int h0 = (int)kh * p.group + share * p.prep_heads, heads = h0 + p.prep_heads;
   auto rows_of = [&](int h) { return p.rows + ((b * a.heads + h) * p.chunks + c) * (kRowFields * kC); };
@@ -498,13 +499,21 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(DeltaParams p) {
       f4 pv = {0, 0, 0, 0};
       if (n <= m) {
         f4 av;
+        double sum_n[BWD ? 1 : 4];
+        int run_n[BWD ? 1 : 4];
+#pragma unroll
+        for (int e = 0; e < (BWD ? 1 : 4); ++e) {
+          const int j = 16 * n + (BWD ? col : 4 * g + e);
+          sum_n[e] = sh.sum[j], run_n[e] = sh.run[j];
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
+          const int y = BWD ? 0 : e;
           const int x = BWD ? e : 0, i = 16 * m + (BWD ? 4 * g + e : col), j = 16 * n + (BWD ? col : 4 * g + e);
-          const bool seen = j <= i && run_m[x] == sh.run[j];
-          const float d = seen ? exp2_of(sum_m[x] - sh.sum[j]) : 0.0f;
-          av[e] = seen && j < i ? beta_m[x] * d * kk[n][e] : 0.0f;
-          pv[e] = seen ? a.scale * d * qk[n][e] : 0.0f;
+          const bool seen = (j <= i) & (run_m[x] == run_n[y]);
+          const float d = exp2_of(sum_m[x] - sum_n[y]), av_e = beta_m[x] * d * kk[n][e], pv_e = a.scale * d * qk[n][e];
+          av[e] = seen & (j < i) ? av_e : 0.0f;
+          pv[e] = seen ? pv_e : 0.0f;
         }
         if constexpr (BWD) {
 #pragma unroll
