@@ -1603,14 +1603,15 @@ __global__ __launch_bounds__((kGradWaves<T, DK>) * 64, kPieces<T> > 1 ? 1 : 2) v
       for (int i = 0; i < PAIRS; ++i)
         if (w + NW * i < 10) {
           const Pair t(w + NW * i);
-          const int r = 16 * t.m + col;
+          const int r = 16 * t.m + col, j0 = 16 * t.n + 4 * g, run_r = run[r];
+          const double sum_r = sum[r];
           f4 x;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int j = 16 * t.n + 4 * g + e;
-            const bool seen = (round ? j < r : j <= r) && run[r] == run[j];
-            const float d = seen ? exp2_of(sum[r] - sum[j]) : 0.0f;
-            x[e] = seen ? (round ? d * gr[i][e] : p.scale * d * go[i][e]) : 0.0f;
+            const int j = j0 + e;
+            const bool seen = (round ? j < r : j <= r) & (run_r == run[j]);
+            const float d = exp2_of(sum_r - sum[j]), y = round ? d * gr[i][e] : p.scale * d * go[i][e];
+            x[e] = seen ? y : 0.0f;
           }
           *reinterpret_cast<f4*>(&gl[r * LG + 16 * t.n + 4 * g]) = x;
         }
