@@ -49,31 +49,31 @@ def update(**kw):
 
 
 @pytest.mark.parametrize("kw,msg", [
-    (dict(state=torch.zeros(3, 4, 8, 6)), "on the device of k"),
-    (dict(state_indices=torch.zeros(3, dtype=torch.int32)), "on the device of k"),
-    (dict(q=z(3, 2, 8, dtype=F)), "the dtype of k"),
-    (dict(q=z(3, 2, 8).requires_grad_()), "no backward"),
-    (dict(beta=z(3, 4).requires_grad_()), "no backward"),
-    (dict(state=z(3, 4, 8, 6, dtype=F).requires_grad_()), "no backward"),
+    (lambda: dict(state=torch.zeros(3, 4, 8, 6)), "on the device of k"),
+    (lambda: dict(state_indices=torch.zeros(3, dtype=torch.int32)), "on the device of k"),
+    (lambda: dict(q=z(3, 2, 8, dtype=F)), "the dtype of k"),
+    (lambda: dict(q=z(3, 2, 8).requires_grad_()), "no backward"),
+    (lambda: dict(beta=z(3, 4).requires_grad_()), "no backward"),
+    (lambda: dict(state=z(3, 4, 8, 6, dtype=F).requires_grad_()), "no backward"),
 ])
 def test_update(kw, msg):
     with pytest.raises(AssertionError) as e:
-        update(**kw)
+        update(**kw())
     assert msg in str(e.value)
 
 
 @pytest.mark.parametrize("kw,err,msg", [
-    (dict(residual=torch.zeros(3, 8)), AssertionError, "on the device of x"),
-    (dict(post_weight=torch.zeros(8)), AssertionError, "on the device of x"),
-    (dict(scale=torch.zeros(8)), AssertionError, "on the device of x"),
-    (dict(gate=z(3, 8, dtype=F)), AssertionError, "gate must have the dtype of x"),
-    (dict(residual=z(3, 8, dtype=torch.float16)), AssertionError, "the dtype of x or be fp32"),
-    (dict(post_weight=z(8, dtype=torch.float64)), TypeError, "unsupported dtype"),
-    (dict(residual=z(3, 8, dtype=torch.int32)), TypeError, "unsupported dtype"),
+    (lambda: dict(residual=torch.zeros(3, 8)), AssertionError, "on the device of x"),
+    (lambda: dict(post_weight=torch.zeros(8)), AssertionError, "on the device of x"),
+    (lambda: dict(scale=torch.zeros(8)), AssertionError, "on the device of x"),
+    (lambda: dict(gate=z(3, 8, dtype=F)), AssertionError, "gate must have the dtype of x"),
+    (lambda: dict(residual=z(3, 8, dtype=torch.float16)), AssertionError, "the dtype of x or be fp32"),
+    (lambda: dict(post_weight=z(8, dtype=torch.float64)), TypeError, "unsupported dtype"),
+    (lambda: dict(residual=z(3, 8, dtype=torch.int32)), TypeError, "unsupported dtype"),
 ])
 def test_norm(kw, err, msg):
     with pytest.raises(err) as e:
-        block_norm_fn(**{**dict(x=z(3, 8), post_weight=z(8)), **kw})
+        block_norm_fn(**{**dict(x=z(3, 8), post_weight=z(8)), **kw()})
     assert msg in str(e.value)
 
 
