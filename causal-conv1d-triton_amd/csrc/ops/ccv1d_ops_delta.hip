@@ -80,7 +80,8 @@ hipError_t run(const ccv1d_delta_args& a, bool backward, hipStream_t s) {
   p.a = a;
   p.chunks = (int32_t)z.chunks;
   p.group = (int32_t)(a.heads / a.key_heads);
-  // Up to 512 workgroups run at once with some room: below that a head each is quicker, though each reads q and k anew.
+  // Up to 512 workgroups run at once with some room: below that a head each is quicker, though each reads q and k anew
+  // (B=4 T=256, 16 heads of 128 over 8 key heads: 128 workgroups of two heads 21 us, 256 of one 17).
   p.prep_heads = a.batch * a.key_heads * z.chunks < 512 ? 1 : p.group;
   p.dk = (int32_t)z.dk, p.dvp = (int32_t)z.dvp, p.tiles = (int32_t)z.tiles;
   char* ws = static_cast<char*>(a.workspace);
@@ -101,7 +102,8 @@ hipError_t run(const ccv1d_delta_args& a, bool backward, hipStream_t s) {
 // One token of a request and head, 64 value columns a workgroup: four a lane, the keys' elements over 16 groups of
 // lanes, ROWS each. One reading of the state gives S^T k and S^T q, from which
 //   u = beta (v - a S^T k),  o = scale (a S^T q + (q.k) u),  S <- a S + k u^T,  a = exp(g).
-// Bound by memory: the states are read and written once.
+// Bound by memory: the states are read and written once, at 128 rows of 32 heads of 128 by 128 537 MB in 107 us (5.0 TB/s,
+// a copy's rate); 4 rows of 8 heads take 6.7 us, the latency of a reading, a sum over waves and a launch.
 template <typename T, int ROWS>
 __global__ __launch_bounds__(256) void delta_update_kernel(ccv1d_delta_update_args p, int32_t group, int32_t cols) {
   typedef float f4 __attribute__((ext_vector_type(4)));
