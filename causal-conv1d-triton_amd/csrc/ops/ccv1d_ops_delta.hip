@@ -18,7 +18,7 @@ __global__ __launch_bounds__(256) void delta_empty_kernel(const float* from, flo
 struct Sizes {
   int64_t chunks, dk, dvp, tiles;
   int64_t kfrag;  // units of 16 bytes of the fragments of k by rows in a chunk, as the others of q and k
-  int64_t tri, pieces_out;
+  int64_t tri, units_p;  // units of a triangle's fragments; of one of P in the forward
 };
 
 Sizes sizes_of(const ccv1d_delta_args& a) {
@@ -30,7 +30,7 @@ Sizes sizes_of(const ccv1d_delta_args& a) {
   const int64_t pieces = a.dtype == CCV1D_BF16 ? 1 : a.dtype == CCV1D_F16 ? 2 : 3;
   z.kfrag = CCV1D_DELTA_CHUNK * z.dk / 8 * pieces;
   z.tri = 6 * 64;
-  z.pieces_out = a.dtype == CCV1D_F32 ? 3 : 2;
+  z.units_p = a.dtype == CCV1D_F32 ? 3 : 2;
   return z;
 }
 
@@ -54,7 +54,7 @@ Places places_of(const ccv1d_delta_args& a, const Sizes& z, bool backward) {
   p.kt = next(kc * z.kfrag * 16);
   p.qt = next(backward ? kc * z.kfrag * 16 : 0);
   p.tf = next(hc * z.tri * 3 * 16);
-  p.pf = next(hc * z.tri * (backward ? 3 : z.pieces_out) * 16);
+  p.pf = next(hc * z.tri * (backward ? 3 : z.units_p) * 16);
   p.rows = next(hc * kRowFloats * 4);
   p.ds = next(backward ? hc * z.dk * z.dvp * 4 : 0);
   p.dr = next(backward ? hc * CCV1D_DELTA_CHUNK * z.dvp * 4 : 0);

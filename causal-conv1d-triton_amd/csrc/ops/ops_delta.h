@@ -22,9 +22,9 @@
 //
 // Products run on the bf16 matrix cores (16x16x32), fp32 operands as sums of bf16 pieces: cut after 8 bits each, three
 // pieces are the fp32 number itself, and the products of pieces i + j <= 2 leave out 2^-22 of the largest term.
-// bf16 inputs are one piece, fp16 inputs two (11 bits), fp32 three. Nothing that reaches a state or a gradient is
-// rounded to fewer than fp32's bits; what reaches an output in 16 bits alone (P and U in P U, S0 in Q S0) keeps
-// two pieces, 2^-15 or better. By the rates of the instructions (16x16x32 in 16 bits 16 cycles, 16x16x4 in fp32
+// bf16 inputs are one piece, fp16 inputs two (11 bits), fp32 three. Nothing but the results themselves is rounded to fewer
+// than fp32's bits: with two pieces of P, U and S0 in the outputs' products, 2^-15, one bf16 output in a hundred was the
+// number beside the nearest. By the rates of the instructions (16x16x32 in 16 bits 16 cycles, 16x16x4 in fp32
 // 32) three pieces against a bf16 input take 3/16 of fp32's time, against three pieces 6/16.
 //
 // A row that holds an infinity or NaN spoils its sequence from there on and nothing else, though the products run over all
@@ -54,9 +54,9 @@ constexpr double kLog2eDouble = 1.4426950408889634074;
 
 template <typename T>
 constexpr int kPieces = std::is_same_v<T, __bf16> ? 1 : std::is_same_v<T, _Float16> ? 2 : 3;
-// Pieces and limit of what reaches an output of type T alone.
+// Units of 16 bytes a lane of a fragment of P: its pieces, or, in 16 bits, the eight fp32 numbers.
 template <typename T>
-constexpr int kOutPieces = sizeof(T) == 4 ? 3 : 2;
+constexpr int kUnitsP = sizeof(T) == 4 ? 3 : 2;
 
 // A wave's number, known to be the same in all lanes.
 __device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
@@ -369,7 +369,7 @@ struct RowLoader {
 template <typename T, int DK, bool BWD>
 __global__ __launch_bounds__(256, 3) void delta_prep_kernel(DeltaParams p) {
   constexpr int NI = kPieces<T>, KS = DK / 32, LD = DK + 16 / sizeof(T), LA = 68;
-  constexpr int NP = BWD ? 3 : kOutPieces<T>;
+  constexpr int NP = BWD ? 3 : kUnitsP<T>;
   // q and k, and once the fragments are made, A (then T) and T's tiles on the diagonal
   constexpr size_t kRowsBytes = 2 * kC * LD * sizeof(T), kMatrixBytes = (kC * LA + 4 * 16 * 20) * sizeof(float);
   __shared__ __attribute__((aligned(16))) char room[kRowsBytes > kMatrixBytes ? kRowsBytes : kMatrixBytes];
@@ -524,13 +524,17 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(DeltaParams p) {
       } else if (m & 1) {
         continue;  // no half of a fragment that is read
       }
-      u2 w[NP];
-      split4<NP>(pv, w);
+      if constexpr (NP == 2) {
+        reinterpret_cast<f4*>(pf)[(lower_frag(m, n / 2) * 2 + (n & 1)) * 64 + lane] = pv;
+        continue;
+      }
+      u2 w[3];
+      split4<3>(pv, w);
       if constexpr (BWD) {
         // rows j of tile n, sum over i of tile m; the tile m of a pair in front of n's is zero
-        store_half<NP>(pf + upper_frag(n, m / 2) * (NP * 64) + lane, m & 1, w);
+        store_half<3>(pf + upper_frag(n, m / 2) * (NP * 64) + lane, m & 1, w);
       } else {
-        store_half<NP>(pf + lower_frag(m, n / 2) * (NP * 64) + lane, n & 1, w);
+        store_half<3>(pf + lower_frag(m, n / 2) * (NP * 64) + lane, n & 1, w);
       }
     }
     lds_barrier();
@@ -745,17 +749,17 @@ __device__ __forceinline__ f4 sum_apart(const u4 (&a)[2][NA], const u4 (*f)[NB][
 
 // The chain of states forward: a workgroup has CT tiles of 16 value columns of a head. Bound by latency: three
 // products after one another a chunk, each behind a barrier; the waves that make the outputs run beside them. At B=4
-// T=4096, 16 heads of 128 in bf16, training, 290 us, of which states and corrections kept take 90 and operands out of
+// T=4096, 16 heads of 128 in bf16, training, 300 us, of which states and corrections kept take 90 and operands out of
 // the caches 80; VALUs are 21 %, matrix cores 13 %, LDS 16 % busy. Without the four waves beside 378; 64 columns a
 // workgroup with the operands through LDS 490 to 914; 16 columns a wave on its own 1525; operands requested into the L2 two
 // chunks ahead 306 (then 276).
 template <typename T, int DK, int CT, bool SAVE>
 __global__ __launch_bounds__(512) void delta_fwd_kernel(DeltaParams p) {
   using L = Chain<DK>;
-  constexpr int NI = kPieces<T>, KS = L::kKS, KB = L::kKB, NO = kOutPieces<T>, LO = NO - 1;
+  constexpr int NI = kPieces<T>, KS = L::kKS, KB = L::kKB, NP = kUnitsP<T>;
   constexpr bool AHEAD = kLoadAhead<T, DK>;
   __shared__ f4 red[CT][L::kParts][4][64];
-  __shared__ u4 sp[CT][KS][NO][64], rb[CT][2][3][64], ub[CT][2][3][64], uo[CT][2][NO][64];
+  __shared__ u4 sp[CT][KS][3][64], rb[CT][2][3][64], ub[CT][2][3][64], uo[CT][2][3][64];
   const ccv1d_delta_args& a = p.a;
   const ChainPlace at = chain_place<CT>(p);
   if (!at.any) return;
@@ -770,14 +774,14 @@ __global__ __launch_bounds__(512) void delta_fwd_kernel(DeltaParams p) {
   const u4* qf = p.qf + (b * a.key_heads + kh) * N * (4 * KS * NI * 64);
   const u4* kt = p.kt + (b * a.key_heads + kh) * N * (DK / 16 * 2 * NI * 64);
   const u4* tf = p.tf + at.head * N * (kTri * 3 * 64);
-  const u4* pf = p.pf + at.head * N * (kTri * NO * 64);
+  const u4* pf = p.pf + at.head * N * (kTri * NP * 64);
   const float* rows = p.rows + at.head * N * (kRowFields * kC);
   auto runs_of = [&](int64_t c) {
     return reinterpret_cast<const int*>(rows + c * (kRowFields * kC) + 7 * kC);
   };
 
   if (wave >= 4) {  // outputs: O = scale e^G Q S0 + P U of a tile of rows
-    u4 qx[KS][NI], px[2][NO];
+    u4 qx[KS][NI], raw[2][NP], px[2][3];
     f4 into, live;
     auto load_q = [&](int64_t c) {
 #pragma unroll
@@ -788,7 +792,7 @@ __global__ __launch_bounds__(512) void delta_fwd_kernel(DeltaParams p) {
       live = *reinterpret_cast<const f4*>(rows + c * (kRowFields * kC) + 3 * kC + row);
 #pragma unroll
       for (int s = 0; s < 2; ++s)
-        if (s <= w / 2) load_frag(pf + c * (kTri * NO * 64) + lower_frag(w, s) * (NO * 64), lane, px[s]);
+        if (s <= w / 2) load_frag(pf + c * (kTri * NP * 64) + lower_frag(w, s) * (NP * 64), lane, raw[s]);
     };
     const int64_t stride = a.heads * a.value_dim;
     T* out = static_cast<T*>(a.out) + (b * a.seqlen + row) * stride + h * a.value_dim + dv;
@@ -797,24 +801,42 @@ __global__ __launch_bounds__(512) void delta_fwd_kernel(DeltaParams p) {
     for (int64_t c = 0; c < N; ++c) {
       const int64_t next = c + 1 < N ? c + 1 : c;
       lds_barrier();
-      f4 o[CT], base[CT];
+      f4 o[CT], base[CT], y[CT][2] = {};
+      auto state_part = [&](int from, int to) {  // steps of Q S0
 #pragma unroll
-      for (int n = 0; n < CT; ++n) {
-        f4 y[2] = {};
+        for (int n = 0; n < CT; ++n)
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          u4 so[NO];
-          load_frag(&sp[n][s][0][0], lane, so);
-          y[s & 1] = mac<LO>(qx[s], so, y[s & 1]);
-        }
+          for (int s = from; s < to; ++s) {
+            u4 so[3];
+            load_frag(&sp[n][s][0][0], lane, so);
+            y[n][s & 1] = mac<2>(qx[s], so, y[n][s & 1]);
+          }
+      };
+      state_part(0, KS / 4);  // the chain's waves have more to do behind this barrier than in front of it
+      lds_barrier();
+      state_part(KS / 4, KS);
+#pragma unroll
+      for (int n = 0; n < CT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          o[n][e] = a.scale * into[e] * (y[0][e] + y[1][e]);
+          o[n][e] = a.scale * into[e] * (y[n][0][e] + y[n][1][e]);
           if (into[e] == 0.0f) o[n][e] = 0.0f;  // not a product with zero: the state may hold no number
         }
-      }
+      // Here, not later: the next rows' factors would get other registers, and wait to be moved.
+#pragma unroll
+      for (int n = 0; n < CT; ++n) asm volatile("" : "+v"(o[n]));
       load_q(next);
-      lds_barrier();
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (s <= w / 2) {
+          if constexpr (NP == 2) {
+            asm volatile("" : "+v"(raw[s][0]), "+v"(raw[s][1]));  // not before: right behind the loads it would wait for them
+            split8<3>(__builtin_bit_cast(f4, raw[s][0]), __builtin_bit_cast(f4, raw[s][1]), px[s]);
+          } else {
+#pragma unroll
+            for (int n = 0; n < 3; ++n) px[s][n] = raw[s][n];
+          }
+        }
       lds_barrier();
 #pragma unroll
       for (int n = 0; n < CT; ++n) {
@@ -822,15 +844,15 @@ __global__ __launch_bounds__(512) void delta_fwd_kernel(DeltaParams p) {
 #pragma unroll
         for (int s = 0; s < 2; ++s)
           if (s <= w / 2) {
-            u4 u[NO];
+            u4 u[3];
             load_frag(&uo[n][s][0][0], lane, u);
-            o[n] = mac<LO>(px[s], u, o[n]);
+            o[n] = mac<2>(px[s], u, o[n]);
           }
       }
       if (any_not_finite(o))
 #pragma unroll
         for (int n = 0; n < CT; ++n)
-          o[n] = sum_apart<false, true, LO>(px, uo[n], lane, 0, w / 2, base[n], runs_of(c), row);
+          o[n] = sum_apart<false, true, 2>(px, uo[n], lane, 0, w / 2, base[n], runs_of(c), row);
       T* to = out + c * (kC * stride);
 #pragma unroll
       for (int n = 0; n < CT; ++n)
@@ -924,7 +946,7 @@ __global__ __launch_bounds__(512) void delta_fwd_kernel(DeltaParams p) {
           split8<3>(state[n][2 * i], state[n][2 * i + 1], sb);
           if (keeper)
 #pragma unroll
-            for (int j = 0; j < NO; ++j) sp[n][part * KB + i][j][lane] = sb[j];
+            for (int j = 0; j < 3; ++j) sp[n][part * KB + i][j][lane] = sb[j];
 #pragma unroll
           for (int m = 0; m < L::kRows; ++m) x[n][m] = mac<2>(kx[i][m], sb, x[n][m]);
         }
@@ -997,11 +1019,11 @@ __global__ __launch_bounds__(512) void delta_fwd_kernel(DeltaParams p) {
       if (!plain)
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = rest[e] != 0.0f ? y[e] : 0.0f;
-      u2 half[3], out[NO];
+      u2 half[3];
       split4<3>(y, half);
       store_half<3>(&ub[n][w / 2][0][lane], w & 1, half);
-      split4<NO>(u[n], out);
-      store_half<NO>(&uo[n][w / 2][0][lane], w & 1, out);
+      split4<3>(u[n], half);
+      store_half<3>(&uo[n][w / 2][0][lane], w & 1, half);
     }
     if constexpr (SAVE) {
       float* to = us + c * (kC * (int64_t)p.dvp);
