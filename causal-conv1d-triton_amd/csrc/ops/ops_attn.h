@@ -387,21 +387,28 @@ __global__ __launch_bounds__(kAttnWaves* kWave, sizeof(T) * DH > 768 ? 1 : 2) vo
 
     // Scores.
     float x[kMine];
+    f32x4 s[kTiles];
     const bool tail = Dh % (4 * kE) != 0 || Dh < DH;
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
-      f32x4 s = {0, 0, 0, 0};
+      s[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
         if (tail && (4 * c + g) * kE >= Dh) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) kw[t][c][i] = 0;
         }
-        s = product32<T>(kw[t][c], q[c], s);
+        s[t] = product32<T>(kw[t][c], q[c], s[t]);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[4 * t + i] = s[i] * to2;
     }
+    // The waits that a matrix instruction's result needs, in full: around the branches above the compiler counts them along
+    // the longer path alone, and in 16 bits, heads of 64, left out one of eight on the shorter one. (In fp32, where none is
+    // left out, heads of 256 would take 463 us in place of 437.)
+    if constexpr (sizeof(T) == 2)
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) asm volatile("s_nop 7" : "+v"(s[t]));
+#pragma unroll
+    for (int e = 0; e < kMine; ++e) x[e] = s[e / 4][e % 4] * to2;
     if constexpr (kLate) {
       __builtin_amdgcn_sched_barrier(0);
       load_values();

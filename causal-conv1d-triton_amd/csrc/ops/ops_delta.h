@@ -379,6 +379,9 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(DeltaParams p) {
   T *kl = reinterpret_cast<T*>(room), *ql = kl + kC * LD;
   float *al = reinterpret_cast<float*>(room), *td = al + kC * LA;
   const ccv1d_delta_args& a = p.a;
+  // The wave's number is not known to be the same in all lanes here: with branches on a scalar the compiler leaves out 7 of
+  // the 10 waits behind the last product of T, keys above 128, backward, and every fourth row of T lacks a term
+  // (tests/test_matrix_waits.py reads the built kernels for such places).
   const int lane = threadIdx.x & 63, m = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
   const uint32_t shares = p.group / p.prep_heads, share = blockIdx.x % shares;
   const uint32_t unit = blockIdx.x / shares;  // (batch, key head, chunk); 32 bits, in which divisions are short
