@@ -21,7 +21,8 @@ from torch import Tensor
 from ._ops import native
 
 
-# The two passes as torch.library operators, for torch.compile. Absent outputs are empty tensors.
+# The two passes as torch.library operators, for torch.compile, and the forward without what the backward needs. Absent
+# outputs are empty tensors.
 
 
 @torch.library.custom_op("causal_conv1d_amd::gated_delta", mutates_args=(), device_types="cuda")
@@ -75,6 +76,20 @@ def _op_backward(ctx, dout, dfinal, _):
 _fwd_op.register_autograd(_op_backward, setup_context=_op_setup)
 
 
+@torch.library.custom_op("causal_conv1d_amd::gated_delta_infer", mutates_args=(), device_types="cuda")
+def _infer_op(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor, seq_idx: Tensor | None,
+              initial_states: Tensor | None, scale: float, final_states: bool) -> tuple[Tensor, Tensor]:
+    out, fin, _ = native().delta_fwd(q, k, v, log_decay, beta, seq_idx, initial_states, scale, final_states, False)
+    return out, v.new_empty(0) if fin is None else fin
+
+
+@_infer_op.register_fake
+def _infer_fake(q, k, v, log_decay, beta, seq_idx, initial_states, scale, final_states):
+    B, T, H, Dv = v.shape
+    return (v.new_empty(B, T, H, Dv),
+            v.new_empty(B, H, k.shape[3], Dv, dtype=torch.float32) if final_states else v.new_empty(0))
+
+
 def gated_delta_fn(
     q: Tensor,
     k: Tensor,
@@ -109,12 +124,16 @@ def gated_delta_fn(
     Gradients: q, k, v, log_decay, beta and initial_states. Results are deterministic. Training keeps, beside the
     inputs, key_dim / 64 + 1 fp32 numbers for each of v's until the backward.
     """
+    train = torch.is_grad_enabled() and any(
+        getattr(t, "requires_grad", False) for t in (q, k, v, log_decay, beta, initial_states))
     if torch.compiler.is_compiling():
         if scale is None:
             scale = k.shape[-1] ** -0.5
-        out, final, _ = _fwd_op(q, k, v, log_decay, beta, seq_idx, initial_states, scale)
-    elif torch.is_grad_enabled() and any(
-            getattr(t, "requires_grad", False) for t in (q, k, v, log_decay, beta, initial_states)):
+        if train:
+            out, final, _ = _fwd_op(q, k, v, log_decay, beta, seq_idx, initial_states, scale)
+        else:
+            out, final = _infer_op(q, k, v, log_decay, beta, seq_idx, initial_states, scale, return_final_states)
+    elif train:
         out, final = native().delta_train(q, k, v, log_decay, beta, seq_idx, initial_states, scale,
                                           return_final_states)
     else:
