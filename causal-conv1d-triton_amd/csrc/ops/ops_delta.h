@@ -299,6 +299,11 @@ __device__ __forceinline__ ChunkRows chunk_row(const ccv1d_delta_args& a, const 
 
 __device__ __forceinline__ float exp2_of(double x) { return __builtin_amdgcn_exp2f((float)x); }
 
+// The decay of a state to a row that it reaches: never zero, which says that it does not, so that an infinity or NaN in
+// it stays there however small the decay (the hardware's is zero below 2^-126). Of numbers up to 2^20 the smallest
+// denormal number leaves less than 2^-128.
+__device__ __forceinline__ float reaching(double x) { return fmaxf(exp2_of(x), 0x1p-149f); }
+
 struct ChunkShared {
   double sum[kC];
   int run[kC];
@@ -312,11 +317,11 @@ __device__ __forceinline__ bool share_rows(const ccv1d_delta_args& a, const RawG
   sh.sum[lane] = r.sum, sh.run[lane] = r.run, sh.beta[lane] = r.beta;
   const double end = __shfl(r.sum, 63);
   const int last = __shfl(r.run, 63);
-  rows[lane] = r.live && r.run == 0 ? exp2_of(r.sum) : 0.0f;
-  rows[kC + lane] = r.live && r.run == last ? exp2_of(end - r.sum) : 0.0f;
+  rows[lane] = r.live && r.run == 0 ? reaching(r.sum) : 0.0f;
+  rows[kC + lane] = r.live && r.run == last ? reaching(end - r.sum) : 0.0f;
   rows[2 * kC + lane] = r.spoilt ? __builtin_nanf("") : r.beta;
   rows[3 * kC + lane] = r.live ? 1.0f : 0.0f;
-  rows[4 * kC + lane] = lane == 0 && last == 0 ? exp2_of(end) : 0.0f;
+  rows[4 * kC + lane] = lane == 0 && last == 0 ? reaching(end) : 0.0f;
   reinterpret_cast<double*>(rows + 5 * kC)[lane] = r.sum;
   reinterpret_cast<int*>(rows + 7 * kC)[lane] = r.run;
   return r.live;
