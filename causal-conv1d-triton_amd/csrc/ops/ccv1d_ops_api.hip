@@ -142,7 +142,8 @@ int check_norm(const ccv1d_norm_args* a) {
   if (!dtype_ok(a->dtype)) return invalid("dtype must be fp32, fp16 or bf16");
   if (a->residual_dtype != a->dtype && a->residual_dtype != CCV1D_F32)
     return invalid("residual_dtype must be dtype or fp32");
-  if (a->residual_dtype != a->dtype && !a->residual) return invalid("residual_dtype is dtype without residual");
+  if (a->residual_dtype != a->dtype && !a->residual && a->outer > 0 && a->inner > 0)  // of no rows a residual is null, too
+    return invalid("residual_dtype is dtype without residual");
   if (!a->post_weight && !a->pre_weight) return invalid("post_weight and pre_weight are null");
   if ((a->post_weight && !dtype_ok(a->post_dtype)) || (a->scale_weight && !dtype_ok(a->scale_dtype)) ||
       (a->pre_weight && !dtype_ok(a->pre_dtype)))
