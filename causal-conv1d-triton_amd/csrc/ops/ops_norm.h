@@ -22,7 +22,10 @@ namespace ccv1d {
 namespace ops {
 
 constexpr int kVec = 8;       // elements a lane and step
+// log2 e in two parts, and ln 2.
 constexpr float kLog2eNorm = 1.44269504088896340736f;
+constexpr float kLog2eRest = (float)(1.44269504088896340736 - (double)kLog2eNorm);
+constexpr float kLn2Norm = 0.693147180559945309417f;
 
 // Eight elements from an address that is aligned to one.
 template <typename T>
@@ -82,9 +85,12 @@ __device__ __forceinline__ void load_weight(const void* p, int type, int64_t at,
 }
 
 // act(z) and act'(z). The hardware's exp2 and reciprocal, 1 ulp each; exp(-z) past fp32's range is infinity, and the
-// sigmoid zero.
+// sigmoid zero. What the rounding of -z log2 e leaves, up to 2^-18 for z = -80, comes as a factor 1 + rest ln 2; where
+// that product is beyond fp32's exponents, infinite or NaN, there is none.
 __device__ __forceinline__ float sigmoid_of(float z) {
-  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2eNorm * z));
+  const float t = -kLog2eNorm * z;
+  const float rest = fmaf(-kLog2eRest, z, fmaf(-kLog2eNorm, z, -t));
+  return __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_exp2f(t), fabsf(t) < 256.0f ? fmaf(rest, kLn2Norm, 1.0f) : 1.0f, 1.0f));
 }
 __device__ __forceinline__ float act_of(float z, int act) {
   if (act == CCV1D_NORM_IDENTITY) return z;
