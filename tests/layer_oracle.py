@@ -143,3 +143,31 @@ def norm_close(got, want, name, t):
                              if t.get(n) is not None and t[n].numel()])
         bound = 64 * U * (size + parts)
     close(got, want, bound, name)
+
+
+# Root mean squares, in units of 2^-24 of the tensor's own. A step of a sum in fp32 rounds by 0.3 units of its result in
+# the mean; a product over the keys' elements or the rows is up to 48 steps (8 instructions for each of six pairs of
+# pieces), whose partial sums are smaller than the last: 2 units. Three such products follow one another in a chunk, a chunk's
+# error shrinks with its state, and the backward goes through as many again: 5 units. The gradient of the log-decays is
+# a difference of sums over the rows behind, whose parts are up to three times as large.
+RMS_UNITS = {"g": 24}
+
+
+def rms_units(got, want):
+    off = (got.detach().double().cpu() - want).square().mean().sqrt()
+    return float(off / want.square().mean().sqrt()) / U
+
+
+def rms_close(got, want, name):
+    assert got.dtype == torch.float32 and got.shape == want.shape
+    if want.any():
+        units = rms_units(got, want)
+        assert units <= RMS_UNITS.get(name, 8), (name, units)
+    else:
+        assert not got.any(), name
+
+
+def share_beside(got, want):
+    """Of results of 16 bits of a quarter of their root mean square and more, the share that is not the nearest number."""
+    large = want.abs() >= 0.25 * want.square().mean().sqrt()
+    return float((got.cpu() != want.to(got.dtype))[large].double().mean())

@@ -7,6 +7,7 @@ import torch
 import layer_oracle as oracle
 from causal_conv1d_triton.norm import block_norm_fn
 from test_layer_delta import BF, F, HF, make, run
+from test_layer_norm import make as make_norm, run as run_norm
 
 pytestmark = pytest.mark.gpu
 
@@ -19,10 +20,62 @@ def test_outputs_of_16_bits_are_the_nearest(dtype, Dk):
     square, eight units of fp32, and outputs of a quarter of that and more, whose steps are more than 2^-8 (bf16) or
     2^-11 (fp16) of themselves: 2^-10 or 2^-7 of them."""
     t = make(Dk, B=2, T=300, Hk=2, H=4, Dk=Dk, Dv=64, dtype=dtype, init=True, grad=False)
-    got, want = run(t)["out"].cpu(), oracle.delta_all(t)["out"]
-    large = want.abs() >= 0.25 * want.square().mean().sqrt()
-    share = float((got != want.to(dtype))[large].double().mean())
+    share = oracle.share_beside(run(t)["out"], oracle.delta_all(t)["out"])
     assert share <= {BF: 2.0 ** -10, HF: 2.0 ** -7}[dtype], share
+
+
+def trained(seed, **kw):
+    t = make(seed, init=True, **kw)
+    t["beta"] = t["beta"].float()
+    final = torch.randn(t["init"].shape, generator=torch.Generator().manual_seed(seed))
+    return run(t, final), oracle.delta_all(t, final)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("Dk,Dv,T", [(64, 40, 64), (64, 64, 300), (100, 33, 129), (128, 64, 300), (130, 40, 70), (256, 64, 300)])
+@pytest.mark.parametrize("dtype", [F, BF, HF])
+def test_delta_in_fp32(dtype, Dk, Dv, T, packed):
+    """Everything that is kept in fp32, in the root mean square; results of 16 bits are the nearest numbers."""
+    got, want = trained(Dk + T, B=2, T=T, Hk=2, H=4, Dk=Dk, Dv=Dv, dtype=dtype, packed=packed)
+    for n, x in got.items():
+        if x.dtype == F:
+            oracle.rms_close(x, want[n], n)
+        else:
+            # as the outputs above, with the means of e = 2^-20: sums over heads and small tensors
+            assert oracle.share_beside(x, want[n]) <= {BF: 2.0 ** -9, HF: 2.0 ** -6}[dtype], n
+
+
+@pytest.mark.parametrize("dtype", [F, BF, HF])
+def test_update_in_fp32(dtype):
+    from causal_conv1d_triton.delta import gated_delta_update
+    t = make(41, B=1, T=50, Hk=2, H=4, Dk=128, Dv=128, dtype=dtype, grad=False)
+    gen = torch.Generator().manual_seed(1)
+    state = torch.randn(50, 4, 128, 128, generator=gen)
+    names = ("q", "k", "v", "g", "beta")
+    one = {n: t[n][0][:, None] for n in names}
+    want = oracle.delta_all(dict(one, init=state))
+    pool = state.cuda()
+    with torch.no_grad():
+        out = gated_delta_update(*(t[n][0].cuda() for n in names), pool)
+    oracle.rms_close(pool, want["final"], "final")
+    if dtype == F:
+        oracle.rms_close(out[:, None], want["out"], "out")
+    else:
+        assert oracle.share_beside(out[:, None], want["out"]) <= {BF: 2.0 ** -10, HF: 2.0 ** -7}[dtype]
+
+
+@pytest.mark.parametrize("rows,D", [(33, 64), (33, 300), (1025, 2048), (7, 8192), (40000, 128)])
+@pytest.mark.parametrize("dtype", [F, BF, HF])
+def test_norms_in_fp32(dtype, rows, D):
+    """The weights' gradients, sums over all rows in 32 lines of 1024 at most, and in fp32 everything, in the root mean
+    square: a row left out of 40000 would be 5000 units and more, a sum kept in 16 bits 74."""
+    t = make_norm(rows + D, (rows, D), dtype, F, True, True, "tensor", True)
+    got, want = run_norm(t), oracle.norm_all(t)
+    for n, x in got.items():
+        if x.dtype == F:
+            oracle.rms_close(x, want[n], n)
+        else:
+            assert oracle.share_beside(x, want[n]) <= {BF: 2.0 ** -9, HF: 2.0 ** -6}[dtype], n
 
 
 @pytest.mark.parametrize("activation", ["silu", "sigmoid"])
