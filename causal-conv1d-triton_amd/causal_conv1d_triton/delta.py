@@ -113,8 +113,9 @@ def gated_delta_fn(
       seq_idx: optional (batch, seqlen) integer ids marking packed sequences: the state starts at zero in each
          row whose id differs from the row before; rows with a negative id are padding, whose outputs and
          gradients are zero whatever the inputs hold there. initial_states belong to the sequence of seq_idx[:, 0].
-         An infinity or NaN in a row that is no padding spoils that sequence from there on (and its gradients),
-         no other; only finite keys so long that the products of 64 rows overflow fp32 can.
+         An infinity or NaN in a row that is no padding, or a log-decay above 88.7, whose exponential is infinite in
+         fp32, on a state, spoils that sequence from there on (and its gradients), no other; only finite keys so long,
+         or log-decays of several rows so far above zero, that the products of 64 rows overflow fp32 can.
       initial_states: optional (batch, heads, key_dim, value_dim), any float type, the state in front of row 0.
       return_final_states: also return the state behind the last row (zero where that is padding), of the shape of
          initial_states in fp32, which is the initial_states of a following chunk; gradients flow through it.

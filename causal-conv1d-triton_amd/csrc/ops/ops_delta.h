@@ -280,10 +280,11 @@ __device__ __forceinline__ ChunkRows chunk_row(const ccv1d_delta_args& a, const 
   r.reset = in && (raw.id < 0 || raw.id != raw.before);
   float g = r.live ? RawGates::number(raw.g, a.log_decay_dtype) : 0.0f;
   r.beta = r.live ? RawGates::number(raw.beta, a.beta_dtype) : 0.0f;
-  r.spoilt = r.live && (bad_key || g != g || g == INFINITY || !__builtin_isfinite(r.beta));
+  const bool infinite = g > 88.72f && !r.reset;  // its exponential, in fp32
+  r.spoilt = r.live && (bad_key || g != g || g == INFINITY || infinite || !__builtin_isfinite(r.beta));
   if (g < -104.0f) r.reset = true;
   if (r.spoilt) r.beta = 0.0f;
-  if (g != g || g == INFINITY) g = 0.0f;
+  if (g != g || g == INFINITY || infinite) g = 0.0f;
   const uint64_t resets = __ballot(r.reset);
   r.run = __popcll(resets & (~uint64_t(0) >> (63 - lane)));
   double s = r.reset ? 0.0 : (double)g * kLog2eDouble;

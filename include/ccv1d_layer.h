@@ -33,8 +33,9 @@ extern "C" {
  * fp32) empties the state. With seq_idx the state starts at zero in each row whose id differs from the row
  * before it; initial_states belong to the sequence of seq_idx[:, 0]; rows of a negative id are padding:
  * their output is zero, the state behind them zero, whatever they hold, and no gradient leaves them. An
- * infinity or NaN in another row spoils its own sequence alone: outputs from that row on (in q: that row's; in v:
- * its column's), gradients. Only finite keys so long that 64 rows' products overflow fp32 can spoil more.
+ * infinity or NaN in another row, or a log-decay above 88.7 (whose exponential is infinite in fp32) on a state, spoils its
+ * own sequence alone: outputs from that row on (in q: that row's; in v: its column's), gradients. Only finite keys so long,
+ * or log-decays of several rows so far above zero, that 64 rows' products overflow fp32 can spoil more.
  * ------------------------------------------------------------------------------------------- */
 
 /* Rows of a chunk: the forward hands the backward the state in front of every chunk, and the corrections u
@@ -67,8 +68,8 @@ struct ccv1d_delta_args {
   /* forward */
   void* out;           /* (batch, seqlen, heads, value_dim) contiguous, type dtype */
   float* final_states; /* (batch, heads, key_dim, value_dim): the state behind the last row; or NULL */
-  float* saved;        /* ccv1d_delta_saved_floats() floats: forward: written when not NULL; backward: what
-                          the forward wrote */
+  float* saved;        /* ccv1d_delta_saved_floats() floats, aligned to 16 bytes: forward: written when not NULL;
+                          backward: what the forward wrote */
   /* backward */
   const void* dout; /* (batch, seqlen, heads, value_dim), type dtype, unit last stride */
   int64_t dout_stride_b, dout_stride_t, dout_stride_h;

@@ -57,3 +57,24 @@ def test_gradients_in_front_of_a_strong_decay(dtype, Dk):
     assert torch.equal(got["init"], clean["init"]) and torch.equal(got["out"], clean["out"])
     t["seq"] = None
     assert not torch.isfinite(run(t)["init"]).any()
+
+
+@pytest.mark.parametrize("row", [50, 70])
+@pytest.mark.parametrize("dtype,Dk", [(BF, 64), (HF, 128), (F, 100), (BF, 256)])
+def test_an_infinite_decay_spoils_its_own_sequence(dtype, Dk, row):
+    """A finite log-decay whose exponential is infinite in fp32; in the first row of a sequence it multiplies nothing."""
+    t = make(34, B=1, T=270, Hk=1, H=2, Dk=Dk, Dv=40, dtype=dtype, init=True)
+    starts = torch.tensor([0, 17, 40, 75, 90, 150, 192, 263])
+    t["seq"] = (torch.arange(270)[:, None] >= starts).sum(1).int()[None]
+    clean = run(t)
+    t["g"] = t["g"].clone()
+    t["g"][:, row] = 200.0
+    t["g"][:, 90] = 200.0
+    got = run(t)
+    own = (torch.arange(270) >= 40) & (torch.arange(270) < 75)
+    for n in ("out", "q", "k", "v", "g", "beta"):
+        assert torch.equal(got[n][:, ~own], clean[n][:, ~own]), n
+    for n in ("final", "init"):
+        assert torch.equal(got[n], clean[n]), n
+    assert torch.equal(got["out"][:, 40:row], clean["out"][:, 40:row])
+    assert not torch.isfinite(got["out"][:, row:75]).any()
