@@ -117,13 +117,15 @@ def gated_delta_fn(
          fp32, on a state, spoils that sequence from there on (and its gradients), no other; only finite keys so long,
          or log-decays of several rows so far above zero, that the products of 64 rows overflow fp32 can.
       initial_states: optional (batch, heads, key_dim, value_dim), any float type, the state in front of row 0.
-      return_final_states: also return the state behind the last row (zero where that is padding), of the shape of
-         initial_states in fp32, which is the initial_states of a following chunk; gradients flow through it.
+      return_final_states: also return the state behind the last row (zero where that is padding, so prompts of
+         unequal length take a call each), of the shape of initial_states in fp32, which is the initial_states of a
+         following chunk; gradients flow through it.
       scale: of the outputs, key_dim ** -0.5 without.
 
     Returns `out` (batch, seqlen, heads, value_dim), rounded once to v's dtype, or `(out, final_states)`.
     Gradients: q, k, v, log_decay, beta and initial_states. Results are deterministic. Training keeps, beside the
-    inputs, key_dim / 64 + 1 fp32 numbers for each of v's until the backward.
+    inputs, ceil(seqlen / 64) * (K + 64) * V fp32 numbers of each batch and head until the backward, K being key_dim
+    raised to 64, 128 or 256 and V value_dim to a multiple of 32; the backward takes as many again while it runs.
     """
     train = torch.is_grad_enabled() and any(
         getattr(t, "requires_grad", False) for t in (q, k, v, log_decay, beta, initial_states))

@@ -84,7 +84,8 @@ def block_norm_fn(
         r = residual + scale * m                         back to the residual stream
         y = r * pre_weight / sqrt(mean(r^2) + eps)       the norm before the next block
 
-    over the last dimension, in fp32 whatever the types, every result rounded once (y from the unrounded r).
+    over the last dimension, in fp32 whatever the types, every result rounded once (y from the unrounded r). So a row whose
+    squares add up to more than fp32 holds, with elements beyond 1e17 or so, comes out of a norm as zero.
 
     Arguments:
       x: (..., dim) on a GPU, bf16, fp16 or fp32, dim at most 8192. Unit last stride and rows that two

@@ -102,8 +102,9 @@ hipError_t run(const ccv1d_delta_args& a, bool backward, hipStream_t s) {
 // One token of a request and head, 64 value columns a workgroup: four a lane, the keys' elements over 16 groups of
 // lanes, ROWS each. One reading of the state gives S^T k and S^T q, from which
 //   u = beta (v - a S^T k),  o = scale (a S^T q + (q.k) u),  S <- a S + k u^T,  a = exp(g).
-// Bound by memory: the states are read and written once, at 128 rows of 32 heads of 128 by 128 537 MB in 107 us (5.0 TB/s,
-// a copy's rate); 4 rows of 8 heads take 6.7 us, the latency of a reading, a sum over waves and a launch.
+// Bound by memory: the states are read and written once, at 128 rows of 32 heads of 128 by 128 537 MB, 126 us a call on a
+// pool that lies outside the caches (4.3 TB/s, 0.84 of a copy's rate), 107 on one that stays in them. 4 rows of 8
+// heads take 6.7 us, the latency of the slot's number, a reading of its state and a sum over waves.
 template <typename T, int ROWS>
 __global__ __launch_bounds__(256) void delta_update_kernel(ccv1d_delta_update_args p, int32_t group, int32_t cols) {
   typedef float f4 __attribute__((ext_vector_type(4)));

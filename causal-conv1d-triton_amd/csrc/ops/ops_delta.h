@@ -761,7 +761,7 @@ __device__ __forceinline__ f4 sum_apart(const u4 (&a)[2][NA], const u4 (*f)[NB][
 // The chain of states forward: a workgroup has CT tiles of 16 value columns of a head. Bound by latency: three
 // products after one another a chunk, each behind a barrier; the waves that make the outputs run beside them. At B=4
 // T=4096, 16 heads of 128 in bf16, training, 300 us, of which states and corrections kept take 90 and operands out of
-// the caches 80; VALUs are 21 %, matrix cores 13 %, LDS 16 % busy. Without the four waves beside 378; 64 columns a
+// the caches 80; VALUs are 23 %, matrix cores 15 %, LDS 18 % busy. Without the four waves beside 378; 64 columns a
 // workgroup with the operands through LDS 490 to 914; 16 columns a wave on its own 1525; operands requested into the L2 two
 // chunks ahead 306 (then 276).
 template <typename T, int DK, int CT, bool SAVE>

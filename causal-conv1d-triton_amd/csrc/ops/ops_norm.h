@@ -2,7 +2,7 @@
 //
 // A row lies in the registers of 16 to 512 lanes, 8 elements a lane and step, so that each tensor is read once and
 // written once per direction; its sums go through the wave and, for rows of several waves, LDS. Bound by memory:
-// forward at 32768 rows of 4096 in bf16 with all parts 263 us (5.1 TB/s, a copy's rate), at 16384 rows of 2048 with an
+// forward at 32768 rows of 4096 in bf16 with all parts 265 us (5.1 TB/s, a copy's rate), at 16384 rows of 2048 with an
 // fp32 stream 78 us (5.2 TB/s), backward there 178 (3.5 TB/s; VALUs 40 % busy, rows one after another: a row requested ahead
 // 196, three waves a SIMD 206), weights' sums 7.
 // Backward, with h1 = x inv1, h2 = r inv2, t2 = w2 dy, inv = 1 / sqrt(mean(.^2) + eps):
